@@ -1619,6 +1619,143 @@ bool emitFmhaF32(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::s
   return true;
 }
 
+// ---------------------------------------------------------------------------
+// The families of a decoding step.  Everything that a model fixes (heads, page, strides, types, options) is a parameter; how many
+// tokens, requests and pages there are is an argument of the kernel, a whole number of 64 bits, since it is another in every step, and
+// the caller gives the grid.
+bool whole(const KernelSpec& s, const char* key, int64_t low, int64_t high, std::string& err) {
+  const int64_t v = s.get(key, low - 1);
+  if (v >= low && v <= high) return true;
+  err = s.family + ": " + key + " must be in [" + std::to_string(low) + "," + std::to_string(high) + "]";
+  return false;
+}
+
+bool powerOfTwo(int64_t v) { return v > 0 && (v & (v - 1)) == 0; }
+
+// Strides of an 8-bit cache in bytes: the rows are read in runs of 16 bytes.
+bool cacheShape(KernelSpec& s, std::initializer_list<const char*> strides, std::string& err) {
+  if (!whole(s, "H", 1, 65536, err) || !whole(s, "D", 32, 256, err) || !whole(s, "PAGE", 16, 256, err)) return false;
+  if (s.p["D"] % 32) { err = s.family + ": D must be a multiple of 32"; return false; }
+  if (!powerOfTwo(s.p["PAGE"])) { err = s.family + ": PAGE must be a power of two"; return false; }
+  for (auto key : strides)
+    if (!whole(s, key, 0, (int64_t)1 << 40, err)) return false;
+    else if (s.p[key] % 16) { err = s.family + ": " + key + " must be a multiple of 16 bytes"; return false; }
+  return true;
+}
+
+const char* typeName(int64_t f16) { return f16 == 0 ? "float" : f16 == 1 ? "_Float16" : "__bf16"; }      // as in the row kernels
+
+bool emitPageSlots(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::string& err) {
+  const int64_t block = s.get("BLOCK", 1024);
+  if (block < 64 || block > 1024 || block % 64) { err = "page_slots: BLOCK must be a multiple of 64 up to 1024"; return false; }
+  s.p["BLOCK"] = block;
+  Defines d;
+  d.add("PS_NAME", s.name);
+  d.add("PS_BLOCK", block);
+  src = d.wrap(kTpl_page_slots);
+  info.name = s.name;
+  info.block[0] = (uint32_t)block;
+  info.numArgs = 15;
+  return true;
+}
+
+bool emitCacheWrite(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::string& err) {
+  if (!cacheShape(s, {"KP", "KT", "KH", "VP", "VT", "VH"}, err)) return false;
+  if (!whole(s, "F16", 0, 2, err) || !whole(s, "WIN", 1, 64, err)) return false;
+  const int64_t esize = s.p["F16"] ? 2 : 4;
+  for (auto key : {"XKT", "XKH", "XVT", "XVH"})
+    if (!whole(s, key, 0, (int64_t)1 << 40, err)) return false;
+    else if (s.p[key] * esize % 16) { err = std::string("cache_write: ") + key + " must be a multiple of 16 bytes"; return false; }
+  Defines d;
+  d.add("CW_NAME", s.name);
+  d.add("CW_T", std::string(typeName(s.p["F16"])));
+  for (auto key : {"H", "D", "PAGE", "WIN"}) d.add(std::string("CW_") + key, s.p[key]);
+  for (auto key : {"KP", "KT", "KH", "VP", "VT", "VH", "XKT", "XKH", "XVT", "XVH"}) d.add(std::string("CW_") + key, std::to_string(s.p[key]) + "LL");
+  src = d.wrap(kTpl_cache_write);
+  info.name = s.name;
+  info.block[0] = 256;
+  info.numArgs = 9;
+  return true;
+}
+
+bool emitCacheRead(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::string& err) {
+  if (!cacheShape(s, {"KP", "KT", "KH"}, err) || !whole(s, "F16", 0, 2, err)) return false;
+  const int64_t unroll = s.get("UNROLL", 1);
+  if (unroll < 1 || unroll > 8) { err = "cache_read: UNROLL must be in [1,8]"; return false; }
+  s.p["UNROLL"] = unroll;
+  Defines d;
+  d.add("CR_NAME", s.name);
+  d.add("CR_T", std::string(typeName(s.p["F16"])));
+  d.add("CR_H", s.p["H"]); d.add("CR_D", s.p["D"]); d.add("CR_PAGE", s.p["PAGE"]); d.add("CR_UNROLL", unroll);
+  d.add("CR_P", std::to_string(s.p["KP"]) + "LL"); d.add("CR_TS", std::to_string(s.p["KT"]) + "LL"); d.add("CR_HS", std::to_string(s.p["KH"]) + "LL");
+  src = d.wrap(kTpl_cache_read);
+  info.name = s.name;
+  info.block[0] = 256;
+  info.numArgs = 6;
+  return true;
+}
+
+// cache_attention, and cache_join, which adds up what its workgroups leave of tiles that they share: the same parameters.
+bool emitCacheAttention(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::string& err) {
+  if (!cacheShape(s, {"KP", "KT", "KH", "VP", "VT", "VH"}, err)) return false;
+  if (!whole(s, "G", 1, 65536, err) || !whole(s, "RB", 1, 4, err) || !whole(s, "F16", 0, 1, err)) return false;
+  const int64_t rb = s.p["RB"], dh = s.p["D"], g = s.p["G"];
+  if (!powerOfTwo(rb)) { err = "cache_attention: RB must be 1, 2 or 4"; return false; }
+  if (rb == 4 && dh > 128) { err = "cache_attention: 64 rows of more than 128 do not fit the registers"; return false; }
+  for (auto key : {"QT", "QH"})
+    if (!whole(s, key, 0, (int64_t)1 << 40, err)) return false;
+    else if (s.p[key] % 8) { err = std::string("cache_attention: ") + key + " must be a multiple of 16 bytes"; return false; }
+  const bool starts = s.get("STARTS", 0) != 0, slopes = s.get("SLOPES", 0) != 0, wholeTiles = s.get("WHOLE", 0) != 0, join = s.family == "cache_join";
+  const int64_t window = s.get("WINDOW", 0), grid = s.get("GRID", 512), least = s.get("LEAST", 2);
+  if (window < 0 || window > 0x7FFFFFFF) { err = "cache_attention: WINDOW must be in [0,2^31)"; return false; }
+  if (grid < 8 || grid > 65536 || grid % 8) { err = "cache_attention: GRID must be a multiple of 8 up to 65536"; return false; }
+  if (least < 1) { err = "cache_attention: LEAST must be positive"; return false; }
+  if (wholeTiles && (starts || join)) { err = "cache_attention: whole tiles are for one row per request, and need no join"; return false; }
+  const double cap = s.f.count("CAP") ? s.f["CAP"] : 0.0, scale = s.f.count("SCALE") ? s.f["SCALE"] : 1.0;
+  if (!(cap >= 0.0) || !std::isfinite(cap) || !std::isfinite(scale)) { err = "cache_attention: CAP must not be negative, CAP and SCALE must be finite"; return false; }
+  const int64_t rows = 16 * rb, gs = std::min(g, rows);
+  Defines d;
+  d.add("CA_NAME", s.name);
+  d.add("CA_JOIN", join ? 1 : 0);
+  d.add("CA_D", dh); d.add("CA_HKV", s.p["H"]); d.add("CA_G", g); d.add("CA_GS", gs); d.add("CA_PAGE", s.p["PAGE"]);
+  d.add("CA_F16", s.p["F16"]); d.add("CA_RB", rb); d.add("CA_GRID", grid); d.add("CA_WHOLE", wholeTiles ? 1 : 0); d.add("CA_MIN", least);
+  d.add("CA_OCC", s.get("OCC", rb == 4 || dh > (rb == 2 ? 64 : 128) ? 1 : 2));
+  d.add("CA_SCALE", floatLiteral(scale)); d.add("CA_CAP", floatLiteral(cap)); d.add("CA_HAS_CAP", cap > 0.0 ? 1 : 0);
+  d.add("CA_WINDOW", window); d.add("CA_SLOPES", slopes ? 1 : 0); d.add("CA_STARTS", starts ? 1 : 0);
+  for (auto key : {"KP", "KT", "KH", "VP", "VT", "VH", "QT", "QH"}) d.add(std::string("CA_") + key, std::to_string(s.p[key]) + "LL");
+  src = d.wrap(kTpl_cache_attention);
+  info.name = s.name;
+  info.grid[0] = (uint32_t)(join ? grid - 1 : grid);
+  if (join) info.grid[1] = (uint32_t)(rb * dh / 16);
+  info.block[0] = 256;
+  info.numArgs = join ? 7 : 16;
+  return true;
+}
+
+bool emitGemmQ4(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::string& err) {
+  if (!whole(s, "N", 1, 0x7FFFFFF0, err) || !whole(s, "K", 32, 0x7FFFFF00, err) || !whole(s, "GROUP", 32, 0x7FFFFF00, err)) return false;
+  if (!whole(s, "F16", 0, 1, err) || !whole(s, "MB", 1, 4, err)) return false;
+  const int64_t n = s.p["N"], k = s.p["K"], group = s.p["GROUP"], mb = s.p["MB"];
+  if (group != 32 && group != 64 && group % 128) { err = "gemm_q4: GROUP must be 32, 64 or a multiple of 128"; return false; }
+  if (k % group) { err = "gemm_q4: GROUP must divide K"; return false; }
+  const int64_t nt = s.get("NT", 1), waves = s.get("WAVES", 8);
+  if (nt < 1 || nt > 4 || waves < 1 || waves > 16 || waves * mb * nt * 1024 > 163840) { err = "gemm_q4: bad NT or WAVES"; return false; }
+  s.p["NT"] = nt; s.p["WAVES"] = waves;
+  const char* x = s.p["F16"] ? "_Float16" : "__bf16";
+  Defines d;
+  d.add("Q4_NAME", s.name);
+  d.add("Q4_N", n); d.add("Q4_K", k); d.add("Q4_GROUP", group); d.add("Q4_F16", s.p["F16"]); d.add("Q4_ZERO", s.get("ZERO", 0) ? 1 : 0);
+  d.add("Q4_ST", std::string(s.get("SCALE_F32", 0) ? "float" : x));
+  d.add("Q4_YT", std::string(s.get("OUT_F32", 0) ? "float" : x));
+  d.add("Q4_MB", mb); d.add("Q4_NT", nt); d.add("Q4_WAVES", waves);
+  src = d.wrap(kTpl_gemm_q4);
+  info.name = s.name;
+  info.grid[0] = (uint32_t)ceilDiv(n, 16 * nt);
+  info.block[0] = (uint32_t)(64 * waves);
+  info.numArgs = 6;
+  return true;
+}
+
 }  // namespace
 
 const std::string& prelude() {
@@ -1644,6 +1781,11 @@ bool emitKernel(KernelSpec& spec, std::string& src, KernelLaunchInfo& info, std:
   if (spec.family == "gemm_fp8") return emitGemmFp8(spec, src, info, err);
   if (spec.family == "fmha_bf16") return emitFmhaBf16(spec, src, info, err);
   if (spec.family == "fmha_f32") return emitFmhaF32(spec, src, info, err);
+  if (spec.family == "page_slots") return emitPageSlots(spec, src, info, err);
+  if (spec.family == "cache_write") return emitCacheWrite(spec, src, info, err);
+  if (spec.family == "cache_read") return emitCacheRead(spec, src, info, err);
+  if (spec.family == "cache_attention" || spec.family == "cache_join") return emitCacheAttention(spec, src, info, err);
+  if (spec.family == "gemm_q4") return emitGemmQ4(spec, src, info, err);
   err = "unknown kernel family '" + spec.family + "'";
   return false;
 }

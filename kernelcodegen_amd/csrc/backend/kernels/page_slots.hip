@@ -1,0 +1,82 @@
+// ---- page tables and slots of one step's tokens ----
+//   before_b = ceil(length_b / page), after_b = ceil((length_b + added_b) / page); request b takes after_b - before_b pages off the list
+//   of free ones, those of earlier requests first, and its table is continued with them; its new tokens get the positions from
+//   length_b on and the slots table[position / page] * page + position % page (-1 where there is no page)
+// Every workgroup takes the prefix sums of all requests (1024 at a time) and then its share of the pages and tokens, each found by
+// bisection in the sums in LDS: a step of any shape is one launch with two dependent reads per token.
+// Parameters: PS_NAME, PS_BLOCK.
+struct PsSums { int pages[PS_BLOCK + 1], tokens[PS_BLOCK + 1], waves[2][PS_BLOCK / 64]; };
+
+extern "C" __global__ __launch_bounds__(PS_BLOCK)
+void PS_NAME(const int* __restrict__ lengths, const int* __restrict__ added, int* __restrict__ table, const int* __restrict__ free_pages,
+             long long* __restrict__ slots, int* __restrict__ positions, int* __restrict__ starts, int* __restrict__ lengths_out,
+             int* __restrict__ used, long long B_, long long T_, long long W_, long long table_row, long long F_, long long page_) {
+  __shared__ PsSums s;
+  const int B = (int)B_, T = (int)T_, W = (int)W_, F = (int)F_, page = (int)page_;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = blockIdx.x * PS_BLOCK + threadIdx.x, step = gridDim.x * PS_BLOCK;
+  int pages0 = 0, tokens0 = 0;                 // of the requests before this round's
+  for (int b0 = 0; b0 < B; b0 += PS_BLOCK) {
+    const int b = b0 + threadIdx.x, n = B - b0 < PS_BLOCK ? B - b0 : PS_BLOCK;
+    int len = 0, add = 0;
+    if (b < B) {
+      len = lengths[b] > 0 ? lengths[b] : 0;
+      add = added[b] > 0 ? added[b] : 0;
+    }
+    int p = (len + add + page - 1) / page - (len + page - 1) / page, t = add;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int op = __shfl_up(p, off, 64), ot = __shfl_up(t, off, 64);
+      if (lane >= off) { p += op; t += ot; }
+    }
+    if (lane == 63) { s.waves[0][wave] = p; s.waves[1][wave] = t; }
+    __syncthreads();
+    int pb = 0, tb = 0;
+    for (int w = 0; w < wave; ++w) { pb += s.waves[0][w]; tb += s.waves[1][w]; }
+    s.pages[threadIdx.x + 1] = pb + p;
+    s.tokens[threadIdx.x + 1] = tb + t;
+    if (threadIdx.x == 0) s.pages[0] = s.tokens[0] = 0;
+    __syncthreads();
+    if (blockIdx.x == 0 && b < B) {
+      starts[b + 1] = tokens0 + s.tokens[threadIdx.x + 1];
+      lengths_out[b] = len + add;
+      if (b == 0) starts[0] = 0;
+    }
+    // which request of this round: the last whose sum before it is not over `i`
+    auto find = [&](const int* sums, int i) {
+      int lo = 0, hi = n - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (sums[mid] <= i) lo = mid; else hi = mid - 1;
+      }
+      return lo;
+    };
+    for (int i = first; i < s.pages[n]; i += step) {
+      const int r = find(s.pages, i), have = lengths[b0 + r] > 0 ? lengths[b0 + r] : 0;
+      const int column = (have + page - 1) / page + i - s.pages[r];
+      if (column < W && pages0 + i < F) table[(long long)(b0 + r) * table_row + column] = free_pages[pages0 + i];
+    }
+    for (int i = first; i < s.tokens[n] && tokens0 + i < T; i += step) {
+      const int r = find(s.tokens, i), have = lengths[b0 + r] > 0 ? lengths[b0 + r] : 0;
+      const int before = (have + page - 1) / page, at = have + i - s.tokens[r], column = at / page;
+      int id = -1;
+      if (column < W) {
+        if (column < before) {
+          id = table[(long long)(b0 + r) * table_row + column];
+        } else {
+          const int k = pages0 + s.pages[r] + column - before;
+          if (k < F) id = free_pages[k];
+        }
+      }
+      slots[tokens0 + i] = id < 0 ? -1 : (long long)id * page + at % page;
+      positions[tokens0 + i] = at;
+    }
+    pages0 += s.pages[n];
+    tokens0 += s.tokens[n];
+    __syncthreads();
+  }
+  for (int i = tokens0 + first; i < T; i += step) {
+    slots[i] = -1;
+    positions[i] = -1;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) used[0] = pages0 < F ? pages0 : F;
+}

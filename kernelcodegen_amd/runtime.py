@@ -221,22 +221,23 @@ class Kernel:
         holders, arr = self._pack(self._complete(args))
         check(lib().kcg_hip_launch(self.handle, g, b, lds, self._stream(stream), arr), "kcg_hip_launch")
 
-    def bind(self, scalars=0):
+    def bind(self, scalars=0, grid=None):
         """launch() on the current stream for a kernel without a workspace, as a function of the arguments' values: device
-        pointers as integers, then `scalars` fp32 numbers.  Everything that is the same for all launches is prepared here:
+        pointers (and arguments that are whole numbers) as integers, then `scalars` fp32 numbers; `grid` for a kernel whose
+        launch info leaves it to the caller.  Everything that is the same for all launches is prepared here:
         the general launch() spends most of a small call on ctypes objects (an eight-call block 148 us, 41 this way).
         Where the native launches are built, this is one of them, whose result() also allocates the output."""
         info = self.info
         if info["workspace_bytes"]:
             raise ValueError("the kernel takes a workspace")
-        n = info["num_args"]
+        n, grid = info["num_args"], info["grid"] if grid is None else (*grid, 1, 1)[:3]
         native = _native_launch() if isinstance(lib(), C.CDLL) else None
         if native is not None:
             return native(C.cast(lib().kcg_hip_launch_packed, C.c_void_p).value, self.handle.value,
-                          (*info["grid"], *info["block"], info["lds_bytes"]), n - scalars, scalars,
+                          (*grid, *info["block"], info["lds_bytes"]), n - scalars, scalars,
                           lambda rc: check(rc, "kcg_hip_launch_packed"), self)
         pack = struct.Struct("<" + "Q" * (n - scalars) + "f4x" * scalars).pack
-        dims = (C.c_uint32 * 7)(*info["grid"], *info["block"], info["lds_bytes"])
+        dims = (C.c_uint32 * 7)(*grid, *info["block"], info["lds_bytes"])
         address, handle, entry, stream = C.addressof(dims), self.handle, lib().kcg_hip_launch_packed, _current_stream()
 
         def run(*values, _keep=(dims, self)):
