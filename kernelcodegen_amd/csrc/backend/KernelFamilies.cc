@@ -1714,45 +1714,58 @@ bool emitCacheAttention(KernelSpec& s, std::string& src, KernelLaunchInfo& info,
   const double cap = s.f.count("CAP") ? s.f["CAP"] : 0.0, scale = s.f.count("SCALE") ? s.f["SCALE"] : 1.0;
   if (!(cap >= 0.0) || !std::isfinite(cap) || !std::isfinite(scale)) { err = "cache_attention: CAP must not be negative, CAP and SCALE must be finite"; return false; }
   const int64_t rows = 16 * rb, gs = std::min(g, rows);
+  // wavefronts per SIMD that the registers hold
+  const int64_t occ = s.get("OCC", rb == 4 ? 1 : rb == 2 ? (dh > 128 ? 1 : dh > 64 ? 2 : 3) : dh > 192 ? 2 : dh > 96 ? 3 : 4);
   Defines d;
   d.add("CA_NAME", s.name);
   d.add("CA_JOIN", join ? 1 : 0);
   d.add("CA_D", dh); d.add("CA_HKV", s.p["H"]); d.add("CA_G", g); d.add("CA_GS", gs); d.add("CA_PAGE", s.p["PAGE"]);
   d.add("CA_F16", s.p["F16"]); d.add("CA_RB", rb); d.add("CA_GRID", grid); d.add("CA_WHOLE", wholeTiles ? 1 : 0); d.add("CA_MIN", least);
-  d.add("CA_OCC", s.get("OCC", rb == 4 || dh > (rb == 2 ? 64 : 128) ? 1 : 2));
+  d.add("CA_OCC", occ); d.add("CA_SPLIT", s.p["F16"] && rb < 4 ? 1 : 0);
   d.add("CA_SCALE", floatLiteral(scale)); d.add("CA_CAP", floatLiteral(cap)); d.add("CA_HAS_CAP", cap > 0.0 ? 1 : 0);
   d.add("CA_WINDOW", window); d.add("CA_SLOPES", slopes ? 1 : 0); d.add("CA_STARTS", starts ? 1 : 0);
   for (auto key : {"KP", "KT", "KH", "VP", "VT", "VH", "QT", "QH"}) d.add(std::string("CA_") + key, std::to_string(s.p[key]) + "LL");
   src = d.wrap(kTpl_cache_attention);
   info.name = s.name;
   info.grid[0] = (uint32_t)(join ? grid - 1 : grid);
-  if (join) info.grid[1] = (uint32_t)(rb * dh / 16);
+  if (join) info.grid[1] = (uint32_t)rb;
   info.block[0] = 256;
   info.numArgs = join ? 7 : 16;
   return true;
 }
 
+// gemm_q4, and gemm_q4_join, which adds up what its workgroups leave where they split k: the same parameters.
 bool emitGemmQ4(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::string& err) {
+  const bool join = s.family == "gemm_q4_join";
   if (!whole(s, "N", 1, 0x7FFFFFF0, err) || !whole(s, "K", 32, 0x7FFFFF00, err) || !whole(s, "GROUP", 32, 0x7FFFFF00, err)) return false;
   if (!whole(s, "F16", 0, 1, err) || !whole(s, "MB", 1, 4, err)) return false;
   const int64_t n = s.p["N"], k = s.p["K"], group = s.p["GROUP"], mb = s.p["MB"];
   if (group != 32 && group != 64 && group % 128) { err = "gemm_q4: GROUP must be 32, 64 or a multiple of 128"; return false; }
   if (k % group) { err = "gemm_q4: GROUP must divide K"; return false; }
-  const int64_t nt = s.get("NT", 1), waves = s.get("WAVES", 8);
-  if (nt < 1 || nt > 4 || waves < 1 || waves > 16 || waves * mb * nt * 1024 > 163840) { err = "gemm_q4: bad NT or WAVES"; return false; }
-  s.p["NT"] = nt; s.p["WAVES"] = waves;
+  const int64_t nt = s.get("NT", 1), wn = s.get("WN", mb > 1 ? 8 : 1), wk = s.get("WK", mb > 1 ? 1 : 8), depth = s.get("DEPTH", 1), split = s.get("SPLIT", 1), mr = s.get("MR", 16 * mb);
+  const int64_t per = group >= 128 ? 1 : 128 / group;
+  const int64_t lds = std::max(wk * (wn > 1 ? 2 : 1) * mr * 528 + wk * wn * (16 * nt * 144 + 2 * per * 16 * nt * 8), wk * wn * mb * nt * 1024);
+  if (nt < 1 || nt > 8 || wn < 1 || wk < 1 || wn * wk > 16 || depth < 1 || depth > 16 || split < 1 || split > 64 || mr < 1 || mr > 16 * mb || (lds > 163840 && !join)) {
+    err = "gemm_q4: bad NT, WN, WK, DEPTH, SPLIT or MR";
+    return false;
+  }
+  s.p["NT"] = nt; s.p["WN"] = wn; s.p["WK"] = wk; s.p["DEPTH"] = depth; s.p["SPLIT"] = split; s.p["MR"] = mr;
   const char* x = s.p["F16"] ? "_Float16" : "__bf16";
   Defines d;
   d.add("Q4_NAME", s.name);
   d.add("Q4_N", n); d.add("Q4_K", k); d.add("Q4_GROUP", group); d.add("Q4_F16", s.p["F16"]); d.add("Q4_ZERO", s.get("ZERO", 0) ? 1 : 0);
   d.add("Q4_ST", std::string(s.get("SCALE_F32", 0) ? "float" : x));
   d.add("Q4_YT", std::string(s.get("OUT_F32", 0) ? "float" : x));
-  d.add("Q4_MB", mb); d.add("Q4_NT", nt); d.add("Q4_WAVES", waves);
+  d.add("Q4_MB", mb); d.add("Q4_NT", nt); d.add("Q4_WN", wn); d.add("Q4_WK", wk); d.add("Q4_DEPTH", depth); d.add("Q4_SPLIT", split); d.add("Q4_MR", mr);
+  // (offsets into the codes, and into 64 rows of X)
+  d.add("Q4_WIDE", s.get("WIDE", (double)n * (double)(k / 2) >= 2147483648.0 || k >= 1 << 24 ? 1 : 0) ? 1 : 0);
+  d.add("Q4_OCC", s.get("OCC", 1)); d.add("Q4_JOIN", join ? 1 : 0);
   src = d.wrap(kTpl_gemm_q4);
   info.name = s.name;
-  info.grid[0] = (uint32_t)ceilDiv(n, 16 * nt);
-  info.block[0] = (uint32_t)(64 * waves);
-  info.numArgs = 6;
+  info.grid[0] = (uint32_t)ceilDiv(n, 16 * nt * wn);
+  info.grid[2] = (uint32_t)split;
+  info.block[0] = (uint32_t)(join ? 256 : 64 * wn * wk);
+  info.numArgs = join ? 3 : 6;
   return true;
 }
 
@@ -1785,7 +1798,7 @@ bool emitKernel(KernelSpec& spec, std::string& src, KernelLaunchInfo& info, std:
   if (spec.family == "cache_write") return emitCacheWrite(spec, src, info, err);
   if (spec.family == "cache_read") return emitCacheRead(spec, src, info, err);
   if (spec.family == "cache_attention" || spec.family == "cache_join") return emitCacheAttention(spec, src, info, err);
-  if (spec.family == "gemm_q4") return emitGemmQ4(spec, src, info, err);
+  if (spec.family == "gemm_q4" || spec.family == "gemm_q4_join") return emitGemmQ4(spec, src, info, err);
   err = "unknown kernel family '" + spec.family + "'";
   return false;
 }

@@ -10,17 +10,19 @@
 // eight keys of that product's lane are taken to be those that the lane has scores of.  The order of the summed index is free in
 // both products: K is read in runs of D / 4 bytes, V in runs of D / 16 of eight keys, which are turned into columns in registers
 // by one v_perm each.  e4m3 numbers are exact in both 16-bit types, so the cache costs no rounding; the probabilities are
-// rounded to IEEE half (11 bits, they lie in [0, 2^CA_LAZY]), whatever the type of q.
+// rounded to IEEE half (11 bits, they lie in [0, 2^CA_LAZY]), whatever the type of q; for results in IEEE half, which that rounding would
+// make 1.4 times less exact than their own does, the rest of the rounding goes through a second product (CA_SPLIT) where rows are few
+// and the cache's bytes bound the launch.
 //
 // A page's vscale goes into the exponent: P' = 2^(s - m) vscale = 2^(s + log2 vscale - m'), with m' the running maximum of that
-// sum, so P' keeps its bits whatever the scales are; the sum of the probabilities takes the rounded P' / vscale in fp32, so that a
+// sum, so P' keeps its bits whatever the scales are; the sum of the probabilities takes P' / vscale as rounded, in fp32, so that a
 // rounding shifts weight between keys and does not scale the result (and two dot products replace four additions).
 //
 // Work: the keys of a tile are cut into units of CA_UK = 128, one step of each of the four wavefronts.  All units of all tiles, head
 // after head, stand in one line that is cut evenly over CA_GRID workgroups (prefix sums of the units of each request, in closed form,
 // taken by every workgroup); a tile cut between workgroups leaves partial results in `part`, which cache_join adds up.  So
 // requests of any lengths fill the part.  CA_WHOLE: one workgroup for each tile of a request (one tile each), nothing to join.
-// Parameters: CA_NAME, CA_D, CA_HKV, CA_G (heads per kv head), CA_GS, CA_PAGE, CA_F16, CA_RB, CA_GRID, CA_WHOLE, CA_MIN (least units of
+// Parameters: CA_NAME, CA_D, CA_HKV, CA_G (heads per kv head), CA_GS, CA_PAGE, CA_F16, CA_SPLIT, CA_RB, CA_GRID, CA_WHOLE, CA_MIN (least units of
 // a workgroup), CA_SCALE, CA_CAP (0: none), CA_WINDOW (0: none), CA_SLOPES, CA_STARTS, CA_KP CA_KT CA_KH / CA_VP CA_VT CA_VH (strides of
 // page, token, head), CA_QT CA_QH (of q), CA_JOIN (this is cache_join).
 typedef _Float16 ca_f16x8 __attribute__((ext_vector_type(8)));
@@ -49,6 +51,7 @@ typedef __bf16 ca_q;
 #define CA_HV (CA_HKV * CA_PARTS)
 #define CA_UK 128
 #define CA_LAZY 6.0f
+#define CA_TINY 1.17549435e-38f               // the least normal number: scales below count as zero
 #define CA_SLOT (CA_ROWS * CA_D + 2 * CA_ROWS)   // floats of a partial result
 
 struct CaRequest { int length, count, first; };       // keys, rows, first row
@@ -71,18 +74,18 @@ __device__ __forceinline__ CaRequest ca_request(const int* __restrict__ lengths,
   return r;
 }
 
-// sum of the whole parts of (a i + b) / m over i < n; a, b >= 0 (the steps of Euclid's algorithm on a and m)
-__device__ __forceinline__ long long ca_floor_sum(long long n, long long a, long long b, long long m) {
-  long long sum = 0;
+// sum of the whole parts of (a i + b) / m over i < n (the steps of Euclid's algorithm on a and m); the sum and a n + b below 2^32
+__device__ __forceinline__ unsigned ca_floor_sum(unsigned n, unsigned a, unsigned b, unsigned m) {
+  unsigned sum = 0;
   while (n > 0) {
-    sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
+    sum += n * (n - 1) / 2 * (a / m) + n * (b / m);        // (a / m is not 0 in later rounds only, where n is small)
     a %= m;
     b %= m;
-    const long long top = a * n + b;
+    const unsigned top = a * n + b;
     if (top < m) break;
     n = top / m;
     b = top % m;
-    const long long t = m;
+    const unsigned t = m;
     m = a;
     a = t;
   }
@@ -104,92 +107,81 @@ __device__ __forceinline__ int ca_units(const CaRequest& r, int tile) {
   return (ca_base(r) + (tile + 1) * ca_tokens(r) + CA_UK - 1) / CA_UK - ca_low(r, tile);
 }
 // Units of the tiles before `tile`: every tile ends with its last token's position (the last tile of several counts as if it were whole).
-__device__ __forceinline__ long long ca_before(const CaRequest& r, int tile) {
+__device__ __forceinline__ int ca_before(const CaRequest& r, int tile) {
   if (tile <= 1) return tile == 0 ? 0 : ca_units(r, 0);
-  const long long p = ca_base(r), t = ca_tokens(r);
-  long long sum = ca_floor_sum(tile, t, p + t + CA_UK - 1, CA_UK);
+  const int p = ca_base(r), t = ca_tokens(r);
+  unsigned sum = ca_floor_sum(tile, t, p + t + CA_UK - 1, CA_UK);
 #if CA_WINDOW
-  long long skip = 0;                      // tiles whose window begins with the first key
+  int skip = 0;                            // tiles whose window begins with the first key
   if (r.length < r.count) skip = tile;
   else if (p < CA_WINDOW) skip = (CA_WINDOW - 1 - p) / t + 1;
   if (tile > skip) sum -= ca_floor_sum(tile - skip, t, p + skip * t - CA_WINDOW + 1, CA_UK);
 #endif
-  return sum;
-}
-__device__ __forceinline__ long long ca_div(long long a, long long b) {      // of numbers that are not negative
-  return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+  return (int)sum;
 }
 
-struct CaScan {
-  long long wave[4], found[2];
-};
-
-// Sum over the threads before this one, and the sum over all of them.
-__device__ __forceinline__ long long ca_scan(long long mine, CaScan& s, long long& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  long long v = mine;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const long long o = __shfl_up(v, off, 64);
-    if (lane >= off) v += o;
-  }
-  if (lane == 63) s.wave[wave] = v;
-  __syncthreads();
-  long long before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w < wave) before += s.wave[w];
-    total += s.wave[w];
-  }
-  return before + v - mine;
+// Sum over the lanes up to and including this one.
+__device__ __forceinline__ int ca_scan(int v) {
+#define CA_DPP(control, rows) v += __builtin_amdgcn_update_dpp(0, v, control, rows, 0xf, false)
+  CA_DPP(0x111, 0xf);        // row_shr 1, 2, 4, 8: over the 16 lanes of a row
+  CA_DPP(0x112, 0xf);
+  CA_DPP(0x114, 0xf);
+  CA_DPP(0x118, 0xf);
+  CA_DPP(0x142, 0xa);        // a row's last lane into the next row, for the second and the fourth,
+  CA_DPP(0x143, 0xc);        // the second row's into the third and the fourth
+#undef CA_DPP
+  return v;
 }
 
-// Where in the line of all units a number of workgroups' shares end.
+// Where in the line of all units a workgroup's share begins.
 struct CaPlace {
-  long long all, chunk, at;     // units of one head, of a workgroup, and the place
+  long long at;                 // the place
+  int all, chunk;               // units of one head, and of a workgroup
   int hv, b, tile, unit;        // what stands there
 };
-// The place where workgroup `piece` begins; false where there is none.
-__device__ __forceinline__ bool ca_locate(int piece, const int* __restrict__ lengths, const int* __restrict__ starts, int B, int T, int most, CaScan& scan, CaPlace& w) {
-  const int requests = B + CA_STARTS;
-  const int per = (requests + 255) / 256, b0 = threadIdx.x * per, b1 = b0 + per < requests ? b0 + per : requests;
-  long long mine = 0;
+// The place where workgroup `piece` begins; false where there is none.  Every wavefront finds it by itself, 64 requests to a round, or
+// more to a lane: a read of the lengths, a sum over lanes, and two reads of lanes.
+__device__ __forceinline__ bool ca_locate(int piece, const int* __restrict__ lengths, const int* __restrict__ starts, int B, int T, int most, CaPlace& w) {
+  const int requests = B + CA_STARTS, lane = threadIdx.x & 63;
+  const int per = (requests + 63) / 64, b0 = lane * per, b1 = b0 + per < requests ? b0 + per : requests;
+  int mine = 0;
   for (int i = b0; i < b1; ++i) {
     const CaRequest r = ca_request(lengths, starts, i, B, T, most);
     mine += ca_before(r, ca_tiles(r));
   }
-  const long long ahead = ca_scan(mine, scan, w.all);
-  const long long even = (w.all * CA_HV + CA_GRID - 1) / CA_GRID;
-  w.chunk = even < CA_MIN ? CA_MIN : even;
-  w.at = piece * w.chunk;
-  if (w.at >= w.all * CA_HV) return false;
-  w.hv = (int)ca_div(w.at, w.all);
-  const long long f = w.at - w.hv * w.all;
-  if (f >= ahead && f < ahead + mine) {
-    long long at = ahead;
+  const int through = ca_scan(mine), ahead = through - mine;
+  w.all = __builtin_amdgcn_readlane(through, 63);
+  const long long total = (long long)w.all * CA_HV, even = (total + CA_GRID - 1) / CA_GRID;
+  w.chunk = even < CA_MIN ? CA_MIN : (int)even;
+  w.at = (long long)piece * w.chunk;
+  if (w.at >= total) return false;
+  w.hv = total >> 32 ? (int)(w.at / w.all) : (int)((unsigned)w.at / (unsigned)w.all);
+  const int f = (int)(w.at - (long long)w.hv * w.all);
+  int b = 0, tile = 0, unit = 0;
+  const bool here = f >= ahead && f < through;
+  if (here) {
+    int at = ahead;
     for (int i = b0; i < b1; ++i) {
       const CaRequest r = ca_request(lengths, starts, i, B, T, most);
-      const int tiles = ca_tiles(r);
-      const long long units = ca_before(r, tiles);
+      const int tiles = ca_tiles(r), units = ca_before(r, tiles);
       if (f < at + units) {
         int lo = 0, hi = tiles - 1;           // the last tile that begins at or before f
         while (lo < hi) {
           const int mid = (lo + hi + 1) >> 1;
           if (at + ca_before(r, mid) <= f) lo = mid; else hi = mid - 1;
         }
-        scan.found[0] = ((long long)i << 32) | (unsigned)lo;
-        scan.found[1] = f - at - ca_before(r, lo);
+        b = i;
+        tile = lo;
+        unit = f - at - ca_before(r, lo);
         break;
       }
       at += units;
     }
   }
-  __syncthreads();
-  w.b = __builtin_amdgcn_readfirstlane((int)(scan.found[0] >> 32));
-  w.tile = __builtin_amdgcn_readfirstlane((int)scan.found[0]);
-  w.unit = __builtin_amdgcn_readfirstlane((int)scan.found[1]);
-  w.hv = __builtin_amdgcn_readfirstlane(w.hv);
+  const int who = __builtin_ctzll(__ballot(here));
+  w.b = __builtin_amdgcn_readlane(b, who);
+  w.tile = __builtin_amdgcn_readlane(tile, who);
+  w.unit = __builtin_amdgcn_readlane(unit, who);
   return true;
 }
 
@@ -225,57 +217,49 @@ __device__ __forceinline__ void ca_store(ca_q* __restrict__ out, const CaRequest
 }
 
 #if CA_JOIN
-// A workgroup for each tile of O^T of each tile of rows: its four wavefronts take the partial results of a row in turn.
+// A workgroup for every end of a share, which has something to do where that is the first one inside of a tile: it adds up the parts of
+// the tile, in order.  A wavefront takes every fourth tile of 16 columns of O.
 extern "C" __global__ __launch_bounds__(256)
 void CA_NAME(const float* __restrict__ part, const int* __restrict__ lengths, const int* __restrict__ starts, long long T_, long long B_,
              long long W_, ca_q* __restrict__ out) {
-  __shared__ CaScan scan;
-  __shared__ kcg_f32x4 red[4][64];
-  __shared__ float top[4][16], sums[4][16];
-  const int T = (int)T_, B = (int)B_, most = (int)W_ * CA_PAGE, rb = blockIdx.y / CA_NT, tt = blockIdx.y % CA_NT;
-  // A workgroup for every end of a share: it has something to do where that is the first one inside of a tile
+  const int T = (int)T_, B = (int)B_, most = (int)W_ * CA_PAGE, rb = blockIdx.y;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15;
   const int second = blockIdx.x + 1;
   CaPlace w;
-  if (!ca_locate(second, lengths, starts, B, T, most, scan, w) || w.unit == 0 || w.unit > w.chunk) return;
+  if (!ca_locate(second, lengths, starts, B, T, most, w) || w.unit == 0 || w.unit > w.chunk) return;
   const CaRequest rq = ca_request(lengths, starts, w.b, B, T, most);
-  const long long f0 = w.at - w.unit;
-  const int w0 = second - 1, w1 = (int)ca_div(f0 + ca_units(rq, w.tile) - 1, w.chunk);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15;
-  // (the piece of the first workgroup is its last one, slot 1, unless its share begins with it)
+  // the parts: of the workgroup before this end (its last piece, slot 1, unless its share begins with it), and of as many behind as
+  // the tile goes on for
+  const int count = 1 + (ca_units(rq, w.tile) - w.unit + w.chunk - 1) / w.chunk;
+  const float* first = part + ((long long)(second - 1) * 2 + (w.unit < w.chunk ? 1 : 0)) * CA_SLOT;
+  const float* later = part + (long long)second * 2 * CA_SLOT;
+  // the largest maximum, and the sum: lane group g takes every fourth part
+  const int at = CA_ROWS * CA_D + (rb * 16 + n) * 2;
   float m = -__builtin_inff(), l = 0.0f;
-  kcg_f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int i = w0 + wave; i <= w1; i += 4) {
-    const int slot = i == w0 && i * w.chunk < f0 ? 1 : 0;
-    const float* p = part + ((long long)i * 2 + slot) * CA_SLOT;
-    const kcg_f32x4 x = *(const kcg_f32x4*)(p + ((rb * CA_NT + tt) * 64 + lane) * 4);
-    const float pm = p[CA_ROWS * CA_D + (rb * 16 + n) * 2], pl = p[CA_ROWS * CA_D + (rb * 16 + n) * 2 + 1];
-    const float mm = fmaxf(m, pm), ref = mm == -__builtin_inff() ? 0.0f : mm;
-    const float fa = __builtin_amdgcn_exp2f(m - ref), fb = __builtin_amdgcn_exp2f(pm - ref);
-    o = o * fa + x * fb;
-    l = l * fa + pl * fb;
-    m = mm;
+  for (int i = lane >> 4; i < count; i += 4) {
+    const float* p = i ? later + (long long)(i - 1) * 2 * CA_SLOT : first;
+    const float pm = p[at], to = fmaxf(m, pm), ref = to == -__builtin_inff() ? 0.0f : to;
+    l = l * __builtin_amdgcn_exp2f(m - ref) + p[at + 1] * __builtin_amdgcn_exp2f(pm - ref);
+    m = to;
   }
-  if (lane < 16) { top[wave][n] = m; sums[wave][n] = l; }
-  red[wave][lane] = o;
-  __syncthreads();
-  if (wave) return;
-  float mm = fmaxf(fmaxf(top[0][n], top[1][n]), fmaxf(top[2][n], top[3][n]));
-  mm = mm == -__builtin_inff() ? 0.0f : mm;
-  kcg_f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-  float total = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float f = __builtin_amdgcn_exp2f(top[i][n] - mm);
-    sum += red[i][lane] * f;
-    total += sums[i][n] * f;
+  const float top = ca_cross(m, true), ref = top == -__builtin_inff() ? 0.0f : top;
+  const float sum = ca_cross(l * __builtin_amdgcn_exp2f(m - ref), false);
+  for (int tt = wave; tt < CA_NT; tt += 4) {
+    kcg_f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) {
+      const float* p = i ? later + (long long)(i - 1) * 2 * CA_SLOT : first;
+      o += *(const kcg_f32x4*)(p + ((rb * CA_NT + tt) * 64 + lane) * 4) * __builtin_amdgcn_exp2f(p[at] - ref);
+    }
+    ca_store(out, rq, w.hv, w.tile, rb, tt, o, sum);
   }
-  ca_store(out, rq, w.hv, w.tile, rb, tt, sum, total);
 }
 #else
 
-struct CaStep {
-  unsigned k[2][CA_KR], v[8][CA_VR];
-  float ks[2], vs[2];
+// What a step has beside its keys and values.
+struct CaMeta {
+  float ks[2], vs[2];      // scales of the pages of its two halves
+  bool there[2];           // false: no such keys, or a page that there is none of
 };
 
 extern "C" __global__ __launch_bounds__(256, CA_OCC)
@@ -289,20 +273,19 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
 
   int hv, b, tile, unit;
-  long long left;                 // units this workgroup has to do
+  int left;                       // units this workgroup has to do
 #if CA_WHOLE
   hv = blockIdx.x % CA_HV;
   b = blockIdx.x / CA_HV;
   tile = unit = 0;
-  left = 1LL << 40;
+  left = 0x7fffffff;
 #else
-  __shared__ CaScan scan;
   const int requests = B + CA_STARTS;
   // neighbouring shares, which have pages in common, on one XCD: workgroups are dealt to the eight in turn
   const int piece = (blockIdx.x & 7) * (CA_GRID / 8) + (blockIdx.x >> 3);
   CaPlace w;
-  if (!ca_locate(piece, lengths, starts, B, T, most, scan, w)) return;
-  left = w.all * CA_HV - w.at < w.chunk ? w.all * CA_HV - w.at : w.chunk;
+  if (!ca_locate(piece, lengths, starts, B, T, most, w)) return;
+  left = (long long)w.all * CA_HV - w.at < w.chunk ? (int)((long long)w.all * CA_HV - w.at) : w.chunk;
   hv = w.hv; b = w.b; tile = w.tile; unit = w.unit;
   bool begun = true;              // the first piece of this workgroup, if it is not a whole tile, goes to slot 0, a later one to slot 1
 #endif
@@ -311,7 +294,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
     const CaRequest rq = ca_request(lengths, starts, b, B, T, most);
     const int t = ca_tokens(rq), tok0 = tile * t, tokens = rq.count - tok0 < t ? rq.count - tok0 : t;
     const int units = ca_units(rq, tile);
-    const int until = left < units - unit ? unit + (int)left : units;      // of this piece
+    const int until = left < units - unit ? unit + left : units;      // of this piece
     const int first = rq.length - rq.count + tok0;                         // position of the tile's first row
     const int hi = first + tokens > 0 ? first + tokens : 0;
     const int lo = CA_WINDOW && first - CA_WINDOW + 1 > 0 ? first - CA_WINDOW + 1 : 0;
@@ -347,60 +330,56 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
     }
 
     const int* row = table + (long long)b * table_row;
-    // Pages of the two halves of a step; -1: no such key, or a page that there is none of.
+    // Entries of the table for the two halves of a step.  What is wrong with them is looked at when they are used, a step later: until
+    // then nobody waits for them.
     auto pagesOf = [&](int at, int (&page)[2]) {
 #pragma unroll
+      for (int h = 0; h < 2; ++h) page[h] = row[(at + h * 16 < hi ? at + h * 16 : hi - 1) / CA_PAGE];
+    };
+    // Addresses: a uniform base and an offset of the lane's
+    const unsigned koff = n * (unsigned)CA_KT + g * (CA_D / 4), voff = g * 4 * (unsigned)CA_VT;
+    unsigned k[2][CA_KR], v[8][CA_VR];
+    // (what is not there is read from somewhere that is)
+    auto loadMeta = [&](int at, const int (&page)[2], long long (&pg)[2], CaMeta& s) {
+#pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int k16 = at + h * 16;
-        page[h] = k16 < hi && k16 + 16 > lo ? row[k16 / CA_PAGE] : -1;
-        if ((unsigned)page[h] >= (unsigned)pages) page[h] = -1;
+        s.there[h] = at + h * 16 < hi && at + h * 16 + 16 > lo && (unsigned)page[h] < (unsigned)pages;
+        pg[h] = s.there[h] ? page[h] : 0;
+        s.ks[h] = kscale[pg[h] * CA_HKV + kvh];
+        s.vs[h] = vscale[pg[h] * CA_HKV + kvh];
       }
     };
-    auto load = [&](int at, const int (&page)[2], CaStep& s) {
+    auto loadK = [&](int at, const long long (&pg)[2]) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const long long pg = page[h] < 0 ? 0 : page[h];         // what is masked is read from somewhere that is there
-        const int token = (at + h * 16) % CA_PAGE;
-        const unsigned char* kp = kc + pg * CA_KP + (long long)token * CA_KT + (long long)kvh * CA_KH + (n * (long long)CA_KT + g * (CA_D / 4));
-        const unsigned char* vp = vc + pg * CA_VP + (long long)token * CA_VT + (long long)kvh * CA_VH + g * 4 * (long long)CA_VT;
+        const unsigned char* kp = kc + (pg[h] * CA_KP + (long long)((at + h * 16) % CA_PAGE) * CA_KT + (long long)kvh * CA_KH);
 #if CA_KR % 4 == 0
 #pragma unroll
-        for (int i = 0; i < CA_KR; i += 4) *(kcg_u32x4*)&s.k[h][i] = *(const kcg_u32x4*)(kp + i * 4);
+        for (int i = 0; i < CA_KR; i += 4) *(kcg_u32x4*)&k[h][i] = *(const kcg_u32x4*)(kp + koff + i * 4);
 #else
 #pragma unroll
-        for (int i = 0; i < CA_KR; i += 2) *(kcg_u32x2*)&s.k[h][i] = *(const kcg_u32x2*)(kp + i * 4);
+        for (int i = 0; i < CA_KR; i += 2) *(kcg_u32x2*)&k[h][i] = *(const kcg_u32x2*)(kp + koff + i * 4);
 #endif
+      }
+    };
+    auto loadV = [&](int at, const long long (&pg)[2]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned char* vp = vc + (pg[h] * CA_VP + (long long)((at + h * 16) % CA_PAGE) * CA_VT + (long long)kvh * CA_VH);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const unsigned char* p = vp + r * (long long)CA_VT;
+          const unsigned off = voff + r * (unsigned)CA_VT;
 #pragma unroll
-          for (int i = 0; i < CA_N8; ++i) *(kcg_u32x2*)&s.v[h * 4 + r][2 * i] = *(const kcg_u32x2*)(p + i * 128 + n * 8);
-          if (CA_N4) s.v[h * 4 + r][2 * CA_N8] = *(const unsigned*)(p + CA_N8 * 128 + n * 4);
-          if (CA_N2) s.v[h * 4 + r][2 * CA_N8 + CA_N4] = *(const unsigned short*)(p + CA_N8 * 128 + CA_N4 * 64 + n * 2);
+          for (int i = 0; i < CA_N8; ++i) *(kcg_u32x2*)&v[h * 4 + r][2 * i] = *(const kcg_u32x2*)(vp + off + (i * 128 + n * 8));
+          if (CA_N4) v[h * 4 + r][2 * CA_N8] = *(const unsigned*)(vp + off + (CA_N8 * 128 + n * 4));
+          if (CA_N2) v[h * 4 + r][2 * CA_N8 + CA_N4] = *(const unsigned short*)(vp + off + (CA_N8 * 128 + CA_N4 * 64 + n * 2));
         }
-        s.ks[h] = kscale[pg * CA_HKV + kvh];
-        s.vs[h] = vscale[pg * CA_HKV + kvh];
       }
     };
 
     float known = 1.0f;            // the last vscale that was not zero
-    // O^T += V^T P^T for the 32 keys of a step: dword w of a lane's eight keys gives four tiles (two where it is half a dword)
-    auto product = [&](const unsigned (&v)[8][CA_VR], int w, int e2, const unsigned (&p)[4], kcg_f32x4 c0, kcg_f32x4 c1, kcg_f32x4& r0, kcg_f32x4& r1) {
-      unsigned x[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = e2 ? CA_CVT16(v[k][w], true) : CA_CVT16(v[k][w], false);
-      const kcg_u32x4 even = {__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u),
-                              __builtin_amdgcn_perm(x[5], x[4], 0x05040100u), __builtin_amdgcn_perm(x[7], x[6], 0x05040100u)};
-      const kcg_u32x4 odd = {__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u),
-                             __builtin_amdgcn_perm(x[5], x[4], 0x07060302u), __builtin_amdgcn_perm(x[7], x[6], 0x07060302u)};
-      const kcg_u32x4 pf = {p[0], p[1], p[2], p[3]};
-      r0 = CA_MFMA16(even, pf, c0);
-      r1 = CA_MFMA16(odd, pf, c1);
-    };
-
-    auto compute = [&](int at, const int (&page)[2], CaStep& s) {
-      // scores
-      kcg_f32x4 sc[CA_RB][2];
+    kcg_f32x4 sc[CA_RB][2];
+    auto scores = [&]() {
 #pragma unroll
       for (int rb = 0; rb < CA_RB; ++rb)
 #pragma unroll
@@ -409,25 +388,27 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < CA_KR; i += 2) {
-          const kcg_u32x4 kf = {CA_CVT(s.k[h][i], false), CA_CVT(s.k[h][i], true), CA_CVT(s.k[h][i + 1], false), CA_CVT(s.k[h][i + 1], true)};
+          const kcg_u32x4 kf = {CA_CVT(k[h][i], false), CA_CVT(k[h][i], true), CA_CVT(k[h][i + 1], false), CA_CVT(k[h][i + 1], true)};
 #pragma unroll
           for (int rb = 0; rb < CA_RB; ++rb) {
             const kcg_u32x4 qv = {qf[rb][2 * i], qf[rb][2 * i + 1], qf[rb][2 * i + 2], qf[rb][2 * i + 3]};
             sc[rb][h] = CA_MFMA(kf, qv, sc[rb][h]);
           }
         }
+    };
+    // Scores to probabilities, and these into the sums; `masked`: not every row sees every key of the step, or a scale is zero.
+    auto weigh = [&](int at, const CaMeta& s, bool masked) __attribute__((always_inline)) {
       // scales; those of zero stand for pages of zeros (or for pages that are not there)
-      float lv[2], iv[2];
+      float ks[2], lv[2], iv[2];
       bool zero[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        zero[h] = page[h] < 0 || s.vs[h] < 1.17549435e-38f;
-        if (page[h] < 0) s.ks[h] = 0.0f;
+        zero[h] = masked && (!s.there[h] || s.vs[h] < CA_TINY);
+        ks[h] = masked && !s.there[h] ? 0.0f : s.ks[h];
         if (!zero[h]) known = s.vs[h];
         lv[h] = __builtin_amdgcn_logf(known);
         iv[h] = __builtin_amdgcn_rcpf(known);
       }
-      const bool masked = at + 32 > first + 1 || (CA_WINDOW && at < first + tokens - CA_WINDOW) || zero[0] || zero[1];
 #pragma unroll
       for (int rb = 0; rb < CA_RB; ++rb)
 #pragma unroll
@@ -436,10 +417,10 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
           for (int r = 0; r < 4; ++r) {
             float x = sc[rb][h][r];
 #if CA_HAS_CAP
-            x = kcg_fast_tanh(x * (s.ks[h] * (CA_SCALE / CA_CAP)));
+            x = kcg_fast_tanh(x * (ks[h] * (CA_SCALE / CA_CAP)));
             x = __builtin_fmaf(x, CA_CAP * 1.44269504088896340736f, lv[h]);
 #else
-            x = __builtin_fmaf(x, s.ks[h] * (CA_SCALE * 1.44269504088896340736f), lv[h]);
+            x = __builtin_fmaf(x, ks[h] * (CA_SCALE * 1.44269504088896340736f), lv[h]);
 #endif
             if (CA_SLOPES) x = __builtin_fmaf(slope[rb], (float)(at + h * 16 + g * 4 + r - pos[rb]), x);
             sc[rb][h][r] = x;
@@ -452,8 +433,8 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const int k = at + h * 16 + g * 4 + r;
-              const bool seen = k <= pos[rb] && (!CA_WINDOW || k > pos[rb] - CA_WINDOW) && page[h] >= 0;
+              const int key16 = at + h * 16 + g * 4 + r;
+              const bool seen = key16 <= pos[rb] && (!CA_WINDOW || key16 > pos[rb] - CA_WINDOW) && s.there[h];
               if (!seen) sc[rb][h][r] = -__builtin_inff();
             }
         // V of keys that no row sees, which may be anything, and of pages whose scale is zero
@@ -461,14 +442,17 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int k = at + h * 16 + g * 4 + r;
-            if (k < lo || k >= hi || zero[h])
+            const int key16 = at + h * 16 + g * 4 + r;
+            if (key16 < lo || key16 >= hi || zero[h])
 #pragma unroll
-              for (int w = 0; w < CA_VR; ++w) s.v[h * 4 + r][w] = 0;
+              for (int w = 0; w < CA_VR; ++w) v[h * 4 + r][w] = 0;
           }
       }
       // running maximum: the sums are brought to a new one only where it is more than 2^CA_LAZY times the old
       unsigned pf[CA_RB][4];
+#if CA_SPLIT
+      unsigned pl[CA_RB][4];           // what the rounding of pf leaves
+#endif
 #pragma unroll
       for (int rb = 0; rb < CA_RB; ++rb) {
         float mx = fmaxf(fmaxf(fmaxf(sc[rb][0][0], sc[rb][0][1]), fmaxf(sc[rb][0][2], sc[rb][0][3])),
@@ -489,9 +473,18 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
           for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(sc[rb][h][r] - ref);
           pf[rb][2 * h] = kcg_pack_f16x2(p[0], p[1]);
           pf[rb][2 * h + 1] = kcg_pack_f16x2(p[2], p[3]);
+#if CA_SPLIT
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const kcg_f16x2 up = __builtin_bit_cast(kcg_f16x2, pf[rb][2 * h + j]);
+            pl[rb][2 * h + j] = kcg_pack_f16x2(p[2 * j] - (float)up[0], p[2 * j + 1] - (float)up[1]);
+          }
+          const float sum = (p[0] + p[1]) + (p[2] + p[3]);
+#else
           const kcg_f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
           const float sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(kcg_f16x2, pf[rb][2 * h]), one,
                                                    __builtin_amdgcn_fdot2(__builtin_bit_cast(kcg_f16x2, pf[rb][2 * h + 1]), one, 0.0f, false), false);
+#endif
           l[rb] = __builtin_fmaf(sum, iv[h], l[rb]);
         }
       }
@@ -501,41 +494,37 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
 #pragma unroll
         for (int k = 0; k < 8; ++k)
 #pragma unroll
-          for (int w = 0; w < CA_VR; ++w) any |= ((s.v[k][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+          for (int w = 0; w < CA_VR; ++w) any |= ((v[k][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
         if (__any(any != 0)) {
-          unsigned where[8][CA_VR];
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
+          for (int w = 0; w < CA_VR; ++w)
 #pragma unroll
-            for (int w = 0; w < CA_VR; ++w) {
-              const unsigned nan = ((((s.v[k][w] & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u);
-              where[k][w] = nan * 0x38u;              // 1.0
-              s.v[k][w] &= ~(nan * 0xffu);
+            for (int e = 0; e < 4; ++e) {
+              if (w * 4 + e >= CA_NT) continue;
+              unsigned x[4];             // 1.0 where column e of dword w is NaN
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                x[j] = ((v[2 * j][w] >> (8 * e) & 0x7f) == 0x7f ? 0x3c00u : 0u) | ((v[2 * j + 1][w] >> (8 * e) & 0x7f) == 0x7f ? 0x3c000000u : 0u);
+              const kcg_u32x4 where = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+              for (int rb = 0; rb < CA_RB; ++rb) {
+                unsigned see[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  see[j] = (sc[rb][j / 2][j % 2 * 2] != -__builtin_inff() ? 0x3c00u : 0u) | (sc[rb][j / 2][j % 2 * 2 + 1] != -__builtin_inff() ? 0x3c000000u : 0u);
+                const kcg_u32x4 who = {see[0], see[1], see[2], see[3]};
+                const kcg_f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+                kcg_f32x4 c = CA_MFMA16(where, who, none);        // how many such keys the row sees
+                c *= 0x1p127f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[rb][w * 4 + e][r] = __builtin_fmaf(c[r] * 0x1p127f, 0.0f, acc[rb][w * 4 + e][r]);      // + 0, or infinity times 0
+              }
+              __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
-          for (int rb = 0; rb < CA_RB; ++rb) {
-            unsigned see[4];
+          for (int k8 = 0; k8 < 8; ++k8)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int r = 0; r < 4; r += 2)
-                see[2 * h + r / 2] = (sc[rb][h][r] != -__builtin_inff() ? 0x3c00u : 0u) | (sc[rb][h][r + 1] != -__builtin_inff() ? 0x3c000000u : 0u);
-#pragma unroll
-            for (int w = 0; w < CA_VR; ++w)
-#pragma unroll
-              for (int e2 = 0; e2 < 2; ++e2) {
-                const int tt = w * 4 + e2 * 2;
-                if (tt >= CA_NT) continue;
-                const kcg_f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
-                kcg_f32x4 c0, c1;
-                product(where, w, e2, see, none, none, c0, c1);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  if (c0[r] > 0.0f) acc[rb][tt][r] = __builtin_nanf("");
-                  if (c1[r] > 0.0f) acc[rb][tt + 1][r] = __builtin_nanf("");
-                }
-              }
-          }
+            for (int w = 0; w < CA_VR; ++w) v[k8][w] &= ~((((v[k8][w] & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u) * 0xffu);
         }
       }
 #pragma unroll
@@ -546,7 +535,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
           if (tt >= CA_NT) continue;
           unsigned x[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] = e2 ? CA_CVT16(s.v[k][w], true) : CA_CVT16(s.v[k][w], false);
+          for (int k = 0; k < 8; ++k) x[k] = e2 ? CA_CVT16(v[k][w], true) : CA_CVT16(v[k][w], false);
           const kcg_u32x4 even = {__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u),
                                   __builtin_amdgcn_perm(x[5], x[4], 0x05040100u), __builtin_amdgcn_perm(x[7], x[6], 0x05040100u)};
           const kcg_u32x4 odd = {__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u),
@@ -556,30 +545,41 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
             const kcg_u32x4 p = {pf[rb][0], pf[rb][1], pf[rb][2], pf[rb][3]};
             acc[rb][tt] = CA_MFMA16(even, p, acc[rb][tt]);
             acc[rb][tt + 1] = CA_MFMA16(odd, p, acc[rb][tt + 1]);
+#if CA_SPLIT
+            const kcg_u32x4 q = {pl[rb][0], pl[rb][1], pl[rb][2], pl[rb][3]};
+            acc[rb][tt] = CA_MFMA16(even, q, acc[rb][tt]);
+            acc[rb][tt + 1] = CA_MFMA16(odd, q, acc[rb][tt + 1]);
+#endif
           }
         }
     };
 
     if (key < end) {
-      CaStep sa, sb;
-      int pa[2], pb[2];
-      pagesOf(key, pa);
-      pagesOf(key + CA_UK, pb);
-      load(key, pa, sa);
+      // The next step's keys are loaded when this one's scores are there, its values when this one's sums are: into the same registers, so
+      // that many wavefronts fit.  Pages are read two steps ahead.
+      const int last = key + (end - 1 - key) / CA_UK * CA_UK;
+      CaMeta meta;
+      int next[2];
+      long long pg[2];
+      pagesOf(key, next);
+      loadMeta(key, next, pg, meta);
+      loadK(key, pg);
+      loadV(key, pg);
+      pagesOf(key + CA_UK < last ? key + CA_UK : last, next);
+#pragma unroll 1
       while (true) {
-        int pn[2];
-        pagesOf(key + 2 * CA_UK, pn);
-        if (key + CA_UK < end) load(key + CA_UK, pb, sb);
-        compute(key, pa, sa);
+        scores();
+        const CaMeta now = meta;
+        const bool more = key < last;
+        if (more) {
+          loadMeta(key + CA_UK, next, pg, meta);
+          loadK(key + CA_UK, pg);
+          pagesOf(key + 2 * CA_UK < last ? key + 2 * CA_UK : last, next);
+        }
+        weigh(key, now, key + 32 > first + 1 || (CA_WINDOW && key < first + tokens - CA_WINDOW) || !now.there[0] || !now.there[1] || now.vs[0] < CA_TINY || now.vs[1] < CA_TINY);
+        if (!more) break;
+        loadV(key + CA_UK, pg);
         key += CA_UK;
-        if (key >= end) break;
-        pagesOf(key + 2 * CA_UK, pa);
-        if (key + CA_UK < end) load(key + CA_UK, pn, sa);
-        compute(key, pb, sb);
-        key += CA_UK;
-        if (key >= end) break;
-        pb[0] = pa[0]; pb[1] = pa[1];
-        pa[0] = pn[0]; pa[1] = pn[1];
       }
     }
 

@@ -10,168 +10,258 @@
 // is the group's part of the result: codes, zeros and X enter unrounded, sums are fp32, the scale is applied in fp32.
 // X is the left operand, so the result's lanes hold one column n and four rows: a group's scale is one number per lane.
 //
-// A dword of codes gives the pairs (0, 4) (1, 5) (2, 6) (3, 7) of its eight, and X is put into that order.  Where a group is 128 or more, a
-// lane of quarter g takes k = 32 g + 8 j .. + 7 of a step of 128 for product j, 16 bytes of codes as they come; smaller groups
-// need products of 32 neighbouring k, so the quarters exchange dwords first (four permlane swaps).
+// A dword of codes gives the pairs (0, 4) (1, 5) (2, 6) (3, 7) of its eight, and X is put into that order on its way into LDS.
 //
-// A workgroup has 16 Q4_NT columns of up to 16 Q4_MB rows; its wavefronts split k (and the grid's z axis, if Q4_SPLIT) and add through LDS.
-// Parameters: Q4_NAME, Q4_N, Q4_K, Q4_GROUP, Q4_F16, Q4_ZERO, Q4_ST (type of the scales), Q4_YT (of the result), Q4_MB, Q4_NT, Q4_WAVES.
+// A wavefront has 16 Q4_NT columns and takes 256 k a step: 128 bytes of a row, whole lines.  Neighbouring lanes load neighbouring bytes
+// and the tile goes through LDS rows that belong to the wavefront alone, where lane l finds column l % 16 (read where a lane needs them,
+// four neighbouring lanes touch four lines).  Q4_WN wavefronts beside one another share the rows of X, Q4_WK groups of them split k and add
+// their sums through LDS, and Q4_SPLIT workgroups split it again, whose fp32 results gemm_q4_join adds in order.
+// Where a group has 128 codes or more, product j of a step's half takes k = 32 g + 8 j .. + 7 for quarter g of the wavefront, 16 bytes
+// of codes as they come; smaller groups need products of 32 neighbouring k, so the quarters exchange dwords (four permlane swaps).
+// Parameters: Q4_NAME, Q4_N, Q4_K, Q4_GROUP, Q4_F16, Q4_ZERO, Q4_ST (type of the scales), Q4_YT (of the result), Q4_MB, Q4_MR (rows of X in
+// LDS, up to 16 Q4_MB), Q4_NT, Q4_WN, Q4_WK, Q4_SPLIT, Q4_DEPTH (steps under way in registers), Q4_WIDE, Q4_JOIN (this is gemm_q4_join).
 typedef _Float16 q4_f16x8 __attribute__((ext_vector_type(8)));
 #if Q4_F16
 typedef _Float16 q4_x;
 #define Q4_MFMA(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q4_f16x8, a), __builtin_bit_cast(q4_f16x8, b), c, 0, 0, 0)
 #define Q4_ONE 0x3c003c00u
 #define Q4_MASK 0x03c003c0u
-#define Q4_PAIR(w, p) (((p) == 0 ? (w) << 6 : (p) == 1 ? (w) << 2 : (p) == 2 ? (w) >> 2 : (w) >> 6) & Q4_MASK | Q4_ONE)
+#define Q4_SHIFT(w, p) ((p) == 0 ? (w) << 6 : (p) == 1 ? (w) << 2 : (p) == 2 ? (w) >> 2 : (w) >> 6)
 #else
 typedef __bf16 q4_x;
 #define Q4_MFMA(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(kcg_bf16x8, a), __builtin_bit_cast(kcg_bf16x8, b), c, 0, 0, 0)
 #define Q4_ONE 0x3f803f80u
 #define Q4_MASK 0x00780078u
-#define Q4_PAIR(w, p) (((p) == 0 ? (w) << 3 : (p) == 1 ? (w) >> 1 : (p) == 2 ? (w) >> 5 : (w) >> 9) & Q4_MASK | Q4_ONE)
+#define Q4_SHIFT(w, p) ((p) == 0 ? (w) << 3 : (p) == 1 ? (w) >> 1 : (p) == 2 ? (w) >> 5 : (w) >> 9)
 #endif
-#define Q4_STEPS ((Q4_K + 127) / 128)
+#define Q4_STEPS ((Q4_K + 255) / 256)
+#define Q4_PARTS (Q4_WK * Q4_SPLIT)
+#define Q4_SHARE ((Q4_STEPS + Q4_PARTS - 1) / Q4_PARTS)       // steps of a wavefront
+#define Q4_EXACT (Q4_K % 256 == 0 && Q4_STEPS == Q4_SHARE * Q4_PARTS)
 #define Q4_GROUPS (Q4_K / Q4_GROUP)
-#define Q4_PER (Q4_GROUP >= 128 ? 1 : 128 / Q4_GROUP)         // groups of a step
-#define Q4_J (4 / Q4_PER)                                     // products of a group of a step
+#if Q4_WIDE            // offsets that 32 bits do not hold
+typedef long long q4_offset;
+#else
+typedef unsigned q4_offset;
+#endif
+#define Q4_PER (Q4_GROUP >= 128 ? 1 : 128 / Q4_GROUP)         // groups of half a step
+#define Q4_J (4 / Q4_PER)                                     // products of a group of half a step
+#define Q4_COLS (16 * Q4_NT)
+#define Q4_XPITCH 528                                         // bytes of a row of X in LDS, and of one of W: 16 more than it holds, so that
+#define Q4_WPITCH 144                                         // eight lanes that read below one another meet all banks
+#define Q4_XC ((Q4_MR * 32 + 64 * Q4_WN - 1) / (64 * Q4_WN))  // chunks of X that a lane brings
+#define Q4_SC ((Q4_COLS * 2 * Q4_PER + 63) / 64)              // scales that a lane brings
 
+#if Q4_JOIN
+extern "C" __global__ __launch_bounds__(256)
+void Q4_NAME(const float* __restrict__ part, long long M, Q4_YT* __restrict__ Y) {
+  const long long total = M * Q4_N, at = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= total) return;
+  float sum = part[at];
+#pragma unroll
+  for (int i = 1; i < Q4_SPLIT; ++i) sum += part[i * total + at];
+  Y[at] = (Q4_YT)sum;
+}
+#else
 struct Q4Step {
-  kcg_u32x4 w[Q4_NT], x[Q4_MB][4];
-  float s[Q4_NT][Q4_PER], z[Q4_NT][Q4_PER];
+  kcg_u32x4 w[2 * Q4_NT], x[Q4_XC];
+  Q4_ST s[Q4_SC];
+  unsigned char z[Q4_SC];
 };
 
-extern "C" __global__ __launch_bounds__(64 * Q4_WAVES)
+extern "C" __global__ __launch_bounds__(64 * Q4_WN * Q4_WK, Q4_OCC)
 void Q4_NAME(const q4_x* __restrict__ X, const unsigned char* __restrict__ W, const Q4_ST* __restrict__ scale, const unsigned char* __restrict__ zero,
-             long long M_, Q4_YT* __restrict__ Y) {
-  __shared__ kcg_f32x4 red[Q4_WAVES][Q4_MB * Q4_NT][64];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-  const int M = (int)M_, n0 = blockIdx.x * (16 * Q4_NT), m0 = blockIdx.y * (16 * Q4_MB);
+             long long M_,
+#if Q4_SPLIT > 1
+             float* __restrict__ part
+#else
+             Q4_YT* __restrict__ Y
+#endif
+) {
+  struct Tiles {
+    __attribute__((aligned(16))) unsigned char x[Q4_WK][Q4_WN > 1 ? 2 : 1][Q4_MR * Q4_XPITCH], w[Q4_WK * Q4_WN][Q4_COLS * Q4_WPITCH];
+    kcg_f32x2 s[Q4_WK * Q4_WN][2 * Q4_PER][Q4_COLS];
+  };
+  union Shared {
+    Tiles t;
+    kcg_f32x4 red[Q4_WK][Q4_WN * Q4_MB * Q4_NT][64];
+  };
+  __shared__ Shared sh;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % Q4_WN, wk = wave / Q4_WN, lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int M = (int)M_, n0 = (blockIdx.x * Q4_WN + wn) * Q4_COLS, m0 = blockIdx.y * (16 * Q4_MB);
   kcg_f32x4 acc[Q4_MB][Q4_NT];
 #pragma unroll
   for (int a = 0; a < Q4_MB; ++a)
 #pragma unroll
     for (int b = 0; b < Q4_NT; ++b) acc[a][b] = kcg_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  // rows and columns behind the last are read as the last; their results are not stored
-  const unsigned char* wp[Q4_NT];
-  int col[Q4_NT];
-#pragma unroll
-  for (int b = 0; b < Q4_NT; ++b) {
-    const int n = n0 + b * 16 + i;
-    col[b] = n < Q4_N ? n : Q4_N - 1;
-    wp[b] = W + (long long)col[b] * (Q4_K / 2);
-  }
-  const q4_x* xp[Q4_MB];
-#pragma unroll
-  for (int a = 0; a < Q4_MB; ++a) {
-    const int m = m0 + a * 16 + i;
-    xp[a] = X + (long long)(m < M ? m : M - 1) * Q4_K;
-  }
+  // mask and one in a scalar and a vector register: one v_and_or_b32 a pair, of which an instruction takes no more than one constant
+  unsigned mask = Q4_MASK, one = Q4_ONE;
+  asm("" : "+s"(mask));
+  asm("" : "+v"(one));
 
-  auto load = [&](int step, Q4Step& s) {
-    const int k0 = step * 128;
-    const int kw = k0 + g * 32;
+  const int share = blockIdx.z * Q4_WK + wk, first = share * Q4_SHARE, kend = (first + Q4_SHARE) * 256 < Q4_K ? (first + Q4_SHARE) * 256 : Q4_K;
+  // Rows and columns behind the last are read as the last, and their results are not stored; k behind the last is read as the first and
+  // takes part with zeros of X.  (All loads are unconditional: one behind a branch would be waited for there.)  Addresses are a uniform
+  // base, which goes on with the steps, and an offset of the lane's.
+  q4_offset wo[2 * Q4_NT], xo[Q4_XC], so[Q4_SC];
 #pragma unroll
-    for (int b = 0; b < Q4_NT; ++b) {
-      s.w[b] = *(const kcg_u32x4*)(wp[b] + (Q4_K % 128 == 0 || kw < Q4_K ? kw : 0) / 2);
+  for (int b = 0; b < 2 * Q4_NT; ++b) {
+    const int n = n0 + b * 8 + lane / 8;
+    wo[b] = (q4_offset)(n < Q4_N ? n : Q4_N - 1) * (Q4_K / 2) + lane % 8 * 16;
+  }
+  int xk[Q4_XC], xat[Q4_XC];
+#pragma unroll
+  for (int c = 0; c < Q4_XC; ++c) {
+    const int u = (c * Q4_WN + wn) * 64 + lane, row = u / 32, m = m0 + row;
+    xk[c] = u % 32 * 8;
+    xo[c] = (q4_offset)((m < M ? m : M - 1) - m0) * Q4_K + xk[c];
+    xat[c] = row < Q4_MR ? row * Q4_XPITCH + u % 32 * 16 : -1;
+  }
+  int se[Q4_SC], sat[Q4_SC];
+#pragma unroll
+  for (int c = 0; c < Q4_SC; ++c) {
+    const int u = c * 64 + lane, col = u / (2 * Q4_PER), n = n0 + col;
+    se[c] = u % (2 * Q4_PER);
+    so[c] = (q4_offset)(n < Q4_N ? n : Q4_N - 1) * Q4_GROUPS;
+    sat[c] = col < Q4_COLS ? se[c] * Q4_COLS + col : -1;
+  }
+  auto load = [&](int n, Q4Step& s) {
+    int k0 = (first + n) * 256;
+    k0 = k0 < Q4_K ? k0 : 0;             // (the last wavefront's may lie behind the last k)
+    // the first group of the step and the second half's; smaller groups follow one another
+    const int g0 = k0 / Q4_GROUP, g1 = Q4_PER > 1 || k0 + 128 < Q4_K ? (k0 + 128) / Q4_GROUP : g0;
+#pragma unroll
+    for (int c = 0; c < Q4_SC; ++c) {
+      int at = Q4_PER > 1 ? g0 + se[c] : se[c] ? g1 : g0;
+      if (Q4_PER > 1 && Q4_K % 256) at = at < Q4_GROUPS ? at : 0;
+      s.s[c] = scale[so[c] + at];
+      if (Q4_ZERO) s.z[c] = zero[so[c] + at];
+    }
+    const unsigned char* wk0 = W + k0 / 2;
+#pragma unroll
+    for (int b = 0; b < 2 * Q4_NT; ++b) s.w[b] = *(const kcg_u32x4*)(wk0 + (Q4_K % 256 == 0 || k0 + lane % 8 * 32 < Q4_K ? wo[b] : wo[b] - lane % 8 * 16));
+    const q4_x* xk0 = X + (long long)m0 * Q4_K + k0;
+#pragma unroll
+    for (int c = 0; c < Q4_XC; ++c) s.x[c] = *(const kcg_u32x4*)(xk0 + (Q4_K % 256 == 0 || k0 + xk[c] < Q4_K ? xo[c] : xo[c] - xk[c]));
+  };
+  auto stage = [&](int n, Q4Step& s, unsigned char* xs) {
+    const int k0 = (first + n) * 256;
+#pragma unroll
+    for (int c = 0; c < Q4_XC; ++c) {
+      const kcg_u32x4 v = Q4_EXACT || k0 + xk[c] < kend ? s.x[c] : kcg_u32x4{0, 0, 0, 0};
+      const kcg_u32x4 o = {__builtin_amdgcn_perm(v[2], v[0], 0x05040100u), __builtin_amdgcn_perm(v[2], v[0], 0x07060302u),
+                           __builtin_amdgcn_perm(v[3], v[1], 0x05040100u), __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)};
+      if (Q4_MR * 32 % (64 * Q4_WN) == 0 || xat[c] >= 0) *(kcg_u32x4*)(xs + xat[c]) = o;
+    }
+#pragma unroll
+    for (int b = 0; b < 2 * Q4_NT; ++b) *(kcg_u32x4*)(sh.t.w[wave] + (b * 8 + lane / 8) * Q4_WPITCH + lane % 8 * 16) = s.w[b];
+#pragma unroll
+    for (int c = 0; c < Q4_SC; ++c)
+      if (Q4_COLS * 2 * Q4_PER % 64 == 0 || sat[c] >= 0)
+        (&sh.t.s[wave][0][0])[sat[c]] = kcg_f32x2{(float)s.s[c], Q4_ZERO ? -1.0f - (float)s.z[c] * 0.0625f : -1.5f};
+  };
+  auto multiply = [&](const unsigned char* xs) {
+    const kcg_f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+    const kcg_u32x4 ones = {one, one, one, one};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      kcg_u32x4 w4[Q4_NT];
+#pragma unroll
+      for (int b = 0; b < Q4_NT; ++b) {
+        w4[b] = *(const kcg_u32x4*)(sh.t.w[wave] + (b * 16 + i) * Q4_WPITCH + (h * 4 + g) * 16);
+#if Q4_PER > 1
+        // dword j of quarter g becomes dword g of quarter j
+        auto x02 = __builtin_amdgcn_permlane32_swap(w4[b][0], w4[b][2], false, false);
+        auto x13 = __builtin_amdgcn_permlane32_swap(w4[b][1], w4[b][3], false, false);
+        auto x01 = __builtin_amdgcn_permlane16_swap(x02[0], x13[0], false, false);
+        auto x23 = __builtin_amdgcn_permlane16_swap(x02[1], x13[1], false, false);
+        w4[b] = kcg_u32x4{x01[0], x01[1], x23[0], x23[1]};
+#endif
+      }
 #pragma unroll
       for (int p = 0; p < Q4_PER; ++p) {
-        int at = (k0 + p * 128 / Q4_PER) / Q4_GROUP;
-        if (Q4_K % 128 != 0 && at >= Q4_GROUPS) at = Q4_GROUPS - 1;
-        s.s[b][p] = (float)scale[(long long)col[b] * Q4_GROUPS + at];
-        s.z[b][p] = Q4_ZERO ? 1.0f + (float)zero[(long long)col[b] * Q4_GROUPS + at] * 0.0625f : 1.5f;
-      }
-    }
+        kcg_f32x4 u[Q4_MB], t[Q4_MB][Q4_NT];
 #pragma unroll
-    for (int a = 0; a < Q4_MB; ++a)
+        for (int a = 0; a < Q4_MB; ++a) {
+          u[a] = none;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = Q4_PER == 1 ? kw + j * 8 : k0 + j * 32 + g * 8;
-        if (Q4_K % 128 == 0 || k < Q4_K)
-          s.x[a][j] = *(const kcg_u32x4*)(xp[a] + k);
-        else
-          s.x[a][j] = kcg_u32x4{0, 0, 0, 0};          // takes the codes read in place of those behind the row out of all sums
-      }
-  };
-
-  auto compute = [&](Q4Step& s) {
-    const kcg_f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
-    const kcg_u32x4 ones = {Q4_ONE, Q4_ONE, Q4_ONE, Q4_ONE};
+          for (int b = 0; b < Q4_NT; ++b) t[a][b] = none;
+        }
 #pragma unroll
-    for (int a = 0; a < Q4_MB; ++a)
+        for (int j = p * Q4_J; j < (p + 1) * Q4_J; ++j) {
+          kcg_u32x4 x[Q4_MB];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const kcg_u32x4 v = s.x[a][j];
-        s.x[a][j] = kcg_u32x4{__builtin_amdgcn_perm(v[2], v[0], 0x05040100u), __builtin_amdgcn_perm(v[2], v[0], 0x07060302u),
-                              __builtin_amdgcn_perm(v[3], v[1], 0x05040100u), __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)};
-      }
-#if Q4_PER > 1
-    // dword j of quarter g becomes dword g of quarter j
+          for (int a = 0; a < Q4_MB; ++a) {
+            const int row = a * 16 + i < Q4_MR ? a * 16 + i : Q4_MR - 1;
+            x[a] = *(const kcg_u32x4*)(xs + row * Q4_XPITCH + h * 256 + (Q4_PER == 1 ? g * 4 + j : j * 4 + g) * 16);
+            u[a] = Q4_MFMA(x[a], ones, u[a]);
+          }
 #pragma unroll
-    for (int b = 0; b < Q4_NT; ++b) {
-      auto x02 = __builtin_amdgcn_permlane32_swap(s.w[b][0], s.w[b][2], false, false);
-      auto x13 = __builtin_amdgcn_permlane32_swap(s.w[b][1], s.w[b][3], false, false);
-      auto x01 = __builtin_amdgcn_permlane16_swap(x02[0], x13[0], false, false);
-      auto x23 = __builtin_amdgcn_permlane16_swap(x02[1], x13[1], false, false);
-      s.w[b] = kcg_u32x4{x01[0], x01[1], x23[0], x23[1]};
-    }
-#endif
+          for (int b = 0; b < Q4_NT; ++b) {
+            const unsigned w = w4[b][j];
+            const kcg_u32x4 f = {Q4_SHIFT(w, 0) & mask | one, Q4_SHIFT(w, 1) & mask | one, Q4_SHIFT(w, 2) & mask | one, Q4_SHIFT(w, 3) & mask | one};
 #pragma unroll
-    for (int p = 0; p < Q4_PER; ++p) {
-      kcg_f32x4 u[Q4_MB], t[Q4_MB][Q4_NT];
-#pragma unroll
-      for (int a = 0; a < Q4_MB; ++a) {
-        u[a] = none;
-#pragma unroll
-        for (int b = 0; b < Q4_NT; ++b) t[a][b] = none;
-      }
-#pragma unroll
-      for (int j = p * Q4_J; j < (p + 1) * Q4_J; ++j) {
-#pragma unroll
-        for (int a = 0; a < Q4_MB; ++a) u[a] = Q4_MFMA(s.x[a][j], ones, u[a]);
+            for (int a = 0; a < Q4_MB; ++a) t[a][b] = Q4_MFMA(x[a], f, t[a][b]);
+          }
+        }
 #pragma unroll
         for (int b = 0; b < Q4_NT; ++b) {
-          const unsigned w = s.w[b][j];
-          const kcg_u32x4 f = {Q4_PAIR(w, 0), Q4_PAIR(w, 1), Q4_PAIR(w, 2), Q4_PAIR(w, 3)};
+          const kcg_f32x2 s = sh.t.s[wave][h * Q4_PER + p][b * 16 + i];
 #pragma unroll
-          for (int a = 0; a < Q4_MB; ++a) t[a][b] = Q4_MFMA(s.x[a][j], f, t[a][b]);
+          for (int a = 0; a < Q4_MB; ++a)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[a][b][r] = __builtin_fmaf(s[0], __builtin_fmaf(s[1], u[a][r], t[a][b][r]), acc[a][b][r]);
         }
       }
-#pragma unroll
-      for (int a = 0; a < Q4_MB; ++a)
-#pragma unroll
-        for (int b = 0; b < Q4_NT; ++b)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            acc[a][b][r] = __builtin_fmaf(s.s[b][p], __builtin_fmaf(-s.z[b][p], u[a][r], t[a][b][r]), acc[a][b][r]);
     }
   };
 
-  if (wave < Q4_STEPS) {
-    Q4Step sa, sb;
-    load(wave, sa);
-    for (int step = wave; step < Q4_STEPS; step += 2 * Q4_WAVES) {
-      if (step + Q4_WAVES < Q4_STEPS) load(step + Q4_WAVES, sb);
-      compute(sa);
-      if (step + Q4_WAVES >= Q4_STEPS) break;
-      if (step + 2 * Q4_WAVES < Q4_STEPS) load(step + 2 * Q4_WAVES, sa);
-      compute(sb);
+  // Every wavefront makes Q4_SHARE steps; one that has fewer multiplies zeros in those behind its last.  All passes over the registers but
+  // the last load ahead: what they load is used, but for a few steps where the last pass is not a whole one.
+  Q4Step ring[Q4_DEPTH];
+  auto pass = [&](int from, int steps, bool more) __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < Q4_DEPTH; ++d) {
+      if (d >= steps) break;
+      __builtin_amdgcn_sched_barrier(0);
+      unsigned char* xs = sh.t.x[wk][Q4_WN > 1 ? (Q4_DEPTH % 2 ? (from + d) & 1 : d & 1) : 0];
+      stage(from + d, ring[d], xs);
+      if (more) load(from + d + Q4_DEPTH, ring[d]);
+      // the rows of X are there, and those of the step before last have been read (a wavefront's own LDS accesses are carried out in order)
+      if (Q4_WN > 1) __syncthreads(); else __builtin_amdgcn_wave_barrier();
+      multiply(xs);
     }
-  }
+  };
+#pragma unroll
+  for (int d = 0; d < Q4_DEPTH; ++d)
+    if (d < Q4_SHARE) load(d, ring[d]);
+  constexpr int PASSES = (Q4_SHARE + Q4_DEPTH - 1) / Q4_DEPTH, REST = Q4_SHARE - (PASSES - 1) * Q4_DEPTH;
+#pragma unroll 1
+  for (int p = 0; p < PASSES - 1; ++p) pass(p * Q4_DEPTH, Q4_DEPTH, true);
+  pass((PASSES - 1) * Q4_DEPTH, REST, false);
+  __syncthreads();
 #pragma unroll
   for (int a = 0; a < Q4_MB; ++a)
 #pragma unroll
-    for (int b = 0; b < Q4_NT; ++b) red[wave][a * Q4_NT + b][lane] = acc[a][b];
+    for (int b = 0; b < Q4_NT; ++b) sh.red[wk][(wn * Q4_MB + a) * Q4_NT + b][lane] = acc[a][b];
   __syncthreads();
-  for (int u = wave; u < Q4_MB * Q4_NT; u += Q4_WAVES) {
-    kcg_f32x4 sum = red[0][u][lane];
+  for (int u = wave; u < Q4_WN * Q4_MB * Q4_NT; u += Q4_WN * Q4_WK) {
+    kcg_f32x4 sum = sh.red[0][u][lane];
 #pragma unroll
-    for (int w = 1; w < Q4_WAVES; ++w) sum += red[w][u][lane];
-    const int n = n0 + (u % Q4_NT) * 16 + i;
+    for (int w = 1; w < Q4_WK; ++w) sum += sh.red[w][u][lane];
+    const int n = (blockIdx.x * Q4_WN + u / (Q4_MB * Q4_NT)) * Q4_COLS + (u % Q4_NT) * 16 + i;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int m = m0 + (u / Q4_NT) * 16 + g * 4 + r;
-      if (n < Q4_N && m < M) Y[(long long)m * Q4_N + n] = (Q4_YT)(16.0f * sum[r]);
+      const int m = m0 + (u / Q4_NT % Q4_MB) * 16 + g * 4 + r;
+      if (n < Q4_N && m < M) {
+#if Q4_SPLIT > 1
+        part[((long long)blockIdx.z * M + m) * Q4_N + n] = 16.0f * sum[r];
+#else
+        Y[(long long)m * Q4_N + n] = (Q4_YT)(16.0f * sum[r]);
+#endif
+      }
     }
   }
 }
+#endif

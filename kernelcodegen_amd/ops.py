@@ -521,9 +521,12 @@ def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, length
         raise ValueError("starts is [B + 1]")
     if slopes is not None and tuple(slopes.shape) != (heads,):
         raise ValueError("slopes is [heads]")
+    group = heads // kv_heads
+    # the kernel counts pieces of 128 keys of all tiles of 16 rows and more in 32 bits
+    if (tokens * min(group, 64) // 16 + batch + 1) * (width * page // 128 + 2) >= 1 << 31:
+        raise ValueError("too many rows times keys for one launch")
     if not 0.0 <= cap < math.inf or window < 0:
         raise ValueError("cap and window must not be negative")
-    group = heads // kv_heads
     # rows that the average request has of a kv head
     rows = group * -(-tokens // batch)
     blocks = 1 if rows <= 16 else 2 if rows <= 32 or d > 128 else 4
@@ -535,13 +538,13 @@ def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, length
         parts = -(-group // (16 * blocks))
         kern = R.get_kernel("cache_attention", WHOLE=1, **params)
         return _into_last(kern.bind(grid=(batch * kv_heads * parts,)), tuple(q.shape), q.dtype), None, 0
-    grid = 256 if blocks == 4 else 512
+    grid = 256 if blocks == 4 else 512 if blocks == 2 else 768
     kern, join = R.get_kernel("cache_attention", GRID=grid, **params), R.get_kernel("cache_join", GRID=grid, **params)
     floats = 2 * grid * (16 * blocks * d + 32 * blocks)
     return _into_last(kern.bind(), tuple(q.shape), q.dtype), join.bind(), floats
 
 
-def matmul_q4(x, w, scale, zero=None, out_dtype=None):
+def matmul_q4(x, w, scale, zero=None, out_dtype=None, **cfg):
     """x times the transpose of a matrix of 4-bit numbers: y[..., n] = sum over k of x[..., k] * scale[n, k / group] * (code[n, k] - zero).
 
     x: [..., K], IEEE half or bfloat16; w: uint8 [N, K / 2], the code of an even k in the low four bits; scale: [N, K / group], fp32 or x's
@@ -553,17 +556,18 @@ def matmul_q4(x, w, scale, zero=None, out_dtype=None):
         _need_cuda(zero)
     key = ("matmul_q4", dims, x.dtype, w.shape, w.dtype, scale.shape, scale.dtype, None if zero is None else (zero.shape, zero.dtype), out_dtype,
            (x.data_ptr() | w.data_ptr()) & 15)
-    hit = _bound.get(key)
+    hit = None if cfg else _bound.get(key)
     if hit is None:
-        hit = _matmul_q4_launch(x, w, scale, zero, out_dtype)
-        _bound[key] = hit
+        hit = _matmul_q4_launch(x, w, scale, zero, out_dtype, cfg)
+        if not cfg:
+            _bound[key] = hit
     run, rows = hit
     if rows == 0:
         return torch.empty(dims[:-1] + (w.shape[0],), dtype=out_dtype or x.dtype, device=x.device)
     return run(x, w, scale, 0 if zero is None else zero.data_ptr(), rows)
 
 
-def _matmul_q4_launch(x, w, scale, zero, out_dtype):
+def _matmul_q4_launch(x, w, scale, zero, out_dtype, cfg):
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if x.dtype not in (torch.float16, torch.bfloat16) or out_dtype not in (x.dtype, torch.float32) or scale.dtype not in (x.dtype, torch.float32):
         raise ValueError("x is IEEE half or bfloat16, result and scales have x's type or are fp32")
@@ -584,5 +588,5 @@ def _matmul_q4_launch(x, w, scale, zero, out_dtype):
     if rows == 0:
         return None, 0
     kern = R.get_kernel("gemm_q4", N=n, K=k, GROUP=group, F16=int(x.dtype == torch.float16), ZERO=int(zero is not None),
-                        SCALE_F32=int(scale.dtype == torch.float32), OUT_F32=int(out_dtype == torch.float32), MB=blocks)
+                        SCALE_F32=int(scale.dtype == torch.float32), OUT_F32=int(out_dtype == torch.float32), MB=blocks, **cfg)
     return _into_last(kern.bind(grid=(kern.info["grid"][0], -(-rows // (16 * blocks)))), tuple(x.shape[:-1]) + (n,), out_dtype), rows

@@ -44,7 +44,7 @@ def test_every_form_compiles_for_gfx950(family, params, nargs):
     ("cache_attention", attention(128, SCALE=float("inf"))), ("cache_attention", attention(128, WINDOW=-1)), ("cache_attention", attention(128, WHOLE=1, STARTS=1)),
     ("cache_join", attention(128, WHOLE=1)), ("cache_attention", attention(128, F16=2)),
     ("gemm_q4", dict(N=100, K=100, GROUP=50, F16=0, MB=1)), ("gemm_q4", dict(N=100, K=192, GROUP=128, F16=0, MB=1)), ("gemm_q4", dict(N=100, K=192, GROUP=96, F16=0, MB=1)),
-    ("gemm_q4", dict(N=0, K=128, GROUP=128, F16=0, MB=1)), ("gemm_q4", dict(N=100, K=128, GROUP=128, F16=0, MB=5)), ("gemm_q4", dict(N=100, K=128, GROUP=128, F16=0, MB=4, WAVES=16, NT=4))])
+    ("gemm_q4", dict(N=0, K=128, GROUP=128, F16=0, MB=1)), ("gemm_q4", dict(N=100, K=128, GROUP=128, F16=0, MB=5)), ("gemm_q4", dict(N=100, K=128, GROUP=128, F16=0, MB=4, WK=16, NT=4))])
 def test_bad_parameters_are_refused(family, params):
     with pytest.raises(_lib.KcgError):
         R.emit_kernel(family, "kernel0", **params)
@@ -78,7 +78,7 @@ int main() {
       long long sum = 0;
       for (int i = 0; i < tiles; ++i) {
         const int units = ca_units(r, i), low = ca_low(r, i) * CA_UK;
-        if (ca_before(r, i) != sum || units < 1) { printf("count %%d length %%d tile %%d: %%lld, counted %%lld\n", count, length, i, ca_before(r, i), sum); return 1; }
+        if (ca_before(r, i) != sum || units < 1) { printf("count %%d length %%d tile %%d: %%d, counted %%lld\n", count, length, i, ca_before(r, i), sum); return 1; }
         sum += units;
         for (int row = i * t; row < (i + 1) * t && row < count; ++row) {
           const int pos = length - count + row;
@@ -103,7 +103,7 @@ int main() {
 @pytest.mark.parametrize("rows", [1, 4, 12, 64])
 def test_units_of_tiles_in_closed_form(tmp_path, window, rows):
     text = open(os.path.join(ROOT, "kernelcodegen_amd", "csrc", "backend", "kernels", "cache_attention.hip")).read()
-    part = text[text.index("struct CaRequest"):text.index("// Request b; b == B")] + text[text.index("// sum of the whole parts"):text.index("struct CaScan")]
+    part = text[text.index("struct CaRequest"):text.index("// Request b; b == B")] + text[text.index("// sum of the whole parts"):text.index("// Sum over the lanes up to")]
     source = tmp_path / "units.cc"
     source.write_text("#define CA_WINDOW %d\n#define CA_TOK %d\n#define CA_UK 128\n" % (window, rows) + HARNESS % part)
     exe = str(tmp_path / "units")
