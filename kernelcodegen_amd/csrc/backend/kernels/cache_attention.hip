@@ -5,11 +5,13 @@
 // and kv head; table[b] lists the pages of request b, lengths[b] its keys, starts[b] its first row of q.
 //
 // The rows that read the same keys (the CA_GS heads of a group, of CA_TOK tokens) form a tile of 16 * CA_RB rows, so that a key is
-// read once for all of them.  A wavefront takes 32 keys a step, without LDS: K is the left operand of S^T = K Q^T, whose result layout
-// (a lane holds one row's scores of four neighbouring keys) is the layout in which the right operand of O^T = V^T P^T is read, when the
-// eight keys of that product's lane are taken to be those that the lane has scores of.  The order of the summed index is free in
-// both products: K is read in runs of D / 4 bytes, V in runs of D / 16 of eight keys, which are turned into columns in registers
-// by one v_perm each.  e4m3 numbers are exact in both 16-bit types, so the cache costs no rounding; the probabilities are
+// read once for all of them.  A wavefront takes 32 keys a step.  K is the left operand of S^T = K Q^T as it lies in memory, in 8 bits:
+// it is the queries that are converted, once, each row divided by a power of two and written as a sum of two e4m3 numbers (four bits each:
+// all of a bfloat16's) or three (IEEE half), whose products are added; what that leaves out is below 2^-18 of the row's
+// largest element.  The result's layout (a lane holds one row's scores of four neighbouring keys) is the layout in which the right
+// operand of O^T = V^T P^T is read, when the eight keys of that product's lane are taken to be those that the lane has scores of.  V goes
+// through LDS rows that belong to the wavefront alone, from which transposing reads give a lane its eight keys of one column, and is
+// converted to IEEE half, exactly.  The probabilities are
 // rounded to IEEE half (11 bits, they lie in [0, 2^CA_LAZY]), whatever the type of q; for results in IEEE half, which that rounding would
 // make 1.4 times less exact than their own does, the rest of the rounding goes through a second product (CA_SPLIT) where rows are few
 // and the cache's bytes bound the launch.
@@ -18,38 +20,38 @@
 // sum, so P' keeps its bits whatever the scales are; the sum of the probabilities takes P' / vscale as rounded, in fp32, so that a
 // rounding shifts weight between keys and does not scale the result (and two dot products replace four additions).
 //
-// Work: the keys of a tile are cut into units of CA_UK = 128, one step of each of the four wavefronts.  All units of all tiles, head
-// after head, stand in one line that is cut evenly over CA_GRID workgroups (prefix sums of the units of each request, in closed form,
+// Work: the keys of a tile are cut into units of CA_UK = 32 CA_WAVES, one step of each wavefront of a workgroup.  All units of all tiles of a head
+// stand in one line that is cut evenly between CA_PIECES workgroups (prefix sums of the units of each request, in closed form,
 // taken by every workgroup); a tile cut between workgroups leaves partial results in `part`, which cache_join adds up.  So
 // requests of any lengths fill the part.  CA_WHOLE: one workgroup for each tile of a request (one tile each), nothing to join.
-// Parameters: CA_NAME, CA_D, CA_HKV, CA_G (heads per kv head), CA_GS, CA_PAGE, CA_F16, CA_SPLIT, CA_RB, CA_GRID, CA_WHOLE, CA_MIN (least units of
+// Parameters: CA_NAME, CA_D, CA_HKV, CA_G (heads per kv head), CA_GS, CA_PAGE, CA_F16, CA_SPLIT, CA_RB, CA_WAVES, CA_PIECES, CA_WHOLE, CA_MIN (least units of
 // a workgroup), CA_SCALE, CA_CAP (0: none), CA_WINDOW (0: none), CA_SLOPES, CA_STARTS, CA_KP CA_KT CA_KH / CA_VP CA_VT CA_VH (strides of
 // page, token, head), CA_QT CA_QH (of q), CA_JOIN (this is cache_join).
 typedef _Float16 ca_f16x8 __attribute__((ext_vector_type(8)));
 #if CA_F16
 typedef _Float16 ca_q;
-#define CA_MFMA(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ca_f16x8, a), __builtin_bit_cast(ca_f16x8, b), c, 0, 0, 0)
-#define CA_CVT(w, hi) __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, hi))
 #define CA_PACK kcg_pack_f16x2
+#define CA_QN 3                              // e4m3 numbers that a query's element is written as
 #else
 typedef __bf16 ca_q;
-#define CA_MFMA(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(kcg_bf16x8, a), __builtin_bit_cast(kcg_bf16x8, b), c, 0, 0, 0)
-#define CA_CVT(w, hi) __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, hi))
 #define CA_PACK kcg_pack_bf16x2
+#define CA_QN 2
 #endif
 #define CA_MFMA16(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ca_f16x8, a), __builtin_bit_cast(ca_f16x8, b), c, 0, 0, 0)
 #define CA_CVT16(w, hi) __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, hi))
 #define CA_NT (CA_D / 16)                    // tiles of 16 rows of O^T
 #define CA_KR (CA_D / 16)                    // dwords of a lane's share of a key
-#define CA_N8 (CA_D / 128)                   // V: pieces of 8 bytes per lane,
-#define CA_N4 ((CA_D % 128) / 64)            // of 4
-#define CA_N2 ((CA_D % 64) / 32)             // and of 2
-#define CA_VR (2 * CA_N8 + CA_N4 + CA_N2)    // dwords of a lane's share of a key
+#define CA_VL (CA_D / 32)                    // chunks of 16 bytes of a step's V that a lane brings
+// Bytes of a key's V in LDS, an odd multiple of 32, the keys of the second half 16 bytes further: the 16 rows of 16 bytes that 32 lanes read
+// together then meet all banks.
+#define CA_VP_ ((CA_D + 31) / 64 * 64 + 32)
+#define CA_VROW(key) ((key) * CA_VP_ + (key) / 16 * 16)
+#define CA_KP_ (CA_D + 16)                   // of its K: eight lanes that read below one another meet all banks
 #define CA_ROWS (16 * CA_RB)
 #define CA_TOK (CA_ROWS / CA_GS)             // tokens of a tile
 #define CA_PARTS ((CA_G + CA_GS - 1) / CA_GS)    // tiles that the heads of a group are cut into
 #define CA_HV (CA_HKV * CA_PARTS)
-#define CA_UK 128
+#define CA_UK (32 * CA_WAVES)
 #define CA_LAZY 6.0f
 #define CA_TINY 1.17549435e-38f               // the least normal number: scales below count as zero
 #define CA_SLOT (CA_ROWS * CA_D + 2 * CA_ROWS)   // floats of a partial result
@@ -133,36 +135,35 @@ __device__ __forceinline__ int ca_scan(int v) {
   return v;
 }
 
-// Where in the line of all units a workgroup's share begins.
+// What stands at the beginning of a workgroup's share.
 struct CaPlace {
-  long long at;                 // the place
-  int all, chunk;               // units of one head, and of a workgroup
-  int hv, b, tile, unit;        // what stands there
+  int left, chunk;              // units of this share, and of every whole one
+  CaRequest request;
+  int b, tile, unit;
 };
-// The place where workgroup `piece` begins; false where there is none.  Every wavefront finds it by itself, 64 requests to a round, or
-// more to a lane: a read of the lengths, a sum over lanes, and two reads of lanes.
+// The beginning of share `piece` of the units of a head; false where nothing is left.  Every wavefront finds it by itself, 64 requests to a
+// round, or more to a lane: one read of the lengths, a sum over lanes, and reads of lanes.
 __device__ __forceinline__ bool ca_locate(int piece, const int* __restrict__ lengths, const int* __restrict__ starts, int B, int T, int most, CaPlace& w) {
   const int requests = B + CA_STARTS, lane = threadIdx.x & 63;
   const int per = (requests + 63) / 64, b0 = lane * per, b1 = b0 + per < requests ? b0 + per : requests;
+  CaRequest r = {0, 0, 0};
   int mine = 0;
   for (int i = b0; i < b1; ++i) {
-    const CaRequest r = ca_request(lengths, starts, i, B, T, most);
+    r = ca_request(lengths, starts, i, B, T, most);
     mine += ca_before(r, ca_tiles(r));
   }
-  const int through = ca_scan(mine), ahead = through - mine;
-  w.all = __builtin_amdgcn_readlane(through, 63);
-  const long long total = (long long)w.all * CA_HV, even = (total + CA_GRID - 1) / CA_GRID;
-  w.chunk = even < CA_MIN ? CA_MIN : (int)even;
-  w.at = (long long)piece * w.chunk;
-  if (w.at >= total) return false;
-  w.hv = total >> 32 ? (int)(w.at / w.all) : (int)((unsigned)w.at / (unsigned)w.all);
-  const int f = (int)(w.at - (long long)w.hv * w.all);
-  int b = 0, tile = 0, unit = 0;
+  const int through = ca_scan(mine), ahead = through - mine, all = __builtin_amdgcn_readlane(through, 63);
+  const int even = (all + CA_PIECES - 1) / CA_PIECES;
+  w.chunk = even < CA_MIN ? CA_MIN : even;
+  if (piece >= (all + w.chunk - 1) / w.chunk) return false;
+  const int f = piece * w.chunk;
+  w.left = all - f < w.chunk ? all - f : w.chunk;
+  int b = b0, tile = 0, unit = 0;
   const bool here = f >= ahead && f < through;
   if (here) {
     int at = ahead;
-    for (int i = b0; i < b1; ++i) {
-      const CaRequest r = ca_request(lengths, starts, i, B, T, most);
+    for (; b < b1; ++b) {
+      if (per > 1) r = ca_request(lengths, starts, b, B, T, most);
       const int tiles = ca_tiles(r), units = ca_before(r, tiles);
       if (f < at + units) {
         int lo = 0, hi = tiles - 1;           // the last tile that begins at or before f
@@ -170,7 +171,6 @@ __device__ __forceinline__ bool ca_locate(int piece, const int* __restrict__ len
           const int mid = (lo + hi + 1) >> 1;
           if (at + ca_before(r, mid) <= f) lo = mid; else hi = mid - 1;
         }
-        b = i;
         tile = lo;
         unit = f - at - ca_before(r, lo);
         break;
@@ -182,6 +182,9 @@ __device__ __forceinline__ bool ca_locate(int piece, const int* __restrict__ len
   w.b = __builtin_amdgcn_readlane(b, who);
   w.tile = __builtin_amdgcn_readlane(tile, who);
   w.unit = __builtin_amdgcn_readlane(unit, who);
+  w.request.length = __builtin_amdgcn_readlane(r.length, who);
+  w.request.count = __builtin_amdgcn_readlane(r.count, who);
+  w.request.first = __builtin_amdgcn_readlane(r.first, who);
   return true;
 }
 
@@ -196,102 +199,114 @@ __device__ __forceinline__ float ca_cross(float v, bool max) {      // over the 
   return max ? fmaxf(p, q) : p + q;
 }
 
-// Index in a row of O of element `r` of tile `tt`, of a lane of group g: the inverse of the order in which V is read.
-__device__ __forceinline__ int ca_column(int tt, int g, int r) {
-  const int w = tt / 4, e = tt % 4, m = g * 4 + r;
-  if (w < 2 * CA_N8) return (w / 2) * 128 + m * 8 + (w & 1) * 4 + e;
-  if (CA_N4 && w == 2 * CA_N8) return CA_N8 * 128 + m * 4 + e;
-  return CA_N8 * 128 + CA_N4 * 64 + m * 2 + e;
+// One row block's tile of O^T to the rows of `out`, of `tokens` tokens from `first` on.
+__device__ __forceinline__ void ca_store(ca_q* __restrict__ out, int first, int tokens, int hv, int rb, int tt, kcg_f32x4 o, float sum) {
+  const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4, row = rb * 16 + n;
+  const int token = row / CA_GS, head = row - token * CA_GS, h = (hv / CA_PARTS) * CA_G + (hv % CA_PARTS) * CA_GS + head;
+  if (token >= tokens || (hv % CA_PARTS) * CA_GS + head >= CA_G) return;
+  const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);       // (a NaN stays one)
+  ca_q* p = out + ((long long)(first + token) * (CA_HKV * CA_G) + h) * CA_D;
+  *(kcg_u32x2*)(p + tt * 16 + g * 4) = kcg_u32x2{CA_PACK(o[0] * inv, o[1] * inv), CA_PACK(o[2] * inv, o[3] * inv)};
 }
 
-// One row block's tile of O^T to the rows of `out`.
-__device__ __forceinline__ void ca_store(ca_q* __restrict__ out, const CaRequest& rq, int hv, int tile, int rb, int tt, kcg_f32x4 o, float sum) {
-  const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4, row = rb * 16 + n;
-  const int token = row / CA_GS, head = row - token * CA_GS, t = ca_tokens(rq);
-  const int h = (hv / CA_PARTS) * CA_G + (hv % CA_PARTS) * CA_GS + head;
-  if (token >= t || tile * t + token >= rq.count || (hv % CA_PARTS) * CA_GS + head >= CA_G) return;
-  const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);       // (a NaN stays one)
-  ca_q* p = out + ((long long)(rq.first + tile * t + token) * (CA_HKV * CA_G) + h) * CA_D;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) p[ca_column(tt, g, r)] = (ca_q)(o[r] * inv);
-}
+// What the workgroup of a share tells the join about the tile that its share begins inside of.
+struct CaEnd { int first, tokens, parts, slot; };      // rows, parts (0: nothing to join, or an earlier share does), slot of the part before
+#define CA_ENDS (4 * CA_HV * CA_PIECES)                // floats of all of them, in front of the parts
 
 #if CA_JOIN
-// A workgroup for every end of a share, which has something to do where that is the first one inside of a tile: it adds up the parts of
-// the tile, in order.  A wavefront takes every fourth tile of 16 columns of O.
-extern "C" __global__ __launch_bounds__(256)
-void CA_NAME(const float* __restrict__ part, const int* __restrict__ lengths, const int* __restrict__ starts, long long T_, long long B_,
-             long long W_, ca_q* __restrict__ out) {
-  const int T = (int)T_, B = (int)B_, most = (int)W_ * CA_PAGE, rb = blockIdx.y;
+// A workgroup for every beginning of a share and two tiles of 16 columns of O; it has something to do where that is the first one inside
+// of a tile of rows, and adds up the parts of the tile.  Four wavefronts take every fourth part of the same columns.
+extern "C" __global__ __launch_bounds__(512)
+void CA_NAME(const float* __restrict__ part, ca_q* __restrict__ out) {
+  __shared__ kcg_f32x4 red[8][64];
+  __shared__ float ml[8][16][2];
+  const int hv = blockIdx.x % CA_HV, piece = blockIdx.x / CA_HV + 1, id = hv * CA_PIECES + piece;
+  const CaEnd e = ((const CaEnd*)part)[id];
+  if (e.parts == 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15;
-  const int second = blockIdx.x + 1;
-  CaPlace w;
-  if (!ca_locate(second, lengths, starts, B, T, most, w) || w.unit == 0 || w.unit > w.chunk) return;
-  const CaRequest rq = ca_request(lengths, starts, w.b, B, T, most);
-  // the parts: of the workgroup before this end (its last piece, slot 1, unless its share begins with it), and of as many behind as
-  // the tile goes on for
-  const int count = 1 + (ca_units(rq, w.tile) - w.unit + w.chunk - 1) / w.chunk;
-  const float* first = part + ((long long)(second - 1) * 2 + (w.unit < w.chunk ? 1 : 0)) * CA_SLOT;
-  const float* later = part + (long long)second * 2 * CA_SLOT;
-  // the largest maximum, and the sum: lane group g takes every fourth part
-  const int at = CA_ROWS * CA_D + (rb * 16 + n) * 2;
+  const int rb = blockIdx.y / (CA_NT / 2), tt = blockIdx.y % (CA_NT / 2) * 2 + (wave & 1);
+  const float* later = part + CA_ENDS + ((long long)id * 2 - 2) * CA_SLOT;       // part i > 0 is slot 0 of share id + i - 1
+  const int at = CA_ROWS * CA_D + (rb * 16 + n) * 2, of = ((rb * CA_NT + tt) * 64 + lane) * 4;
   float m = -__builtin_inff(), l = 0.0f;
-  for (int i = lane >> 4; i < count; i += 4) {
-    const float* p = i ? later + (long long)(i - 1) * 2 * CA_SLOT : first;
-    const float pm = p[at], to = fmaxf(m, pm), ref = to == -__builtin_inff() ? 0.0f : to;
-    l = l * __builtin_amdgcn_exp2f(m - ref) + p[at + 1] * __builtin_amdgcn_exp2f(pm - ref);
+  kcg_f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int i = wave >> 1; i < e.parts; i += 4) {
+    const float* p = later + ((long long)i * 2 + (i ? 0 : e.slot)) * CA_SLOT;
+    const kcg_f32x4 x = *(const kcg_f32x4*)(p + of);
+    const float pm = p[at], pl = p[at + 1], to = fmaxf(m, pm), ref = to == -__builtin_inff() ? 0.0f : to;
+    const float fa = __builtin_amdgcn_exp2f(m - ref), fb = __builtin_amdgcn_exp2f(pm - ref);
+    o = o * fa + x * fb;
+    l = l * fa + pl * fb;
     m = to;
   }
-  const float top = ca_cross(m, true), ref = top == -__builtin_inff() ? 0.0f : top;
-  const float sum = ca_cross(l * __builtin_amdgcn_exp2f(m - ref), false);
-  for (int tt = wave; tt < CA_NT; tt += 4) {
-    kcg_f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int i = 0; i < count; ++i) {
-      const float* p = i ? later + (long long)(i - 1) * 2 * CA_SLOT : first;
-      o += *(const kcg_f32x4*)(p + ((rb * CA_NT + tt) * 64 + lane) * 4) * __builtin_amdgcn_exp2f(p[at] - ref);
-    }
-    ca_store(out, rq, w.hv, w.tile, rb, tt, o, sum);
+  if (lane < 16) {
+    ml[wave][n][0] = m;
+    ml[wave][n][1] = l;
   }
+  red[wave][lane] = o;
+  __syncthreads();
+  if (wave > 1) return;
+  const float top = fmaxf(fmaxf(ml[wave][n][0], ml[wave + 2][n][0]), fmaxf(ml[wave + 4][n][0], ml[wave + 6][n][0]));
+  const float ref = top == -__builtin_inff() ? 0.0f : top;
+  kcg_f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  float total = 0.0f;
+#pragma unroll
+  for (int w = wave; w < 8; w += 2) {
+    const float f = __builtin_amdgcn_exp2f(ml[w][n][0] - ref);
+    sum += red[w][lane] * f;
+    total += ml[w][n][1] * f;
+  }
+  ca_store(out, e.first, e.tokens, hv, rb, tt, sum, total);
 }
 #else
 
-// What a step has beside its keys and values.
-struct CaMeta {
-  float ks[2], vs[2];      // scales of the pages of its two halves
-  bool there[2];           // false: no such keys, or a page that there is none of
-};
-
-extern "C" __global__ __launch_bounds__(256, CA_OCC)
+extern "C" __global__ __launch_bounds__(64 * CA_WAVES, CA_OCC)
 void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, const unsigned char* __restrict__ vc,
              const float* __restrict__ kscale, const float* __restrict__ vscale, const int* __restrict__ table,
              const int* __restrict__ lengths, const int* __restrict__ starts, const float* __restrict__ slopes,
              float* __restrict__ part, long long T_, long long B_, long long W_, long long table_row, long long pages_, ca_q* __restrict__ out) {
-  __shared__ kcg_f32x4 red[4][CA_NT][64];
-  __shared__ float ml[4][CA_ROWS][2];
+  union Shared {
+    kcg_f32x4 red[CA_WAVES][CA_NT][64];
+    struct {
+      __attribute__((aligned(16))) unsigned char v[CA_WAVES][CA_VROW(31) + CA_VP_], k[CA_WAVES][32 * CA_KP_];
+    } tile;
+  };
+  __shared__ Shared sh;
+  __shared__ float ml[CA_WAVES][CA_ROWS][2];
   const int T = (int)T_, B = (int)B_, most = (int)W_ * CA_PAGE, pages = (int)pages_;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
 
-  int hv, b, tile, unit;
-  int left;                       // units this workgroup has to do
+  // neighbouring heads, whose rows of a token lie beside one another, walk over their keys at the same time, and a head's workgroups, which
+  // have keys in common where there are many rows, lie on one XCD where the number of heads allows (workgroups are dealt to the eight in turn)
+  const int hv = blockIdx.x % CA_HV;
+  CaRequest rq;
+  int b, tile, unit, left;                       // left: units this workgroup has to do
 #if CA_WHOLE
-  hv = blockIdx.x % CA_HV;
   b = blockIdx.x / CA_HV;
+  rq = ca_request(lengths, starts, b, B, T, most);
   tile = unit = 0;
   left = 0x7fffffff;
 #else
-  const int requests = B + CA_STARTS;
-  // neighbouring shares, which have pages in common, on one XCD: workgroups are dealt to the eight in turn
-  const int piece = (blockIdx.x & 7) * (CA_GRID / 8) + (blockIdx.x >> 3);
+  const int requests = B + CA_STARTS, piece = blockIdx.x / CA_HV, id = hv * CA_PIECES + piece;
   CaPlace w;
-  if (!ca_locate(piece, lengths, starts, B, T, most, w)) return;
-  left = (long long)w.all * CA_HV - w.at < w.chunk ? (int)((long long)w.all * CA_HV - w.at) : w.chunk;
-  hv = w.hv; b = w.b; tile = w.tile; unit = w.unit;
+  const bool some = ca_locate(piece, lengths, starts, B, T, most, w);
+  if (threadIdx.x == 0) {
+    CaEnd e = {0, 0, 0, 0};
+    if (some && w.unit > 0 && w.unit <= w.chunk) {
+      const int t = ca_tokens(w.request), at = w.tile * t;
+      e.first = w.request.first + at;
+      e.tokens = w.request.count - at < t ? w.request.count - at : t;
+      e.parts = 1 + (ca_units(w.request, w.tile) - w.unit + w.chunk - 1) / w.chunk;
+      e.slot = w.unit < w.chunk ? 1 : 0;          // the share before has it as its last piece, or as its only one
+    }
+    ((CaEnd*)part)[id] = e;
+  }
+  if (!some) return;
+  rq = w.request; b = w.b; tile = w.tile; unit = w.unit; left = w.left;
   bool begun = true;              // the first piece of this workgroup, if it is not a whole tile, goes to slot 0, a later one to slot 1
 #endif
 
   while (left > 0) {
-    const CaRequest rq = ca_request(lengths, starts, b, B, T, most);
     const int t = ca_tokens(rq), tok0 = tile * t, tokens = rq.count - tok0 < t ? rq.count - tok0 : t;
     const int units = ca_units(rq, tile);
     const int until = left < units - unit ? unit + left : units;      // of this piece
@@ -303,8 +318,9 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
     int key = base + unit * CA_UK + wave * 32;
     const int end = base + until * CA_UK < hi ? base + until * CA_UK : hi;
 
-    // rows: query fragments, positions
-    unsigned qf[CA_RB][CA_KR * 2];
+    // rows: queries in 8 bits, positions
+    unsigned qf[CA_RB][CA_QN][CA_KR];
+    float qs[CA_RB];               // the power of two that a row was divided by
     int pos[CA_RB];
     float slope[CA_RB];
 #pragma unroll
@@ -315,8 +331,38 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
       pos[rb] = first + token;
       slope[rb] = CA_SLOPES ? slopes[head] * 1.44269504088896340736f : 0.0f;
       const ca_q* p = q + (long long)(rq.first + tok0 + token) * CA_QT + (long long)head * CA_QH + g * (CA_D / 4);
+      typedef ca_q ca_q8 __attribute__((ext_vector_type(8)));
+      ca_q8 raw[CA_KR / 2];
+      float top = 0.0f;
 #pragma unroll
-      for (int i = 0; i < CA_KR * 2; i += 4) *(kcg_u32x4*)&qf[rb][i] = *(const kcg_u32x4*)(p + i * 2);
+      for (int i = 0; i < CA_KR / 2; ++i) raw[i] = *(const ca_q8*)(p + i * 8);
+#pragma unroll
+      for (int i = 0; i < CA_KR * 4; ++i) top = fmaxf(top, __builtin_fabsf((float)raw[i / 8][i % 8]));
+      top = ca_cross(top, true);
+      // the least power of two whose 448-fold (1.75 * 2^8) reaches the row's largest element
+      const unsigned bits = __builtin_bit_cast(unsigned, top);
+      int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+      e = e < -100 ? -100 : e;
+      qs[rb] = __builtin_bit_cast(float, (unsigned)(e + 127) << 23);
+      const float inv = __builtin_bit_cast(float, (unsigned)(127 - e) << 23);
+#pragma unroll
+      for (int i = 0; i < CA_KR; ++i) {
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = (float)raw[i / 2][i % 2 * 4 + j] * inv;
+#pragma unroll
+        for (int c = 0; c < CA_QN; ++c) {
+          int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+          w = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], w, true);
+          qf[rb][c][i] = (unsigned)w;
+          if (c + 1 < CA_QN) {
+            f[0] -= __builtin_amdgcn_cvt_f32_fp8(w, 0);
+            f[1] -= __builtin_amdgcn_cvt_f32_fp8(w, 1);
+            f[2] -= __builtin_amdgcn_cvt_f32_fp8(w, 2);
+            f[3] -= __builtin_amdgcn_cvt_f32_fp8(w, 3);
+          }
+        }
+      }
     }
 
     kcg_f32x4 acc[CA_RB][CA_NT];
@@ -330,85 +376,102 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
     }
 
     const int* row = table + (long long)b * table_row;
-    // Entries of the table for the two halves of a step.  What is wrong with them is looked at when they are used, a step later: until
-    // then nobody waits for them.
-    auto pagesOf = [&](int at, int (&page)[2]) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) page[h] = row[(at + h * 16 < hi ? at + h * 16 : hi - 1) / CA_PAGE];
+    // Pages and scales of the halves of 32 steps, a lane each (lane 2 s + h half h of step s), read while the 32 steps before are worked on and
+    // their pages while those before are: by vector loads, since a scalar load would be waited for by every LDS access.
+    struct Block { int page; float ks, vs; };       // page -1: no such keys, or a page that there is none of
+    auto pagesOf = [&](int from) {
+      const int at = from + (lane >> 1) * CA_UK + (lane & 1) * 16;
+      const int page = row[(at < hi ? at : hi - 1) / CA_PAGE];
+      return at < hi && at + 16 > lo && (unsigned)page < (unsigned)pages ? page : -1;
+    };
+    auto scalesOf = [&](int page) {
+      const long long at = (long long)(page < 0 ? 0 : page) * CA_HKV + kvh;       // (what is not there is read from somewhere that is)
+      return Block{page, kscale[at], vscale[at]};
     };
     // Addresses: a uniform base and an offset of the lane's
-    const unsigned koff = n * (unsigned)CA_KT + g * (CA_D / 4), voff = g * 4 * (unsigned)CA_VT;
-    unsigned k[2][CA_KR], v[8][CA_VR];
-    // (what is not there is read from somewhere that is)
-    auto loadMeta = [&](int at, const int (&page)[2], long long (&pg)[2], CaMeta& s) {
+    // K and V go in chunks of 16 bytes, neighbouring lanes neighbouring chunks (read where a lane needs them, four neighbouring lanes touch
+    // four lines)
+    kcg_u32x4 k[CA_VL], v[CA_VL];
+    unsigned koff[CA_VL], voff[CA_VL], kat[CA_VL], vat[CA_VL];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        s.there[h] = at + h * 16 < hi && at + h * 16 + 16 > lo && (unsigned)page[h] < (unsigned)pages;
-        pg[h] = s.there[h] ? page[h] : 0;
-        s.ks[h] = kscale[pg[h] * CA_HKV + kvh];
-        s.vs[h] = vscale[pg[h] * CA_HKV + kvh];
-      }
+    for (int u = 0; u < CA_VL; ++u) {
+      const int c = u * 64 + lane, key32 = c / (CA_D / 16), part16 = c % (CA_D / 16) * 16;
+      koff[u] = (key32 % 16) * (unsigned)CA_KT + part16;
+      voff[u] = (key32 % 16) * (unsigned)CA_VT + part16;
+      kat[u] = key32 * CA_KP_ + part16;
+      vat[u] = CA_VROW(key32) + part16;
+    }
+    // the half that a chunk's key lies in is the same for all lanes where 64 chunks are whole halves
+#define CA_HALF(u) (CA_D % 64 == 0 ? (u) * 64 / CA_D : ((u) * 64 + lane) / CA_D)
+    auto loadK = [&](int at, const int (&pg)[2]) {
+      const unsigned char* kp[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        kp[h] = kc + ((long long)(pg[h] < 0 ? 0 : pg[h]) * CA_KP + (long long)((at + h * 16) % CA_PAGE) * CA_KT + (long long)kvh * CA_KH);
+#pragma unroll
+      for (int u = 0; u < CA_VL; ++u) k[u] = *(const kcg_u32x4*)((CA_HALF(u) ? kp[1] : kp[0]) + koff[u]);
     };
-    auto loadK = [&](int at, const long long (&pg)[2]) {
+    auto loadV = [&](int at, const int (&pg)[2]) {
+      const unsigned char* vp[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const unsigned char* kp = kc + (pg[h] * CA_KP + (long long)((at + h * 16) % CA_PAGE) * CA_KT + (long long)kvh * CA_KH);
-#if CA_KR % 4 == 0
+      for (int h = 0; h < 2; ++h)
+        vp[h] = vc + ((long long)(pg[h] < 0 ? 0 : pg[h]) * CA_VP + (long long)((at + h * 16) % CA_PAGE) * CA_VT + (long long)kvh * CA_VH);
 #pragma unroll
-        for (int i = 0; i < CA_KR; i += 4) *(kcg_u32x4*)&k[h][i] = *(const kcg_u32x4*)(kp + koff + i * 4);
-#else
-#pragma unroll
-        for (int i = 0; i < CA_KR; i += 2) *(kcg_u32x2*)&k[h][i] = *(const kcg_u32x2*)(kp + koff + i * 4);
-#endif
-      }
+      for (int u = 0; u < CA_VL; ++u) v[u] = *(const kcg_u32x4*)((CA_HALF(u) ? vp[1] : vp[0]) + voff[u]);
     };
-    auto loadV = [&](int at, const long long (&pg)[2]) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const unsigned char* vp = vc + (pg[h] * CA_VP + (long long)((at + h * 16) % CA_PAGE) * CA_VT + (long long)kvh * CA_VH);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const unsigned off = voff + r * (unsigned)CA_VT;
-#pragma unroll
-          for (int i = 0; i < CA_N8; ++i) *(kcg_u32x2*)&v[h * 4 + r][2 * i] = *(const kcg_u32x2*)(vp + off + (i * 128 + n * 8));
-          if (CA_N4) v[h * 4 + r][2 * CA_N8] = *(const unsigned*)(vp + off + (CA_N8 * 128 + n * 4));
-          if (CA_N2) v[h * 4 + r][2 * CA_N8 + CA_N4] = *(const unsigned short*)(vp + off + (CA_N8 * 128 + CA_N4 * 64 + n * 2));
-        }
-      }
-    };
+    typedef __attribute__((address_space(3))) unsigned char* ca_lds;
+    typedef int ca_i32x2 __attribute__((ext_vector_type(2)));
+    unsigned char *ks_ = sh.tile.k[wave], *vs = sh.tile.v[wave];
+    // this lane's address for the transposing reads of tile 0: within each group of 16 lanes, lanes 2 j and 2 j + 1 give the two halves of row
+    // j, and lane i receives column i of the eight rows.  The rows are the keys that lane group g has scores of.
+    const int key8 = n / 2 < 4 ? g * 4 + n / 2 : 16 + g * 4 + n / 2 - 4;
+    const ca_lds vread = (ca_lds)vs + CA_VROW(key8) + (n & 1) * 8;
 
-    float known = 1.0f;            // the last vscale that was not zero
+    float lvk = 0.0f;              // logarithm of the last vscale that was not zero
     kcg_f32x4 sc[CA_RB][2];
-    auto scores = [&]() {
+    // `behind` is called when the registers of K are free
+    auto scores = [&](auto behind) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < CA_VL; ++u) *(kcg_u32x4*)(ks_ + kat[u]) = k[u];
+      behind();
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int rb = 0; rb < CA_RB; ++rb)
 #pragma unroll
         for (int h = 0; h < 2; ++h) sc[rb][h] = kcg_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int h = 0; h < 2; ++h)
+#if CA_D % 128 == 0
+#pragma unroll
+        for (int i = 0; i < CA_KR; i += 8) {
+          const unsigned char* p = ks_ + (h * 16 + n) * CA_KP_ + g * (CA_D / 4) + i * 4;
+          const kcg_i32x4 k0 = *(const kcg_i32x4*)p, k1 = *(const kcg_i32x4*)(p + 16);
+          const kcg_i32x8 kf = {k0[0], k0[1], k0[2], k0[3], k1[0], k1[1], k1[2], k1[3]};
+#pragma unroll
+          for (int rb = 0; rb < CA_RB; ++rb)
+#pragma unroll
+            for (int c = 0; c < CA_QN; ++c) {
+              const unsigned (&w)[CA_KR] = qf[rb][c];
+              const kcg_i32x8 qv = {(int)w[i], (int)w[i + 1], (int)w[i + 2], (int)w[i + 3], (int)w[i + 4], (int)w[i + 5], (int)w[i + 6], (int)w[i + 7]};
+              sc[rb][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qv, sc[rb][h], 0, 0, 0, 0, 0, 0);
+            }
+        }
+#else
 #pragma unroll
         for (int i = 0; i < CA_KR; i += 2) {
-          const kcg_u32x4 kf = {CA_CVT(k[h][i], false), CA_CVT(k[h][i], true), CA_CVT(k[h][i + 1], false), CA_CVT(k[h][i + 1], true)};
+          const long kf = *(const long*)(ks_ + (h * 16 + n) * CA_KP_ + g * (CA_D / 4) + i * 4);
 #pragma unroll
-          for (int rb = 0; rb < CA_RB; ++rb) {
-            const kcg_u32x4 qv = {qf[rb][2 * i], qf[rb][2 * i + 1], qf[rb][2 * i + 2], qf[rb][2 * i + 3]};
-            sc[rb][h] = CA_MFMA(kf, qv, sc[rb][h]);
-          }
+          for (int rb = 0; rb < CA_RB; ++rb)
+#pragma unroll
+            for (int c = 0; c < CA_QN; ++c)
+              sc[rb][h] = __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(kf, (long)((unsigned long)qf[rb][c][i + 1] << 32 | qf[rb][c][i]), sc[rb][h], 0, 0, 0);
         }
+#endif
     };
     // Scores to probabilities, and these into the sums; `masked`: not every row sees every key of the step, or a scale is zero.
-    auto weigh = [&](int at, const CaMeta& s, bool masked) __attribute__((always_inline)) {
-      // scales; those of zero stand for pages of zeros (or for pages that are not there)
-      float ks[2], lv[2], iv[2];
-      bool zero[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        zero[h] = masked && (!s.there[h] || s.vs[h] < CA_TINY);
-        ks[h] = masked && !s.there[h] ? 0.0f : s.ks[h];
-        if (!zero[h]) known = s.vs[h];
-        lv[h] = __builtin_amdgcn_logf(known);
-        iv[h] = __builtin_amdgcn_rcpf(known);
-      }
+    // `behind` is called when the registers of V are free.
+    auto weigh = [&](int at, const bool (&there)[2], const bool (&zero)[2], const float (&ks)[2], const float (&lv)[2], const float (&iv)[2], bool masked,
+                     auto behind) __attribute__((always_inline)) {
 #pragma unroll
       for (int rb = 0; rb < CA_RB; ++rb)
 #pragma unroll
@@ -417,10 +480,10 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
           for (int r = 0; r < 4; ++r) {
             float x = sc[rb][h][r];
 #if CA_HAS_CAP
-            x = kcg_fast_tanh(x * (ks[h] * (CA_SCALE / CA_CAP)));
+            x = kcg_fast_tanh(x * (ks[h] * (CA_SCALE / CA_CAP) * qs[rb]));
             x = __builtin_fmaf(x, CA_CAP * 1.44269504088896340736f, lv[h]);
 #else
-            x = __builtin_fmaf(x, ks[h] * (CA_SCALE * 1.44269504088896340736f), lv[h]);
+            x = __builtin_fmaf(x, ks[h] * (CA_SCALE * 1.44269504088896340736f) * qs[rb], lv[h]);
 #endif
             if (CA_SLOPES) x = __builtin_fmaf(slope[rb], (float)(at + h * 16 + g * 4 + r - pos[rb]), x);
             sc[rb][h][r] = x;
@@ -434,19 +497,9 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const int key16 = at + h * 16 + g * 4 + r;
-              const bool seen = key16 <= pos[rb] && (!CA_WINDOW || key16 > pos[rb] - CA_WINDOW) && s.there[h];
+              const bool seen = key16 <= pos[rb] && (!CA_WINDOW || key16 > pos[rb] - CA_WINDOW) && there[h];
               if (!seen) sc[rb][h][r] = -__builtin_inff();
             }
-        // V of keys that no row sees, which may be anything, and of pages whose scale is zero
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int key16 = at + h * 16 + g * 4 + r;
-            if (key16 < lo || key16 >= hi || zero[h])
-#pragma unroll
-              for (int w = 0; w < CA_VR; ++w) v[h * 4 + r][w] = 0;
-          }
       }
       // running maximum: the sums are brought to a new one only where it is more than 2^CA_LAZY times the old
       unsigned pf[CA_RB][4];
@@ -488,136 +541,163 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
           l[rb] = __builtin_fmaf(sum, iv[h], l[rb]);
         }
       }
+      auto stage = [&]() __attribute__((always_inline)) {      // (a wavefront's own LDS accesses are carried out in order)
+#pragma unroll
+        for (int u = 0; u < CA_VL; ++u) *(kcg_u32x4*)(vs + vat[u]) = v[u];
+        __builtin_amdgcn_wave_barrier();
+      };
+      auto column = [&](int tt) __attribute__((always_inline)) {
+        const ca_i32x2 raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) ca_i32x2*)(vread + tt * 16));
+        const unsigned w0 = (unsigned)raw[0], w1 = (unsigned)raw[1];
+        return kcg_u32x4{CA_CVT16(w0, false), CA_CVT16(w0, true), CA_CVT16(w1, false), CA_CVT16(w1, true)};
+      };
       if (masked) {
-        // NaN in V where some rows see the key and some do not: it goes to those that do, by a product of where V is NaN and who sees
-        unsigned any = 0;
+        // V of keys that no row sees, which may be anything, and of pages whose scale is zero, counts as zero
+        unsigned nan = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int u = 0; u < CA_VL; ++u) {
+          const int key32 = (u * 64 + lane) / (CA_D / 16);
+          if (at + key32 < lo || at + key32 >= hi || (key32 < 16 ? zero[0] : zero[1])) v[u] = kcg_u32x4{0, 0, 0, 0};
 #pragma unroll
-          for (int w = 0; w < CA_VR; ++w) any |= ((v[k][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-        if (__any(any != 0)) {
+          for (int i = 0; i < 4; ++i) nan |= ((v[u][i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        }
+        if (__any(nan != 0)) {
+          // NaN where some rows see the key and some may not: it goes to those that do, by a product of where V is NaN and who sees
+          kcg_u32x4 whole[CA_VL];
 #pragma unroll
-          for (int w = 0; w < CA_VR; ++w)
+          for (int u = 0; u < CA_VL; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (w * 4 + e >= CA_NT) continue;
-              unsigned x[4];             // 1.0 where column e of dword w is NaN
+            for (int i = 0; i < 4; ++i) {
+              const unsigned bytes = ((v[u][i] & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u;
+              whole[u][i] = v[u][i] & ~(bytes * 0xffu);
+              v[u][i] = bytes * 0x38u;               // 1.0
+            }
+          stage();
+#pragma unroll
+          for (int u = 0; u < CA_VL; ++u) v[u] = whole[u];
+#pragma unroll
+          for (int tt = 0; tt < CA_NT; ++tt) {
+            const kcg_u32x4 where = column(tt);
+#pragma unroll
+            for (int rb = 0; rb < CA_RB; ++rb) {
+              unsigned see[4];
 #pragma unroll
               for (int j = 0; j < 4; ++j)
-                x[j] = ((v[2 * j][w] >> (8 * e) & 0x7f) == 0x7f ? 0x3c00u : 0u) | ((v[2 * j + 1][w] >> (8 * e) & 0x7f) == 0x7f ? 0x3c000000u : 0u);
-              const kcg_u32x4 where = {x[0], x[1], x[2], x[3]};
+                see[j] = (sc[rb][j / 2][j % 2 * 2] != -__builtin_inff() ? 0x3c00u : 0u) | (sc[rb][j / 2][j % 2 * 2 + 1] != -__builtin_inff() ? 0x3c000000u : 0u);
+              const kcg_u32x4 who = {see[0], see[1], see[2], see[3]};
+              const kcg_f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+              kcg_f32x4 c = CA_MFMA16(where, who, none);          // how many such keys the row sees
+              c *= 0x1p127f;
 #pragma unroll
-              for (int rb = 0; rb < CA_RB; ++rb) {
-                unsigned see[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  see[j] = (sc[rb][j / 2][j % 2 * 2] != -__builtin_inff() ? 0x3c00u : 0u) | (sc[rb][j / 2][j % 2 * 2 + 1] != -__builtin_inff() ? 0x3c000000u : 0u);
-                const kcg_u32x4 who = {see[0], see[1], see[2], see[3]};
-                const kcg_f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
-                kcg_f32x4 c = CA_MFMA16(where, who, none);        // how many such keys the row sees
-                c *= 0x1p127f;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) acc[rb][w * 4 + e][r] = __builtin_fmaf(c[r] * 0x1p127f, 0.0f, acc[rb][w * 4 + e][r]);      // + 0, or infinity times 0
-              }
-              __builtin_amdgcn_sched_barrier(0);
+              for (int r = 0; r < 4; ++r) acc[rb][tt][r] = __builtin_fmaf(c[r] * 0x1p127f, 0.0f, acc[rb][tt][r]);      // + 0, or infinity times 0
             }
-#pragma unroll
-          for (int k8 = 0; k8 < 8; ++k8)
-#pragma unroll
-            for (int w = 0; w < CA_VR; ++w) v[k8][w] &= ~((((v[k8][w] & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u) * 0xffu);
-        }
-      }
-#pragma unroll
-      for (int w = 0; w < CA_VR; ++w)
-#pragma unroll
-        for (int e2 = 0; e2 < 2; ++e2) {
-          const int tt = w * 4 + e2 * 2;
-          if (tt >= CA_NT) continue;
-          unsigned x[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] = e2 ? CA_CVT16(v[k][w], true) : CA_CVT16(v[k][w], false);
-          const kcg_u32x4 even = {__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u),
-                                  __builtin_amdgcn_perm(x[5], x[4], 0x05040100u), __builtin_amdgcn_perm(x[7], x[6], 0x05040100u)};
-          const kcg_u32x4 odd = {__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u),
-                                 __builtin_amdgcn_perm(x[5], x[4], 0x07060302u), __builtin_amdgcn_perm(x[7], x[6], 0x07060302u)};
-#pragma unroll
-          for (int rb = 0; rb < CA_RB; ++rb) {
-            const kcg_u32x4 p = {pf[rb][0], pf[rb][1], pf[rb][2], pf[rb][3]};
-            acc[rb][tt] = CA_MFMA16(even, p, acc[rb][tt]);
-            acc[rb][tt + 1] = CA_MFMA16(odd, p, acc[rb][tt + 1]);
-#if CA_SPLIT
-            const kcg_u32x4 q = {pl[rb][0], pl[rb][1], pl[rb][2], pl[rb][3]};
-            acc[rb][tt] = CA_MFMA16(even, q, acc[rb][tt]);
-            acc[rb][tt + 1] = CA_MFMA16(odd, q, acc[rb][tt + 1]);
-#endif
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
+      }
+      stage();
+      behind();
+#pragma unroll
+      for (int tt = 0; tt < CA_NT; ++tt) {
+        const kcg_u32x4 vf = column(tt);
+#pragma unroll
+        for (int rb = 0; rb < CA_RB; ++rb) {
+          const kcg_u32x4 p = {pf[rb][0], pf[rb][1], pf[rb][2], pf[rb][3]};
+          acc[rb][tt] = CA_MFMA16(vf, p, acc[rb][tt]);
+#if CA_SPLIT
+          const kcg_u32x4 q = {pl[rb][0], pl[rb][1], pl[rb][2], pl[rb][3]};
+          acc[rb][tt] = CA_MFMA16(vf, q, acc[rb][tt]);
+#endif
+        }
+      }
     };
 
     if (key < end) {
-      // The next step's keys are loaded when this one's scores are there, its values when this one's sums are: into the same registers, so
-      // that many wavefronts fit.  Pages are read two steps ahead.
+      // The next step's keys are loaded when this one's scores are there, its values when this one's are in LDS: into the same registers, so
+      // that many wavefronts fit.
       const int last = key + (end - 1 - key) / CA_UK * CA_UK;
-      CaMeta meta;
-      int next[2];
-      long long pg[2];
-      pagesOf(key, next);
-      loadMeta(key, next, pg, meta);
+      Block now = scalesOf(pagesOf(key)), soon;
+      int later = pagesOf(key + 32 * CA_UK);
+      int pg[2] = {__builtin_amdgcn_readlane(now.page, 0), __builtin_amdgcn_readlane(now.page, 1)};
       loadK(key, pg);
       loadV(key, pg);
-      pagesOf(key + CA_UK < last ? key + CA_UK : last, next);
+      int step = 0;
 #pragma unroll 1
       while (true) {
-        scores();
-        const CaMeta now = meta;
-        const bool more = key < last;
-        if (more) {
-          loadMeta(key + CA_UK, next, pg, meta);
-          loadK(key + CA_UK, pg);
-          pagesOf(key + 2 * CA_UK < last ? key + 2 * CA_UK : last, next);
+        if (step == 0) {
+          soon = scalesOf(later);
+          later = pagesOf(key + 64 * CA_UK);
+          // (scales of zero stand for pages of zeros)
+          now.ks = now.page < 0 ? 0.0f : now.ks;
+          now.vs = now.page < 0 || now.vs < CA_TINY ? -__builtin_inff() : __builtin_amdgcn_logf(now.vs);
         }
-        weigh(key, now, key + 32 > first + 1 || (CA_WINDOW && key < first + tokens - CA_WINDOW) || !now.there[0] || !now.there[1] || now.vs[0] < CA_TINY || now.vs[1] < CA_TINY);
+        bool there[2], zero[2];
+        float ks[2], lv[2], iv[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          there[h] = pg[h] >= 0;
+          ks[h] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, now.ks), 2 * step + h));
+          lv[h] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, now.vs), 2 * step + h));
+          zero[h] = lv[h] == -__builtin_inff();
+          if (zero[h]) lv[h] = lvk;
+          lvk = lv[h];
+          iv[h] = __builtin_amdgcn_exp2f(-lv[h]);
+        }
+        const bool more = key < last;
+        if (++step == 32) {
+          step = 0;
+          now = soon;
+        }
+        pg[0] = __builtin_amdgcn_readlane(now.page, 2 * step);
+        pg[1] = __builtin_amdgcn_readlane(now.page, 2 * step + 1);
+        scores([&]() { if (more) loadK(key + CA_UK, pg); });
+        const bool masked = key + 32 > first + 1 || (CA_WINDOW && key < first + tokens - CA_WINDOW) || zero[0] || zero[1];
+        weigh(key, there, zero, ks, lv, iv, masked, [&]() { if (more) loadV(key + CA_UK, pg); });
         if (!more) break;
-        loadV(key + CA_UK, pg);
         key += CA_UK;
       }
     }
 
-    // the four wavefronts' results, brought to one maximum and added through LDS
-#pragma unroll
-    for (int rb = 0; rb < CA_RB; ++rb) {
-      l[rb] = ca_cross(l[rb], false);
-      if (g == 0) {
-        ml[wave][rb * 16 + n][0] = m[rb];
-        ml[wave][rb * 16 + n][1] = l[rb];
-      }
-    }
-    __syncthreads();
+    // the wavefronts' results, added through LDS
 #if CA_WHOLE
     const bool whole = true;
     float* slot = nullptr;
 #else
     const bool whole = unit == 0 && until == units;
-    float* slot = part + ((long long)piece * 2 + (begun ? 0 : 1)) * CA_SLOT;
+    float* slot = part + CA_ENDS + ((long long)id * 2 + (begun ? 0 : 1)) * CA_SLOT;
     begun = false;
 #endif
 #pragma unroll
     for (int rb = 0; rb < CA_RB; ++rb) {
       const int at = rb * 16 + n;
-      const float top = fmaxf(fmaxf(ml[0][at][0], ml[1][at][0]), fmaxf(ml[2][at][0], ml[3][at][0]));
+      l[rb] = ca_cross(l[rb], false);
+      if (g == 0) {
+        ml[wave][at][0] = m[rb];
+        ml[wave][at][1] = l[rb];
+      }
+      if (CA_WAVES > 1) __syncthreads();           // (everybody has read the sums of the row block before, or V)
+#pragma unroll
+      for (int i = 0; i < CA_NT; ++i) sh.red[wave][i][lane] = acc[rb][i];
+      if (CA_WAVES > 1) __syncthreads();
+      float top = ml[0][at][0];
+#pragma unroll
+      for (int w = 1; w < CA_WAVES; ++w) top = fmaxf(top, ml[w][at][0]);
       const float ref = top == -__builtin_inff() ? 0.0f : top;
-      float sum = 0.0f;
+      float sum = 0.0f, f[CA_WAVES];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) sum = __builtin_fmaf(ml[w][at][1], __builtin_amdgcn_exp2f(ml[w][at][0] - ref), sum);
-      const float f = __builtin_amdgcn_exp2f(m[rb] - ref);
-      if (rb) __syncthreads();
+      for (int w = 0; w < CA_WAVES; ++w) {
+        f[w] = __builtin_amdgcn_exp2f(ml[w][at][0] - ref);
+        sum = __builtin_fmaf(ml[w][at][1], f[w], sum);
+      }
 #pragma unroll
-      for (int i = 0; i < CA_NT; ++i) red[wave][i][lane] = acc[rb][i] * f;
-      __syncthreads();
-      for (int i = wave; i < CA_NT; i += 4) {
-        const kcg_f32x4 o = (red[0][i][lane] + red[1][i][lane]) + (red[2][i][lane] + red[3][i][lane]);
+      for (int j = 0; j < (CA_NT + CA_WAVES - 1) / CA_WAVES; ++j) {
+        const int i = j * CA_WAVES + wave;
+        if (i >= CA_NT) break;
+        kcg_f32x4 o = sh.red[0][i][lane] * f[0];
+#pragma unroll
+        for (int w = 1; w < CA_WAVES; ++w) o += sh.red[w][i][lane] * f[w];
         if (whole)
-          ca_store(out, rq, hv, tile, rb, i, o, sum);
+          ca_store(out, rq.first + tok0, tokens, hv, rb, i, o, sum);
         else
           *(kcg_f32x4*)(slot + ((rb * CA_NT + i) * 64 + lane) * 4) = o;
       }
@@ -632,14 +712,11 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
     __syncthreads();
     left -= until - unit;
     unit = 0;
-    if (left > 0 && ++tile >= ca_tiles(rq)) {      // the next tile that there is: of a later request, or of the next head
+    if (left > 0 && ++tile >= ca_tiles(rq)) {      // the next tile that there is
       tile = 0;
-      while (true) {
-        if (++b >= requests) {
-          b = 0;
-          ++hv;
-        }
-        if (ca_request(lengths, starts, b, B, T, most).count > 0) break;
+      while (++b < requests) {
+        rq = ca_request(lengths, starts, b, B, T, most);
+        if (rq.count > 0) break;
       }
     }
 #endif

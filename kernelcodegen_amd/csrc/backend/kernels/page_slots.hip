@@ -9,8 +9,8 @@ struct PsSums { int pages[PS_BLOCK + 1], tokens[PS_BLOCK + 1], waves[2][PS_BLOCK
 
 extern "C" __global__ __launch_bounds__(PS_BLOCK)
 void PS_NAME(const int* __restrict__ lengths, const int* __restrict__ added, int* __restrict__ table, const int* __restrict__ free_pages,
-             long long* __restrict__ slots, int* __restrict__ positions, int* __restrict__ starts, int* __restrict__ lengths_out,
-             int* __restrict__ used, long long B_, long long T_, long long W_, long long table_row, long long F_, long long page_) {
+             long long B_, long long T_, long long W_, long long table_row, long long F_, long long page_, long long* __restrict__ slots,
+             int* __restrict__ positions, int* __restrict__ starts, int* __restrict__ lengths_out, int* __restrict__ used) {
   __shared__ PsSums s;
   const int B = (int)B_, T = (int)T_, W = (int)W_, F = (int)F_, page = (int)page_;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = blockIdx.x * PS_BLOCK + threadIdx.x, step = gridDim.x * PS_BLOCK;

@@ -15,6 +15,9 @@
 //   launch.result(shape, dtype)            a Launch whose call leaves the last pointer out: call(tensor, ..., number, ...)
 //                                          allocates it on the first tensor's device and returns it
 //   launch.result(None, None)              the result is like the first tensor
+//   launch.results((shape, dtype), ...)    a Launch whose call leaves the last pointers out and returns a tuple of their tensors
+//   signature(tensor or None, ...)         what a kernel can depend on of its operands, as bytes: device, type, sizes, strides and how
+//                                          far each address is from a multiple of 16
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -39,7 +42,8 @@ struct Launch {
   void* handle;
   uint32_t dims[7];
   int pointers, scalars;
-  int result;                     // 0: no result, 1: shape and dtype, 2: like the first tensor
+  int result;                     // 0: no result, 1: shape and dtype, 2: like the first tensor, 3: several
+  std::vector<std::pair<std::vector<int64_t>, at::ScalarType>>* several;
   std::vector<int64_t>* shape;
   at::ScalarType dtype;
   PyObject *fail, *keep;
@@ -74,7 +78,7 @@ PyObject* callLaunch(PyObject* me, PyObject* const* args, size_t nargsf, PyObjec
   HANDLE_TH_ERRORS
   Launch* self = (Launch*)me;
   const Py_ssize_t n = PyVectorcall_NARGS(nargsf);
-  const int given = self->pointers - (self->result ? 1 : 0);
+  const int given = self->pointers - (self->result == 3 ? (int)self->several->size() : self->result ? 1 : 0);
   if ((kwnames && PyTuple_GET_SIZE(kwnames)) || n != given + self->scalars) {
     PyErr_Format(PyExc_TypeError, "a launch of this kernel takes %d pointers and %d numbers", given, self->scalars);
     return nullptr;
@@ -105,6 +109,31 @@ PyObject* callLaunch(PyObject* me, PyObject* const* args, size_t nargsf, PyObjec
   if (!given || !THPVariable_Check(args[0])) {
     PyErr_SetString(PyExc_TypeError, "the first operand must be a tensor");
     return nullptr;
+  }
+  if (self->result == 3) {
+    std::vector<at::Tensor> outs;
+    outs.reserve(self->several->size());
+    {
+      const auto options = THPVariable_Unpack(args[0]).options().requires_grad(false);
+      pybind11::gil_scoped_release unlocked;
+      for (const auto& [shape, dtype] : *self->several) {
+        outs.push_back(at::empty(shape, options.dtype(dtype)));
+        slots[given + outs.size() - 1] = (uint64_t)(uintptr_t)outs.back().data_ptr();
+      }
+      rc = launch(self, slots);
+    }
+    if (rc) return failed(self, rc);
+    PyObject* tuple = PyTuple_New((Py_ssize_t)outs.size());
+    if (!tuple) return nullptr;
+    for (size_t i = 0; i < outs.size(); ++i) {
+      PyObject* o = THPVariable_Wrap(outs[i]);
+      if (!o) {
+        Py_DECREF(tuple);
+        return nullptr;
+      }
+      PyTuple_SET_ITEM(tuple, (Py_ssize_t)i, o);
+    }
+    return tuple;
   }
   at::Tensor out;
   {
@@ -146,6 +175,7 @@ PyObject* newLaunch(PyTypeObject* type, PyObject* args, PyObject* kwargs) {
   self->scalars = scalars;
   self->result = 0;
   self->shape = nullptr;
+  self->several = nullptr;
   Py_INCREF(fail);
   self->fail = fail;
   Py_INCREF(keep);
@@ -154,29 +184,28 @@ PyObject* newLaunch(PyTypeObject* type, PyObject* args, PyObject* kwargs) {
   END_HANDLE_TH_ERRORS
 }
 
-PyObject* withResult(PyObject* me, PyObject* args) {
-  HANDLE_TH_ERRORS
-  Launch* self = (Launch*)me;
-  PyObject *shape, *dtype;
-  if (!PyArg_ParseTuple(args, "OO", &shape, &dtype)) return nullptr;
-  std::vector<int64_t> sizes;
-  if (shape != Py_None) {
-    PyObject* seq = PySequence_Fast(shape, "the shape is a sequence of whole numbers");
-    if (!seq) return nullptr;
-    for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq); ++i) {
-      const long long v = PyLong_AsLongLong(PySequence_Fast_GET_ITEM(seq, i));
-      if (v == -1 && PyErr_Occurred()) {
-        Py_DECREF(seq);
-        return nullptr;
-      }
-      sizes.push_back(v);
+// The sizes and type of a result; false with an error set.
+bool shapeOf(PyObject* shape, PyObject* dtype, std::vector<int64_t>& sizes) {
+  PyObject* seq = PySequence_Fast(shape, "the shape is a sequence of whole numbers");
+  if (!seq) return false;
+  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq); ++i) {
+    const long long v = PyLong_AsLongLong(PySequence_Fast_GET_ITEM(seq, i));
+    if (v == -1 && PyErr_Occurred()) {
+      Py_DECREF(seq);
+      return false;
     }
-    Py_DECREF(seq);
-    if (!THPDtype_Check(dtype)) {
-      PyErr_SetString(PyExc_TypeError, "a shape needs a torch dtype");
-      return nullptr;
-    }
+    sizes.push_back(v);
   }
+  Py_DECREF(seq);
+  if (!THPDtype_Check(dtype)) {
+    PyErr_SetString(PyExc_TypeError, "a shape needs a torch dtype");
+    return false;
+  }
+  return true;
+}
+
+// A Launch of the same kernel; what it gives is set by the caller.
+Launch* again(Launch* self) {
   Launch* made = (Launch*)LaunchType.tp_alloc(&LaunchType, 0);
   if (!made) return nullptr;
   made->call = callLaunch;
@@ -185,31 +214,102 @@ PyObject* withResult(PyObject* me, PyObject* args) {
   memcpy(made->dims, self->dims, sizeof made->dims);
   made->pointers = self->pointers;
   made->scalars = self->scalars;
-  made->result = shape == Py_None ? 2 : 1;
+  made->result = 0;
   made->shape = nullptr;
-  if (shape != Py_None) {
-    made->shape = new std::vector<int64_t>(std::move(sizes));
-    made->dtype = ((THPDtype*)dtype)->scalar_type;
-  }
+  made->several = nullptr;
   Py_INCREF(self->fail);
   made->fail = self->fail;
   Py_INCREF(self->keep);
   made->keep = self->keep;
+  return made;
+}
+
+PyObject* withResult(PyObject* me, PyObject* args) {
+  HANDLE_TH_ERRORS
+  PyObject *shape, *dtype;
+  if (!PyArg_ParseTuple(args, "OO", &shape, &dtype)) return nullptr;
+  std::vector<int64_t> sizes;
+  if (shape != Py_None && !shapeOf(shape, dtype, sizes)) return nullptr;
+  Launch* made = again((Launch*)me);
+  if (!made) return nullptr;
+  made->result = shape == Py_None ? 2 : 1;
+  if (shape != Py_None) {
+    made->shape = new std::vector<int64_t>(std::move(sizes));
+    made->dtype = ((THPDtype*)dtype)->scalar_type;
+  }
   return (PyObject*)made;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* withResults(PyObject* me, PyObject* args) {
+  HANDLE_TH_ERRORS
+  std::vector<std::pair<std::vector<int64_t>, at::ScalarType>> several;
+  for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(args); ++i) {
+    PyObject *shape, *dtype;
+    if (!PyArg_ParseTuple(PyTuple_GET_ITEM(args, i), "OO", &shape, &dtype)) return nullptr;
+    several.emplace_back();
+    if (!shapeOf(shape, dtype, several.back().first)) return nullptr;
+    several.back().second = ((THPDtype*)dtype)->scalar_type;
+  }
+  if (several.empty() || (int)several.size() >= ((Launch*)me)->pointers) {
+    PyErr_SetString(PyExc_ValueError, "results: one or more, and fewer than the kernel has pointers");
+    return nullptr;
+  }
+  Launch* made = again((Launch*)me);
+  if (!made) return nullptr;
+  made->result = 3;
+  made->several = new std::vector<std::pair<std::vector<int64_t>, at::ScalarType>>(std::move(several));
+  return (PyObject*)made;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* signature(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  // (a tensor of d dimensions takes 2 d + 2 numbers of 8 bytes)
+  int64_t out[256];
+  size_t at = 0;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    if (args[i] == Py_None) {
+      if (at + 1 > 256) break;
+      out[at++] = -1;
+      continue;
+    }
+    if (!THPVariable_Check(args[i])) {
+      PyErr_SetString(PyExc_TypeError, "operands must be tensors");
+      return nullptr;
+    }
+    const at::Tensor& t = THPVariable_Unpack(args[i]);
+    const int64_t d = t.dim();
+    if (at + 2 * d + 2 > 256) {
+      PyErr_SetString(PyExc_ValueError, "too many dimensions");
+      return nullptr;
+    }
+    const auto device = t.device();
+    out[at++] = d | (int64_t)t.scalar_type() << 8 | (int64_t)device.type() << 16 | (int64_t)(uint8_t)device.index() << 24 |
+                (int64_t)t.layout() << 32;
+    for (int64_t j = 0; j < d; ++j) out[at++] = t.size(j);
+    for (int64_t j = 0; j < d; ++j) out[at++] = t.stride(j);
+    out[at++] = (int64_t)((uintptr_t)t.data_ptr() & 15);
+  }
+  return PyBytes_FromStringAndSize((const char*)out, (Py_ssize_t)(at * sizeof out[0]));
   END_HANDLE_TH_ERRORS
 }
 
 void freeLaunch(PyObject* me) {
   Launch* self = (Launch*)me;
   delete self->shape;
+  delete self->several;
   Py_XDECREF(self->fail);
   Py_XDECREF(self->keep);
   Py_TYPE(me)->tp_free(me);
 }
 
 PyMethodDef methods[] = {{"result", withResult, METH_VARARGS, "result(shape, dtype): a Launch that allocates and returns its last pointer's tensor"},
+                         {"results", withResults, METH_VARARGS, "results((shape, dtype), ...): a Launch that allocates and returns its last pointers' tensors"},
                          {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", "bound kernel launches on torch tensors", -1, nullptr};
+PyMethodDef functions[] = {{"signature", (PyCFunction)(void (*)(void))signature, METH_FASTCALL, "what a kernel can depend on of its operands"},
+                           {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", "bound kernel launches on torch tensors", -1, functions};
 
 }  // namespace
 

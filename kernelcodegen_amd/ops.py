@@ -317,28 +317,21 @@ def softmax(x, inplace=False):
 
 # ---- a decoding step: pages, the cache in 8 bits, attention over it, weights of 4 bits ----
 
-def _bound_kernel(key, family, grid, **params):
-    """The bound launch of a kernel whose grid goes by the call, kept under `key`."""
-    run = R.get_kernel(family, **params).bind(grid=grid)
-    _bound[key] = run
-    return run
-
-
-def _into_last(run, shape, dtype):
-    """_into for a kernel whose other arguments are pointers and whole numbers in any order: its result is the last one."""
-    native = getattr(run, "result", None)
-    if native is not None:
-        return native(shape, dtype)
+def _into_last(run, *results):
+    """_into for a kernel whose other arguments are pointers and whole numbers in any order: its results, each a (shape, dtype), are the last
+    ones; several are given as a tuple."""
+    if hasattr(run, "results"):
+        return run.result(*results[0]) if len(results) == 1 else run.results(*results)
 
     def call(*operands):
-        out = torch.empty(shape, dtype=dtype, device=operands[0].device)
-        run(*[t.data_ptr() if isinstance(t, torch.Tensor) else t for t in operands], out.data_ptr())
-        return out
+        device = operands[0].device
+        outs = tuple([torch.empty(shape, dtype=dtype, device=device) for shape, dtype in results])
+        run(*[t.data_ptr() if isinstance(t, torch.Tensor) else t for t in operands], *[t.data_ptr() for t in outs])
+        return outs if len(outs) > 1 else outs[0]
     return call
 
 
 def _on_device(*ts):
-    """What every call looks at: a bound launch hands on addresses, whatever they are of."""
     for t in ts:
         if not t.is_cuda:
             raise ValueError("operands must be device tensors")
@@ -359,6 +352,14 @@ def page_slots(lengths, added, table, free, page_size, tokens):
     [B], number of pages taken int32 [1]): slot = page * page_size + place in the page, what cache_write takes; -1 for padding and for
     tokens that have no page, because `free` or the table is too short.  starts and the new lengths are what cache_attention takes."""
     page_size, tokens = operator.index(page_size), operator.index(tokens)
+    key = ("page_slots", R.signature(lengths, added, table, free), page_size, tokens)
+    run = _bound.get(key)
+    if run is None:
+        _bound[key] = run = _page_slots_launch(lengths, added, table, free, page_size, tokens)
+    return run(lengths, added, table, free, table.shape[0], tokens, table.shape[1], table.stride(0), free.shape[0], page_size)
+
+
+def _page_slots_launch(lengths, added, table, free, page_size, tokens):
     _vectors(torch.int32, lengths, added, free)
     if lengths.dim() != 1 or lengths.shape != added.shape or free.dim() != 1 or table.dim() != 2 or table.shape[0] != lengths.shape[0]:
         raise ValueError("lengths and added are [B], table is [B, W], free is [F]")
@@ -366,18 +367,12 @@ def page_slots(lengths, added, table, free, page_size, tokens):
         raise ValueError("the table must be an int32 device tensor with rows of neighbouring entries")
     if page_size < 1 or tokens < 0 or tokens > 0x7FFFFFFF:
         raise ValueError("bad page size or number of tokens")
-    batch, width = table.shape
-    device = lengths.device
-    slots = torch.empty(tokens, dtype=torch.int64, device=device)
-    positions, rest = torch.empty(tokens, dtype=torch.int32, device=device), torch.empty(2 * batch + 2, dtype=torch.int32, device=device)
-    starts, lengths_out, used = rest[:batch + 1], rest[batch + 1:2 * batch + 1], rest[2 * batch + 1:]
+    batch = table.shape[0]
     # two tokens a lane, as far as that needs no more workgroups than the part has CUs
-    grid = max(1, min(256, -(-tokens // 2048)))
-    key = ("page_slots", batch > 256 or tokens > 512, grid)
-    run = _bound.get(key) or _bound_kernel(key, "page_slots", (grid,), BLOCK=1024 if key[1] else 256)
-    run(lengths.data_ptr(), added.data_ptr(), table.data_ptr(), free.data_ptr(), slots.data_ptr(), positions.data_ptr(), starts.data_ptr(),
-        lengths_out.data_ptr(), used.data_ptr(), batch, tokens, width, table.stride(0), free.numel(), page_size)
-    return slots, positions, starts, lengths_out, used
+    kern = R.get_kernel("page_slots", BLOCK=1024 if batch > 256 or tokens > 512 else 256)
+    i32 = torch.int32
+    return _into_last(kern.bind(grid=(max(1, min(256, -(-tokens // 2048))),)), ((tokens,), torch.int64), ((tokens,), i32), ((batch + 1,), i32), ((batch,), i32),
+                      ((1,), i32))
 
 
 def _cache_strides(cache, scale):
@@ -413,52 +408,54 @@ def cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots):
     left out.  The tokens of a page stand together and in order, as page_slots gives them.  A page's scale is the least power of two by
     which its rows fit the format; where a page has earlier rows, these are converted when the scale has to grow.  A page whose
     first row is written is taken to be new.  Infinities become the largest numbers that the scale allows."""
-    if tuple(k.shape) != tuple(v.shape) or k.dtype != v.dtype or k_cache.shape != v_cache.shape:
-        raise ValueError("keys and values, and their caches, must have one shape and type")
-    if k.dim() == 3 and k.shape[0] == 0:
-        return
+    key = ("cache_write", R.signature(k, v, k_cache, v_cache, k_scale, v_scale, slots))
+    run = _bound.get(key)
+    if run is None:
+        _bound[key] = run = _cache_write_launch(k, v, k_cache, v_cache, k_scale, v_scale, slots)
+    tokens = slots.shape[0]
+    if tokens:
+        run(k, v, k_cache, v_cache, k_scale, v_scale, slots, tokens, k_cache.shape[0])
+
+
+def _cache_write_launch(k, v, k_cache, v_cache, k_scale, v_scale, slots):
     _on_device(k, v, k_cache, v_cache)
     _vectors(torch.int64, slots)
     _vectors(torch.float32, k_scale, v_scale)
-    tokens = slots.numel()
-    key = ("cache_write", tokens, k.shape, k.dtype, k.stride(), v.stride(), k_cache.shape, k_cache.stride(), v_cache.stride(), k_cache.dtype, v_cache.dtype,
-           k_scale.shape, v_scale.shape, (k.data_ptr() | v.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15)
-    run = _bound.get(key)
-    if run is None:
-        ks, vs = _cache_strides(k_cache, k_scale), _cache_strides(v_cache, v_scale)
-        xk, xv = _row_strides(k, k_cache, _STORAGE), _row_strides(v, v_cache, _STORAGE)
-        if k.shape[1] != k_cache.shape[2] or tokens != k.shape[0] or tokens > 0x7FFFFFFF:
-            raise ValueError("one slot per token, and the cache's heads, are needed")
-        heads = k.shape[1]
-        win = 1 if tokens <= 512 else 16
-        jobs = 2 * heads * -(-tokens // win)
-        run = _bound_kernel(key, "cache_write", (-(-jobs // 4),), H=heads, D=k.shape[2], PAGE=k_cache.shape[1], F16=_STORAGE[k.dtype], WIN=win,
-                            KP=ks[0], KT=ks[1], KH=ks[2], VP=vs[0], VT=vs[1], VH=vs[2], XKT=xk[0], XKH=xk[1], XVT=xv[0], XVH=xv[1])
-    run(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slots.data_ptr(), tokens,
-        k_cache.shape[0])
+    if k.shape != v.shape or k.dtype != v.dtype or k_cache.shape != v_cache.shape:
+        raise ValueError("keys and values, and their caches, must have one shape and type")
+    ks, vs = _cache_strides(k_cache, k_scale), _cache_strides(v_cache, v_scale)
+    xk, xv = _row_strides(k, k_cache, _STORAGE), _row_strides(v, v_cache, _STORAGE)
+    tokens, heads, d = k.shape
+    if heads != k_cache.shape[2] or tuple(slots.shape) != (tokens,) or tokens > 0x7FFFFFFF:
+        raise ValueError("one slot per token, and the cache's heads, are needed")
+    win = 1 if tokens <= 512 else 16
+    kern = R.get_kernel("cache_write", H=heads, D=d, PAGE=k_cache.shape[1], F16=_STORAGE[k.dtype], WIN=win, KP=ks[0], KT=ks[1], KH=ks[2],
+                        VP=vs[0], VT=vs[1], VH=vs[2], XKT=xk[0], XKH=xk[1], XVT=xv[0], XVH=xv[1])
+    run = kern.bind(grid=(max(1, -(-2 * heads * -(-tokens // win) // 4)),))
+    return run if hasattr(run, "results") else lambda *a: run(*[x.data_ptr() if isinstance(x, torch.Tensor) else x for x in a])
 
 
 def cache_read(cache, scale, slots, dtype=torch.bfloat16):
     """Rows of a paged cache in 8 bits: [tokens, heads, d] in fp32, IEEE half or bfloat16 for slots int64 [tokens]; zeros for a slot that is
     none of the cache's (-1)."""
+    key = ("cache_read", R.signature(cache, scale, slots), dtype)
+    run = _bound.get(key)
+    if run is None:
+        _bound[key] = run = _cache_read_launch(cache, scale, slots, dtype)
+    return run(cache, scale, slots, slots.shape[0], cache.shape[0])
+
+
+def _cache_read_launch(cache, scale, slots, dtype):
     _on_device(cache)
     _vectors(torch.int64, slots)
     _vectors(torch.float32, scale)
     if dtype not in _STORAGE or slots.dim() != 1:
         raise ValueError("rows are given in fp32, IEEE half or bfloat16, for slots [tokens]")
-    tokens = slots.numel()
-    key = ("cache_read", tokens, cache.shape, cache.stride(), cache.dtype, scale.shape, dtype, cache.data_ptr() & 15)
-    hit = _bound.get(key)
-    if hit is None:
-        s = _cache_strides(cache, scale)
-        pages, page, heads, d = cache.shape
-        if tokens == 0:
-            return torch.empty((0, heads, d), dtype=dtype, device=cache.device)
-        units, unroll = tokens * heads * d // 8, 1
-        hit = _into_last(R.get_kernel("cache_read", H=heads, D=d, PAGE=page, F16=_STORAGE[dtype], KP=s[0], KT=s[1], KH=s[2], UNROLL=unroll)
-                    .bind(grid=(-(-units // (256 * unroll)),)), (tokens, heads, d), dtype)
-        _bound[key] = hit
-    return hit(cache, scale, slots, tokens, cache.shape[0])
+    s = _cache_strides(cache, scale)
+    page, heads, d = cache.shape[1:]
+    tokens = slots.shape[0]
+    kern = R.get_kernel("cache_read", H=heads, D=d, PAGE=page, F16=_STORAGE[dtype], KP=s[0], KT=s[1], KH=s[2], UNROLL=1)
+    return _into_last(kern.bind(grid=(max(1, -(-tokens * heads * d // 2048)),)), ((tokens, heads, d), dtype))
 
 
 def cache_attention(q, k_cache, v_cache, k_scale, v_scale, table, lengths, starts=None, scale=None, cap=None, window=None, slopes=None):
@@ -471,40 +468,32 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, table, lengths, start
       score = scale * q.k (scale: d^-0.5), then cap * tanh(score / cap), then + slopes[head] * (key's position - row's), slopes fp32
       [heads]; a row sees the keys up to its own position, of these the last `window`.
     Entries of the table behind a request's length are not read; keys on pages that are not the cache's count as not there."""
-    _on_device(q, k_cache, v_cache, table)
-    _vectors(torch.float32, k_scale, v_scale)
-    _vectors(torch.int32, lengths)
-    if starts is not None:
-        _vectors(torch.int32, starts)
-    if slopes is not None:
-        _vectors(torch.float32, slopes)
-    if q.dim() == 3 and q.shape[0] == 0:
-        return torch.empty_like(q)
     scale, cap, window = None if scale is None else float(scale), float(cap or 0.0), operator.index(window or 0)
-    key = ("cache_attention", q.shape, q.dtype, q.stride(), k_cache.shape, k_cache.stride(), v_cache.shape, v_cache.stride(), k_cache.dtype, v_cache.dtype,
-           k_scale.shape, v_scale.shape, table.shape, table.dtype, table.stride(), lengths.shape, None if starts is None else starts.shape,
-           None if slopes is None else slopes.shape, scale, cap, window,
-           (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15)
+    key = ("cache_attention", R.signature(q, k_cache, v_cache, k_scale, v_scale, table, lengths, starts, slopes), scale, cap, window)
     hit = _bound.get(key)
     if hit is None:
-        hit = _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, lengths, starts, scale, cap, window, slopes)
-        _bound[key] = hit
+        _bound[key] = hit = _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, lengths, starts, scale, cap, window, slopes)
     run, join, floats = hit
-    tokens, batch, width = q.shape[0], table.shape[0], table.shape[1]
-    first = 0 if starts is None else starts.data_ptr()
-    part = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-    at = part.data_ptr() if floats else 0
-    out = run(q, k_cache, v_cache, k_scale, v_scale, table, lengths, first, 0 if slopes is None else slopes.data_ptr(), at, tokens, batch, width,
-              table.stride(0), k_cache.shape[0])
+    if not q.shape[0]:
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
+    batch, width = table.shape
+    part = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else 0
+    out = run(q, k_cache, v_cache, k_scale, v_scale, table, lengths, 0 if starts is None else starts, 0 if slopes is None else slopes, part, q.shape[0], batch,
+              width, table.stride(0), k_cache.shape[0])
     if join is not None:
-        join(at, lengths.data_ptr(), first, tokens, batch, width, out.data_ptr())
+        join(part.data_ptr(), out.data_ptr())
     return out
 
 
 def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, lengths, starts, scale, cap, window, slopes):
+    _on_device(q, k_cache, v_cache, table)
+    _vectors(torch.float32, k_scale, v_scale, *(() if slopes is None else (slopes,)))
+    _vectors(torch.int32, lengths, *(() if starts is None else (starts,)))
     ks, vs = _cache_strides(k_cache, k_scale), _cache_strides(v_cache, v_scale)
     if k_cache.shape != v_cache.shape:
         raise ValueError("the caches of keys and values must have one shape")
+    if max(ks[1], vs[1]) >= 1 << 27:
+        raise ValueError("neighbouring tokens of a page must lie less than 2^27 bytes apart")
     qs = _row_strides(q, k_cache, (torch.float16, torch.bfloat16))
     tokens, heads, d = q.shape
     page, kv_heads = k_cache.shape[1:3]
@@ -522,13 +511,13 @@ def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, length
     if slopes is not None and tuple(slopes.shape) != (heads,):
         raise ValueError("slopes is [heads]")
     group = heads // kv_heads
-    # the kernel counts pieces of 128 keys of all tiles of 16 rows and more in 32 bits
-    if (tokens * min(group, 64) // 16 + batch + 1) * (width * page // 128 + 2) >= 1 << 31:
+    # the kernel counts pieces of 32 keys and more of all tiles of 16 rows and more in 32 bits
+    if (tokens * min(group, 64) // 16 + batch + 1) * (width * page // 32 + 2) >= 1 << 31:
         raise ValueError("too many rows times keys for one launch")
     if not 0.0 <= cap < math.inf or window < 0:
         raise ValueError("cap and window must not be negative")
     # rows that the average request has of a kv head
-    rows = group * -(-tokens // batch)
+    rows = group * max(1, -(-tokens // batch))
     blocks = 1 if rows <= 16 else 2 if rows <= 32 or d > 128 else 4
     whole = starts is None and width * page <= 512
     params = dict(H=kv_heads, D=d, PAGE=page, G=group, F16=int(q.dtype == torch.float16), RB=blocks, STARTS=int(starts is not None), CAP=cap, WINDOW=window,
@@ -537,11 +526,13 @@ def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, length
     if whole:
         parts = -(-group // (16 * blocks))
         kern = R.get_kernel("cache_attention", WHOLE=1, **params)
-        return _into_last(kern.bind(grid=(batch * kv_heads * parts,)), tuple(q.shape), q.dtype), None, 0
-    grid = 256 if blocks == 4 else 512 if blocks == 2 else 768
-    kern, join = R.get_kernel("cache_attention", GRID=grid, **params), R.get_kernel("cache_join", GRID=grid, **params)
-    floats = 2 * grid * (16 * blocks * d + 32 * blocks)
-    return _into_last(kern.bind(), tuple(q.shape), q.dtype), join.bind(), floats
+        return _into_last(kern.bind(grid=(batch * kv_heads * parts,)), (tuple(q.shape), q.dtype)), None, 0
+    grid = 256 if blocks == 4 or (blocks == 2 and d > 128) else 512
+    kern = R.get_kernel("cache_attention", GRID=grid, **params)
+    shares, alone = kern.info["grid"][0], kern.info["grid"][0] == kv_heads * -(-group // (16 * blocks))
+    # for each share four whole numbers, and two parts of a tile: its sums, and maximum and sum of the probabilities of each row
+    floats = shares * (4 + 2 * (16 * blocks * d + 32 * blocks))
+    return _into_last(kern.bind(), (tuple(q.shape), q.dtype)), None if alone else R.get_kernel("cache_join", GRID=grid, **params).bind(), floats
 
 
 def matmul_q4(x, w, scale, zero=None, out_dtype=None, **cfg):
@@ -550,12 +541,7 @@ def matmul_q4(x, w, scale, zero=None, out_dtype=None, **cfg):
     x: [..., K], IEEE half or bfloat16; w: uint8 [N, K / 2], the code of an even k in the low four bits; scale: [N, K / group], fp32 or x's
     type, group 32, 64 or a multiple of 128; zero: uint8 [N, K / group], None for 8.  Codes and x enter the sums unrounded, the sums are fp32; the
     result has x's type (default) or is fp32.  For the few rows of a decoding step: the weights are read once for each 64 rows."""
-    dims = x.shape
-    _need_cuda(x, w, scale)
-    if zero is not None:
-        _need_cuda(zero)
-    key = ("matmul_q4", dims, x.dtype, w.shape, w.dtype, scale.shape, scale.dtype, None if zero is None else (zero.shape, zero.dtype), out_dtype,
-           (x.data_ptr() | w.data_ptr()) & 15)
+    key = ("matmul_q4", R.signature(x, w, scale, zero), out_dtype)
     hit = None if cfg else _bound.get(key)
     if hit is None:
         hit = _matmul_q4_launch(x, w, scale, zero, out_dtype, cfg)
@@ -563,11 +549,12 @@ def matmul_q4(x, w, scale, zero=None, out_dtype=None, **cfg):
             _bound[key] = hit
     run, rows = hit
     if rows == 0:
-        return torch.empty(dims[:-1] + (w.shape[0],), dtype=out_dtype or x.dtype, device=x.device)
-    return run(x, w, scale, 0 if zero is None else zero.data_ptr(), rows)
+        return torch.empty(x.shape[:-1] + (w.shape[0],), dtype=out_dtype or x.dtype, device=x.device)
+    return run(x, w, scale, 0 if zero is None else zero, rows)
 
 
 def _matmul_q4_launch(x, w, scale, zero, out_dtype, cfg):
+    _need_cuda(x, w, scale, *(() if zero is None else (zero,)))
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if x.dtype not in (torch.float16, torch.bfloat16) or out_dtype not in (x.dtype, torch.float32) or scale.dtype not in (x.dtype, torch.float32):
         raise ValueError("x is IEEE half or bfloat16, result and scales have x's type or are fp32")
@@ -589,4 +576,4 @@ def _matmul_q4_launch(x, w, scale, zero, out_dtype, cfg):
         return None, 0
     kern = R.get_kernel("gemm_q4", N=n, K=k, GROUP=group, F16=int(x.dtype == torch.float16), ZERO=int(zero is not None),
                         SCALE_F32=int(scale.dtype == torch.float32), OUT_F32=int(out_dtype == torch.float32), MB=blocks, **cfg)
-    return _into_last(kern.bind(grid=(kern.info["grid"][0], -(-rows // (16 * blocks)))), tuple(x.shape[:-1]) + (n,), out_dtype), rows
+    return _into_last(kern.bind(grid=(kern.info["grid"][0], -(-rows // (16 * blocks)))), (tuple(x.shape[:-1]) + (n,), out_dtype)), rows

@@ -2,6 +2,7 @@
 pick up a code object built ahead of time), load it, launch it on torch's
 current stream.  torch supplies device memory and the stream handle only."""
 import ctypes as C
+import importlib
 import os
 import struct
 
@@ -166,6 +167,18 @@ def _native_launch():
             warnings.warn("the native launches are not used, ctypes takes their place: " + why, RuntimeWarning)
         _launch_type = found
     return _launch_type or None
+
+
+def _plain_signature(*tensors):
+    return tuple([None if t is None else (t.device, t.dtype, t.layout, t.shape, t.stride(), t.data_ptr() & 15) for t in tensors])
+
+
+def signature(*tensors):
+    """What a kernel can depend on of its operands (tensors, or None): device, type, sizes, strides, and how far each address is from a
+    multiple of 16.  The key under which a bound launch is kept: whoever has it need not look at the operands again."""
+    global signature
+    signature = importlib.import_module(__package__ + "._launch").signature if _native_launch() else _plain_signature
+    return signature(*tensors)
 
 
 class Kernel:

@@ -21,7 +21,7 @@ def attention(d, **more):
 
 WRITE = dict(F16=2, WIN=1, XKT=256, XKH=128, XVT=256, XVH=128)
 GOOD = [("page_slots", dict(), 15), ("cache_write", dict(cache(128), **WRITE), 9), ("cache_write", dict(cache(96), **{**WRITE, "F16": 0, "WIN": 16}), 9),
-        ("cache_read", dict(cache(64), F16=0), 6), ("cache_join", attention(128), 7), ("cache_join", attention(256, RB=2, STARTS=1, WINDOW=100), 7),
+        ("cache_read", dict(cache(64), F16=0), 6), ("cache_join", attention(128), 2), ("cache_join", attention(256, RB=2, STARTS=1, WINDOW=100), 2),
         ("gemm_q4", dict(N=100, K=4096, GROUP=128, F16=0, MB=1), 6), ("gemm_q4", dict(N=4096, K=1088, GROUP=64, F16=1, MB=4, ZERO=1, SCALE_F32=1, OUT_F32=1), 6)]
 GOOD += [("cache_attention", attention(d, RB=rb, F16=d // 32 % 2), 16) for d in (32, 64, 96, 128) for rb in (1, 2, 4)]
 GOOD += [("cache_attention", attention(d, RB=rb), 16) for d in (160, 192, 224, 256) for rb in (1, 2)]
@@ -39,8 +39,8 @@ def test_every_form_compiles_for_gfx950(family, params, nargs):
     ("page_slots", dict(BLOCK=100)), ("cache_read", dict(cache(48), F16=0)), ("cache_read", dict(cache(288), F16=0)), ("cache_read", dict(cache(64, page=8), F16=0)),
     ("cache_read", dict(cache(64, page=48), F16=0)), ("cache_read", dict(cache(64), F16=3)), ("cache_read", dict(cache(64))), ("cache_read", dict(cache(64), F16=0, KT=8)),
     ("cache_read", dict(cache(64), F16=0, KP=-16)), ("cache_write", dict(cache(128), **{**WRITE, "WIN": 65})), ("cache_write", dict(cache(128), **{**WRITE, "XKT": 4})),
-    ("cache_attention", attention(128, RB=3)), ("cache_attention", attention(256, RB=4)), ("cache_attention", attention(128, G=0)), ("cache_attention", attention(128, QT=4)),
-    ("cache_attention", attention(128, GRID=100)), ("cache_attention", attention(128, CAP=-1.0)), ("cache_attention", attention(128, CAP=float("nan"))),
+    ("cache_attention", attention(128, RB=3)), ("cache_attention", attention(256, RB=4)), ("cache_attention", attention(128, G=0)), ("cache_attention", attention(128, QT=4)), ("cache_attention", attention(128, KT=1 << 27)),
+    ("cache_attention", attention(128, GRID=0)), ("cache_attention", attention(128, CAP=-1.0)), ("cache_attention", attention(128, CAP=float("nan"))),
     ("cache_attention", attention(128, SCALE=float("inf"))), ("cache_attention", attention(128, WINDOW=-1)), ("cache_attention", attention(128, WHOLE=1, STARTS=1)),
     ("cache_join", attention(128, WHOLE=1)), ("cache_attention", attention(128, F16=2)),
     ("gemm_q4", dict(N=100, K=100, GROUP=50, F16=0, MB=1)), ("gemm_q4", dict(N=100, K=192, GROUP=128, F16=0, MB=1)), ("gemm_q4", dict(N=100, K=192, GROUP=96, F16=0, MB=1)),
@@ -100,12 +100,12 @@ int main() {
 
 
 @pytest.mark.parametrize("window", [0, 1, 100, 1000])
-@pytest.mark.parametrize("rows", [1, 4, 12, 64])
-def test_units_of_tiles_in_closed_form(tmp_path, window, rows):
+@pytest.mark.parametrize("rows,keys", [(1, 128), (4, 32), (4, 64), (12, 128), (64, 128), (64, 32)])
+def test_units_of_tiles_in_closed_form(tmp_path, window, rows, keys):
     text = open(os.path.join(ROOT, "kernelcodegen_amd", "csrc", "backend", "kernels", "cache_attention.hip")).read()
     part = text[text.index("struct CaRequest"):text.index("// Request b; b == B")] + text[text.index("// sum of the whole parts"):text.index("// Sum over the lanes up to")]
     source = tmp_path / "units.cc"
-    source.write_text("#define CA_WINDOW %d\n#define CA_TOK %d\n#define CA_UK 128\n" % (window, rows) + HARNESS % part)
+    source.write_text("#define CA_WINDOW %d\n#define CA_TOK %d\n#define CA_UK %d\n" % (window, rows, keys) + HARNESS % part)
     exe = str(tmp_path / "units")
     subprocess.run(["g++", "-O1", "-o", exe, str(source)], check=True)
     done = subprocess.run([exe], capture_output=True, text=True)
