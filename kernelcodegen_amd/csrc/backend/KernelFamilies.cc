@@ -1698,12 +1698,10 @@ bool emitCacheRead(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std:
 // cache_attention, and cache_join, which adds up what its workgroups leave of tiles that they share: the same parameters.
 bool emitCacheAttention(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::string& err) {
   if (!cacheShape(s, {"KP", "KT", "KH", "VP", "VT", "VH"}, err)) return false;
-  if (!whole(s, "G", 1, 65536, err) || !whole(s, "RB", 1, 4, err) || !whole(s, "F16", 0, 1, err)) return false;
+  if (!whole(s, "G", 1, 65536, err) || !whole(s, "RB", 1, 2, err) || !whole(s, "F16", 0, 1, err)) return false;
   const int64_t rb = s.p["RB"], dh = s.p["D"], g = s.p["G"];
   for (auto key : {"KT", "VT"})
     if (s.p[key] >= (int64_t)1 << 27) { err = std::string("cache_attention: ") + key + " must be below 2^27 (16 tokens lie within 32 bits)"; return false; }
-  if (!powerOfTwo(rb)) { err = "cache_attention: RB must be 1, 2 or 4"; return false; }
-  if (rb == 4 && dh > 128) { err = "cache_attention: 64 rows of more than 128 do not fit the registers"; return false; }
   for (auto key : {"QT", "QH"})
     if (!whole(s, key, 0, (int64_t)1 << 40, err)) return false;
     else if (s.p[key] % 8) { err = std::string("cache_attention: ") + key + " must be a multiple of 16 bytes"; return false; }
@@ -1711,31 +1709,33 @@ bool emitCacheAttention(KernelSpec& s, std::string& src, KernelLaunchInfo& info,
   const int64_t window = s.get("WINDOW", 0), grid = s.get("GRID", 512), least = s.get("LEAST", 2);
   if (window < 0 || window > 0x7FFFFFFF) { err = "cache_attention: WINDOW must be in [0,2^31)"; return false; }
   if (grid < 1 || grid > 65536) { err = "cache_attention: GRID must be in [1,65536]"; return false; }
-  const int64_t waves = s.get("WAVES", 4);
-  if (waves != 1 && waves != 2 && waves != 4) { err = "cache_attention: WAVES must be 1, 2 or 4"; return false; }
   if (least < 1) { err = "cache_attention: LEAST must be positive"; return false; }
   if (wholeTiles && (starts || join)) { err = "cache_attention: whole tiles are for one row per request, and need no join"; return false; }
   const double cap = s.f.count("CAP") ? s.f["CAP"] : 0.0, scale = s.f.count("SCALE") ? s.f["SCALE"] : 1.0;
   if (!(cap >= 0.0) || !std::isfinite(cap) || !std::isfinite(scale)) { err = "cache_attention: CAP must not be negative, CAP and SCALE must be finite"; return false; }
-  const int64_t rows = 16 * rb, gs = std::min(g, rows);
+  const int64_t waves = s.get("WAVES", 4);
+  if (waves != 1 && waves != 2 && waves != 4) { err = "cache_attention: WAVES must be 1, 2 or 4"; return false; }
+  const bool share = s.get("SHARE", 0) != 0;
+  if (share && wholeTiles) { err = "cache_attention: whole tiles are for one row per request"; return false; }
+  const int64_t blocks = share ? rb * waves : rb, rows = 16 * blocks, gs = std::min(g, rows);
   // shares that a head's work is cut into, of about GRID workgroups in all
   const int64_t hv = s.p["H"] * ceilDiv(g, gs), pieces = std::max<int64_t>(1, grid / hv);
   // wavefronts per SIMD that the registers are given for: more hide no more of the loads (64 requests of up to 4096 keys, 32 heads on 8: two
   // 53.8 us, three 57)
-  const int64_t occ = s.get("OCC", rb == 4 || (rb == 2 && dh > 128) ? 1 : 2);
+  const int64_t occ = s.get("OCC", rb == 2 && dh > 128 ? 1 : 2);
   Defines d;
   d.add("CA_NAME", s.name);
   d.add("CA_JOIN", join ? 1 : 0);
   d.add("CA_D", dh); d.add("CA_HKV", s.p["H"]); d.add("CA_G", g); d.add("CA_GS", gs); d.add("CA_PAGE", s.p["PAGE"]);
-  d.add("CA_F16", s.p["F16"]); d.add("CA_RB", rb); d.add("CA_WAVES", waves); d.add("CA_PIECES", pieces); d.add("CA_WHOLE", wholeTiles ? 1 : 0); d.add("CA_MIN", least);
-  d.add("CA_OCC", occ); d.add("CA_SPLIT", s.p["F16"] && rb < 4 ? 1 : 0);
+  d.add("CA_F16", s.p["F16"]); d.add("CA_RB", rb); d.add("CA_WAVES", waves); d.add("CA_SHARE", share ? 1 : 0); d.add("CA_PIECES", pieces); d.add("CA_WHOLE", wholeTiles ? 1 : 0); d.add("CA_MIN", least);
+  d.add("CA_OCC", occ); d.add("CA_SPLIT", s.p["F16"] && !share ? 1 : 0);
   d.add("CA_SCALE", floatLiteral(scale)); d.add("CA_CAP", floatLiteral(cap)); d.add("CA_HAS_CAP", cap > 0.0 ? 1 : 0);
   d.add("CA_WINDOW", window); d.add("CA_SLOPES", slopes ? 1 : 0); d.add("CA_STARTS", starts ? 1 : 0);
   for (auto key : {"KP", "KT", "KH", "VP", "VT", "VH", "QT", "QH"}) d.add(std::string("CA_") + key, std::to_string(s.p[key]) + "LL");
   src = d.wrap(kTpl_cache_attention);
   info.name = s.name;
   info.grid[0] = (uint32_t)((join ? std::max<int64_t>(1, pieces - 1) : pieces) * hv);
-  if (join) info.grid[1] = (uint32_t)(rb * dh / 32);
+  if (join) info.grid[1] = (uint32_t)(blocks * dh / 32);
   info.block[0] = (uint32_t)(join ? 512 : 64 * waves);
   info.numArgs = join ? 2 : 16;
   return true;

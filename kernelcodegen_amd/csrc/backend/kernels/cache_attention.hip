@@ -24,7 +24,7 @@
 // stand in one line that is cut evenly between CA_PIECES workgroups (prefix sums of the units of each request, in closed form,
 // taken by every workgroup); a tile cut between workgroups leaves partial results in `part`, which cache_join adds up.  So
 // requests of any lengths fill the part.  CA_WHOLE: one workgroup for each tile of a request (one tile each), nothing to join.
-// Parameters: CA_NAME, CA_D, CA_HKV, CA_G (heads per kv head), CA_GS, CA_PAGE, CA_F16, CA_SPLIT, CA_RB, CA_WAVES, CA_PIECES, CA_WHOLE, CA_MIN (least units of
+// Parameters: CA_NAME, CA_D, CA_HKV, CA_G (heads per kv head), CA_GS, CA_PAGE, CA_F16, CA_SPLIT, CA_RB, CA_WAVES, CA_SHARE, CA_PIECES, CA_WHOLE, CA_MIN (least units of
 // a workgroup), CA_SCALE, CA_CAP (0: none), CA_WINDOW (0: none), CA_SLOPES, CA_STARTS, CA_KP CA_KT CA_KH / CA_VP CA_VT CA_VH (strides of
 // page, token, head), CA_QT CA_QH (of q), CA_JOIN (this is cache_join).
 typedef _Float16 ca_f16x8 __attribute__((ext_vector_type(8)));
@@ -47,11 +47,12 @@ typedef __bf16 ca_q;
 #define CA_VP_ ((CA_D + 31) / 64 * 64 + 32)
 #define CA_VROW(key) ((key) * CA_VP_ + (key) / 16 * 16)
 #define CA_KP_ (CA_D + 16)                   // of its K: eight lanes that read below one another meet all banks
-#define CA_ROWS (16 * CA_RB)
+#define CA_BLOCKS (CA_SHARE ? CA_RB * CA_WAVES : CA_RB)      // blocks of 16 rows of a tile
+#define CA_ROWS (16 * CA_BLOCKS)
 #define CA_TOK (CA_ROWS / CA_GS)             // tokens of a tile
 #define CA_PARTS ((CA_G + CA_GS - 1) / CA_GS)    // tiles that the heads of a group are cut into
 #define CA_HV (CA_HKV * CA_PARTS)
-#define CA_UK (32 * CA_WAVES)
+#define CA_UK (CA_SHARE ? 64 : 32 * CA_WAVES)
 #define CA_LAZY 6.0f
 #define CA_TINY 1.17549435e-38f               // the least normal number: scales below count as zero
 #define CA_SLOT (CA_ROWS * CA_D + 2 * CA_ROWS)   // floats of a partial result
@@ -260,6 +261,419 @@ void CA_NAME(const float* __restrict__ part, ca_q* __restrict__ out) {
 }
 #else
 
+// The queries of a lane's row in 8 bits: a sum of CA_QN e4m3 numbers times the power of two that is returned.
+__device__ __forceinline__ float ca_query(const ca_q* __restrict__ p, unsigned (&qf)[CA_QN][CA_KR]) {
+  typedef ca_q ca_q8 __attribute__((ext_vector_type(8)));
+  ca_q8 raw[CA_KR / 2];
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < CA_KR / 2; ++i) raw[i] = *(const ca_q8*)(p + i * 8);
+#pragma unroll
+  for (int i = 0; i < CA_KR * 4; ++i) top = fmaxf(top, __builtin_fabsf((float)raw[i / 8][i % 8]));
+  top = ca_cross(top, true);
+  // the least power of two whose 448-fold (1.75 * 2^8) reaches the row's largest element
+  const unsigned bits = __builtin_bit_cast(unsigned, top);
+  int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  e = e < -100 ? -100 : e;
+  const float inv = __builtin_bit_cast(float, (unsigned)(127 - e) << 23);
+#pragma unroll
+  for (int i = 0; i < CA_KR; ++i) {
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = (float)raw[i / 2][i % 2 * 4 + j] * inv;
+#pragma unroll
+    for (int c = 0; c < CA_QN; ++c) {
+      int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+      w = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], w, true);
+      qf[c][i] = (unsigned)w;
+      if (c + 1 < CA_QN) {
+        f[0] -= __builtin_amdgcn_cvt_f32_fp8(w, 0);
+        f[1] -= __builtin_amdgcn_cvt_f32_fp8(w, 1);
+        f[2] -= __builtin_amdgcn_cvt_f32_fp8(w, 2);
+        f[3] -= __builtin_amdgcn_cvt_f32_fp8(w, 3);
+      }
+    }
+  }
+  return __builtin_bit_cast(float, (unsigned)(e + 127) << 23);
+}
+
+// The scores of 16 keys, whose K is row `n` of `p`, and of row blocks with the queries `qf`.
+template <int RB>
+__device__ __forceinline__ void ca_scores(const unsigned char* p, const unsigned (&qf)[RB][CA_QN][CA_KR], kcg_f32x4 (&sc)[RB]) {
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) sc[rb] = kcg_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#if CA_D % 128 == 0
+#pragma unroll
+  for (int i = 0; i < CA_KR; i += 8) {
+    const kcg_i32x4 k0 = *(const kcg_i32x4*)(p + i * 4), k1 = *(const kcg_i32x4*)(p + i * 4 + 16);
+    const kcg_i32x8 kf = {k0[0], k0[1], k0[2], k0[3], k1[0], k1[1], k1[2], k1[3]};
+#pragma unroll
+    for (int c = 0; c < CA_QN; ++c)
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        const unsigned (&w)[CA_KR] = qf[rb][c];
+        const kcg_i32x8 qv = {(int)w[i], (int)w[i + 1], (int)w[i + 2], (int)w[i + 3], (int)w[i + 4], (int)w[i + 5], (int)w[i + 6], (int)w[i + 7]};
+        sc[rb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qv, sc[rb], 0, 0, 0, 0, 0, 0);
+      }
+  }
+#else
+#pragma unroll
+  for (int i = 0; i < CA_KR; i += 2) {
+    const long kf = *(const long*)(p + i * 4);
+#pragma unroll
+    for (int c = 0; c < CA_QN; ++c)
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+        sc[rb] = __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(kf, (long)((unsigned long)qf[rb][c][i + 1] << 32 | qf[rb][c][i]), sc[rb], 0, 0, 0);
+  }
+#endif
+}
+
+typedef __attribute__((address_space(3))) unsigned char* ca_lds;
+typedef int ca_i32x2 __attribute__((ext_vector_type(2)));
+// Eight keys of one column of V, by a transposing read, as IEEE half.
+__device__ __forceinline__ kcg_u32x4 ca_columns(ca_lds p) {
+  const ca_i32x2 raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) ca_i32x2*)p);
+  const unsigned w0 = (unsigned)raw[0], w1 = (unsigned)raw[1];
+  return kcg_u32x4{CA_CVT16(w0, false), CA_CVT16(w0, true), CA_CVT16(w1, false), CA_CVT16(w1, true)};
+}
+__device__ __forceinline__ unsigned ca_nan_bytes(unsigned w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u; }
+// NaN for the rows (columns of `who`, 1.0 where the row sees the key) that see a key whose V is NaN (1.0 in `where`).
+__device__ __forceinline__ void ca_spread_nan(kcg_u32x4 where, kcg_u32x4 who, kcg_f32x4& acc) {
+  const kcg_f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+  kcg_f32x4 c = CA_MFMA16(where, who, none);          // how many such keys the row sees
+  c *= 0x1p127f;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(c[r] * 0x1p127f, 0.0f, acc[r]);      // + 0, or infinity times 0
+}
+
+// The beginning of a workgroup's share, and what the join has to know of it; false where nothing is left.
+__device__ __forceinline__ bool ca_begin(int id, int piece, float* __restrict__ part, const int* __restrict__ lengths, const int* __restrict__ starts, int B, int T,
+                                         int most, CaPlace& w) {
+  const bool some = ca_locate(piece, lengths, starts, B, T, most, w);
+  if (threadIdx.x == 0) {
+    CaEnd e = {0, 0, 0, 0};
+    if (some && w.unit > 0 && w.unit <= w.chunk) {
+      const int t = ca_tokens(w.request), at = w.tile * t;
+      e.first = w.request.first + at;
+      e.tokens = w.request.count - at < t ? w.request.count - at : t;
+      e.parts = 1 + (ca_units(w.request, w.tile) - w.unit + w.chunk - 1) / w.chunk;
+      e.slot = w.unit < w.chunk ? 1 : 0;          // the share before has it as its last piece, or as its only one
+    }
+    ((CaEnd*)part)[id] = e;
+  }
+  return some;
+}
+
+#if CA_SHARE
+// Many rows: every wavefront has 16 CA_RB rows of the tile of its own, and all of them work on the same 64 keys a step, which they bring into two
+// LDS buffers together; so a key is read once for 16 CA_RB CA_WAVES rows and nothing is added up between wavefronts.
+#define CA_SL ((4 * CA_D + 64 * CA_WAVES - 1) / (64 * CA_WAVES))     // chunks of 16 bytes of a step's K, and of its V, that a lane brings
+extern "C" __global__ __launch_bounds__(64 * CA_WAVES, CA_OCC)
+void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, const unsigned char* __restrict__ vc,
+             const float* __restrict__ kscale, const float* __restrict__ vscale, const int* __restrict__ table,
+             const int* __restrict__ lengths, const int* __restrict__ starts, const float* __restrict__ slopes,
+             float* __restrict__ part, long long T_, long long B_, long long W_, long long table_row, long long pages_, ca_q* __restrict__ out) {
+  struct Shared {
+    __attribute__((aligned(16))) unsigned char k[2][64 * CA_KP_], v[2][CA_VROW(63) + CA_VP_];
+    int nan[4];                  // whether a step has NaN in V where that matters, steps in turn
+  };
+  __shared__ Shared sh;
+  const int T = (int)T_, B = (int)B_, most = (int)W_ * CA_PAGE, pages = (int)pages_;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int hv = blockIdx.x % CA_HV, requests = B + CA_STARTS, piece = blockIdx.x / CA_HV, id = hv * CA_PIECES + piece;
+  CaPlace w;
+  if (!ca_begin(id, piece, part, lengths, starts, B, T, most, w)) return;
+  CaRequest rq = w.request;
+  int b = w.b, tile = w.tile, unit = w.unit, left = w.left;
+  bool begun = true;              // the first piece of this workgroup, if it is not a whole tile, goes to slot 0, a later one to slot 1
+  if (threadIdx.x < 4) sh.nan[threadIdx.x] = 0;
+  __syncthreads();
+  unsigned koff[CA_SL], voff[CA_SL], kat[CA_SL], vat[CA_SL];
+  int of[CA_SL];                  // key of the step that a chunk belongs to
+#pragma unroll
+  for (int u = 0; u < CA_SL; ++u) {
+    int c = u * 64 * CA_WAVES + threadIdx.x;
+    c = c < 4 * CA_D ? c : 4 * CA_D - 1;            // (behind the last chunk that one again)
+    const int part16 = c % (CA_D / 16) * 16;
+    of[u] = c / (CA_D / 16);
+    koff[u] = (of[u] % 16) * (unsigned)CA_KT + part16;
+    voff[u] = (of[u] % 16) * (unsigned)CA_VT + part16;
+    kat[u] = of[u] * CA_KP_ + part16;
+    vat[u] = CA_VROW(of[u]) + part16;
+  }
+  const int key8 = n / 2 < 4 ? g * 4 + n / 2 : 16 + g * 4 + n / 2 - 4;        // the row that this lane gives the address of in transposing reads
+  int count = 0;                  // steps so far
+
+  while (left > 0) {
+    const int t = ca_tokens(rq), tok0 = tile * t, tokens = rq.count - tok0 < t ? rq.count - tok0 : t;
+    const int units = ca_units(rq, tile);
+    const int until = left < units - unit ? unit + left : units;           // of this piece
+    const int first = rq.length - rq.count + tok0;                         // position of the tile's first row
+    const int hi = first + tokens > 0 ? first + tokens : 0;
+    const int lo = CA_WINDOW && first - CA_WINDOW + 1 > 0 ? first - CA_WINDOW + 1 : 0;
+    const int kvh = hv / CA_PARTS, head0 = kvh * CA_G + (hv % CA_PARTS) * CA_GS;
+    const int base = ca_low(rq, tile) * CA_UK;
+    int key = base + unit * CA_UK;
+    const int end = base + until * CA_UK < hi ? base + until * CA_UK : hi;
+    // tokens of this wavefront's rows; it has none where the first is not there
+    const int t0 = wave * 16 * CA_RB / CA_GS, t1 = (wave * 16 * CA_RB + 16 * CA_RB - 1) / CA_GS;
+    const bool mine = t0 < tokens;
+    const int pos0 = first + t0, pos1 = first + (t1 < tokens ? t1 : tokens - 1);
+
+    unsigned qf[CA_RB][CA_QN][CA_KR];
+    float qs[CA_RB], slope[CA_RB], m[CA_RB], l[CA_RB];
+    int pos[CA_RB];
+    kcg_f32x4 acc[CA_RB][CA_NT];
+#pragma unroll
+    for (int rb = 0; rb < CA_RB; ++rb) {
+      const int row = (wave * CA_RB + rb) * 16 + n, tk = row / CA_GS, hd = row - tk * CA_GS;
+      const bool real = tk < tokens && (hv % CA_PARTS) * CA_GS + hd < CA_G;
+      const int token = real ? tk : 0, head = real ? head0 + hd : head0;
+      pos[rb] = first + token;
+      slope[rb] = CA_SLOPES ? slopes[head] * 1.44269504088896340736f : 0.0f;
+      qs[rb] = ca_query(q + (long long)(rq.first + tok0 + token) * CA_QT + (long long)head * CA_QH + g * (CA_D / 4), qf[rb]);
+      m[rb] = -__builtin_inff();
+      l[rb] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < CA_NT; ++i) acc[rb][i] = kcg_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    if (key < end) {
+      const int* row = table + (long long)b * table_row;
+      // Pages and scales of the quarters of 16 steps, a lane each, read while the 16 steps before are worked on
+      struct Block { int page; float ks, vs; };       // page -1: no such keys, or a page that there is none of
+      auto pagesOf = [&](int from) {
+        const int at = from + (lane >> 2) * CA_UK + (lane & 3) * 16;
+        const int page = row[(at < hi ? at : hi - 1) / CA_PAGE];
+        return at < hi && at + 16 > lo && (unsigned)page < (unsigned)pages ? page : -1;
+      };
+      auto scalesOf = [&](int page) {
+        const long long at = (long long)(page < 0 ? 0 : page) * CA_HKV + kvh;       // (what is not there is read from somewhere that is)
+        return Block{page, kscale[at], vscale[at]};
+      };
+      auto ready = [&](Block& x) {
+        x.ks = x.page < 0 ? 0.0f : x.ks;
+        x.vs = x.page < 0 || x.vs < CA_TINY ? -__builtin_inff() : __builtin_amdgcn_logf(x.vs);      // (scales of zero stand for pages of zeros)
+      };
+      kcg_u32x4 k[CA_SL], v[CA_SL];
+      auto load = [&](int at, int step, const Block& x) {
+#pragma unroll
+        for (int u = 0; u < CA_SL; ++u) {
+          int page = __shfl(x.page, step * 4 + of[u] / 16, 64);
+          page = page < 0 ? 0 : page;
+          const long long token = (at + of[u] / 16 * 16) % CA_PAGE;
+          k[u] = *(const kcg_u32x4*)(kc + ((long long)page * CA_KP + token * CA_KT + (long long)kvh * CA_KH) + koff[u]);
+          v[u] = *(const kcg_u32x4*)(vc + ((long long)page * CA_VP + token * CA_VT + (long long)kvh * CA_VH) + voff[u]);
+        }
+      };
+      Block now = scalesOf(pagesOf(key)), soon;
+      int later = pagesOf(key + 16 * CA_UK), step = 0;
+      load(key, 0, now);
+      ready(now);
+      float lvk = 0.0f;              // logarithm of the last vscale that was not zero
+#pragma unroll 1
+      while (true) {
+        if (step == 0) {
+          soon = scalesOf(later);
+          later = pagesOf(key + 32 * CA_UK);
+        }
+        float ks[4], lv[4], iv[4];
+        bool there[4], zeros = false;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          there[h] = __builtin_amdgcn_readlane(now.page, 4 * step + h) >= 0;
+          ks[h] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, now.ks), 4 * step + h));
+          lv[h] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, now.vs), 4 * step + h));
+          const bool zero = lv[h] == -__builtin_inff();
+          zeros |= zero;
+          if (zero) lv[h] = lvk;
+          lvk = lv[h];
+          iv[h] = __builtin_amdgcn_exp2f(-lv[h]);
+        }
+        unsigned char *kb = sh.k[count & 1], *vb = sh.v[count & 1];
+        // not every row of the tile sees every key of the step, or a scale is zero
+        bool flagged = false;
+        if (key + 64 > first + 1 || (CA_WINDOW && key < first + tokens - CA_WINDOW) || zeros) {
+          // V of keys that no row sees, which may be anything, and of pages whose scale is zero, counts as zero
+          unsigned nan = 0;
+#pragma unroll
+          for (int u = 0; u < CA_SL; ++u) {
+            const float scale = __shfl(now.vs, step * 4 + of[u] / 16, 64);
+            if (key + of[u] < lo || key + of[u] >= hi || scale == -__builtin_inff()) v[u] = kcg_u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) nan |= ca_nan_bytes(v[u][i]);
+          }
+          if (nan != 0) sh.nan[count & 3] = 1;
+          __syncthreads();
+          flagged = __builtin_amdgcn_readfirstlane(sh.nan[count & 3]) != 0;
+        }
+#pragma unroll
+        for (int u = 0; u < CA_SL; ++u) {
+          *(kcg_u32x4*)(kb + kat[u]) = k[u];
+          kcg_u32x4 x = v[u];
+          if (flagged)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = ca_nan_bytes(x[i]) * 0x38u;       // 1.0 where V is NaN, first
+          *(kcg_u32x4*)(vb + vat[u]) = x;
+        }
+        if (threadIdx.x == 0) sh.nan[(count + 2) & 3] = 0;                       // (read last two steps ago)
+        const bool more = key + CA_UK < end;
+        if (++step == 16) {
+          step = 0;
+          now = soon;
+          ready(now);
+        }
+        if (more && !flagged) load(key + CA_UK, step, now);
+        __syncthreads();           // the step is in LDS, and everybody has finished with the one before
+
+        const bool work = mine && key <= pos1 && (!CA_WINDOW || key + 63 > pos0 - CA_WINDOW);
+        unsigned pf[CA_RB][8];
+        kcg_f32x4 sc[CA_RB][4];
+        if (work) {
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            kcg_f32x4 s[CA_RB];
+            ca_scores<CA_RB>(kb + (h * 16 + n) * CA_KP_ + g * (CA_D / 4), qf, s);
+#pragma unroll
+            for (int rb = 0; rb < CA_RB; ++rb) sc[rb][h] = s[rb];
+          }
+          const bool masked = key + 64 > pos0 + 1 || (CA_WINDOW && key <= pos1 - CA_WINDOW) || zeros;
+          const bool general = CA_HAS_CAP || CA_SLOPES || !(CA_SCALE > 0.0f) || masked || !(ks[0] > 0.0f && ks[1] > 0.0f && ks[2] > 0.0f && ks[3] > 0.0f);
+#pragma unroll
+          for (int rb = 0; rb < CA_RB; ++rb) {
+            // the exponent of a score x is by * x + plus
+            float by[4], plus[4];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              by[h] = ks[h] * (CA_SCALE * 1.44269504088896340736f) * qs[rb];
+              plus[h] = lv[h];
+            }
+            if (general) {
+#pragma unroll
+              for (int h = 0; h < 4; ++h) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const int at = key + h * 16 + g * 4 + r;
+                  float x = sc[rb][h][r];
+#if CA_HAS_CAP
+                  x = kcg_fast_tanh(x * (ks[h] * (CA_SCALE / CA_CAP) * qs[rb]));
+                  x = __builtin_fmaf(x, CA_CAP * 1.44269504088896340736f, lv[h]);
+#else
+                  x = __builtin_fmaf(x, by[h], lv[h]);
+#endif
+                  if (CA_SLOPES) x = __builtin_fmaf(slope[rb], (float)(at - pos[rb]), x);
+                  const bool seen = !masked || (at <= pos[rb] && (!CA_WINDOW || at > pos[rb] - CA_WINDOW) && there[h]);
+                  sc[rb][h][r] = seen ? x : -__builtin_inff();
+                }
+                by[h] = 1.0f;
+                plus[h] = 0.0f;
+              }
+            }
+            float mx = -__builtin_inff();
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+              mx = fmaxf(mx, __builtin_fmaf(fmaxf(fmaxf(sc[rb][h][0], sc[rb][h][1]), fmaxf(sc[rb][h][2], sc[rb][h][3])), by[h], plus[h]));
+            mx = ca_cross(mx, true);
+            if (__any(mx > m[rb] + CA_LAZY)) {
+              const float to = fmaxf(m[rb], mx), f = to == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m[rb] - to);
+              m[rb] = to;
+              l[rb] *= f;
+#pragma unroll
+              for (int i = 0; i < CA_NT; ++i) acc[rb][i] *= f;
+            }
+            const float ref = m[rb] == -__builtin_inff() ? 0.0f : m[rb];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              float p[4];
+#pragma unroll
+              for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][h][r], by[h], plus[h] - ref));
+              pf[rb][2 * h] = kcg_pack_f16x2(p[0], p[1]);
+              pf[rb][2 * h + 1] = kcg_pack_f16x2(p[2], p[3]);
+              const kcg_f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
+              const float sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(kcg_f16x2, pf[rb][2 * h]), one,
+                                                       __builtin_amdgcn_fdot2(__builtin_bit_cast(kcg_f16x2, pf[rb][2 * h + 1]), one, 0.0f, false), false);
+              l[rb] = __builtin_fmaf(sum, iv[h], l[rb]);
+            }
+          }
+        }
+        const ca_lds vread = (ca_lds)vb + CA_VROW(key8) + (n & 1) * 8;
+        if (flagged) {
+          // NaN where some rows see the key and some may not: it goes to those that do, by a product of where V is NaN and who sees
+          if (work)
+#pragma unroll
+            for (int rb = 0; rb < CA_RB; ++rb)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                unsigned see[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  see[j] = (sc[rb][2 * h + j / 2][j % 2 * 2] != -__builtin_inff() ? 0x3c00u : 0u) | (sc[rb][2 * h + j / 2][j % 2 * 2 + 1] != -__builtin_inff() ? 0x3c000000u : 0u);
+                const kcg_u32x4 who = {see[0], see[1], see[2], see[3]};
+#pragma unroll
+                for (int tt = 0; tt < CA_NT; ++tt) ca_spread_nan(ca_columns(vread + h * CA_VROW(32) + tt * 16), who, acc[rb][tt]);
+              }
+          __syncthreads();
+#pragma unroll
+          for (int u = 0; u < CA_SL; ++u) {
+            kcg_u32x4 x = v[u];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] &= ~(ca_nan_bytes(x[i]) * 0xffu);
+            *(kcg_u32x4*)(vb + vat[u]) = x;
+          }
+          if (more) load(key + CA_UK, step, now);
+          __syncthreads();
+        }
+        if (work) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int tt = 0; tt < CA_NT; ++tt) {
+              const kcg_u32x4 vf = ca_columns(vread + h * CA_VROW(32) + tt * 16);
+#pragma unroll
+              for (int rb = 0; rb < CA_RB; ++rb) {
+                const kcg_u32x4 p = {pf[rb][4 * h], pf[rb][4 * h + 1], pf[rb][4 * h + 2], pf[rb][4 * h + 3]};
+                acc[rb][tt] = CA_MFMA16(vf, p, acc[rb][tt]);
+              }
+            }
+        }
+        ++count;
+        if (!more) break;
+        key += CA_UK;
+      }
+    }
+
+    const bool whole = unit == 0 && until == units;
+    float* slot = part + CA_ENDS + ((long long)id * 2 + (begun ? 0 : 1)) * CA_SLOT;
+    begun = false;
+#pragma unroll
+    for (int rb = 0; rb < CA_RB; ++rb) {
+      const int block = wave * CA_RB + rb, at = block * 16 + n;
+      l[rb] = ca_cross(l[rb], false);
+#pragma unroll
+      for (int i = 0; i < CA_NT; ++i) {
+        if (whole)
+          ca_store(out, rq.first + tok0, tokens, hv, block, i, acc[rb][i], l[rb]);
+        else
+          *(kcg_f32x4*)(slot + ((block * CA_NT + i) * 64 + lane) * 4) = acc[rb][i];
+      }
+      if (!whole && g == 0) {
+        slot[CA_ROWS * CA_D + at * 2] = m[rb];
+        slot[CA_ROWS * CA_D + at * 2 + 1] = l[rb];
+      }
+    }
+    left -= until - unit;
+    unit = 0;
+    if (left > 0 && ++tile >= ca_tiles(rq)) {      // the next tile that there is
+      tile = 0;
+      while (++b < requests) {
+        rq = ca_request(lengths, starts, b, B, T, most);
+        if (rq.count > 0) break;
+      }
+    }
+  }
+}
+#else
 extern "C" __global__ __launch_bounds__(64 * CA_WAVES, CA_OCC)
 void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, const unsigned char* __restrict__ vc,
              const float* __restrict__ kscale, const float* __restrict__ vscale, const int* __restrict__ table,
@@ -289,19 +703,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
 #else
   const int requests = B + CA_STARTS, piece = blockIdx.x / CA_HV, id = hv * CA_PIECES + piece;
   CaPlace w;
-  const bool some = ca_locate(piece, lengths, starts, B, T, most, w);
-  if (threadIdx.x == 0) {
-    CaEnd e = {0, 0, 0, 0};
-    if (some && w.unit > 0 && w.unit <= w.chunk) {
-      const int t = ca_tokens(w.request), at = w.tile * t;
-      e.first = w.request.first + at;
-      e.tokens = w.request.count - at < t ? w.request.count - at : t;
-      e.parts = 1 + (ca_units(w.request, w.tile) - w.unit + w.chunk - 1) / w.chunk;
-      e.slot = w.unit < w.chunk ? 1 : 0;          // the share before has it as its last piece, or as its only one
-    }
-    ((CaEnd*)part)[id] = e;
-  }
-  if (!some) return;
+  if (!ca_begin(id, piece, part, lengths, starts, B, T, most, w)) return;
   rq = w.request; b = w.b; tile = w.tile; unit = w.unit; left = w.left;
   bool begun = true;              // the first piece of this workgroup, if it is not a whole tile, goes to slot 0, a later one to slot 1
 #endif
@@ -331,38 +733,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
       pos[rb] = first + token;
       slope[rb] = CA_SLOPES ? slopes[head] * 1.44269504088896340736f : 0.0f;
       const ca_q* p = q + (long long)(rq.first + tok0 + token) * CA_QT + (long long)head * CA_QH + g * (CA_D / 4);
-      typedef ca_q ca_q8 __attribute__((ext_vector_type(8)));
-      ca_q8 raw[CA_KR / 2];
-      float top = 0.0f;
-#pragma unroll
-      for (int i = 0; i < CA_KR / 2; ++i) raw[i] = *(const ca_q8*)(p + i * 8);
-#pragma unroll
-      for (int i = 0; i < CA_KR * 4; ++i) top = fmaxf(top, __builtin_fabsf((float)raw[i / 8][i % 8]));
-      top = ca_cross(top, true);
-      // the least power of two whose 448-fold (1.75 * 2^8) reaches the row's largest element
-      const unsigned bits = __builtin_bit_cast(unsigned, top);
-      int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-      e = e < -100 ? -100 : e;
-      qs[rb] = __builtin_bit_cast(float, (unsigned)(e + 127) << 23);
-      const float inv = __builtin_bit_cast(float, (unsigned)(127 - e) << 23);
-#pragma unroll
-      for (int i = 0; i < CA_KR; ++i) {
-        float f[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = (float)raw[i / 2][i % 2 * 4 + j] * inv;
-#pragma unroll
-        for (int c = 0; c < CA_QN; ++c) {
-          int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
-          w = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], w, true);
-          qf[rb][c][i] = (unsigned)w;
-          if (c + 1 < CA_QN) {
-            f[0] -= __builtin_amdgcn_cvt_f32_fp8(w, 0);
-            f[1] -= __builtin_amdgcn_cvt_f32_fp8(w, 1);
-            f[2] -= __builtin_amdgcn_cvt_f32_fp8(w, 2);
-            f[3] -= __builtin_amdgcn_cvt_f32_fp8(w, 3);
-          }
-        }
-      }
+      qs[rb] = ca_query(p, qf[rb]);
     }
 
     kcg_f32x4 acc[CA_RB][CA_NT];
@@ -419,8 +790,6 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
 #pragma unroll
       for (int u = 0; u < CA_VL; ++u) v[u] = *(const kcg_u32x4*)((CA_HALF(u) ? vp[1] : vp[0]) + voff[u]);
     };
-    typedef __attribute__((address_space(3))) unsigned char* ca_lds;
-    typedef int ca_i32x2 __attribute__((ext_vector_type(2)));
     unsigned char *ks_ = sh.tile.k[wave], *vs = sh.tile.v[wave];
     // this lane's address for the transposing reads of tile 0: within each group of 16 lanes, lanes 2 j and 2 j + 1 give the two halves of row
     // j, and lane i receives column i of the eight rows.  The rows are the keys that lane group g has scores of.
@@ -436,37 +805,12 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
       behind();
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int rb = 0; rb < CA_RB; ++rb)
+      for (int h = 0; h < 2; ++h) {
+        kcg_f32x4 s[CA_RB];
+        ca_scores<CA_RB>(ks_ + (h * 16 + n) * CA_KP_ + g * (CA_D / 4), qf, s);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) sc[rb][h] = kcg_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#if CA_D % 128 == 0
-#pragma unroll
-        for (int i = 0; i < CA_KR; i += 8) {
-          const unsigned char* p = ks_ + (h * 16 + n) * CA_KP_ + g * (CA_D / 4) + i * 4;
-          const kcg_i32x4 k0 = *(const kcg_i32x4*)p, k1 = *(const kcg_i32x4*)(p + 16);
-          const kcg_i32x8 kf = {k0[0], k0[1], k0[2], k0[3], k1[0], k1[1], k1[2], k1[3]};
-#pragma unroll
-          for (int rb = 0; rb < CA_RB; ++rb)
-#pragma unroll
-            for (int c = 0; c < CA_QN; ++c) {
-              const unsigned (&w)[CA_KR] = qf[rb][c];
-              const kcg_i32x8 qv = {(int)w[i], (int)w[i + 1], (int)w[i + 2], (int)w[i + 3], (int)w[i + 4], (int)w[i + 5], (int)w[i + 6], (int)w[i + 7]};
-              sc[rb][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qv, sc[rb][h], 0, 0, 0, 0, 0, 0);
-            }
-        }
-#else
-#pragma unroll
-        for (int i = 0; i < CA_KR; i += 2) {
-          const long kf = *(const long*)(ks_ + (h * 16 + n) * CA_KP_ + g * (CA_D / 4) + i * 4);
-#pragma unroll
-          for (int rb = 0; rb < CA_RB; ++rb)
-#pragma unroll
-            for (int c = 0; c < CA_QN; ++c)
-              sc[rb][h] = __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(kf, (long)((unsigned long)qf[rb][c][i + 1] << 32 | qf[rb][c][i]), sc[rb][h], 0, 0, 0);
-        }
-#endif
+        for (int rb = 0; rb < CA_RB; ++rb) sc[rb][h] = s[rb];
+      }
     };
     // Scores to probabilities, and these into the sums; `masked`: not every row sees every key of the step, or a scale is zero.
     // `behind` is called when the registers of V are free.
@@ -546,11 +890,6 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
         for (int u = 0; u < CA_VL; ++u) *(kcg_u32x4*)(vs + vat[u]) = v[u];
         __builtin_amdgcn_wave_barrier();
       };
-      auto column = [&](int tt) __attribute__((always_inline)) {
-        const ca_i32x2 raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) ca_i32x2*)(vread + tt * 16));
-        const unsigned w0 = (unsigned)raw[0], w1 = (unsigned)raw[1];
-        return kcg_u32x4{CA_CVT16(w0, false), CA_CVT16(w0, true), CA_CVT16(w1, false), CA_CVT16(w1, true)};
-      };
       if (masked) {
         // V of keys that no row sees, which may be anything, and of pages whose scale is zero, counts as zero
         unsigned nan = 0;
@@ -559,7 +898,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
           const int key32 = (u * 64 + lane) / (CA_D / 16);
           if (at + key32 < lo || at + key32 >= hi || (key32 < 16 ? zero[0] : zero[1])) v[u] = kcg_u32x4{0, 0, 0, 0};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) nan |= ((v[u][i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+          for (int i = 0; i < 4; ++i) nan |= ca_nan_bytes(v[u][i]);
         }
         if (__any(nan != 0)) {
           // NaN where some rows see the key and some may not: it goes to those that do, by a product of where V is NaN and who sees
@@ -568,7 +907,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
           for (int u = 0; u < CA_VL; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const unsigned bytes = ((v[u][i] & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u;
+              const unsigned bytes = ca_nan_bytes(v[u][i]);
               whole[u][i] = v[u][i] & ~(bytes * 0xffu);
               v[u][i] = bytes * 0x38u;               // 1.0
             }
@@ -577,7 +916,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
           for (int u = 0; u < CA_VL; ++u) v[u] = whole[u];
 #pragma unroll
           for (int tt = 0; tt < CA_NT; ++tt) {
-            const kcg_u32x4 where = column(tt);
+            const kcg_u32x4 where = ca_columns(vread + tt * 16);
 #pragma unroll
             for (int rb = 0; rb < CA_RB; ++rb) {
               unsigned see[4];
@@ -585,11 +924,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
               for (int j = 0; j < 4; ++j)
                 see[j] = (sc[rb][j / 2][j % 2 * 2] != -__builtin_inff() ? 0x3c00u : 0u) | (sc[rb][j / 2][j % 2 * 2 + 1] != -__builtin_inff() ? 0x3c000000u : 0u);
               const kcg_u32x4 who = {see[0], see[1], see[2], see[3]};
-              const kcg_f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
-              kcg_f32x4 c = CA_MFMA16(where, who, none);          // how many such keys the row sees
-              c *= 0x1p127f;
-#pragma unroll
-              for (int r = 0; r < 4; ++r) acc[rb][tt][r] = __builtin_fmaf(c[r] * 0x1p127f, 0.0f, acc[rb][tt][r]);      // + 0, or infinity times 0
+              ca_spread_nan(where, who, acc[rb][tt]);
             }
             __builtin_amdgcn_sched_barrier(0);
           }
@@ -599,7 +934,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
       behind();
 #pragma unroll
       for (int tt = 0; tt < CA_NT; ++tt) {
-        const kcg_u32x4 vf = column(tt);
+        const kcg_u32x4 vf = ca_columns(vread + tt * 16);
 #pragma unroll
         for (int rb = 0; rb < CA_RB; ++rb) {
           const kcg_u32x4 p = {pf[rb][0], pf[rb][1], pf[rb][2], pf[rb][3]};
@@ -722,4 +1057,5 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
 #endif
   }
 }
+#endif
 #endif

@@ -458,7 +458,7 @@ def _cache_read_launch(cache, scale, slots, dtype):
     return _into_last(kern.bind(grid=(max(1, -(-tokens * heads * d // 2048)),)), ((tokens, heads, d), dtype))
 
 
-def cache_attention(q, k_cache, v_cache, k_scale, v_scale, table, lengths, starts=None, scale=None, cap=None, window=None, slopes=None):
+def cache_attention(q, k_cache, v_cache, k_scale, v_scale, table, lengths, starts=None, scale=None, cap=None, window=None, slopes=None, **cfg):
     """Attention of new tokens over a paged cache in 8 bits, which holds their own keys and values already.
 
     q: [tokens, heads, d], IEEE half or bfloat16, heads a multiple of the cache's; caches and scales as for cache_write; table: int32
@@ -467,12 +467,15 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, table, lengths, start
     and rows behind the last request's, are zeros.
       score = scale * q.k (scale: d^-0.5), then cap * tanh(score / cap), then + slopes[head] * (key's position - row's), slopes fp32
       [heads]; a row sees the keys up to its own position, of these the last `window`.
-    Entries of the table behind a request's length are not read; keys on pages that are not the cache's count as not there."""
+    Entries of the table behind a request's length are not read; keys on pages that are not the cache's count as not there.  `cfg`
+    overrides kernel parameters (RB, WAVES, GRID, LEAST, OCC, WHOLE)."""
     scale, cap, window = None if scale is None else float(scale), float(cap or 0.0), operator.index(window or 0)
     key = ("cache_attention", R.signature(q, k_cache, v_cache, k_scale, v_scale, table, lengths, starts, slopes), scale, cap, window)
-    hit = _bound.get(key)
+    hit = None if cfg else _bound.get(key)
     if hit is None:
-        _bound[key] = hit = _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, lengths, starts, scale, cap, window, slopes)
+        hit = _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, lengths, starts, scale, cap, window, slopes, cfg)
+        if not cfg:
+            _bound[key] = hit
     run, join, floats = hit
     if not q.shape[0]:
         return torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -485,7 +488,7 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, table, lengths, start
     return out
 
 
-def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, lengths, starts, scale, cap, window, slopes):
+def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, lengths, starts, scale, cap, window, slopes, cfg):
     _on_device(q, k_cache, v_cache, table)
     _vectors(torch.float32, k_scale, v_scale, *(() if slopes is None else (slopes,)))
     _vectors(torch.int32, lengths, *(() if starts is None else (starts,)))
@@ -516,23 +519,27 @@ def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, length
         raise ValueError("too many rows times keys for one launch")
     if not 0.0 <= cap < math.inf or window < 0:
         raise ValueError("cap and window must not be negative")
-    # rows that the average request has of a kv head
+    # Rows that the average request has of a kv head: up to 32 form a tile, whose keys the wavefronts of a workgroup split; more are split
+    # between the wavefronts
     rows = group * max(1, -(-tokens // batch))
-    blocks = 1 if rows <= 16 else 2 if rows <= 32 or d > 128 else 4
-    whole = starts is None and width * page <= 512
-    params = dict(H=kv_heads, D=d, PAGE=page, G=group, F16=int(q.dtype == torch.float16), RB=blocks, STARTS=int(starts is not None), CAP=cap, WINDOW=window,
+    blocks, share = (1 if rows <= 16 else 2), int(rows > 32)
+    params = dict(H=kv_heads, D=d, PAGE=page, G=group, F16=int(q.dtype == torch.float16), RB=blocks, WAVES=4, SHARE=share, STARTS=int(starts is not None), CAP=cap, WINDOW=window,
                   SLOPES=int(slopes is not None), SCALE=d ** -0.5 if scale is None else scale, KP=ks[0], KT=ks[1], KH=ks[2], VP=vs[0], VT=vs[1], VH=vs[2],
-                  QT=qs[0], QH=qs[1])
-    if whole:
-        parts = -(-group // (16 * blocks))
-        kern = R.get_kernel("cache_attention", WHOLE=1, **params)
-        return _into_last(kern.bind(grid=(batch * kv_heads * parts,)), (tuple(q.shape), q.dtype)), None, 0
-    grid = 256 if blocks == 4 or (blocks == 2 and d > 128) else 512
-    kern = R.get_kernel("cache_attention", GRID=grid, **params)
-    shares, alone = kern.info["grid"][0], kern.info["grid"][0] == kv_heads * -(-group // (16 * blocks))
+                  QT=qs[0], QH=qs[1], WHOLE=int(starts is None and width * page <= 512),
+                  GRID=256 if blocks == 2 and d > 128 else 512)
+    if not cfg.keys() <= {"RB", "WAVES", "SHARE", "GRID", "LEAST", "OCC", "WHOLE"}:
+        raise ValueError("unknown kernel parameters")
+    params.update(cfg)
+    blocks = params["RB"] * (params["WAVES"] if params["SHARE"] else 1)
+    tiles = kv_heads * -(-group // (16 * blocks))         # of a token's heads
+    kern = R.get_kernel("cache_attention", **params)
+    if params["WHOLE"]:
+        return _into_last(kern.bind(grid=(batch * tiles,)), (tuple(q.shape), q.dtype)), None, 0
+    shares = kern.info["grid"][0]
     # for each share four whole numbers, and two parts of a tile: its sums, and maximum and sum of the probabilities of each row
     floats = shares * (4 + 2 * (16 * blocks * d + 32 * blocks))
-    return _into_last(kern.bind(), (tuple(q.shape), q.dtype)), None if alone else R.get_kernel("cache_join", GRID=grid, **params).bind(), floats
+    join = None if shares == tiles else R.get_kernel("cache_join", **params).bind()
+    return _into_last(kern.bind(), (tuple(q.shape), q.dtype)), join, floats
 
 
 def matmul_q4(x, w, scale, zero=None, out_dtype=None, **cfg):
