@@ -1749,24 +1749,24 @@ bool emitGemmQ4(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::st
   const int64_t n = s.p["N"], k = s.p["K"], group = s.p["GROUP"], mb = s.p["MB"];
   if (group != 32 && group != 64 && group % 128) { err = "gemm_q4: GROUP must be 32, 64 or a multiple of 128"; return false; }
   if (k % group) { err = "gemm_q4: GROUP must divide K"; return false; }
-  const int64_t nt = s.get("NT", 1), wn = s.get("WN", mb > 1 ? 8 : 1), wk = s.get("WK", mb > 1 ? 1 : 8), depth = s.get("DEPTH", 1), split = s.get("SPLIT", 1), mr = s.get("MR", 16 * mb);
+  const int64_t nt = s.get("NT", 1), wn = s.get("WN", 1), wk = s.get("WK", mb > 1 ? 1 : 8), split = s.get("SPLIT", 1), mr = s.get("MR", 16 * mb);
   const int64_t per = group >= 128 ? 1 : 128 / group;
-  const int64_t lds = std::max(wk * (wn > 1 ? 2 : 1) * mr * 528 + wk * wn * (16 * nt * 144 + 2 * per * 16 * nt * 8), wk * wn * mb * nt * 1024);
-  if (nt < 1 || nt > 8 || wn < 1 || wk < 1 || wn * wk > 16 || depth < 1 || depth > 16 || split < 1 || split > 64 || mr < 1 || mr > 16 * mb || (lds > 163840 && !join)) {
-    err = "gemm_q4: bad NT, WN, WK, DEPTH, SPLIT or MR";
+  const int64_t lds = std::max(wk * (wn > 1 ? 2 : 1) * mr * 528 + wk * wn * (16 * nt * 144 + 2 * per * 16 * nt * 8) + wk * (wn > 1 ? 2 : 1) * 2 * per * 16 * mb * 4 + 64, wk * wn * mb * nt * 1024);
+  if (nt < 1 || nt > 8 || wn < 1 || wk < 1 || wn * wk > 16 || split < 1 || split > 64 || mr < 1 || mr > 16 * mb || (lds > 163840 && !join)) {
+    err = "gemm_q4: bad NT, WN, WK, SPLIT or MR";
     return false;
   }
-  s.p["NT"] = nt; s.p["WN"] = wn; s.p["WK"] = wk; s.p["DEPTH"] = depth; s.p["SPLIT"] = split; s.p["MR"] = mr;
+  s.p["NT"] = nt; s.p["WN"] = wn; s.p["WK"] = wk; s.p["SPLIT"] = split; s.p["MR"] = mr;
   const char* x = s.p["F16"] ? "_Float16" : "__bf16";
   Defines d;
   d.add("Q4_NAME", s.name);
   d.add("Q4_N", n); d.add("Q4_K", k); d.add("Q4_GROUP", group); d.add("Q4_F16", s.p["F16"]); d.add("Q4_ZERO", s.get("ZERO", 0) ? 1 : 0);
   d.add("Q4_ST", std::string(s.get("SCALE_F32", 0) ? "float" : x));
   d.add("Q4_YT", std::string(s.get("OUT_F32", 0) ? "float" : x));
-  d.add("Q4_MB", mb); d.add("Q4_NT", nt); d.add("Q4_WN", wn); d.add("Q4_WK", wk); d.add("Q4_DEPTH", depth); d.add("Q4_SPLIT", split); d.add("Q4_MR", mr);
+  d.add("Q4_MB", mb); d.add("Q4_NT", nt); d.add("Q4_WN", wn); d.add("Q4_WK", wk); d.add("Q4_SPLIT", split); d.add("Q4_MR", mr);
   // (offsets into the codes, and into 64 rows of X)
   d.add("Q4_WIDE", s.get("WIDE", (double)n * (double)(k / 2) >= 2147483648.0 || k >= 1 << 24 ? 1 : 0) ? 1 : 0);
-  d.add("Q4_OCC", s.get("OCC", 1)); d.add("Q4_JOIN", join ? 1 : 0);
+  d.add("Q4_JOIN", join ? 1 : 0);
   src = d.wrap(kTpl_gemm_q4);
   info.name = s.name;
   info.grid[0] = (uint32_t)ceilDiv(n, 16 * nt * wn);

@@ -5,9 +5,9 @@
 //
 // The weights are read once and bound the launch, so they are spent as little on as they can be: the bits of a code are shifted into
 // the mantissa of 1.0, which gives 1 + code / 16 exactly in either 16-bit type, eight codes in eight instructions.  The matrix
-// product takes these, and a second one with ones in the weights' place sums X; from a group's two fp32 sums t and u
-//   16 scale (t - (1 + zero / 16) u)
-// is the group's part of the result: codes, zeros and X enter unrounded, sums are fp32, the scale is applied in fp32.
+// product takes these and begins a group at -(1 + zero / 16) times the group's sum of X, which the wavefronts take on X's way into LDS;
+// 16 scale times what comes out is the group's part of the result: codes, zeros and X enter unrounded, sums are fp32, the scale is applied in
+// fp32.
 // X is the left operand, so the result's lanes hold one column n and four rows: a group's scale is one number per lane.
 //
 // A dword of codes gives the pairs (0, 4) (1, 5) (2, 6) (3, 7) of its eight, and X is put into that order on its way into LDS.
@@ -18,20 +18,27 @@
 // their sums through LDS, and Q4_SPLIT workgroups split it again, whose fp32 results gemm_q4_join adds in order.
 // Where a group has 128 codes or more, product j of a step's half takes k = 32 g + 8 j .. + 7 for quarter g of the wavefront, 16 bytes
 // of codes as they come; smaller groups need products of 32 neighbouring k, so the quarters exchange dwords (four permlane swaps).
+// Measured: 1 row, N = K = 4096, bf16, groups of 128: 4.4 us (2.0 TB/s; reading as many bytes alone takes 3.0); 16 rows, N 11008, K 4096, half
+// precision with zeros: 9.5 us (2.5 TB/s; reading alone 5.1); 61 rows, N 4096, K 11008, groups of 64: 20.7 us with the join's 3.  One row is
+// bound by the launch and one trip to memory; many rows by reading X from LDS (half the time of the last case) and turning codes into
+// numbers (a third), for which every wavefront's 16 or 32 columns pay anew.  The sums of X taken by the matrix product itself, with ones in
+// the weights' place, cost the last case 1.5 us.
 // Parameters: Q4_NAME, Q4_N, Q4_K, Q4_GROUP, Q4_F16, Q4_ZERO, Q4_ST (type of the scales), Q4_YT (of the result), Q4_MB, Q4_MR (rows of X in
-// LDS, up to 16 Q4_MB), Q4_NT, Q4_WN, Q4_WK, Q4_SPLIT, Q4_DEPTH (steps under way in registers), Q4_WIDE, Q4_JOIN (this is gemm_q4_join).
+// LDS, up to 16 Q4_MB), Q4_NT, Q4_WN, Q4_WK, Q4_SPLIT, Q4_WIDE, Q4_JOIN (this is gemm_q4_join).
 typedef _Float16 q4_f16x8 __attribute__((ext_vector_type(8)));
 #if Q4_F16
 typedef _Float16 q4_x;
 #define Q4_MFMA(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q4_f16x8, a), __builtin_bit_cast(q4_f16x8, b), c, 0, 0, 0)
 #define Q4_ONE 0x3c003c00u
 #define Q4_MASK 0x03c003c0u
+#define Q4_DOT(a, c) __builtin_amdgcn_fdot2(__builtin_bit_cast(kcg_f16x2, a), __builtin_bit_cast(kcg_f16x2, Q4_ONE), c, false)
 #define Q4_SHIFT(w, p) ((p) == 0 ? (w) << 6 : (p) == 1 ? (w) << 2 : (p) == 2 ? (w) >> 2 : (w) >> 6)
 #else
 typedef __bf16 q4_x;
 #define Q4_MFMA(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(kcg_bf16x8, a), __builtin_bit_cast(kcg_bf16x8, b), c, 0, 0, 0)
 #define Q4_ONE 0x3f803f80u
 #define Q4_MASK 0x00780078u
+#define Q4_DOT(a, c) __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(kcg_bf16x2, a), __builtin_bit_cast(kcg_bf16x2, Q4_ONE), c, false)
 #define Q4_SHIFT(w, p) ((p) == 0 ? (w) << 3 : (p) == 1 ? (w) >> 1 : (p) == 2 ? (w) >> 5 : (w) >> 9)
 #endif
 #define Q4_STEPS ((Q4_K + 255) / 256)
@@ -69,7 +76,7 @@ struct Q4Step {
   unsigned char z[Q4_SC];
 };
 
-extern "C" __global__ __launch_bounds__(64 * Q4_WN * Q4_WK, Q4_OCC)
+extern "C" __global__ __launch_bounds__(64 * Q4_WN * Q4_WK, 1)
 void Q4_NAME(const q4_x* __restrict__ X, const unsigned char* __restrict__ W, const Q4_ST* __restrict__ scale, const unsigned char* __restrict__ zero,
              long long M_,
 #if Q4_SPLIT > 1
@@ -81,6 +88,7 @@ void Q4_NAME(const q4_x* __restrict__ X, const unsigned char* __restrict__ W, co
   struct Tiles {
     __attribute__((aligned(16))) unsigned char x[Q4_WK][Q4_WN > 1 ? 2 : 1][Q4_MR * Q4_XPITCH], w[Q4_WK * Q4_WN][Q4_COLS * Q4_WPITCH];
     kcg_f32x2 s[Q4_WK * Q4_WN][2 * Q4_PER][Q4_COLS];
+    __attribute__((aligned(16))) float u[Q4_WK][Q4_WN > 1 ? 2 : 1][2 * Q4_PER][16 * Q4_MB];        // sums of X of a group
   };
   union Shared {
     Tiles t;
@@ -145,7 +153,7 @@ void Q4_NAME(const q4_x* __restrict__ X, const unsigned char* __restrict__ W, co
 #pragma unroll
     for (int c = 0; c < Q4_XC; ++c) s.x[c] = *(const kcg_u32x4*)(xk0 + (Q4_K % 256 == 0 || k0 + xk[c] < Q4_K ? xo[c] : xo[c] - xk[c]));
   };
-  auto stage = [&](int n, Q4Step& s, unsigned char* xs) {
+  auto stage = [&](int n, Q4Step& s, unsigned char* xs, float* us) {
     const int k0 = (first + n) * 256;
 #pragma unroll
     for (int c = 0; c < Q4_XC; ++c) {
@@ -153,17 +161,23 @@ void Q4_NAME(const q4_x* __restrict__ X, const unsigned char* __restrict__ W, co
       const kcg_u32x4 o = {__builtin_amdgcn_perm(v[2], v[0], 0x05040100u), __builtin_amdgcn_perm(v[2], v[0], 0x07060302u),
                            __builtin_amdgcn_perm(v[3], v[1], 0x05040100u), __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)};
       if (Q4_MR * 32 % (64 * Q4_WN) == 0 || xat[c] >= 0) *(kcg_u32x4*)(xs + xat[c]) = o;
+      // the sum over the lanes that have a group of the row (16, 8 or 4), times -1.5 where that is 1 + zero / 16 for all columns
+      const unsigned v0 = v[0], v1 = v[1], v2 = v[2], v3 = v[3];      // (bit_cast of a vector's element takes the first)
+      float sum = Q4_DOT(v0, Q4_DOT(v1, Q4_DOT(v2, Q4_DOT(v3, 0.0f))));
+      sum += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, sum), 0xb1, 0xf, 0xf, true));      // quad_perm: 1 0 3 2
+      sum += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, sum), 0x4e, 0xf, 0xf, true));      // quad_perm: 2 3 0 1
+      if (Q4_PER < 4) sum += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, sum), 0x141, 0xf, 0xf, true));      // row_half_mirror
+      if (Q4_PER < 2) sum += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, sum), 0x140, 0xf, 0xf, true));      // row_mirror
+      if (lane % (16 / Q4_PER) == 0 && xat[c] >= 0) us[(lane % 32) / (16 / Q4_PER) * (16 * Q4_MB) + xat[c] / Q4_XPITCH] = Q4_ZERO ? sum : -1.5f * sum;
     }
 #pragma unroll
     for (int b = 0; b < 2 * Q4_NT; ++b) *(kcg_u32x4*)(sh.t.w[wave] + (b * 8 + lane / 8) * Q4_WPITCH + lane % 8 * 16) = s.w[b];
 #pragma unroll
     for (int c = 0; c < Q4_SC; ++c)
       if (Q4_COLS * 2 * Q4_PER % 64 == 0 || sat[c] >= 0)
-        (&sh.t.s[wave][0][0])[sat[c]] = kcg_f32x2{(float)s.s[c], Q4_ZERO ? -1.0f - (float)s.z[c] * 0.0625f : -1.5f};
+        (&sh.t.s[wave][0][0])[sat[c]] = kcg_f32x2{(float)s.s[c], Q4_ZERO ? -1.0f - (float)s.z[c] * 0.0625f : 0.0f};
   };
-  auto multiply = [&](const unsigned char* xs) {
-    const kcg_f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
-    const kcg_u32x4 ones = {one, one, one, one};
+  auto multiply = [&](const unsigned char* xs, const float* us) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       kcg_u32x4 w4[Q4_NT];
@@ -181,12 +195,17 @@ void Q4_NAME(const q4_x* __restrict__ X, const unsigned char* __restrict__ W, co
       }
 #pragma unroll
       for (int p = 0; p < Q4_PER; ++p) {
-        kcg_f32x4 u[Q4_MB], t[Q4_MB][Q4_NT];
+        kcg_f32x4 t[Q4_MB][Q4_NT];
+        float by[Q4_NT];
 #pragma unroll
-        for (int a = 0; a < Q4_MB; ++a) {
-          u[a] = none;
+        for (int b = 0; b < Q4_NT; ++b) {
+          const kcg_f32x2 s = sh.t.s[wave][h * Q4_PER + p][b * 16 + i];
+          by[b] = s[0];
 #pragma unroll
-          for (int b = 0; b < Q4_NT; ++b) t[a][b] = none;
+          for (int a = 0; a < Q4_MB; ++a) {
+            t[a][b] = *(const kcg_f32x4*)(us + (h * Q4_PER + p) * (16 * Q4_MB) + a * 16 + g * 4);
+            if (Q4_ZERO) t[a][b] *= s[1];
+          }
         }
 #pragma unroll
         for (int j = p * Q4_J; j < (p + 1) * Q4_J; ++j) {
@@ -195,7 +214,6 @@ void Q4_NAME(const q4_x* __restrict__ X, const unsigned char* __restrict__ W, co
           for (int a = 0; a < Q4_MB; ++a) {
             const int row = a * 16 + i < Q4_MR ? a * 16 + i : Q4_MR - 1;
             x[a] = *(const kcg_u32x4*)(xs + row * Q4_XPITCH + h * 256 + (Q4_PER == 1 ? g * 4 + j : j * 4 + g) * 16);
-            u[a] = Q4_MFMA(x[a], ones, u[a]);
           }
 #pragma unroll
           for (int b = 0; b < Q4_NT; ++b) {
@@ -206,40 +224,31 @@ void Q4_NAME(const q4_x* __restrict__ X, const unsigned char* __restrict__ W, co
           }
         }
 #pragma unroll
-        for (int b = 0; b < Q4_NT; ++b) {
-          const kcg_f32x2 s = sh.t.s[wave][h * Q4_PER + p][b * 16 + i];
+        for (int b = 0; b < Q4_NT; ++b)
 #pragma unroll
           for (int a = 0; a < Q4_MB; ++a)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[a][b][r] = __builtin_fmaf(s[0], __builtin_fmaf(s[1], u[a][r], t[a][b][r]), acc[a][b][r]);
-        }
+            for (int r = 0; r < 4; ++r) acc[a][b][r] = __builtin_fmaf(by[b], t[a][b][r], acc[a][b][r]);
       }
     }
   };
 
-  // Every wavefront makes Q4_SHARE steps; one that has fewer multiplies zeros in those behind its last.  All passes over the registers but
-  // the last load ahead: what they load is used, but for a few steps where the last pass is not a whole one.
-  Q4Step ring[Q4_DEPTH];
-  auto pass = [&](int from, int steps, bool more) __attribute__((always_inline)) {
-#pragma unroll
-    for (int d = 0; d < Q4_DEPTH; ++d) {
-      if (d >= steps) break;
-      __builtin_amdgcn_sched_barrier(0);
-      unsigned char* xs = sh.t.x[wk][Q4_WN > 1 ? (Q4_DEPTH % 2 ? (from + d) & 1 : d & 1) : 0];
-      stage(from + d, ring[d], xs);
-      if (more) load(from + d + Q4_DEPTH, ring[d]);
-      // the rows of X are there, and those of the step before last have been read (a wavefront's own LDS accesses are carried out in order)
-      if (Q4_WN > 1) __syncthreads(); else __builtin_amdgcn_wave_barrier();
-      multiply(xs);
-    }
+  // Every wavefront makes Q4_SHARE steps; one that has fewer multiplies zeros in those behind its last.  A step is under way in registers
+  // while the one before it is multiplied (two or three were no faster in any form).
+  Q4Step next;
+  load(0, next);
+  auto step = [&](int n, bool more) __attribute__((always_inline)) {
+    const int buffer = Q4_WN > 1 ? n & 1 : 0;
+    __builtin_amdgcn_sched_barrier(0);
+    stage(n, next, sh.t.x[wk][buffer], &sh.t.u[wk][buffer][0][0]);
+    if (more) load(n + 1, next);
+    // the rows of X are there, and those of the step before last have been read (a wavefront's own LDS accesses are carried out in order)
+    if (Q4_WN > 1) __syncthreads(); else __builtin_amdgcn_wave_barrier();
+    multiply(sh.t.x[wk][buffer], &sh.t.u[wk][buffer][0][0]);
   };
-#pragma unroll
-  for (int d = 0; d < Q4_DEPTH; ++d)
-    if (d < Q4_SHARE) load(d, ring[d]);
-  constexpr int PASSES = (Q4_SHARE + Q4_DEPTH - 1) / Q4_DEPTH, REST = Q4_SHARE - (PASSES - 1) * Q4_DEPTH;
 #pragma unroll 1
-  for (int p = 0; p < PASSES - 1; ++p) pass(p * Q4_DEPTH, Q4_DEPTH, true);
-  pass((PASSES - 1) * Q4_DEPTH, REST, false);
+  for (int n = 0; n < Q4_SHARE - 1; ++n) step(n, true);
+  step(Q4_SHARE - 1, false);
   __syncthreads();
 #pragma unroll
   for (int a = 0; a < Q4_MB; ++a)

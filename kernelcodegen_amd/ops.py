@@ -554,10 +554,11 @@ def matmul_q4(x, w, scale, zero=None, out_dtype=None, **cfg):
         hit = _matmul_q4_launch(x, w, scale, zero, out_dtype, cfg)
         if not cfg:
             _bound[key] = hit
-    run, rows = hit
+    run, join, rows = hit
     if rows == 0:
         return torch.empty(x.shape[:-1] + (w.shape[0],), dtype=out_dtype or x.dtype, device=x.device)
-    return run(x, w, scale, 0 if zero is None else zero, rows)
+    out = run(x, w, scale, 0 if zero is None else zero, rows)
+    return out if join is None else join(out, rows)
 
 
 def _matmul_q4_launch(x, w, scale, zero, out_dtype, cfg):
@@ -578,9 +579,42 @@ def _matmul_q4_launch(x, w, scale, zero, out_dtype, cfg):
     if (x.data_ptr() | w.data_ptr()) % 16:
         raise ValueError("x and w must start on multiples of 16 bytes")
     rows = math.prod(x.shape[:-1])
-    blocks = 1 if rows <= 16 else 2 if rows <= 32 else 4
     if rows == 0:
-        return None, 0
-    kern = R.get_kernel("gemm_q4", N=n, K=k, GROUP=group, F16=int(x.dtype == torch.float16), ZERO=int(zero is not None),
-                        SCALE_F32=int(scale.dtype == torch.float32), OUT_F32=int(out_dtype == torch.float32), MB=blocks, **cfg)
-    return _into_last(kern.bind(grid=(kern.info["grid"][0], -(-rows // (16 * blocks)))), (tuple(x.shape[:-1]) + (n,), out_dtype)), rows
+        return None, None, 0
+    if not cfg.keys() <= {"MB", "MR", "NT", "WN", "WK", "SPLIT"}:
+        raise ValueError("unknown kernel parameters")
+    params = dict(N=n, K=k, GROUP=group, F16=int(x.dtype == torch.float16), ZERO=int(zero is not None), SCALE_F32=int(scale.dtype == torch.float32),
+                  OUT_F32=int(out_dtype == torch.float32), **{**_matmul_q4_form(rows, n, k, group), **cfg})
+    kern = R.get_kernel("gemm_q4", **params)
+    shape, split = tuple(x.shape[:-1]) + (n,), kern.info["grid"][2]
+    grid = (kern.info["grid"][0], -(-rows // (16 * params["MB"])), split)
+    if split == 1:
+        return _into_last(kern.bind(grid=grid), (shape, out_dtype)), None, rows
+    join = R.get_kernel("gemm_q4_join", **params).bind(grid=(-(-rows * n // 256),))
+    return _into_last(kern.bind(grid=grid), ((split, rows, n), torch.float32)), _into_last(join, (shape, out_dtype)), rows
+
+
+def _matmul_q4_form(rows, n, k, group):
+    """The tiles and the splitting of k, by the columns of a workgroup and the rows of X that every workgroup reads again.
+
+    Up to 16 rows, a wavefront's 16 columns are a workgroup while few workgroups read few rows (a product with its neighbours' would need
+    fewer, but wait for one another), else 64 columns; more rows take 64 columns and two shares of k in a workgroup, or, where there is more
+    to do, 256 columns, 32 to a wavefront, which reads the rows from LDS half as often.  A form whose workgroups do not fill the 256 units
+    splits k, at two launches' price, where a wavefront has four steps of 256 k or more.  Measured, in us (bf16, groups of 128):
+      rows 1, N = K = 4096: 16 columns 4.2, 64 columns with k split 6.2;  1, N 32000, K 4096: 18.9, 17.1
+      rows 16, N = K = 4096: 6.0, 7.1;  4, N 11008, K 4096: 7.6, 8.3;  8: 9.5, 8.9;  16: 14.9, 10.0
+      rows 32, N = K = 4096: 64 columns 8.2, 256 columns 8.9;  64: 12.4, 12.9;  128: 17.1, 15.7
+      rows 32, N 4096, K 11008: 15.2, 13.9;  64: 24.1, 21.3;  128: 37.0, 28.6;  64, N 32000, K 4096: 51.6, 39.3
+      rows 64, N 1024, K 4096: k in four 9.9, in eight 8.2;  N = K = 1024: in one 7.5, in two 7.3"""
+    blocks = min(4, -(-rows // 16))
+    form = dict(MB=blocks, NT=1, WN=4, WK=2)
+    if blocks == 1:
+        form["MR"] = 1 << (rows - 1).bit_length()
+        tall = -(-n // 16)
+        form.update(dict(WN=1, WK=8) if tall <= 1024 and tall * form["MR"] <= 4096 else dict(NT=2, WN=2, WK=4))
+    elif n * k * -(-rows // 64) >= 1 << 25 or (blocks == 4 and group == 32):        # (64 rows, two shares and groups of 32: LDS is too small)
+        form.update(NT=2, WN=8, WK=1)
+    workgroups = -(-n // (16 * form["NT"] * form["WN"])) * -(-rows // (16 * blocks))
+    steps = -(-k // 256) // form["WK"]
+    form["SPLIT"] = max(1, min(256 // workgroups, steps, 64)) if form["WN"] > 1 and steps >= 4 else 1
+    return form

@@ -408,7 +408,8 @@ def test_cache_attention_offsets_beyond_32_bits():
 @pytest.mark.parametrize("m,n,k,group,zero,scale32,out32", [
     (1, 16, 128, 128, False, False, False), (1, 1, 32, 32, True, True, True), (3, 37, 96, 32, True, False, True), (16, 100, 4096, 128, True, False, False),
     (17, 333, 1088, 64, False, True, False), (33, 48, 1024, 256, True, False, True), (64, 129, 544, 32, False, False, False), (130, 65, 1920, 64, True, False, False),
-    (5, 1001, 2176, 128, True, True, True), (2, 4097, 640, 640, False, False, False)])
+    (5, 1001, 2176, 128, True, True, True), (2, 4097, 640, 640, False, False, False), (9, 8203, 288, 32, True, False, False), (16, 4211, 4160, 64, False, False, False),
+    (20, 2100, 16384, 128, True, False, False), (70, 1030, 16448, 64, False, True, True), (33, 200, 4352, 128, False, False, False)])
 def test_matmul_q4(dtype, m, n, k, group, zero, scale32, out32):
     g = generator(m * n + k)
     x = (torch.randn((m, k), generator=g, device="cuda") + 0.5).to(DTYPE[dtype])
@@ -442,6 +443,18 @@ def test_matmul_q4_keeps_infinities_to_their_rows():
     w, s = torch.full((20, 64), 0x99, device="cuda", dtype=torch.uint8), torch.ones((20, 1), device="cuda", dtype=torch.bfloat16)
     got = ops.matmul_q4(x, w, s)
     assert bool(got[3].isnan().all()) and bool((got[[0, 1, 2, 4]] == 128).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_matmul_q4_of_subnormal_rows(dtype):
+    # the rows times 2^-20 are subnormal in half precision; they are whole multiples of 2^-20, and sums of 512 of them times a code need no more
+    # than 24 bits, so that the result is 2^-20 of the other one
+    x = (torch.arange(3 * 512, device="cuda").view(3, 512) % 13 + 16).to(DTYPE[dtype])
+    w = torch.arange(24 * 256, device="cuda").view(24, 256).mul(37).to(torch.uint8)
+    s = torch.ones((24, 4), device="cuda", dtype=torch.float32)
+    want = ops.matmul_q4(x, w, s, out_dtype=torch.float32)
+    got = ops.matmul_q4(x * 2.0 ** -20, w, s, out_dtype=torch.float32)
+    assert torch.equal(got * 2.0 ** 20, want)
 
 
 # ---- refusals, streams ----
