@@ -1661,14 +1661,14 @@ bool emitPageSlots(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std:
 
 bool emitCacheWrite(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::string& err) {
   if (!cacheShape(s, {"KP", "KT", "KH", "VP", "VT", "VH"}, err)) return false;
-  if (!whole(s, "F16", 0, 2, err) || !whole(s, "WIN", 1, 64, err)) return false;
+  if (!whole(s, "F16", 0, 2, err) || !whole(s, "WIN", 1, 16, err)) return false;
   const int64_t esize = s.p["F16"] ? 2 : 4;
   for (auto key : {"XKT", "XKH", "XVT", "XVH"})
     if (!whole(s, key, 0, (int64_t)1 << 40, err)) return false;
     else if (s.p[key] * esize % 16) { err = std::string("cache_write: ") + key + " must be a multiple of 16 bytes"; return false; }
   Defines d;
   d.add("CW_NAME", s.name);
-  d.add("CW_T", std::string(typeName(s.p["F16"])));
+  d.add("CW_T", std::string(typeName(s.p["F16"]))); d.add("CW_ESIZE", esize);
   for (auto key : {"H", "D", "PAGE", "WIN"}) d.add(std::string("CW_") + key, s.p[key]);
   for (auto key : {"KP", "KT", "KH", "VP", "VT", "VH", "XKT", "XKH", "XVT", "XVH"}) d.add(std::string("CW_") + key, std::to_string(s.p[key]) + "LL");
   src = d.wrap(kTpl_cache_write);

@@ -5,7 +5,20 @@
 // Every workgroup takes the prefix sums of all requests (1024 at a time) and then its share of the pages and tokens, each found by
 // bisection in the sums in LDS: a step of any shape is one launch with two dependent reads per token.
 // Parameters: PS_NAME, PS_BLOCK.
-struct PsSums { int pages[PS_BLOCK + 1], tokens[PS_BLOCK + 1], waves[2][PS_BLOCK / 64]; };
+struct PsSums { int pages[PS_BLOCK + 1], tokens[PS_BLOCK + 1], lengths[PS_BLOCK], waves[2][PS_BLOCK / 64]; };
+
+// Sum over the lanes up to and including this one.
+__device__ __forceinline__ int ps_scan(int v) {
+#define PS_DPP(control, rows) v += __builtin_amdgcn_update_dpp(0, v, control, rows, 0xf, false)
+  PS_DPP(0x111, 0xf);        // row_shr 1, 2, 4, 8: over the 16 lanes of a row
+  PS_DPP(0x112, 0xf);
+  PS_DPP(0x114, 0xf);
+  PS_DPP(0x118, 0xf);
+  PS_DPP(0x142, 0xa);        // a row's last lane into the next row, for the second and the fourth,
+  PS_DPP(0x143, 0xc);        // the second row's into the third and the fourth
+#undef PS_DPP
+  return v;
+}
 
 extern "C" __global__ __launch_bounds__(PS_BLOCK)
 void PS_NAME(const int* __restrict__ lengths, const int* __restrict__ added, int* __restrict__ table, const int* __restrict__ free_pages,
@@ -22,16 +35,17 @@ void PS_NAME(const int* __restrict__ lengths, const int* __restrict__ added, int
       len = lengths[b] > 0 ? lengths[b] : 0;
       add = added[b] > 0 ? added[b] : 0;
     }
-    int p = (len + add + page - 1) / page - (len + page - 1) / page, t = add;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int op = __shfl_up(p, off, 64), ot = __shfl_up(t, off, 64);
-      if (lane >= off) { p += op; t += ot; }
-    }
+    const int p = ps_scan((len + add + page - 1) / page - (len + page - 1) / page), t = ps_scan(add);
     if (lane == 63) { s.waves[0][wave] = p; s.waves[1][wave] = t; }
     __syncthreads();
     int pb = 0, tb = 0;
-    for (int w = 0; w < wave; ++w) { pb += s.waves[0][w]; tb += s.waves[1][w]; }
+#pragma unroll
+    for (int w = 0; w < PS_BLOCK / 64 - 1; ++w) {
+      const int pw = s.waves[0][w], tw = s.waves[1][w];
+      pb += w < wave ? pw : 0;
+      tb += w < wave ? tw : 0;
+    }
+    s.lengths[threadIdx.x] = len;
     s.pages[threadIdx.x + 1] = pb + p;
     s.tokens[threadIdx.x + 1] = tb + t;
     if (threadIdx.x == 0) s.pages[0] = s.tokens[0] = 0;
@@ -51,12 +65,12 @@ void PS_NAME(const int* __restrict__ lengths, const int* __restrict__ added, int
       return lo;
     };
     for (int i = first; i < s.pages[n]; i += step) {
-      const int r = find(s.pages, i), have = lengths[b0 + r] > 0 ? lengths[b0 + r] : 0;
+      const int r = find(s.pages, i), have = s.lengths[r];
       const int column = (have + page - 1) / page + i - s.pages[r];
       if (column < W && pages0 + i < F) table[(long long)(b0 + r) * table_row + column] = free_pages[pages0 + i];
     }
     for (int i = first; i < s.tokens[n] && tokens0 + i < T; i += step) {
-      const int r = find(s.tokens, i), have = lengths[b0 + r] > 0 ? lengths[b0 + r] : 0;
+      const int r = find(s.tokens, i), have = s.lengths[r];
       const int before = (have + page - 1) / page, at = have + i - s.tokens[r], column = at / page;
       int id = -1;
       if (column < W) {
@@ -67,7 +81,7 @@ void PS_NAME(const int* __restrict__ lengths, const int* __restrict__ added, int
           if (k < F) id = free_pages[k];
         }
       }
-      slots[tokens0 + i] = id < 0 ? -1 : (long long)id * page + at % page;
+      slots[tokens0 + i] = id < 0 ? -1 : (long long)id * page + (at - column * page);
       positions[tokens0 + i] = at;
     }
     pages0 += s.pages[n];

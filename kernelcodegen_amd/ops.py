@@ -426,7 +426,7 @@ def _cache_write_launch(k, v, k_cache, v_cache, k_scale, v_scale, slots):
     ks, vs = _cache_strides(k_cache, k_scale), _cache_strides(v_cache, v_scale)
     xk, xv = _row_strides(k, k_cache, _STORAGE), _row_strides(v, v_cache, _STORAGE)
     tokens, heads, d = k.shape
-    if heads != k_cache.shape[2] or tuple(slots.shape) != (tokens,) or tokens > 0x7FFFFFFF:
+    if heads != k_cache.shape[2] or tuple(slots.shape) != (tokens,) or tokens > 0x7FFFFE00:
         raise ValueError("one slot per token, and the cache's heads, are needed")
     win = 1 if tokens <= 512 else 16
     kern = R.get_kernel("cache_write", H=heads, D=d, PAGE=k_cache.shape[1], F16=_STORAGE[k.dtype], WIN=win, KP=ks[0], KT=ks[1], KH=ks[2],
