@@ -76,7 +76,7 @@ def build_launch(force=False, verbose=False):
                "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, '-DKCG_TORCH_VERSION="%s"' % torch.__version__,
                "-I", inc, "-I", os.path.join(inc, "torch", "csrc", "api", "include"),
                "-I", os.path.join(ROCM, "include"), "-I", sysconfig.get_paths()["include"], src, "-o", LAUNCH, "-L", os.path.join(base, "lib"),
-               "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"]
+               "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"]
         stamp = hashlib.sha256((open(src).read() + " ".join(cmd)).encode()).hexdigest()
         if not force and os.path.exists(LAUNCH) and os.path.exists(stamp_file) and open(stamp_file).read() == stamp:
             return LAUNCH

@@ -1649,13 +1649,14 @@ bool emitPageSlots(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std:
   const int64_t block = s.get("BLOCK", 1024);
   if (block < 64 || block > 1024 || block % 64) { err = "page_slots: BLOCK must be a multiple of 64 up to 1024"; return false; }
   s.p["BLOCK"] = block;
+  if (!whole(s, "PAGE", 1, 0x7FFFFFFF, err)) return false;
   Defines d;
   d.add("PS_NAME", s.name);
-  d.add("PS_BLOCK", block);
+  d.add("PS_BLOCK", block); d.add("PS_PAGE", s.p["PAGE"]);
   src = d.wrap(kTpl_page_slots);
   info.name = s.name;
   info.block[0] = (uint32_t)block;
-  info.numArgs = 15;
+  info.numArgs = 14;
   return true;
 }
 

@@ -2,9 +2,10 @@
 //   before_b = ceil(length_b / page), after_b = ceil((length_b + added_b) / page); request b takes after_b - before_b pages off the list
 //   of free ones, those of earlier requests first, and its table is continued with them; its new tokens get the positions from
 //   length_b on and the slots table[position / page] * page + position % page (-1 where there is no page)
-// Every workgroup takes the prefix sums of all requests (1024 at a time) and then its share of the pages and tokens, each found by
-// bisection in the sums in LDS: a step of any shape is one launch with two dependent reads per token.
-// Parameters: PS_NAME, PS_BLOCK.
+// Every workgroup takes the prefix sums of all requests (PS_BLOCK at a time) and then its share of the pages and tokens, each found in the
+// sums in LDS: a step of any shape is one launch.  Bound by what waits for one another: the lengths, the sums, the table or the
+// list, the stores.
+// Parameters: PS_NAME, PS_BLOCK, PS_PAGE.
 struct PsSums { int pages[PS_BLOCK + 1], tokens[PS_BLOCK + 1], lengths[PS_BLOCK], waves[2][PS_BLOCK / 64]; };
 
 // Sum over the lanes up to and including this one.
@@ -22,10 +23,11 @@ __device__ __forceinline__ int ps_scan(int v) {
 
 extern "C" __global__ __launch_bounds__(PS_BLOCK)
 void PS_NAME(const int* __restrict__ lengths, const int* __restrict__ added, int* __restrict__ table, const int* __restrict__ free_pages,
-             long long B_, long long T_, long long W_, long long table_row, long long F_, long long page_, long long* __restrict__ slots,
+             long long B_, long long T_, long long W_, long long table_row, long long F_, long long* __restrict__ slots,
              int* __restrict__ positions, int* __restrict__ starts, int* __restrict__ lengths_out, int* __restrict__ used) {
   __shared__ PsSums s;
-  const int B = (int)B_, T = (int)T_, W = (int)W_, F = (int)F_, page = (int)page_;
+  const int B = (int)B_, T = (int)T_, W = (int)W_, F = (int)F_;
+  constexpr int page = PS_PAGE;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = blockIdx.x * PS_BLOCK + threadIdx.x, step = gridDim.x * PS_BLOCK;
   int pages0 = 0, tokens0 = 0;                 // of the requests before this round's
   for (int b0 = 0; b0 < B; b0 += PS_BLOCK) {
@@ -55,34 +57,36 @@ void PS_NAME(const int* __restrict__ lengths, const int* __restrict__ added, int
       lengths_out[b] = len + add;
       if (b == 0) starts[0] = 0;
     }
-    // which request of this round: the last whose sum before it is not over `i`
+    // Which request of this round: the last whose sum before it is not over `i`.  Of eight parts at a time, since the reads of one step are
+    // under way together: a round of 256 takes three.
     auto find = [&](const int* sums, int i) {
-      int lo = 0, hi = n - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (sums[mid] <= i) lo = mid; else hi = mid - 1;
+      int lo = 0;
+#pragma unroll
+      for (int part = PS_BLOCK > 512 ? 512 : 64; part > 0; part /= 8) {
+        const int from = lo;
+#pragma unroll
+        for (int j = 1; j < 8 && j * part < PS_BLOCK; ++j) {
+          const int at = from + j * part;
+          lo = sums[at < n ? at : n] <= i && at < n ? at : lo;
+        }
       }
       return lo;
     };
-    for (int i = first; i < s.pages[n]; i += step) {
-      const int r = find(s.pages, i), have = s.lengths[r];
-      const int column = (have + page - 1) / page + i - s.pages[r];
-      if (column < W && pages0 + i < F) table[(long long)(b0 + r) * table_row + column] = free_pages[pages0 + i];
-    }
-    for (int i = first; i < s.tokens[n] && tokens0 + i < T; i += step) {
-      const int r = find(s.tokens, i), have = s.lengths[r];
-      const int before = (have + page - 1) / page, at = have + i - s.tokens[r], column = at / page;
-      int id = -1;
-      if (column < W) {
-        if (column < before) {
-          id = table[(long long)(b0 + r) * table_row + column];
-        } else {
-          const int k = pages0 + s.pages[r] + column - before;
-          if (k < F) id = free_pages[k];
-        }
+    // page i off the list and token i: both numbers' loads, from some length where there is none, then the stores
+    const int pages = s.pages[n], tokens = s.tokens[n], most = pages > tokens ? pages : tokens;
+    for (int i = first; i < most; i += step) {
+      const int rp = find(s.pages, i), place = (s.lengths[rp] + page - 1) / page + i - s.pages[rp];
+      const bool put = i < pages && place < W && pages0 + i < F;
+      const int fresh = *(put ? free_pages + pages0 + i : lengths);
+      const int r = find(s.tokens, i), have = s.lengths[r], at = have + i - s.tokens[r], before = (have + page - 1) / page, column = at / page;
+      const int k = pages0 + s.pages[r] + column - before;
+      const bool token = i < tokens && tokens0 + i < T, old = column < before, page_there = token && column < W && (old || k < F);
+      const int id = *(!page_there ? lengths : old ? table + (long long)(b0 + r) * table_row + column : free_pages + k);
+      if (put) table[(long long)(b0 + rp) * table_row + place] = fresh;
+      if (token) {
+        slots[tokens0 + i] = !page_there || id < 0 ? -1 : (long long)id * page + (at - column * page);
+        positions[tokens0 + i] = at;
       }
-      slots[tokens0 + i] = id < 0 ? -1 : (long long)id * page + (at - column * page);
-      positions[tokens0 + i] = at;
     }
     pages0 += s.pages[n];
     tokens0 += s.tokens[n];

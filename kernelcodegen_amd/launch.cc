@@ -15,7 +15,8 @@
 //   launch.result(shape, dtype)            a Launch whose call leaves the last pointer out: call(tensor, ..., number, ...)
 //                                          allocates it on the first tensor's device and returns it
 //   launch.result(None, None)              the result is like the first tensor
-//   launch.results((shape, dtype), ...)    a Launch whose call leaves the last pointers out and returns a tuple of their tensors
+//   launch.results((shape, dtype), ...)    a Launch whose call leaves the last pointers out and returns a tuple of their tensors,
+//                                          parts of one allocation
 //   signature(tensor or None, ...)         what a kernel can depend on of its operands, as bytes: device, type, sizes, strides and how
 //                                          far each address is from a multiple of 16
 #include <torch/csrc/Exceptions.h>
@@ -23,6 +24,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -53,6 +55,19 @@ struct Launch {
 int launch(const Launch* self, const uint64_t* slots) {
   void* stream = (void*)c10::hip::getCurrentHIPStream().stream();
   return self->entry(self->handle, self->dims, stream, slots, self->pointers + self->scalars);
+}
+
+// A new tensor on `like`'s device: on the part without the dispatcher, which takes as long as the allocation itself.
+at::Tensor fresh(const at::Tensor& like, at::IntArrayRef shape, at::ScalarType dtype) {
+  if (like.is_cuda()) return at::Tensor(at::detail::empty_cuda(shape, dtype, like.device(), std::nullopt));
+  return at::empty(shape, like.options().dtype(dtype).requires_grad(false));
+}
+
+// The bytes of a result, up to the next multiple of 256.
+int64_t bytesOf(const std::vector<int64_t>& shape, at::ScalarType dtype) {
+  int64_t n = (int64_t)c10::elementSize(dtype);
+  for (int64_t s : shape) n *= s;
+  return (n + 255) / 256 * 256;
 }
 
 bool scalar(PyObject* o, uint64_t& slot) {
@@ -114,11 +129,20 @@ PyObject* callLaunch(PyObject* me, PyObject* const* args, size_t nargsf, PyObjec
     std::vector<at::Tensor> outs;
     outs.reserve(self->several->size());
     {
-      const auto options = THPVariable_Unpack(args[0]).options().requires_grad(false);
+      const at::Tensor& like = THPVariable_Unpack(args[0]);
       pybind11::gil_scoped_release unlocked;
+      // one allocation, of which each result is a part that begins at a multiple of 256 bytes: one each takes 0.6 us
+      int64_t bytes = 0;
+      for (const auto& [shape, dtype] : *self->several) bytes += bytesOf(shape, dtype);
+      const at::Tensor all = fresh(like, {bytes}, at::kByte);
+      int64_t at = 0;
       for (const auto& [shape, dtype] : *self->several) {
-        outs.push_back(at::empty(shape, options.dtype(dtype)));
-        slots[given + outs.size() - 1] = (uint64_t)(uintptr_t)outs.back().data_ptr();
+        auto part = c10::make_intrusive<at::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(dtype));
+        part->set_storage_offset(at / (int64_t)c10::elementSize(dtype));
+        part->set_sizes_contiguous(shape);
+        outs.emplace_back(std::move(part));
+        slots[given + outs.size() - 1] = (uint64_t)(uintptr_t)all.data_ptr() + (uint64_t)at;
+        at += bytesOf(shape, dtype);
       }
       rc = launch(self, slots);
     }
@@ -139,7 +163,7 @@ PyObject* callLaunch(PyObject* me, PyObject* const* args, size_t nargsf, PyObjec
   {
     const at::Tensor& like = THPVariable_Unpack(args[0]);
     pybind11::gil_scoped_release unlocked;
-    out = self->result == 2 ? at::empty_like(like) : at::empty(*self->shape, like.options().dtype(self->dtype).requires_grad(false));
+    out = self->result == 2 ? at::empty_like(like) : fresh(like, *self->shape, self->dtype);
     slots[given] = (uint64_t)(uintptr_t)out.data_ptr();
     rc = launch(self, slots);
   }

@@ -356,7 +356,7 @@ def page_slots(lengths, added, table, free, page_size, tokens):
     run = _bound.get(key)
     if run is None:
         _bound[key] = run = _page_slots_launch(lengths, added, table, free, page_size, tokens)
-    return run(lengths, added, table, free, table.shape[0], tokens, table.shape[1], table.stride(0), free.shape[0], page_size)
+    return run(lengths, added, table, free, table.shape[0], tokens, table.shape[1], table.stride(0), free.shape[0])
 
 
 def _page_slots_launch(lengths, added, table, free, page_size, tokens):
@@ -365,11 +365,11 @@ def _page_slots_launch(lengths, added, table, free, page_size, tokens):
         raise ValueError("lengths and added are [B], table is [B, W], free is [F]")
     if not table.is_cuda or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
         raise ValueError("the table must be an int32 device tensor with rows of neighbouring entries")
-    if page_size < 1 or tokens < 0 or tokens > 0x7FFFFFFF:
+    if not 1 <= page_size <= 0x7FFFFFFF or tokens < 0 or tokens > 0x7FFFFFFF:
         raise ValueError("bad page size or number of tokens")
     batch = table.shape[0]
     # two tokens a lane, as far as that needs no more workgroups than the part has CUs
-    kern = R.get_kernel("page_slots", BLOCK=1024 if batch > 256 or tokens > 512 else 256)
+    kern = R.get_kernel("page_slots", PAGE=page_size, BLOCK=1024 if batch > 256 or tokens > 512 else 256)
     i32 = torch.int32
     return _into_last(kern.bind(grid=(max(1, min(256, -(-tokens // 2048))),)), ((tokens,), torch.int64), ((tokens,), i32), ((batch + 1,), i32), ((batch,), i32),
                       ((1,), i32))

@@ -457,6 +457,18 @@ def test_matmul_q4_of_subnormal_rows(dtype):
     assert torch.equal(got * 2.0 ** 20, want)
 
 
+def test_results_of_one_launch_live_on_their_own():
+    args = (ints([5, 0, 31]), ints([1, 2, 3]), ints([[7, 0, 0], [0, 0, 0], [3, 4, 0]]), ints([20, 21, 22]))
+    slots, positions, starts, lengths, used = ops.page_slots(*args, 16, 6)
+    for r in (slots, positions, starts, lengths, used):
+        assert r.is_contiguous() and r.data_ptr() % 256 == 0
+    kept = slots.view(2, 3)
+    del slots, positions, starts, lengths, used
+    again = [ops.page_slots(*args, 16, 6) for _ in range(20)]
+    torch.cuda.synchronize()
+    assert kept.flatten().tolist() == [7 * 16 + 5, 20 * 16, 20 * 16 + 1, 4 * 16 + 15, 21 * 16, 21 * 16 + 1] and len(again) == 20
+
+
 # ---- refusals, streams ----
 
 def test_refusals():
