@@ -226,8 +226,10 @@ void CA_NAME(const float* __restrict__ part, ca_q* __restrict__ out) {
   if (e.parts == 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15;
   const int rb = blockIdx.y / (CA_NT / 2), tt = blockIdx.y % (CA_NT / 2) * 2 + (wave & 1);
+  if (rb * 16 >= e.tokens * CA_GS) return;
+  const int row = rb * 16 + n < e.tokens * CA_GS ? n : 0;                       // (rows that there are not were not written)
   const float* later = part + CA_ENDS + ((long long)id * 2 - 2) * CA_SLOT;       // part i > 0 is slot 0 of share id + i - 1
-  const int at = CA_ROWS * CA_D + (rb * 16 + n) * 2, of = ((rb * CA_NT + tt) * 64 + lane) * 4;
+  const int at = CA_ROWS * CA_D + (rb * 16 + row) * 2, of = ((rb * CA_NT + tt) * 64 + lane - n + row) * 4;
   float m = -__builtin_inff(), l = 0.0f;
   kcg_f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
@@ -261,13 +263,18 @@ void CA_NAME(const float* __restrict__ part, ca_q* __restrict__ out) {
 }
 #else
 
-// The queries of a lane's row in 8 bits: a sum of CA_QN e4m3 numbers times the power of two that is returned.
-__device__ __forceinline__ float ca_query(const ca_q* __restrict__ p, unsigned (&qf)[CA_QN][CA_KR]) {
-  typedef ca_q ca_q8 __attribute__((ext_vector_type(8)));
-  ca_q8 raw[CA_KR / 2];
-  float top = 0.0f;
+// A lane's part of a row of queries, and the same in 8 bits: a sum of CA_QN e4m3 numbers times the power of two that is returned.
+typedef ca_q ca_q8 __attribute__((ext_vector_type(8)));
+struct CaQuery { ca_q8 raw[CA_KR / 2]; };
+__device__ __forceinline__ CaQuery ca_query_load(const ca_q* __restrict__ p) {
+  CaQuery r;
 #pragma unroll
-  for (int i = 0; i < CA_KR / 2; ++i) raw[i] = *(const ca_q8*)(p + i * 8);
+  for (int i = 0; i < CA_KR / 2; ++i) r.raw[i] = *(const ca_q8*)(p + i * 8);
+  return r;
+}
+__device__ __forceinline__ float ca_query(const CaQuery& r, unsigned (&qf)[CA_QN][CA_KR]) {
+  const auto& raw = r.raw;
+  float top = 0.0f;
 #pragma unroll
   for (int i = 0; i < CA_KR * 4; ++i) top = fmaxf(top, __builtin_fabsf((float)raw[i / 8][i % 8]));
   top = ca_cross(top, true);
@@ -432,7 +439,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
       const int token = real ? tk : 0, head = real ? head0 + hd : head0;
       pos[rb] = first + token;
       slope[rb] = CA_SLOPES ? slopes[head] * 1.44269504088896340736f : 0.0f;
-      qs[rb] = ca_query(q + (long long)(rq.first + tok0 + token) * CA_QT + (long long)head * CA_QH + g * (CA_D / 4), qf[rb]);
+      qs[rb] = ca_query(ca_query_load(q + (long long)(rq.first + tok0 + token) * CA_QT + (long long)head * CA_QH + g * (CA_D / 4)), qf[rb]);
       m[rb] = -__builtin_inff();
       l[rb] = 0.0f;
 #pragma unroll
@@ -708,33 +715,136 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
   bool begun = true;              // the first piece of this workgroup, if it is not a whole tile, goes to slot 0, a later one to slot 1
 #endif
 
-  while (left > 0) {
-    const int t = ca_tokens(rq), tok0 = tile * t, tokens = rq.count - tok0 < t ? rq.count - tok0 : t;
-    const int units = ca_units(rq, tile);
-    const int until = left < units - unit ? unit + left : units;      // of this piece
-    const int first = rq.length - rq.count + tok0;                         // position of the tile's first row
-    const int hi = first + tokens > 0 ? first + tokens : 0;
-    const int lo = CA_WINDOW && first - CA_WINDOW + 1 > 0 ? first - CA_WINDOW + 1 : 0;
-    const int kvh = hv / CA_PARTS, head0 = kvh * CA_G + (hv % CA_PARTS) * CA_GS;
+  // What this workgroup has to do of a tile: rows, keys, and the keys that this wavefront begins with.
+  struct Piece { CaRequest rq; int b, tile, unit, until, units, tok0, tokens, first, lo, hi, key, end; };
+  const int kvh = hv / CA_PARTS, head0 = kvh * CA_G + (hv % CA_PARTS) * CA_GS;
+  auto pieceOf = [&](const CaRequest& rq, int b, int tile, int unit, int left) {
+    Piece s;
+    s.rq = rq;
+    s.b = b;
+    s.tile = tile;
+    s.unit = unit;
+    const int t = ca_tokens(rq);
+    s.tok0 = tile * t;
+    s.tokens = rq.count - s.tok0 < t ? rq.count - s.tok0 : t;
+    s.units = ca_units(rq, tile);
+    s.until = left < s.units - unit ? unit + left : s.units;
+    s.first = rq.length - rq.count + s.tok0;                             // position of the tile's first row
+    s.hi = s.first + s.tokens > 0 ? s.first + s.tokens : 0;
+    s.lo = CA_WINDOW && s.first - CA_WINDOW + 1 > 0 ? s.first - CA_WINDOW + 1 : 0;
     const int base = ca_low(rq, tile) * CA_UK;
-    int key = base + unit * CA_UK + wave * 32;
-    const int end = base + until * CA_UK < hi ? base + until * CA_UK : hi;
+    s.key = base + unit * CA_UK + wave * 32;
+    s.end = base + s.until * CA_UK < s.hi ? base + s.until * CA_UK : s.hi;
+    return s;
+  };
+  // Pages and scales of the halves of 32 steps, a lane each (lane 2 s + h half h of step s), read while the 32 steps before are worked on and
+  // their pages while those before are: by vector loads, since a scalar load would be waited for by every LDS access.
+  struct Block { int page; float ks, vs; };       // page -1: no such keys, or a page that there is none of
+  auto pagesOf = [&](const Piece& s, int from) {
+    const int at = from + (lane >> 1) * CA_UK + (lane & 1) * 16;
+    const int page = table[(long long)(s.b < B ? s.b : 0) * table_row + (at < s.hi ? at : s.hi > 0 ? s.hi - 1 : 0) / CA_PAGE];
+    return at < s.hi && at + 16 > s.lo && (unsigned)page < (unsigned)pages ? page : -1;
+  };
+  auto scalesOf = [&](int page) {
+    const long long at = (long long)(page < 0 ? 0 : page) * CA_HKV + kvh;       // (what is not there is read from somewhere that is)
+    return Block{page, kscale[at], vscale[at]};
+  };
+  // Addresses: a uniform base and an offset of the lane's
+  // K and V go in chunks of 16 bytes, neighbouring lanes neighbouring chunks (read where a lane needs them, four neighbouring lanes touch
+  // four lines)
+  kcg_u32x4 k[CA_VL], v[CA_VL];
+  unsigned koff[CA_VL], voff[CA_VL], kat[CA_VL], vat[CA_VL];
+#pragma unroll
+  for (int u = 0; u < CA_VL; ++u) {
+    const int c = u * 64 + lane, key32 = c / (CA_D / 16), part16 = c % (CA_D / 16) * 16;
+    koff[u] = (key32 % 16) * (unsigned)CA_KT + part16;
+    voff[u] = (key32 % 16) * (unsigned)CA_VT + part16;
+    kat[u] = key32 * CA_KP_ + part16;
+    vat[u] = CA_VROW(key32) + part16;
+  }
+  // the half that a chunk's key lies in is the same for all lanes where 64 chunks are whole halves
+#define CA_HALF(u) (CA_D % 64 == 0 ? (u) * 64 / CA_D : ((u) * 64 + lane) / CA_D)
+  auto loadK = [&](int at, const int (&pg)[2]) {
+    const unsigned char* kp[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      kp[h] = kc + ((long long)(pg[h] < 0 ? 0 : pg[h]) * CA_KP + (long long)((at + h * 16) % CA_PAGE) * CA_KT + (long long)kvh * CA_KH);
+#pragma unroll
+    for (int u = 0; u < CA_VL; ++u) k[u] = *(const kcg_u32x4*)((CA_HALF(u) ? kp[1] : kp[0]) + koff[u]);
+  };
+  auto loadV = [&](int at, const int (&pg)[2]) {
+    const unsigned char* vp[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      vp[h] = vc + ((long long)(pg[h] < 0 ? 0 : pg[h]) * CA_VP + (long long)((at + h * 16) % CA_PAGE) * CA_VT + (long long)kvh * CA_VH);
+#pragma unroll
+    for (int u = 0; u < CA_VL; ++u) v[u] = *(const kcg_u32x4*)((CA_HALF(u) ? vp[1] : vp[0]) + voff[u]);
+  };
+  // A piece's pages are read while the piece before is worked on, its first keys and values, and its queries, while that one's results are added
+  // up: what a short piece would wait for (64 requests of up to 4096 keys 54 us without, 50 with).  A wavefront that has no keys brings some
+  // that nobody uses.
+  CaQuery raw[CA_RB];
+  Block now;
+  int pg[2];
+  auto queries = [&](const Piece& s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int rb = 0; rb < CA_RB; ++rb) {
+      const int row = rb * 16 + n, tk = row / CA_GS, hd = row - tk * CA_GS;
+      const bool real = tk < s.tokens && (hv % CA_PARTS) * CA_GS + hd < CA_G;
+      raw[rb] = ca_query_load(q + (long long)(s.rq.first + s.tok0 + (real ? tk : 0)) * CA_QT + (long long)(real ? head0 + hd : head0) * CA_QH + g * (CA_D / 4));
+    }
+  };
+  // whether registers hold the next piece's first keys and values, and its queries, beside the results (at D 256 that spills: 16
+  // requests of up to 8000 keys 49 us, not 47)
+  constexpr bool AHEAD = CA_D <= 128, EARLY = CA_RB * CA_D <= 128;
+  auto begin = [&](const Piece& s, int page) __attribute__((always_inline)) {
+    if (EARLY) queries(s);
+    now = scalesOf(page);
+    pg[0] = __builtin_amdgcn_readlane(page, 0);
+    pg[1] = __builtin_amdgcn_readlane(page, 1);
+    loadK(s.key, pg);
+    loadV(s.key, pg);
+  };
+  Piece s = pieceOf(rq, b, tile, unit, left);
+  int page = pagesOf(s, s.key), later = pagesOf(s, s.key + 32 * CA_UK);
+  if (AHEAD) begin(s, page);
 
-    // rows: queries in 8 bits, positions
+  while (true) {
+    const int tokens = s.tokens, first = s.first, hi = s.hi, lo = s.lo, end = s.end;
+    int key = s.key;
+#if !CA_WHOLE
+    left -= s.until - s.unit;
+    Piece next = s;
+    int nextPage = -1, nextLater = -1;
+    auto follow = [&]() __attribute__((always_inline)) {      // the next tile that there is
+      if (left <= 0) return;
+      if (++tile >= ca_tiles(rq)) {
+        tile = 0;
+        while (++b < requests) {
+          rq = ca_request(lengths, starts, b, B, T, most);
+          if (rq.count > 0) break;
+        }
+      }
+      next = pieceOf(rq, b, tile, 0, left);
+      nextPage = pagesOf(next, next.key);
+      nextLater = pagesOf(next, next.key + 32 * CA_UK);
+    };
+    if (AHEAD) follow();
+#endif
     unsigned qf[CA_RB][CA_QN][CA_KR];
     float qs[CA_RB];               // the power of two that a row was divided by
     int pos[CA_RB];
     float slope[CA_RB];
+    if (!EARLY) queries(s);
 #pragma unroll
     for (int rb = 0; rb < CA_RB; ++rb) {
       const int row = rb * 16 + n, tk = row / CA_GS, hd = row - tk * CA_GS;
       const bool real = tk < tokens && (hv % CA_PARTS) * CA_GS + hd < CA_G;
-      const int token = real ? tk : 0, head = real ? head0 + hd : head0;
-      pos[rb] = first + token;
-      slope[rb] = CA_SLOPES ? slopes[head] * 1.44269504088896340736f : 0.0f;
-      const ca_q* p = q + (long long)(rq.first + tok0 + token) * CA_QT + (long long)head * CA_QH + g * (CA_D / 4);
-      qs[rb] = ca_query(p, qf[rb]);
+      pos[rb] = first + (real ? tk : 0);
+      slope[rb] = CA_SLOPES ? slopes[real ? head0 + hd : head0] * 1.44269504088896340736f : 0.0f;
+      qs[rb] = ca_query(raw[rb], qf[rb]);
     }
+    if (!AHEAD) begin(s, page);
 
     kcg_f32x4 acc[CA_RB][CA_NT];
     float m[CA_RB], l[CA_RB];
@@ -746,50 +856,6 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
       for (int i = 0; i < CA_NT; ++i) acc[rb][i] = kcg_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    const int* row = table + (long long)b * table_row;
-    // Pages and scales of the halves of 32 steps, a lane each (lane 2 s + h half h of step s), read while the 32 steps before are worked on and
-    // their pages while those before are: by vector loads, since a scalar load would be waited for by every LDS access.
-    struct Block { int page; float ks, vs; };       // page -1: no such keys, or a page that there is none of
-    auto pagesOf = [&](int from) {
-      const int at = from + (lane >> 1) * CA_UK + (lane & 1) * 16;
-      const int page = row[(at < hi ? at : hi - 1) / CA_PAGE];
-      return at < hi && at + 16 > lo && (unsigned)page < (unsigned)pages ? page : -1;
-    };
-    auto scalesOf = [&](int page) {
-      const long long at = (long long)(page < 0 ? 0 : page) * CA_HKV + kvh;       // (what is not there is read from somewhere that is)
-      return Block{page, kscale[at], vscale[at]};
-    };
-    // Addresses: a uniform base and an offset of the lane's
-    // K and V go in chunks of 16 bytes, neighbouring lanes neighbouring chunks (read where a lane needs them, four neighbouring lanes touch
-    // four lines)
-    kcg_u32x4 k[CA_VL], v[CA_VL];
-    unsigned koff[CA_VL], voff[CA_VL], kat[CA_VL], vat[CA_VL];
-#pragma unroll
-    for (int u = 0; u < CA_VL; ++u) {
-      const int c = u * 64 + lane, key32 = c / (CA_D / 16), part16 = c % (CA_D / 16) * 16;
-      koff[u] = (key32 % 16) * (unsigned)CA_KT + part16;
-      voff[u] = (key32 % 16) * (unsigned)CA_VT + part16;
-      kat[u] = key32 * CA_KP_ + part16;
-      vat[u] = CA_VROW(key32) + part16;
-    }
-    // the half that a chunk's key lies in is the same for all lanes where 64 chunks are whole halves
-#define CA_HALF(u) (CA_D % 64 == 0 ? (u) * 64 / CA_D : ((u) * 64 + lane) / CA_D)
-    auto loadK = [&](int at, const int (&pg)[2]) {
-      const unsigned char* kp[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        kp[h] = kc + ((long long)(pg[h] < 0 ? 0 : pg[h]) * CA_KP + (long long)((at + h * 16) % CA_PAGE) * CA_KT + (long long)kvh * CA_KH);
-#pragma unroll
-      for (int u = 0; u < CA_VL; ++u) k[u] = *(const kcg_u32x4*)((CA_HALF(u) ? kp[1] : kp[0]) + koff[u]);
-    };
-    auto loadV = [&](int at, const int (&pg)[2]) {
-      const unsigned char* vp[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        vp[h] = vc + ((long long)(pg[h] < 0 ? 0 : pg[h]) * CA_VP + (long long)((at + h * 16) % CA_PAGE) * CA_VT + (long long)kvh * CA_VH);
-#pragma unroll
-      for (int u = 0; u < CA_VL; ++u) v[u] = *(const kcg_u32x4*)((CA_HALF(u) ? vp[1] : vp[0]) + voff[u]);
-    };
     unsigned char *ks_ = sh.tile.k[wave], *vs = sh.tile.v[wave];
     // this lane's address for the transposing reads of tile 0: within each group of 16 lanes, lanes 2 j and 2 j + 1 give the two halves of row
     // j, and lane i receives column i of the eight rows.  The rows are the keys that lane group g has scores of.
@@ -951,17 +1017,13 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
       // The next step's keys are loaded when this one's scores are there, its values when this one's are in LDS: into the same registers, so
       // that many wavefronts fit.
       const int last = key + (end - 1 - key) / CA_UK * CA_UK;
-      Block now = scalesOf(pagesOf(key)), soon;
-      int later = pagesOf(key + 32 * CA_UK);
-      int pg[2] = {__builtin_amdgcn_readlane(now.page, 0), __builtin_amdgcn_readlane(now.page, 1)};
-      loadK(key, pg);
-      loadV(key, pg);
+      Block soon;
       int step = 0;
 #pragma unroll 1
       while (true) {
         if (step == 0) {
           soon = scalesOf(later);
-          later = pagesOf(key + 64 * CA_UK);
+          later = pagesOf(s, key + 64 * CA_UK);
           // (scales of zero stand for pages of zeros)
           now.ks = now.page < 0 ? 0.0f : now.ks;
           now.vs = now.page < 0 || now.vs < CA_TINY ? -__builtin_inff() : __builtin_amdgcn_logf(now.vs);
@@ -993,12 +1055,15 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
       }
     }
 
+#if !CA_WHOLE
+    if (AHEAD && left > 0) begin(next, nextPage);
+#endif
     // the wavefronts' results, added through LDS
 #if CA_WHOLE
     const bool whole = true;
     float* slot = nullptr;
 #else
-    const bool whole = unit == 0 && until == units;
+    const bool whole = s.unit == 0 && s.until == s.units;
     float* slot = part + CA_ENDS + ((long long)id * 2 + (begun ? 0 : 1)) * CA_SLOT;
     begun = false;
 #endif
@@ -1032,8 +1097,8 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
 #pragma unroll
         for (int w = 1; w < CA_WAVES; ++w) o += sh.red[w][i][lane] * f[w];
         if (whole)
-          ca_store(out, rq.first + tok0, tokens, hv, rb, i, o, sum);
-        else
+          ca_store(out, s.rq.first + s.tok0, tokens, hv, rb, i, o, sum);
+        else if (at < tokens * CA_GS)        // (the join reads no others)
           *(kcg_f32x4*)(slot + ((rb * CA_NT + i) * 64 + lane) * 4) = o;
       }
       if (!whole && wave == 0 && g == 0) {
@@ -1044,16 +1109,12 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
 #if CA_WHOLE
     break;
 #else
+    if (left <= 0) break;
+    if (!AHEAD) follow();
     __syncthreads();
-    left -= until - unit;
-    unit = 0;
-    if (left > 0 && ++tile >= ca_tiles(rq)) {      // the next tile that there is
-      tile = 0;
-      while (++b < requests) {
-        rq = ca_request(lengths, starts, b, B, T, most);
-        if (rq.count > 0) break;
-      }
-    }
+    s = next;
+    page = nextPage;
+    later = nextLater;
 #endif
   }
 }
