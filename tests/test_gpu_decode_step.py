@@ -526,3 +526,73 @@ def test_another_stream_and_no_tokens():
     assert none.shape == (0, 8, 64)
     ops.cache_write(q[:0, :2], q[:0, :2], *caches, *scales, ints([], torch.int64))
     assert ops.cache_read(caches[0], scales[0], ints([], torch.int64)).shape == (0, 2, 64)
+
+
+# ---- all of them in a model ----
+
+def answers(model, prompts, steps, graph):
+    tokens = torch.cat([torch.tensor(p, device="cuda") for p in prompts])
+    scores = [model.step(tokens, ints([len(p) for p in prompts]))]
+    tokens = scores[0].argmax(-1)
+    replay = None
+    for i in range(steps):
+        if graph and i == 1:
+            # (recording runs nothing)
+            replay = model.record(tokens)
+        if replay is None:
+            scores.append(model.step(tokens))
+            tokens.copy_(scores[-1].argmax(-1))
+        else:
+            replay.replay()
+            torch.cuda.synchronize()
+        scores.append(tokens.clone())
+    return scores
+
+
+def test_a_model_answers_the_same_from_a_graph_and_from_other_pages():
+    from kernelcodegen_amd.decode import Decoder
+    prompts = [[5, 9, 200, 3] * 7, [1], [77] * 16, list(range(33))]
+    made = dict(layers=2, heads=8, kv_heads=2, d=64, wide=512, vocab=256, pages=48, width=8, seed=3)
+    eager = answers(Decoder(4, **made), prompts, 20, False)
+    replayed = answers(Decoder(4, **made), prompts, 20, True)
+    for i in range(20):
+        assert torch.equal(eager[2 + 2 * i], replayed[2 + i])
+    other = Decoder(4, **made)
+    other.free.copy_(torch.randperm(48, generator=generator(1), device="cuda").int())
+    moved = answers(other, prompts, 20, False)
+    assert all(torch.equal(a, b) for a, b in zip(eager, moved))
+    assert other.lengths.tolist() == [len(p) + 20 for p in prompts]
+
+
+def test_a_layer_of_the_model_against_the_formulas():
+    from kernelcodegen_amd.decode import Decoder
+    model = Decoder(3, layers=1, heads=4, kv_heads=2, d=32, wide=128, vocab=96, group=32, pages=16, width=4, seed=5)
+    added = [20, 1, 9]
+    tokens = torch.arange(30, device="cuda") * 3
+    got = model.step(tokens, ints(added)).double()
+    layer = model.layers[0]
+
+    def product(x, w, scale, zero):
+        code = torch.stack((w & 15, w >> 4), -1).view(w.shape[0], -1, 32).double()
+        return x @ ((code - zero.double()[..., None]) * scale.double()[..., None]).view(w.shape[0], -1).t()
+
+    def norm(x):
+        return (x - x.mean(-1, keepdim=True)) / (x.var(-1, unbiased=False, keepdim=True) + 1e-5).sqrt()
+
+    x, heads, first = model.embedding.double()[tokens], [], 0
+    q = product(norm(x), *layer["qkv"])[:, :128].view(30, 4, 32)
+    for b, n in enumerate(added):
+        at = torch.tensor([int(model.table[b, t // 16]) * 16 + t % 16 for t in range(n)], device="cuda")
+        k, v = [ops.cache_read(*layer[name], at, torch.float32).double().repeat_interleave(2, 1) for name in ("keys", "values")]
+        s = (q[first:first + n, None] * k[None]).sum(-1) / math.sqrt(32)
+        t = torch.arange(n, device="cuda")
+        s = s + model.slopes.double() * (t[None, :, None] - t[:, None, None])
+        s = s.masked_fill((t[None] > t[:, None])[:, :, None], -math.inf).softmax(1)
+        heads.append((s[..., None] * v[None]).sum(1))
+        first += n
+    x = x + product(torch.cat(heads).view(30, 128), *layer["out"])
+    x = x + product(torch.nn.functional.gelu(product(norm(x), *layer["up"]), approximate="tanh"), *layer["down"])
+    want = product(norm(x), *model.head)[[19, 20, 29]]
+    # Twelve results follow one another, each rounded to 11 bits (2^-11 of its size at most, about a third of it in the root of the mean
+    # square); none is larger than a few times what it is added to.  2^-7 is 16 whole ones.
+    assert float((got - want).norm() / want.norm()) < 2.0 ** -7
