@@ -1711,13 +1711,14 @@ bool emitCacheAttention(KernelSpec& s, std::string& src, KernelLaunchInfo& info,
   if (window < 0 || window > 0x7FFFFFFF) { err = "cache_attention: WINDOW must be in [0,2^31)"; return false; }
   if (grid < 1 || grid > 65536) { err = "cache_attention: GRID must be in [1,65536]"; return false; }
   if (least < 1) { err = "cache_attention: LEAST must be positive"; return false; }
-  if (wholeTiles && (starts || join)) { err = "cache_attention: whole tiles are for one row per request, and need no join"; return false; }
+  if (wholeTiles && join) { err = "cache_attention: whole tiles need no join"; return false; }
   const double cap = s.f.count("CAP") ? s.f["CAP"] : 0.0, scale = s.f.count("SCALE") ? s.f["SCALE"] : 1.0;
   if (!(cap >= 0.0) || !std::isfinite(cap) || !std::isfinite(scale)) { err = "cache_attention: CAP must not be negative, CAP and SCALE must be finite"; return false; }
   const int64_t waves = s.get("WAVES", 4);
   if (waves != 1 && waves != 2 && waves != 4) { err = "cache_attention: WAVES must be 1, 2 or 4"; return false; }
   const bool share = s.get("SHARE", 0) != 0;
-  if (share && wholeTiles) { err = "cache_attention: whole tiles are for one row per request"; return false; }
+  if (!share && rb != 1) { err = "cache_attention: RB 2 is for shared keys"; return false; }
+  if (share && wholeTiles) { err = "cache_attention: shared keys are not for whole tiles"; return false; }
   const int64_t blocks = share ? rb * waves : rb, rows = 16 * blocks, gs = std::min(g, rows);
   // shares that a head's work is cut into, of about GRID workgroups in all
   const int64_t hv = s.p["H"] * ceilDiv(g, gs), pieces = std::max<int64_t>(1, grid / hv);

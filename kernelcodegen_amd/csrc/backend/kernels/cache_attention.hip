@@ -23,7 +23,7 @@
 // Work: the keys of a tile are cut into units of CA_UK = 32 CA_WAVES, one step of each wavefront of a workgroup.  All units of all tiles of a head
 // stand in one line that is cut evenly between CA_PIECES workgroups (prefix sums of the units of each request, in closed form,
 // taken by every workgroup); a tile cut between workgroups leaves partial results in `part`, which cache_join adds up.  So
-// requests of any lengths fill the part.  CA_WHOLE: one workgroup for each tile of a request (one tile each), nothing to join.
+// requests of any lengths fill the part.  CA_WHOLE: one workgroup for each tile, nothing to join.
 // Parameters: CA_NAME, CA_D, CA_HKV, CA_G (heads per kv head), CA_GS, CA_PAGE, CA_F16, CA_SPLIT, CA_RB, CA_WAVES, CA_SHARE, CA_PIECES, CA_WHOLE, CA_MIN (least units of
 // a workgroup), CA_SCALE, CA_CAP (0: none), CA_WINDOW (0: none), CA_SLOPES, CA_STARTS, CA_KP CA_KT CA_KH / CA_VP CA_VT CA_VH (strides of
 // page, token, head), CA_QT CA_QH (of q), CA_JOIN (this is cache_join).
@@ -136,6 +136,9 @@ __device__ __forceinline__ int ca_scan(int v) {
   return v;
 }
 
+// What the shares are cut by: units, or whole tiles where a workgroup takes one.
+__device__ __forceinline__ int ca_cost(const CaRequest& r, int tile) { return CA_WHOLE ? tile : ca_before(r, tile); }
+
 // What stands at the beginning of a workgroup's share.
 struct CaPlace {
   int left, chunk;              // units of this share, and of every whole one
@@ -151,11 +154,11 @@ __device__ __forceinline__ bool ca_locate(int piece, const int* __restrict__ len
   int mine = 0;
   for (int i = b0; i < b1; ++i) {
     r = ca_request(lengths, starts, i, B, T, most);
-    mine += ca_before(r, ca_tiles(r));
+    mine += ca_cost(r, ca_tiles(r));
   }
   const int through = ca_scan(mine), ahead = through - mine, all = __builtin_amdgcn_readlane(through, 63);
   const int even = (all + CA_PIECES - 1) / CA_PIECES;
-  w.chunk = even < CA_MIN ? CA_MIN : even;
+  w.chunk = CA_WHOLE ? 1 : even < CA_MIN ? CA_MIN : even;
   if (piece >= (all + w.chunk - 1) / w.chunk) return false;
   const int f = piece * w.chunk;
   w.left = all - f < w.chunk ? all - f : w.chunk;
@@ -165,15 +168,15 @@ __device__ __forceinline__ bool ca_locate(int piece, const int* __restrict__ len
     int at = ahead;
     for (; b < b1; ++b) {
       if (per > 1) r = ca_request(lengths, starts, b, B, T, most);
-      const int tiles = ca_tiles(r), units = ca_before(r, tiles);
+      const int tiles = ca_tiles(r), units = ca_cost(r, tiles);
       if (f < at + units) {
         int lo = 0, hi = tiles - 1;           // the last tile that begins at or before f
         while (lo < hi) {
           const int mid = (lo + hi + 1) >> 1;
-          if (at + ca_before(r, mid) <= f) lo = mid; else hi = mid - 1;
+          if (at + ca_cost(r, mid) <= f) lo = mid; else hi = mid - 1;
         }
         tile = lo;
-        unit = f - at - ca_before(r, lo);
+        unit = f - at - ca_cost(r, lo);
         break;
       }
       at += units;
@@ -704,9 +707,15 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
   int b, tile, unit, left;                       // left: units this workgroup has to do
 #if CA_WHOLE
   b = blockIdx.x / CA_HV;
-  rq = ca_request(lengths, starts, b, B, T, most);
   tile = unit = 0;
   left = 0x7fffffff;
+#if CA_STARTS
+  CaPlace w;
+  if (!ca_locate(b, lengths, starts, B, T, most, w)) return;
+  rq = w.request; b = w.b; tile = w.tile;
+#else
+  rq = ca_request(lengths, starts, b, B, T, most);
+#endif
 #else
   const int requests = B + CA_STARTS, piece = blockIdx.x / CA_HV, id = hv * CA_PIECES + piece;
   CaPlace w;
@@ -796,9 +805,9 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
   };
   // whether registers hold the next piece's first keys and values, and its queries, beside the results (at D 256 that spills: 16
   // requests of up to 8000 keys 49 us, not 47)
-  constexpr bool AHEAD = CA_D <= 128, EARLY = CA_RB * CA_D <= 128;
+  constexpr bool AHEAD = CA_D <= 128;
   auto begin = [&](const Piece& s, int page) __attribute__((always_inline)) {
-    if (EARLY) queries(s);
+    if (AHEAD) queries(s);
     now = scalesOf(page);
     pg[0] = __builtin_amdgcn_readlane(page, 0);
     pg[1] = __builtin_amdgcn_readlane(page, 1);
@@ -835,7 +844,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
     float qs[CA_RB];               // the power of two that a row was divided by
     int pos[CA_RB];
     float slope[CA_RB];
-    if (!EARLY) queries(s);
+    if (!AHEAD) queries(s);
 #pragma unroll
     for (int rb = 0; rb < CA_RB; ++rb) {
       const int row = rb * 16 + n, tk = row / CA_GS, hd = row - tk * CA_GS;

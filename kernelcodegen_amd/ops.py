@@ -519,14 +519,9 @@ def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, length
         raise ValueError("too many rows times keys for one launch")
     if not 0.0 <= cap < math.inf or window < 0:
         raise ValueError("cap and window must not be negative")
-    # Rows that the average request has of a kv head: up to 32 form a tile, whose keys the wavefronts of a workgroup split; more are split
-    # between the wavefronts
-    rows = group * max(1, -(-tokens // batch))
-    blocks, share = (1 if rows <= 16 else 2), int(rows > 32)
-    params = dict(H=kv_heads, D=d, PAGE=page, G=group, F16=int(q.dtype == torch.float16), RB=blocks, WAVES=4, SHARE=share, STARTS=int(starts is not None), CAP=cap, WINDOW=window,
+    params = dict(H=kv_heads, D=d, PAGE=page, G=group, F16=int(q.dtype == torch.float16), STARTS=int(starts is not None), CAP=cap, WINDOW=window,
                   SLOPES=int(slopes is not None), SCALE=d ** -0.5 if scale is None else scale, KP=ks[0], KT=ks[1], KH=ks[2], VP=vs[0], VT=vs[1], VH=vs[2],
-                  QT=qs[0], QH=qs[1], WHOLE=int(starts is None and width * page <= 512),
-                  GRID=256 if blocks == 2 and d > 128 else 512)
+                  QT=qs[0], QH=qs[1], **_cache_attention_form(batch, tokens, kv_heads, group, d, width * page))
     if not cfg.keys() <= {"RB", "WAVES", "SHARE", "GRID", "LEAST", "OCC", "WHOLE"}:
         raise ValueError("unknown kernel parameters")
     params.update(cfg)
@@ -534,12 +529,40 @@ def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, length
     tiles = kv_heads * -(-group // (16 * blocks))         # of a token's heads
     kern = R.get_kernel("cache_attention", **params)
     if params["WHOLE"]:
-        return _into_last(kern.bind(grid=(batch * tiles,)), (tuple(q.shape), q.dtype)), None, 0
+        # with starts, every request's first tile and what the tokens fill behind it, however they are spread (also behind the last request)
+        whole = batch if starts is None else max(1, min(batch + 1, tokens) + tokens // (16 * blocks // min(group, 16 * blocks)))
+        return _into_last(kern.bind(grid=(whole * tiles,)), (tuple(q.shape), q.dtype)), None, 0
     shares = kern.info["grid"][0]
     # for each share four whole numbers, and two parts of a tile: its sums, and maximum and sum of the probabilities of each row
     floats = shares * (4 + 2 * (16 * blocks * d + 32 * blocks))
     join = None if shares == tiles else R.get_kernel("cache_join", **params).bind()
     return _into_last(kern.bind(), (tuple(q.shape), q.dtype)), join, floats
+
+
+def _cache_attention_form(batch, tokens, kv_heads, group, d, keys):
+    """The tiles and who takes what of them; `keys`: what a request's row of the table has room for.
+
+    A tile has 16 rows of a kv head, whose keys are split between the wavefronts of a workgroup.  Where the average request has more than 32
+    rows, or more than 16 of 256 numbers, which registers hold no more keys beside, it has 64 or 128 rows, 16 or 32 (RB) to a wavefront,
+    and the wavefronts share the keys (SHARE).  About GRID workgroups take equal shares
+    of all keys, so that a few long requests fill the part and a tile may lie in several shares, whose results a second launch joins;
+    where requests are short, a workgroup takes one tile (WHOLE), with as many wavefronts as its keys and the number of tiles ask for.
+    Measured, in us (8 kv heads of 128, 4 heads to each, bf16; lengths spread up to `keys`, a third of it on average):
+      512 tiles, 512 keys: a tile each 10.2, shares 15.5;  4096 tiles: 52, 70;  512 tiles, 1024 keys: 14.2, 21.1;  4096: 94, 101;
+      1024 tiles, 2048 keys: 55.3, 54.2;  4096 keys: 102, 90
+      a tile each, 4096 tiles, of 16 keys: one wavefront 11.5, two 16.1, four 25.1;  512 keys: 55, 52, 56;  64 tiles, 512 keys: 14.7, 9.1, 6.8
+      8 prompts of up to 300 behind up to 600 keys: shared keys with 16 rows a wavefront 41, 32 rows 49, keys split 58;  2 of 1000 behind 6000:
+      202, 167, 195;  64 of up to 16 tokens behind 1000: 35, 54, 44
+      32 heads to one kv head: 8 of up to 32000 keys: keys split, 16 rows a tile 21.6, 32 rows 26.9, shared 26.2;  16 of 16000 of 256: 38, 61, 32"""
+    rows = group * max(1, -(-tokens // batch))
+    share = int(rows > (32 if d <= 128 else 16))
+    blocks = 2 if share and rows * keys >= 1 << 21 else 1
+    tiles = batch * kv_heads * -(-group // 16)
+    whole = int(not share and (keys <= 512 or (keys <= 1024 and tiles >= 512)))
+    waves = 4
+    if whole and keys <= 512:
+        waves = (1 if keys <= 64 else 2) if tiles > 512 else 2 if keys <= 64 else 4
+    return dict(RB=blocks, SHARE=share, WHOLE=whole, WAVES=waves, GRID=256 if blocks == 2 and d > 128 else 512)
 
 
 def matmul_q4(x, w, scale, zero=None, out_dtype=None, **cfg):

@@ -21,10 +21,10 @@ def attention(d, **more):
 
 WRITE = dict(F16=2, WIN=1, XKT=256, XKH=128, XVT=256, XVH=128)
 GOOD = [("page_slots", dict(PAGE=16), 14), ("cache_write", dict(cache(128), **WRITE), 9), ("cache_write", dict(cache(96), **{**WRITE, "F16": 0, "WIN": 16}), 9),
-        ("cache_read", dict(cache(64), F16=0), 6), ("cache_join", attention(128), 2), ("cache_join", attention(256, RB=2, STARTS=1, WINDOW=100), 2),
+        ("cache_read", dict(cache(64), F16=0), 6), ("cache_join", attention(128), 2), ("cache_join", attention(256, RB=2, SHARE=1, STARTS=1, WINDOW=100), 2),
         ("gemm_q4", dict(N=100, K=4096, GROUP=128, F16=0, MB=1), 6), ("gemm_q4", dict(N=4096, K=1088, GROUP=64, F16=1, MB=4, ZERO=1, SCALE_F32=1, OUT_F32=1), 6)]
-GOOD += [("cache_attention", attention(d, RB=rb, F16=d // 32 % 2, SHARE=share, STARTS=share), 16) for d in range(32, 257, 32) for rb in (1, 2) for share in (0, 1)]
-GOOD += [("cache_attention", attention(128, WHOLE=1, CAP=30.0), 16), ("cache_attention", attention(128, STARTS=1, WINDOW=500, SLOPES=1, G=40), 16)]
+GOOD += [("cache_attention", attention(d, RB=rb, F16=d // 32 % 2, SHARE=share, STARTS=share), 16) for d in range(32, 257, 32) for rb, share in ((1, 0), (1, 1), (2, 1))]
+GOOD += [("cache_attention", attention(128, WHOLE=1, CAP=30.0), 16), ("cache_attention", attention(128, WHOLE=1, STARTS=1, WAVES=1), 16), ("cache_attention", attention(128, STARTS=1, WINDOW=500, SLOPES=1, G=40), 16)]
 
 
 @pytest.mark.parametrize("family,params,nargs", GOOD)
@@ -38,9 +38,9 @@ def test_every_form_compiles_for_gfx950(family, params, nargs):
     ("page_slots", dict(PAGE=16, BLOCK=100)), ("page_slots", dict()), ("page_slots", dict(PAGE=0)), ("cache_read", dict(cache(48), F16=0)), ("cache_read", dict(cache(288), F16=0)), ("cache_read", dict(cache(64, page=8), F16=0)),
     ("cache_read", dict(cache(64, page=48), F16=0)), ("cache_read", dict(cache(64), F16=3)), ("cache_read", dict(cache(64))), ("cache_read", dict(cache(64), F16=0, KT=8)),
     ("cache_read", dict(cache(64), F16=0, KP=-16)), ("cache_write", dict(cache(128), **{**WRITE, "WIN": 65})), ("cache_write", dict(cache(128), **{**WRITE, "XKT": 4})),
-    ("cache_attention", attention(128, RB=3)), ("cache_attention", attention(128, RB=4)), ("cache_attention", attention(128, WHOLE=1, SHARE=1)), ("cache_attention", attention(128, WAVES=3)), ("cache_attention", attention(128, G=0)), ("cache_attention", attention(128, QT=4)), ("cache_attention", attention(128, KT=1 << 27)),
+    ("cache_attention", attention(128, RB=3)), ("cache_attention", attention(128, RB=4)), ("cache_attention", attention(128, RB=2)), ("cache_attention", attention(128, WAVES=3)), ("cache_attention", attention(128, G=0)), ("cache_attention", attention(128, QT=4)), ("cache_attention", attention(128, KT=1 << 27)),
     ("cache_attention", attention(128, GRID=0)), ("cache_attention", attention(128, CAP=-1.0)), ("cache_attention", attention(128, CAP=float("nan"))),
-    ("cache_attention", attention(128, SCALE=float("inf"))), ("cache_attention", attention(128, WINDOW=-1)), ("cache_attention", attention(128, WHOLE=1, STARTS=1)),
+    ("cache_attention", attention(128, SCALE=float("inf"))), ("cache_attention", attention(128, WINDOW=-1)), ("cache_attention", attention(128, WHOLE=1, SHARE=1)),
     ("cache_join", attention(128, WHOLE=1)), ("cache_attention", attention(128, F16=2)),
     ("gemm_q4", dict(N=100, K=100, GROUP=50, F16=0, MB=1)), ("gemm_q4", dict(N=100, K=192, GROUP=128, F16=0, MB=1)), ("gemm_q4", dict(N=100, K=192, GROUP=96, F16=0, MB=1)),
     ("gemm_q4", dict(N=0, K=128, GROUP=128, F16=0, MB=1)), ("gemm_q4", dict(N=100, K=128, GROUP=128, F16=0, MB=5)), ("gemm_q4", dict(N=100, K=128, GROUP=128, F16=0, MB=4, WK=16, NT=4))])

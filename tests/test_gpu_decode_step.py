@@ -307,6 +307,18 @@ def test_cache_attention_of_one_row_per_request(case, dtype):
     check_attention(case, counts=None, dtype=dtype, **DECODE[case])
 
 
+def test_cache_attention_forms_agree():
+    """One case by every way of cutting it, with requests of no rows and rows behind the last request's."""
+    lengths, counts = [70, 9, 300, 40, 1], [3, 0, 17, 40, 1]
+    q, caches, scales, table, starts = attention_case(3, lengths, counts, 8, 2, 128, 16, "tokens", "bf16")
+    q = torch.cat([q, torch.ones_like(q[:5])])
+    want = plain_attention(q, *caches, *scales, table, lengths, starts, 128 ** -0.5, 0.0, 0, None)
+    forms = [dict(WHOLE=1, SHARE=0, RB=1, WAVES=w) for w in (1, 2, 4)] + [dict(WHOLE=0, SHARE=0, RB=1, WAVES=w, GRID=g) for w, g in ((4, 512), (4, 7), (2, 64))]
+    for form in forms + [dict(WHOLE=0, SHARE=1, RB=rb, WAVES=4, GRID=g) for rb in (1, 2) for g in (512, 9)]:
+        got = ops.cache_attention(q, *caches, *scales, table, ints(lengths), ints(starts), **form)
+        close(got, want)
+
+
 @pytest.mark.parametrize("options", [dict(cap=5.0), dict(window=100), dict(window=1), dict(slope=True), dict(cap=30.0, window=257, slope=True, scale=0.3)])
 @pytest.mark.parametrize("lengths", [[1, 40, 300], [1700, 2, 129]])
 def test_cache_attention_options(options, lengths):
