@@ -1725,8 +1725,9 @@ bool emitCacheAttention(KernelSpec& s, std::string& src, KernelLaunchInfo& info,
   // wavefronts per SIMD that the registers are given for: more hide no more of the loads (64 requests of up to 4096 keys, 32 heads on 8: two
   // 53.8 us, three 57)
   const int64_t occ = s.get("OCC", rb == 2 && dh > 128 ? 1 : 2);
+  const int64_t jt = share ? 8 : 2;            // tiles that a workgroup of the join takes
   Defines d;
-  d.add("CA_NAME", s.name);
+  d.add("CA_NAME", s.name); d.add("CA_JT", jt);
   d.add("CA_JOIN", join ? 1 : 0);
   d.add("CA_D", dh); d.add("CA_HKV", s.p["H"]); d.add("CA_G", g); d.add("CA_GS", gs); d.add("CA_PAGE", s.p["PAGE"]);
   d.add("CA_F16", s.p["F16"]); d.add("CA_RB", rb); d.add("CA_WAVES", waves); d.add("CA_SHARE", share ? 1 : 0); d.add("CA_PIECES", pieces); d.add("CA_WHOLE", wholeTiles ? 1 : 0); d.add("CA_MIN", least);
@@ -1737,7 +1738,7 @@ bool emitCacheAttention(KernelSpec& s, std::string& src, KernelLaunchInfo& info,
   src = d.wrap(kTpl_cache_attention);
   info.name = s.name;
   info.grid[0] = (uint32_t)((join ? std::max<int64_t>(1, pieces - 1) : pieces) * hv);
-  if (join) info.grid[1] = (uint32_t)(blocks * dh / 32);
+  if (join) info.grid[1] = (uint32_t)(blocks * dh / 16 / jt);
   info.block[0] = (uint32_t)(join ? 512 : 64 * waves);
   info.numArgs = join ? 2 : 16;
   return true;

@@ -24,7 +24,7 @@
 // stand in one line that is cut evenly between CA_PIECES workgroups (prefix sums of the units of each request, in closed form,
 // taken by every workgroup); a tile cut between workgroups leaves partial results in `part`, which cache_join adds up.  So
 // requests of any lengths fill the part.  CA_WHOLE: one workgroup for each tile, nothing to join.
-// Parameters: CA_NAME, CA_D, CA_HKV, CA_G (heads per kv head), CA_GS, CA_PAGE, CA_F16, CA_SPLIT, CA_RB, CA_WAVES, CA_SHARE, CA_PIECES, CA_WHOLE, CA_MIN (least units of
+// Parameters: CA_NAME, CA_D, CA_HKV, CA_G (heads per kv head), CA_GS, CA_PAGE, CA_F16, CA_SPLIT, CA_RB, CA_WAVES, CA_SHARE, CA_PIECES, CA_WHOLE, CA_JT, CA_MIN (least units of
 // a workgroup), CA_SCALE, CA_CAP (0: none), CA_WINDOW (0: none), CA_SLOPES, CA_STARTS, CA_KP CA_KT CA_KH / CA_VP CA_VT CA_VH (strides of
 // page, token, head), CA_QT CA_QH (of q), CA_JOIN (this is cache_join).
 typedef _Float16 ca_f16x8 __attribute__((ext_vector_type(8)));
@@ -218,8 +218,10 @@ struct CaEnd { int first, tokens, parts, slot; };      // rows, parts (0: nothin
 #define CA_ENDS (4 * CA_HV * CA_PIECES)                // floats of all of them, in front of the parts
 
 #if CA_JOIN
-// A workgroup for every beginning of a share and two tiles of 16 columns of O; it has something to do where that is the first one inside
-// of a tile of rows, and adds up the parts of the tile.  Four wavefronts take every fourth part of the same columns.
+// A workgroup for every beginning of a share and CA_JT tiles of 16 rows and 16 columns of O; it has something to do where that is the first one
+// inside of a tile of rows, and adds up the parts of the tile.  8 / CA_JT wavefronts take every so many-th part of the same columns: four
+// in a decoding step, where a tile may have many parts; one, in a quarter of the workgroups, where tiles have 64 rows or more (1000 tokens
+// of 32 heads: 67 us in all, 73 with four).
 extern "C" __global__ __launch_bounds__(512)
 void CA_NAME(const float* __restrict__ part, ca_q* __restrict__ out) {
   __shared__ kcg_f32x4 red[8][64];
@@ -228,7 +230,7 @@ void CA_NAME(const float* __restrict__ part, ca_q* __restrict__ out) {
   const CaEnd e = ((const CaEnd*)part)[id];
   if (e.parts == 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15;
-  const int rb = blockIdx.y / (CA_NT / 2), tt = blockIdx.y % (CA_NT / 2) * 2 + (wave & 1);
+  const int unit = wave % CA_JT, of16 = blockIdx.y * CA_JT + unit, rb = of16 / CA_NT, tt = of16 % CA_NT;
   if (rb * 16 >= e.tokens * CA_GS) return;
   const int row = rb * 16 + n < e.tokens * CA_GS ? n : 0;                       // (rows that there are not were not written)
   const float* later = part + CA_ENDS + ((long long)id * 2 - 2) * CA_SLOT;       // part i > 0 is slot 0 of share id + i - 1
@@ -236,7 +238,7 @@ void CA_NAME(const float* __restrict__ part, ca_q* __restrict__ out) {
   float m = -__builtin_inff(), l = 0.0f;
   kcg_f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-  for (int i = wave >> 1; i < e.parts; i += 4) {
+  for (int i = wave / CA_JT; i < e.parts; i += 8 / CA_JT) {
     const float* p = later + ((long long)i * 2 + (i ? 0 : e.slot)) * CA_SLOT;
     const kcg_f32x4 x = *(const kcg_f32x4*)(p + of);
     const float pm = p[at], pl = p[at + 1], to = fmaxf(m, pm), ref = to == -__builtin_inff() ? 0.0f : to;
@@ -245,24 +247,28 @@ void CA_NAME(const float* __restrict__ part, ca_q* __restrict__ out) {
     l = l * fa + pl * fb;
     m = to;
   }
-  if (lane < 16) {
-    ml[wave][n][0] = m;
-    ml[wave][n][1] = l;
-  }
-  red[wave][lane] = o;
-  __syncthreads();
-  if (wave > 1) return;
-  const float top = fmaxf(fmaxf(ml[wave][n][0], ml[wave + 2][n][0]), fmaxf(ml[wave + 4][n][0], ml[wave + 6][n][0]));
-  const float ref = top == -__builtin_inff() ? 0.0f : top;
-  kcg_f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-  float total = 0.0f;
+  if (CA_JT < 8) {
+    if (lane < 16) {
+      ml[wave][n][0] = m;
+      ml[wave][n][1] = l;
+    }
+    red[wave][lane] = o;
+    __syncthreads();
+    if (wave >= CA_JT) return;
+    float top = m;
 #pragma unroll
-  for (int w = wave; w < 8; w += 2) {
-    const float f = __builtin_amdgcn_exp2f(ml[w][n][0] - ref);
-    sum += red[w][lane] * f;
-    total += ml[w][n][1] * f;
+    for (int w = unit + CA_JT; w < 8; w += CA_JT) top = fmaxf(top, ml[w][n][0]);
+    const float ref = top == -__builtin_inff() ? 0.0f : top;
+    o = kcg_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    l = 0.0f;
+#pragma unroll
+    for (int w = unit; w < 8; w += CA_JT) {
+      const float f = __builtin_amdgcn_exp2f(ml[w][n][0] - ref);
+      o += red[w][lane] * f;
+      l += ml[w][n][1] * f;
+    }
   }
-  ca_store(out, e.first, e.tokens, hv, rb, tt, sum, total);
+  ca_store(out, e.first, e.tokens, hv, rb, tt, o, l);
 }
 #else
 

@@ -20,7 +20,7 @@ def attention(d, **more):
 
 
 WRITE = dict(F16=2, WIN=1, XKT=256, XKH=128, XVT=256, XVH=128)
-GOOD = [("page_slots", dict(PAGE=16), 14), ("cache_write", dict(cache(128), **WRITE), 9), ("cache_write", dict(cache(96), **{**WRITE, "F16": 0, "WIN": 16}), 9),
+GOOD = [("cache_join", attention(96, SHARE=1, STARTS=1), 2), ("page_slots", dict(PAGE=16), 14), ("cache_write", dict(cache(128), **WRITE), 9), ("cache_write", dict(cache(96), **{**WRITE, "F16": 0, "WIN": 16}), 9),
         ("cache_read", dict(cache(64), F16=0), 6), ("cache_join", attention(128), 2), ("cache_join", attention(256, RB=2, SHARE=1, STARTS=1, WINDOW=100), 2),
         ("gemm_q4", dict(N=100, K=4096, GROUP=128, F16=0, MB=1), 6), ("gemm_q4", dict(N=4096, K=1088, GROUP=64, F16=1, MB=4, ZERO=1, SCALE_F32=1, OUT_F32=1), 6)]
 GOOD += [("cache_attention", attention(d, RB=rb, F16=d // 32 % 2, SHARE=share, STARTS=share), 16) for d in range(32, 257, 32) for rb, share in ((1, 0), (1, 1), (2, 1))]
