@@ -1754,7 +1754,7 @@ bool emitGemmQ4(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::st
   if (k % group) { err = "gemm_q4: GROUP must divide K"; return false; }
   const int64_t nt = s.get("NT", 1), wn = s.get("WN", 1), wk = s.get("WK", mb > 1 ? 1 : 8), split = s.get("SPLIT", 1), mr = s.get("MR", 16 * mb);
   const int64_t per = group >= 128 ? 1 : 128 / group;
-  const int64_t lds = std::max(wk * (wn > 1 ? 2 : 1) * mr * 528 + wk * wn * (16 * nt * 144 + 2 * per * 16 * nt * 8) + wk * (wn > 1 ? 2 : 1) * 2 * per * 16 * mb * 4 + 64, wk * wn * mb * nt * 1024);
+  const int64_t lds = std::max(wk * (wn > 1 ? 2 : 1) * mr * 528 + wk * wn * (16 * nt * 160 + 2 * per * 16 * nt * 8) + wk * (wn > 1 ? 2 : 1) * 2 * per * 16 * mb * 4 + 64, wk * wn * mb * nt * 1024);
   if (nt < 1 || nt > 8 || wn < 1 || wk < 1 || wn * wk > 16 || split < 1 || split > 64 || mr < 1 || mr > 16 * mb || (lds > 163840 && !join)) {
     err = "gemm_q4: bad NT, WN, WK, SPLIT or MR";
     return false;

@@ -19,10 +19,10 @@
 // Where a group has 128 codes or more, product j of a step's half takes k = 32 g + 8 j .. + 7 for quarter g of the wavefront, 16 bytes
 // of codes as they come; smaller groups need products of 32 neighbouring k, so the quarters exchange dwords (four permlane swaps).
 // Measured: 1 row, N = K = 4096, bf16, groups of 128: 4.4 us (2.0 TB/s; reading as many bytes alone takes 3.0); 16 rows, N 11008, K 4096, half
-// precision with zeros: 9.5 us (2.5 TB/s; reading alone 5.1); 61 rows, N 4096, K 11008, groups of 64: 20.7 us with the join's 3.  One row is
-// bound by the launch and one trip to memory; many rows by reading X from LDS (half the time of the last case) and turning codes into
-// numbers (a third), for which every wavefront's 16 or 32 columns pay anew.  The sums of X taken by the matrix product itself, with ones in
-// the weights' place, cost the last case 1.5 us.
+// precision with zeros: 9.4 us (2.5 TB/s; reading alone 5.1); 61 rows, N 4096, K 11008, groups of 64: 18.3 us with the join's 3.  One row is
+// bound by the launch and one trip to memory.  At 61 rows vector instructions are under way half of the time (codes to numbers, sums to results), LDS
+// reads, of X by every wavefront's columns anew, 43 %, matrix products 20 %, each step's one after the other.  The sums of X taken by the
+// matrix product itself, with ones in the weights' place, cost this case 1.5 us.
 // Parameters: Q4_NAME, Q4_N, Q4_K, Q4_GROUP, Q4_F16, Q4_ZERO, Q4_ST (type of the scales), Q4_YT (of the result), Q4_MB, Q4_MR (rows of X in
 // LDS, up to 16 Q4_MB), Q4_NT, Q4_WN, Q4_WK, Q4_SPLIT, Q4_WIDE, Q4_JOIN (this is gemm_q4_join).
 typedef _Float16 q4_f16x8 __attribute__((ext_vector_type(8)));
@@ -54,8 +54,13 @@ typedef unsigned q4_offset;
 #define Q4_PER (Q4_GROUP >= 128 ? 1 : 128 / Q4_GROUP)         // groups of half a step
 #define Q4_J (4 / Q4_PER)                                     // products of a group of half a step
 #define Q4_COLS (16 * Q4_NT)
-#define Q4_XPITCH 528                                         // bytes of a row of X in LDS, and of one of W: 16 more than it holds, so that
-#define Q4_WPITCH 144                                         // eight lanes that read below one another meet all banks
+// A read of 16 bytes serves sixteen lanes at a time: rows 0 to 3 and 12 to 15 of one quarter and 4 to 11 of the next.  They meet all banks
+// where rows are an odd number of 16 bytes apart and an odd quarter lies a multiple of 256 bytes behind the even one before it, in X within a
+// row, in W in a plane of its own.
+#define Q4_XPITCH 528                                         // bytes of a row of X in LDS
+#define Q4_WPITCH 80                                          // and of one in a plane of W
+#define Q4_WPLANE (Q4_COLS * Q4_WPITCH)
+#define Q4_XPLACE(g, h, j) (((g) & 1) * 16 + ((g) >> 1) * 8 + (h) * 4 + (j))
 #define Q4_XC ((Q4_MR * 32 + 64 * Q4_WN - 1) / (64 * Q4_WN))  // chunks of X that a lane brings
 #define Q4_SC ((Q4_COLS * 2 * Q4_PER + 63) / 64)              // scales that a lane brings
 
@@ -86,7 +91,7 @@ void Q4_NAME(const q4_x* __restrict__ X, const unsigned char* __restrict__ W, co
 #endif
 ) {
   struct Tiles {
-    __attribute__((aligned(16))) unsigned char x[Q4_WK][Q4_WN > 1 ? 2 : 1][Q4_MR * Q4_XPITCH], w[Q4_WK * Q4_WN][Q4_COLS * Q4_WPITCH];
+    __attribute__((aligned(16))) unsigned char x[Q4_WK][Q4_WN > 1 ? 2 : 1][Q4_MR * Q4_XPITCH], w[Q4_WK * Q4_WN][2 * Q4_WPLANE];
     kcg_f32x2 s[Q4_WK * Q4_WN][2 * Q4_PER][Q4_COLS];
     __attribute__((aligned(16))) float u[Q4_WK][Q4_WN > 1 ? 2 : 1][2 * Q4_PER][16 * Q4_MB];        // sums of X of a group
   };
@@ -124,7 +129,8 @@ void Q4_NAME(const q4_x* __restrict__ X, const unsigned char* __restrict__ W, co
     const int u = (c * Q4_WN + wn) * 64 + lane, row = u / 32, m = m0 + row;
     xk[c] = u % 32 * 8;
     xo[c] = (q4_offset)((m < M ? m : M - 1) - m0) * Q4_K + xk[c];
-    xat[c] = row < Q4_MR ? row * Q4_XPITCH + u % 32 * 16 : -1;
+    const int at = u % 16;                     // chunk of 16 bytes of the half
+    xat[c] = row < Q4_MR ? row * Q4_XPITCH + (Q4_PER == 1 ? Q4_XPLACE(at / 4, u % 32 / 16, at % 4) : Q4_XPLACE(at % 4, u % 32 / 16, at / 4)) * 16 : -1;
   }
   int se[Q4_SC], sat[Q4_SC];
 #pragma unroll
@@ -171,7 +177,7 @@ void Q4_NAME(const q4_x* __restrict__ X, const unsigned char* __restrict__ W, co
       if (lane % (16 / Q4_PER) == 0 && xat[c] >= 0) us[(lane % 32) / (16 / Q4_PER) * (16 * Q4_MB) + xat[c] / Q4_XPITCH] = Q4_ZERO ? sum : -1.5f * sum;
     }
 #pragma unroll
-    for (int b = 0; b < 2 * Q4_NT; ++b) *(kcg_u32x4*)(sh.t.w[wave] + (b * 8 + lane / 8) * Q4_WPITCH + lane % 8 * 16) = s.w[b];
+    for (int b = 0; b < 2 * Q4_NT; ++b) *(kcg_u32x4*)(sh.t.w[wave] + lane % 2 * Q4_WPLANE + (b * 8 + lane / 8) * Q4_WPITCH + lane % 8 / 2 * 16) = s.w[b];
 #pragma unroll
     for (int c = 0; c < Q4_SC; ++c)
       if (Q4_COLS * 2 * Q4_PER % 64 == 0 || sat[c] >= 0)
@@ -183,7 +189,7 @@ void Q4_NAME(const q4_x* __restrict__ X, const unsigned char* __restrict__ W, co
       kcg_u32x4 w4[Q4_NT];
 #pragma unroll
       for (int b = 0; b < Q4_NT; ++b) {
-        w4[b] = *(const kcg_u32x4*)(sh.t.w[wave] + (b * 16 + i) * Q4_WPITCH + (h * 4 + g) * 16);
+        w4[b] = *(const kcg_u32x4*)(sh.t.w[wave] + g % 2 * Q4_WPLANE + (b * 16 + i) * Q4_WPITCH + (h * 2 + g / 2) * 16);
 #if Q4_PER > 1
         // dword j of quarter g becomes dword g of quarter j
         auto x02 = __builtin_amdgcn_permlane32_swap(w4[b][0], w4[b][2], false, false);
@@ -213,7 +219,7 @@ void Q4_NAME(const q4_x* __restrict__ X, const unsigned char* __restrict__ W, co
 #pragma unroll
           for (int a = 0; a < Q4_MB; ++a) {
             const int row = a * 16 + i < Q4_MR ? a * 16 + i : Q4_MR - 1;
-            x[a] = *(const kcg_u32x4*)(xs + row * Q4_XPITCH + h * 256 + (Q4_PER == 1 ? g * 4 + j : j * 4 + g) * 16);
+            x[a] = *(const kcg_u32x4*)(xs + row * Q4_XPITCH + Q4_XPLACE(g, h, j) * 16);
           }
 #pragma unroll
           for (int b = 0; b < Q4_NT; ++b) {

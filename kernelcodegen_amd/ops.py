@@ -622,12 +622,13 @@ def _matmul_q4_form(rows, n, k, group):
 
     Up to 16 rows, a wavefront's 16 columns are a workgroup while few workgroups read few rows (a product with its neighbours' would need
     fewer, but wait for one another), else 64 columns; more rows take 64 columns and two shares of k in a workgroup, or, where there is more
-    to do, 256 columns, 32 to a wavefront, which reads the rows from LDS half as often.  A form whose workgroups do not fill the 256 units
-    splits k, at two launches' price, where a wavefront has four steps of 256 k or more.  Measured, in us (bf16, groups of 128):
-      rows 1, N = K = 4096: 16 columns 4.2, 64 columns with k split 6.2;  1, N 32000, K 4096: 18.9, 17.1
-      rows 16, N = K = 4096: 6.0, 7.1;  4, N 11008, K 4096: 7.6, 8.3;  8: 9.5, 8.9;  16: 14.9, 10.0
-      rows 32, N = K = 4096: 64 columns 8.2, 256 columns 8.9;  64: 12.4, 12.9;  128: 17.1, 15.7
-      rows 32, N 4096, K 11008: 15.2, 13.9;  64: 24.1, 21.3;  128: 37.0, 28.6;  64, N 32000, K 4096: 51.6, 39.3
+    to do, 128 columns, or 256, 32 to a wavefront, where 128 are more workgroups than units.  A form whose workgroups do not fill the 256
+    units splits k, at two launches' price, where a wavefront has four steps of 256 k or more.  Measured, in us (bf16, groups of 128):
+      rows 1, N = K = 4096: 16 columns 4.2, 64 columns with k split 6.2;  1, N 32000, K 4096: 17.5, 17.3
+      rows 16, N = K = 4096: 6.0, 7.1;  4, N 11008, K 4096: 7.9, 8.2;  8: 9.5, 8.9;  16: 14.9, 9.9
+      rows 32, N = K = 4096: 64 columns 8.2, 256 columns 9.0;  64: 11.9, 12.6;  128: 15.9, 15.7
+      rows 32, N 4096, K 11008: 64 columns 15.2, 128 columns 14.0;  64: 24, 20.1;  128: 37, 28.0
+      rows 64, N 32000, K 4096: 64 columns 52, 128 columns 37.2, 256 columns 38.6;  128: 89, 61.8, 49.9
       rows 64, N 1024, K 4096: k in four 9.9, in eight 8.2;  N = K = 1024: in one 7.5, in two 7.3"""
     blocks = min(4, -(-rows // 16))
     form = dict(MB=blocks, NT=1, WN=4, WK=2)
@@ -635,8 +636,8 @@ def _matmul_q4_form(rows, n, k, group):
         form["MR"] = 1 << (rows - 1).bit_length()
         tall = -(-n // 16)
         form.update(dict(WN=1, WK=8) if tall <= 1024 and tall * form["MR"] <= 4096 else dict(NT=2, WN=2, WK=4))
-    elif n * k * -(-rows // 64) >= 1 << 25 or (blocks == 4 and group == 32):        # (64 rows, two shares and groups of 32: LDS is too small)
-        form.update(NT=2, WN=8, WK=1)
+    elif n * k * -(-rows // 64) >= 1 << 25 or (blocks == 4 and group < 128):        # (64 rows, two shares and their small groups' scales: LDS is too small)
+        form.update(NT=1 if -(-n // 128) * -(-rows // 64) <= 256 else 2, WN=8, WK=1)
     workgroups = -(-n // (16 * form["NT"] * form["WN"])) * -(-rows // (16 * blocks))
     steps = -(-k // 256) // form["WK"]
     form["SPLIT"] = max(1, min(256 // workgroups, steps, 64)) if form["WN"] > 1 and steps >= 4 else 1
