@@ -1681,13 +1681,10 @@ bool emitCacheWrite(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std
 
 bool emitCacheRead(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::string& err) {
   if (!cacheShape(s, {"KP", "KT", "KH"}, err) || !whole(s, "F16", 0, 2, err)) return false;
-  const int64_t unroll = s.get("UNROLL", 1);
-  if (unroll < 1 || unroll > 8) { err = "cache_read: UNROLL must be in [1,8]"; return false; }
-  s.p["UNROLL"] = unroll;
   Defines d;
   d.add("CR_NAME", s.name);
   d.add("CR_T", std::string(typeName(s.p["F16"])));
-  d.add("CR_H", s.p["H"]); d.add("CR_D", s.p["D"]); d.add("CR_PAGE", s.p["PAGE"]); d.add("CR_UNROLL", unroll);
+  d.add("CR_H", s.p["H"]); d.add("CR_D", s.p["D"]); d.add("CR_PAGE", s.p["PAGE"]);
   d.add("CR_P", std::to_string(s.p["KP"]) + "LL"); d.add("CR_TS", std::to_string(s.p["KT"]) + "LL"); d.add("CR_HS", std::to_string(s.p["KH"]) + "LL");
   src = d.wrap(kTpl_cache_read);
   info.name = s.name;

@@ -1,7 +1,8 @@
 // ---- rows of a paged cache in 8 bits ----
 //   out[t, h] = e4m3 number * scale[page, h], in CR_T; slots that are no slot of the cache give zeros
-// A lane takes 8 elements, neighbouring lanes one row, and rows of neighbouring heads follow: bound by the bytes written.
-// Parameters: CR_NAME, CR_H, CR_D, CR_PAGE, CR_T, CR_P CR_TS CR_HS (strides of page, token, head, bytes), CR_UNROLL.
+// A lane takes 8 elements, neighbouring lanes one row, and rows of neighbouring heads follow: bound by the bytes written
+// (9000 tokens of 8 heads of 128 in half precision: 6.9 us, 4.0 TB/s; 40000: 27, 4.6; two or four times as many to a lane no faster).
+// Parameters: CR_NAME, CR_H, CR_D, CR_PAGE, CR_T, CR_P CR_TS CR_HS (strides of page, token, head, bytes).
 typedef CR_T cr_t;
 typedef cr_t cr_x8 __attribute__((ext_vector_type(8)));
 #define CR_LPR (CR_D / 8)
@@ -9,37 +10,25 @@ typedef cr_t cr_x8 __attribute__((ext_vector_type(8)));
 extern "C" __global__ __launch_bounds__(256)
 void CR_NAME(const unsigned char* __restrict__ cache, const float* __restrict__ scales, const long long* __restrict__ slots, long long T,
              long long pages, cr_t* __restrict__ out) {
-  const long long total = T * (CR_H * CR_LPR), base = (long long)blockIdx.x * (256 * CR_UNROLL) + threadIdx.x;
-  kcg_u32x2 w[CR_UNROLL];
-  float s[CR_UNROLL];
-#pragma unroll
-  for (int i = 0; i < CR_UNROLL; ++i) {
-    const long long u = base + i * 256;
-    w[i] = kcg_u32x2{0, 0};
-    s[i] = 0.0f;
-    if (u < total) {
-      const long long t = u / (CR_H * CR_LPR);
-      const int at = (int)(u - t * (CR_H * CR_LPR)), h = at / CR_LPR, c = at % CR_LPR;
-      const long long slot = slots[t];
-      if (slot >= 0 && slot < pages * CR_PAGE) {
-        const long long page = slot / CR_PAGE;
-        s[i] = scales[page * CR_H + h];
-        w[i] = *(const kcg_u32x2*)(cache + page * CR_P + (slot - page * CR_PAGE) * CR_TS + (long long)h * CR_HS + c * 8);
-      }
-    }
+  const long long u = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (u >= T * (CR_H * CR_LPR)) return;
+  const long long t = u / (CR_H * CR_LPR);
+  const int at = (int)(u - t * (CR_H * CR_LPR)), h = at / CR_LPR, c = at % CR_LPR;
+  const long long slot = slots[t];
+  kcg_u32x2 w = {0, 0};
+  float s = 0.0f;
+  if (slot >= 0 && slot < pages * CR_PAGE) {
+    const long long page = slot / CR_PAGE;
+    s = scales[page * CR_H + h];
+    w = *(const kcg_u32x2*)(cache + page * CR_P + (slot - page * CR_PAGE) * CR_TS + (long long)h * CR_HS + c * 8);
   }
+  cr_x8 o;
 #pragma unroll
-  for (int i = 0; i < CR_UNROLL; ++i) {
-    const long long u = base + i * 256;
-    if (u >= total) continue;
-    cr_x8 o;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      o[4 * j + 0] = (cr_t)(__builtin_amdgcn_cvt_f32_fp8(w[i][j], 0) * s[i]);
-      o[4 * j + 1] = (cr_t)(__builtin_amdgcn_cvt_f32_fp8(w[i][j], 1) * s[i]);
-      o[4 * j + 2] = (cr_t)(__builtin_amdgcn_cvt_f32_fp8(w[i][j], 2) * s[i]);
-      o[4 * j + 3] = (cr_t)(__builtin_amdgcn_cvt_f32_fp8(w[i][j], 3) * s[i]);
-    }
-    *(cr_x8*)(out + u * 8) = o;
+  for (int j = 0; j < 2; ++j) {
+    o[4 * j + 0] = (cr_t)(__builtin_amdgcn_cvt_f32_fp8(w[j], 0) * s);
+    o[4 * j + 1] = (cr_t)(__builtin_amdgcn_cvt_f32_fp8(w[j], 1) * s);
+    o[4 * j + 2] = (cr_t)(__builtin_amdgcn_cvt_f32_fp8(w[j], 2) * s);
+    o[4 * j + 3] = (cr_t)(__builtin_amdgcn_cvt_f32_fp8(w[j], 3) * s);
   }
+  *(cr_x8*)(out + u * 8) = o;
 }

@@ -11,6 +11,7 @@
 // pages go; then rows and old scale are one more trip to memory, before the stores: what bounds a small step.
 // A lane takes 8 elements, CW_RPP rows a pass; rows are held in registers between the two passes (magnitude, conversion) as far as CW_HOLD
 // passes reach, else read again, from the caches.  Passes behind the last row read the last again, so that no load waits for a branch.
+// Measured, 8 heads of 128: 64 tokens of a page each 2.9 us (an empty launch 1.7); 9000 tokens of whole pages, half precision, 12.5 us, 4.4 TB/s.
 // Parameters: CW_NAME, CW_H, CW_D, CW_PAGE, CW_T (input type), CW_ESIZE, CW_WIN, strides as in cache_attention: CW_KP .. CW_VH (bytes), CW_XKT
 // CW_XKH CW_XVT CW_XVH (of k and v, elements).
 typedef CW_T cw_t;

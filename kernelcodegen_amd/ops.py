@@ -428,7 +428,9 @@ def _cache_write_launch(k, v, k_cache, v_cache, k_scale, v_scale, slots):
     tokens, heads, d = k.shape
     if heads != k_cache.shape[2] or tuple(slots.shape) != (tokens,) or tokens > 0x7FFFFE00:
         raise ValueError("one slot per token, and the cache's heads, are needed")
-    win = 1 if tokens <= 512 else 16
+    # tokens of a wavefront, which takes the pages they lead one after the other: us for tokens of a page each and of whole pages (8 heads of 128)
+    # 128 tokens: one 3.5 and 4, four 5.2 and 3.3;  512: one 6.2 and 8.2, four 6.8 and 4.1, sixteen 15 and 3.6;  9000 of whole pages: 58, 29, 12.5
+    win = 1 if tokens <= 128 else 4 if tokens <= 2048 else 16
     kern = R.get_kernel("cache_write", H=heads, D=d, PAGE=k_cache.shape[1], F16=_STORAGE[k.dtype], WIN=win, KP=ks[0], KT=ks[1], KH=ks[2],
                         VP=vs[0], VT=vs[1], VH=vs[2], XKT=xk[0], XKH=xk[1], XVT=xv[0], XVH=xv[1])
     run = kern.bind(grid=(max(1, -(-2 * heads * -(-tokens // win) // 4)),))
@@ -454,7 +456,7 @@ def _cache_read_launch(cache, scale, slots, dtype):
     s = _cache_strides(cache, scale)
     page, heads, d = cache.shape[1:]
     tokens = slots.shape[0]
-    kern = R.get_kernel("cache_read", H=heads, D=d, PAGE=page, F16=_STORAGE[dtype], KP=s[0], KT=s[1], KH=s[2], UNROLL=1)
+    kern = R.get_kernel("cache_read", H=heads, D=d, PAGE=page, F16=_STORAGE[dtype], KP=s[0], KT=s[1], KH=s[2])
     return _into_last(kern.bind(grid=(max(1, -(-tokens * heads * d // 2048)),)), ((tokens, heads, d), dtype))
 
 
