@@ -469,8 +469,8 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, table, lengths, start
     and rows behind the last request's, are zeros.
       score = scale * q.k (scale: d^-0.5), then cap * tanh(score / cap), then + slopes[head] * (key's position - row's), slopes fp32
       [heads]; a row sees the keys up to its own position, of these the last `window`.
-    Entries of the table behind a request's length are not read; keys on pages that are not the cache's count as not there.  `cfg`
-    overrides kernel parameters (RB, WAVES, GRID, LEAST, OCC, WHOLE)."""
+    Entries of the table behind a request's length have no effect; keys on pages that are not the cache's count as not there.  `cfg`
+    overrides kernel parameters (RB, SHARE, WAVES, WHOLE, GRID, LEAST, OCC)."""
     scale, cap, window = None if scale is None else float(scale), float(cap or 0.0), operator.index(window or 0)
     key = ("cache_attention", R.signature(q, k_cache, v_cache, k_scale, v_scale, table, lengths, starts, slopes), scale, cap, window)
     hit = None if cfg else _bound.get(key)
