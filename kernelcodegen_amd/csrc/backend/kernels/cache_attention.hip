@@ -389,6 +389,9 @@ __device__ __forceinline__ bool ca_begin(int id, int piece, float* __restrict__ 
 // LDS buffers together; so a key is read once for 16 CA_RB CA_WAVES rows and nothing is added up between wavefronts.
 // Measured: 1500 tokens of 32 heads over 8 of 128, behind 2 requests of up to 6000 keys, 162 us with the join, 620 TFLOP/s as 16-bit products
 // would count; vector instructions are under way 59 % of the time (scores, exp2, V to half precision), matrix instructions 29 %.
+// V is converted on its way into LDS, once for all wavefronts, as far as LDS holds two such workgroups (D up to 128).
+#define CA_V16 (CA_D <= 128)
+#define CA_VP16 (2 * CA_D + 32)              // bytes of a key's V in half precision: the eight rows of 32 bytes that 32 lanes read together meet all banks
 #define CA_SL ((4 * CA_D + 64 * CA_WAVES - 1) / (64 * CA_WAVES))     // chunks of 16 bytes of a step's K, and of its V, that a lane brings
 extern "C" __global__ __launch_bounds__(64 * CA_WAVES, CA_OCC)
 void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, const unsigned char* __restrict__ vc,
@@ -396,7 +399,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
              const int* __restrict__ lengths, const int* __restrict__ starts, const float* __restrict__ slopes,
              float* __restrict__ part, long long T_, long long B_, long long W_, long long table_row, long long pages_, ca_q* __restrict__ out) {
   struct Shared {
-    __attribute__((aligned(16))) unsigned char k[2][64 * CA_KP_], v[2][CA_VROW(63) + CA_VP_];
+    __attribute__((aligned(16))) unsigned char k[2][64 * CA_KP_], v[2][CA_V16 ? 64 * CA_VP16 : CA_VROW(63) + CA_VP_];
     int nan[4];                  // whether a step has NaN in V where that matters, steps in turn
   };
   __shared__ Shared sh;
@@ -421,9 +424,32 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
     koff[u] = (of[u] % 16) * (unsigned)CA_KT + part16;
     voff[u] = (of[u] % 16) * (unsigned)CA_VT + part16;
     kat[u] = of[u] * CA_KP_ + part16;
-    vat[u] = CA_VROW(of[u]) + part16;
+    vat[u] = CA_V16 ? of[u] * CA_VP16 + 2 * part16 : CA_VROW(of[u]) + part16;
   }
-  const int key8 = n / 2 < 4 ? g * 4 + n / 2 : 16 + g * 4 + n / 2 - 4;        // the row that this lane gives the address of in transposing reads
+  auto stage = [&](unsigned char* vb, int u, const kcg_u32x4& x) __attribute__((always_inline)) {
+#if CA_V16
+    const unsigned x0 = x[0], x1 = x[1], x2 = x[2], x3 = x[3];
+    *(kcg_u32x4*)(vb + vat[u]) = kcg_u32x4{CA_CVT16(x0, false), CA_CVT16(x0, true), CA_CVT16(x1, false), CA_CVT16(x1, true)};
+    *(kcg_u32x4*)(vb + vat[u] + 16) = kcg_u32x4{CA_CVT16(x2, false), CA_CVT16(x2, true), CA_CVT16(x3, false), CA_CVT16(x3, true)};
+#else
+    *(kcg_u32x4*)(vb + vat[u]) = x;
+#endif
+  };
+  // V of the keys that this lane has scores of, in column n of tile tt and half h of the step.  Of 16 bits a transposing read gives a lane four rows
+  // of its column: lane 4 j + i of a group of 16 gives the address of quarter i of row j.
+  const int key8 = n / 2 < 4 ? g * 4 + n / 2 : 16 + g * 4 + n / 2 - 4;        // the row that this lane gives the address of, of 8 bits
+  const int vof = CA_V16 ? (g * 4 + n / 4) * CA_VP16 + n % 4 * 8 : CA_VROW(key8) + (n & 1) * 8;
+  auto columns = [&](unsigned char* vb, int h, int tt) __attribute__((always_inline)) {
+#if CA_V16
+    typedef short ca_s16x4 __attribute__((ext_vector_type(4)));
+    const ca_lds p = (ca_lds)vb + vof + h * 32 * CA_VP16 + tt * 32;
+    const ca_s16x4 near = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ca_s16x4*)p);
+    const ca_s16x4 far = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ca_s16x4*)(p + 16 * CA_VP16));
+    return __builtin_bit_cast(kcg_u32x4, __builtin_shufflevector(near, far, 0, 1, 2, 3, 4, 5, 6, 7));
+#else
+    return ca_columns((ca_lds)vb + vof + h * CA_VROW(32) + tt * 16);
+#endif
+  };
   int count = 0;                  // steps so far
 
   while (left > 0) {
@@ -536,7 +562,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
           if (flagged)
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = ca_nan_bytes(x[i]) * 0x38u;       // 1.0 where V is NaN, first
-          *(kcg_u32x4*)(vb + vat[u]) = x;
+          stage(vb, u, x);
         }
         if (threadIdx.x == 0) sh.nan[(count + 2) & 3] = 0;                       // (read last two steps ago)
         const bool more = key + CA_UK < end;
@@ -618,7 +644,6 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
             }
           }
         }
-        const ca_lds vread = (ca_lds)vb + CA_VROW(key8) + (n & 1) * 8;
         if (flagged) {
           // NaN where some rows see the key and some may not: it goes to those that do, by a product of where V is NaN and who sees
           if (work)
@@ -632,7 +657,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
                   see[j] = (sc[rb][2 * h + j / 2][j % 2 * 2] != -__builtin_inff() ? 0x3c00u : 0u) | (sc[rb][2 * h + j / 2][j % 2 * 2 + 1] != -__builtin_inff() ? 0x3c000000u : 0u);
                 const kcg_u32x4 who = {see[0], see[1], see[2], see[3]};
 #pragma unroll
-                for (int tt = 0; tt < CA_NT; ++tt) ca_spread_nan(ca_columns(vread + h * CA_VROW(32) + tt * 16), who, acc[rb][tt]);
+                for (int tt = 0; tt < CA_NT; ++tt) ca_spread_nan(columns(vb, h, tt), who, acc[rb][tt]);
               }
           __syncthreads();
 #pragma unroll
@@ -640,7 +665,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
             kcg_u32x4 x = v[u];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] &= ~(ca_nan_bytes(x[i]) * 0xffu);
-            *(kcg_u32x4*)(vb + vat[u]) = x;
+            stage(vb, u, x);
           }
           if (more) load(key + CA_UK, step, now);
           __syncthreads();
@@ -650,7 +675,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int tt = 0; tt < CA_NT; ++tt) {
-              const kcg_u32x4 vf = ca_columns(vread + h * CA_VROW(32) + tt * 16);
+              const kcg_u32x4 vf = columns(vb, h, tt);
 #pragma unroll
               for (int rb = 0; rb < CA_RB; ++rb) {
                 const kcg_u32x4 p = {pf[rb][4 * h], pf[rb][4 * h + 1], pf[rb][4 * h + 2], pf[rb][4 * h + 3]};
