@@ -19,9 +19,9 @@
 // Where a group has 128 codes or more, product j of a step's half takes k = 32 g + 8 j .. + 7 for quarter g of the wavefront, 16 bytes
 // of codes as they come; smaller groups need products of 32 neighbouring k, so the quarters exchange dwords (four permlane swaps).
 // Measured: 1 row, N = K = 4096, bf16, groups of 128: 4.4 us (2.0 TB/s; reading as many bytes alone takes 3.0); 16 rows, N 11008, K 4096, half
-// precision with zeros: 9.4 us (2.5 TB/s; reading alone 5.1); 61 rows, N 4096, K 11008, groups of 64: 18.3 us with the join's 3.  One row is
+// precision with zeros: 9.4 us (2.5 TB/s; reading alone 5.1); 61 rows, N 4096, K 11008, groups of 64: 18.1 us with the join's 3.  One row is
 // bound by the launch and one trip to memory.  At 61 rows vector instructions are under way half of the time (codes to numbers, sums to results), LDS
-// reads, of X by every wavefront's columns anew, 43 %, matrix products 20 %, each step's one after the other.  The sums of X taken by the
+// accesses, of X by every wavefront's columns anew, 57 %, matrix products 20 %, each step's one after the other.  The sums of X taken by the
 // matrix product itself, with ones in the weights' place, cost this case 1.5 us.
 // Parameters: Q4_NAME, Q4_N, Q4_K, Q4_GROUP, Q4_F16, Q4_ZERO, Q4_ST (type of the scales), Q4_YT (of the result), Q4_MB, Q4_MR (rows of X in
 // LDS, up to 16 Q4_MB), Q4_NT, Q4_WN, Q4_WK, Q4_SPLIT, Q4_WIDE, Q4_JOIN (this is gemm_q4_join).
@@ -56,7 +56,7 @@ typedef unsigned q4_offset;
 #define Q4_COLS (16 * Q4_NT)
 // A read of 16 bytes serves sixteen lanes at a time: rows 0 to 3 and 12 to 15 of one quarter and 4 to 11 of the next.  They meet all banks
 // where rows are an odd number of 16 bytes apart and an odd quarter lies a multiple of 256 bytes behind the even one before it, in X within a
-// row, in W in a plane of its own.
+// row, in W in a plane of its own.  Lanes bring the chunks in an order whose writes meet few banks twice.
 #define Q4_XPITCH 528                                         // bytes of a row of X in LDS
 #define Q4_WPITCH 80                                          // and of one in a plane of W
 #define Q4_WPLANE (Q4_COLS * Q4_WPITCH)
@@ -118,19 +118,20 @@ void Q4_NAME(const q4_x* __restrict__ X, const unsigned char* __restrict__ W, co
   // takes part with zeros of X.  (All loads are unconditional: one behind a branch would be waited for there.)  Addresses are a uniform
   // base, which goes on with the steps, and an offset of the lane's.
   q4_offset wo[2 * Q4_NT], xo[Q4_XC], so[Q4_SC];
+  const int wc = lane % 4 * 2 + lane % 8 / 4;        // chunk of a row of W: lanes 0 to 3 the even ones, which go into one plane
 #pragma unroll
   for (int b = 0; b < 2 * Q4_NT; ++b) {
     const int n = n0 + b * 8 + lane / 8;
-    wo[b] = (q4_offset)(n < Q4_N ? n : Q4_N - 1) * (Q4_K / 2) + lane % 8 * 16;
+    wo[b] = (q4_offset)(n < Q4_N ? n : Q4_N - 1) * (Q4_K / 2) + wc * 16;
   }
   int xk[Q4_XC], xat[Q4_XC];
 #pragma unroll
   for (int c = 0; c < Q4_XC; ++c) {
     const int u = (c * Q4_WN + wn) * 64 + lane, row = u / 32, m = m0 + row;
-    xk[c] = u % 32 * 8;
+    const int q = u % 16 / 4, j = u % 4;       // quarter and product that this lane's chunk of 8 k is for
+    xk[c] = u % 32 / 16 * 128 + (Q4_PER == 1 ? q * 4 + j : j * 4 + q) * 8;
     xo[c] = (q4_offset)((m < M ? m : M - 1) - m0) * Q4_K + xk[c];
-    const int at = u % 16;                     // chunk of 16 bytes of the half
-    xat[c] = row < Q4_MR ? row * Q4_XPITCH + (Q4_PER == 1 ? Q4_XPLACE(at / 4, u % 32 / 16, at % 4) : Q4_XPLACE(at % 4, u % 32 / 16, at / 4)) * 16 : -1;
+    xat[c] = row < Q4_MR ? row * Q4_XPITCH + Q4_XPLACE(q, u % 32 / 16, j) * 16 : -1;
   }
   int se[Q4_SC], sat[Q4_SC];
 #pragma unroll
@@ -154,7 +155,7 @@ void Q4_NAME(const q4_x* __restrict__ X, const unsigned char* __restrict__ W, co
     }
     const unsigned char* wk0 = W + k0 / 2;
 #pragma unroll
-    for (int b = 0; b < 2 * Q4_NT; ++b) s.w[b] = *(const kcg_u32x4*)(wk0 + (Q4_K % 256 == 0 || k0 + lane % 8 * 32 < Q4_K ? wo[b] : wo[b] - lane % 8 * 16));
+    for (int b = 0; b < 2 * Q4_NT; ++b) s.w[b] = *(const kcg_u32x4*)(wk0 + (Q4_K % 256 == 0 || k0 + wc * 32 < Q4_K ? wo[b] : wo[b] - wc * 16));
     const q4_x* xk0 = X + (long long)m0 * Q4_K + k0;
 #pragma unroll
     for (int c = 0; c < Q4_XC; ++c) s.x[c] = *(const kcg_u32x4*)(xk0 + (Q4_K % 256 == 0 || k0 + xk[c] < Q4_K ? xo[c] : xo[c] - xk[c]));
@@ -170,14 +171,17 @@ void Q4_NAME(const q4_x* __restrict__ X, const unsigned char* __restrict__ W, co
       // the sum over the lanes that have a group of the row (16, 8 or 4), times -1.5 where that is 1 + zero / 16 for all columns
       const unsigned v0 = v[0], v1 = v[1], v2 = v[2], v3 = v[3];      // (bit_cast of a vector's element takes the first)
       float sum = Q4_DOT(v0, Q4_DOT(v1, Q4_DOT(v2, Q4_DOT(v3, 0.0f))));
-      sum += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, sum), 0xb1, 0xf, 0xf, true));      // quad_perm: 1 0 3 2
-      sum += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, sum), 0x4e, 0xf, 0xf, true));      // quad_perm: 2 3 0 1
-      if (Q4_PER < 4) sum += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, sum), 0x141, 0xf, 0xf, true));      // row_half_mirror
-      if (Q4_PER < 2) sum += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, sum), 0x140, 0xf, 0xf, true));      // row_mirror
-      if (lane % (16 / Q4_PER) == 0 && xat[c] >= 0) us[(lane % 32) / (16 / Q4_PER) * (16 * Q4_MB) + xat[c] / Q4_XPITCH] = Q4_ZERO ? sum : -1.5f * sum;
+#define Q4_ADD(control) sum += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, sum), control, 0xf, 0xf, true))
+      if (Q4_PER < 4) Q4_ADD(0xb1);            // quad_perm: 1 0 3 2
+      if (Q4_PER < 2) Q4_ADD(0x4e);            // quad_perm: 2 3 0 1
+      Q4_ADD(0x124);                           // row_ror 4, 8: over the quarters
+      Q4_ADD(0x128);
+#undef Q4_ADD
+      if (lane % 16 / 4 == 0 && lane % (4 / Q4_PER) == 0 && xat[c] >= 0)
+        us[(lane % 32 / 16 * Q4_PER + lane % 4 / (4 / Q4_PER)) * (16 * Q4_MB) + xat[c] / Q4_XPITCH] = Q4_ZERO ? sum : -1.5f * sum;
     }
 #pragma unroll
-    for (int b = 0; b < 2 * Q4_NT; ++b) *(kcg_u32x4*)(sh.t.w[wave] + lane % 2 * Q4_WPLANE + (b * 8 + lane / 8) * Q4_WPITCH + lane % 8 / 2 * 16) = s.w[b];
+    for (int b = 0; b < 2 * Q4_NT; ++b) *(kcg_u32x4*)(sh.t.w[wave] + lane % 8 / 4 * Q4_WPLANE + (b * 8 + lane / 8) * Q4_WPITCH + lane % 4 * 16) = s.w[b];
 #pragma unroll
     for (int c = 0; c < Q4_SC; ++c)
       if (Q4_COLS * 2 * Q4_PER % 64 == 0 || sat[c] >= 0)
