@@ -457,6 +457,18 @@ def test_matmul_q4_keeps_infinities_to_their_rows():
     assert bool(got[3].isnan().all()) and bool((got[[0, 1, 2, 4]] == 128).all())
 
 
+def test_matmul_q4_of_more_than_2_gib_of_codes():
+    n, k = 65600, 65536
+    w = torch.full((n, k // 2), 0x88, device="cuda", dtype=torch.uint8)
+    scale = torch.ones((n, k // 128), device="cuda", dtype=torch.bfloat16)
+    x = torch.zeros((2, k), device="cuda", dtype=torch.bfloat16)
+    x[0], x[1, -1] = 1, 2
+    w[-1, -1] = 0xf9              # k - 2: 9 - 8, k - 1: 15 - 8
+    w[n - 70, 5] = 0x08
+    got = ops.matmul_q4(x, w, scale, out_dtype=torch.float32)
+    assert got[:, -1].tolist() == [8, 14] and got[:, n - 70].tolist() == [-8, 0] and int((got != 0).sum()) == 3
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_matmul_q4_of_subnormal_rows(dtype):
     # the rows times 2^-20 are subnormal in half precision; they are whole multiples of 2^-20, and sums of 512 of them times a code need no more
@@ -479,6 +491,21 @@ def test_results_of_one_launch_live_on_their_own():
     again = [ops.page_slots(*args, 16, 6) for _ in range(20)]
     torch.cuda.synchronize()
     assert kept.flatten().tolist() == [7 * 16 + 5, 20 * 16, 20 * 16 + 1, 4 * 16 + 15, 21 * 16, 21 * 16 + 1] and len(again) == 20
+
+
+def test_results_in_inference_mode_and_of_operands_with_gradients():
+    args = (ints([5, 0]), ints([1, 2]), ints([[7, 0], [0, 0]]), ints([20, 21]))
+    want = [r.tolist() for r in ops.page_slots(*args, 16, 4)]
+    x = torch.randn((2, 64), device="cuda").half().requires_grad_()
+    w, s = torch.full((8, 32), 0x9a, device="cuda", dtype=torch.uint8), torch.ones((8, 1), device="cuda", dtype=torch.half)
+    plain = ops.matmul_q4(x, w, s)
+    assert not plain.requires_grad
+    with torch.inference_mode():
+        got = ops.page_slots(*args, 16, 4)
+        assert [r.tolist() for r in got] == want and all(r.is_inference() for r in got)
+        assert (got[0] + 1).tolist() == [v + 1 for v in want[0]] and got[1].add_(1).tolist() == [v + 1 for v in want[1]]
+        inside = ops.matmul_q4(x, w, s)
+        assert inside.is_inference() and torch.equal(inside, plain)
 
 
 # ---- refusals, streams ----
