@@ -623,11 +623,12 @@ def _matmul_q4_form(rows, n, k, group):
     """The tiles and the splitting of k, by the columns of a workgroup and the rows of X that every workgroup reads again.
 
     Up to 16 rows, a wavefront's 16 columns are a workgroup while few workgroups read few rows (a product with its neighbours' would need
-    fewer, but wait for one another), else 64 columns; more rows take 64 columns and two shares of k in a workgroup, or, where there is more
+    fewer, but wait for one another), else 32 or 48, where those are no more workgroups than units, or 64; more rows take 64 columns and two shares of k in a workgroup, or, where there is more
     to do, 128 columns, or 256, 32 to a wavefront, where 128 are more workgroups than units.  A form whose workgroups do not fill the 256
     units splits k, at two launches' price, where a wavefront has four steps of 256 k or more.  Measured, in us (bf16, groups of 128):
       rows 1, N = K = 4096: 16 columns 4.2, 64 columns with k split 6.2;  1, N 32000, K 4096: 17.5, 17.3
-      rows 16, N = K = 4096: 6.0, 7.1;  4, N 11008, K 4096: 7.9, 8.2;  8: 9.5, 8.9;  16: 14.9, 9.9
+      rows 16, N = K = 4096: 6.0, 7.1;  4, N 11008, K 4096: 7.9, 8.2;  8: 9.5, 8.9, 48 columns 8.2;  16, half with zeros: 64 columns 10.9, 48 9.9
+      rows 16, N 8192, K 4096: 64 columns 9.1, 32 columns 7.4;  N 14336: 64 columns 10.5, 48 columns 15.5
       rows 32, N = K = 4096: 64 columns 8.2, 256 columns 9.0;  64: 11.9, 12.6;  128: 15.9, 15.7
       rows 32, N 4096, K 11008: 64 columns 15.2, 128 columns 14.0;  64: 24, 20.1;  128: 37, 28.0
       rows 64, N 32000, K 4096: 64 columns 52, 128 columns 37.2, 256 columns 38.6;  128: 89, 61.8, 49.9
@@ -637,7 +638,10 @@ def _matmul_q4_form(rows, n, k, group):
     if blocks == 1:
         form["MR"] = 1 << (rows - 1).bit_length()
         tall = -(-n // 16)
-        form.update(dict(WN=1, WK=8) if tall <= 1024 and tall * form["MR"] <= 4096 else dict(NT=2, WN=2, WK=4))
+        if tall <= 768 or tall <= 1024 and tall * form["MR"] <= 4096:
+            form.update(NT=1 if tall * form["MR"] <= 4096 else -(-tall // 256), WN=1, WK=8)
+        else:
+            form.update(NT=2, WN=2, WK=4)
     elif n * k * -(-rows // 64) >= 1 << 25 or (blocks == 4 and group < 128):        # (64 rows, two shares and their small groups' scales: LDS is too small)
         form.update(NT=1 if -(-n // 128) * -(-rows // 64) <= 256 else 2, WN=8, WK=1)
     workgroups = -(-n // (16 * form["NT"] * form["WN"])) * -(-rows // (16 * blocks))

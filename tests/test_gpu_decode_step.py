@@ -421,7 +421,7 @@ def test_cache_attention_offsets_beyond_32_bits():
     (1, 16, 128, 128, False, False, False), (1, 1, 32, 32, True, True, True), (3, 37, 96, 32, True, False, True), (16, 100, 4096, 128, True, False, False),
     (17, 333, 1088, 64, False, True, False), (33, 48, 1024, 256, True, False, True), (64, 129, 544, 32, False, False, False), (130, 65, 1920, 64, True, False, False),
     (5, 1001, 2176, 128, True, True, True), (2, 4097, 640, 640, False, False, False), (9, 8203, 288, 32, True, False, False), (16, 4211, 4160, 64, False, False, False),
-    (20, 2100, 16384, 128, True, False, False), (70, 1030, 16448, 64, False, True, True), (33, 200, 4352, 128, False, False, False)])
+    (20, 2100, 16384, 128, True, False, False), (70, 1030, 16448, 64, False, True, True), (33, 200, 4352, 128, False, False, False), (11, 9003, 544, 32, True, True, False), (7, 12500, 384, 128, True, False, True)])
 def test_matmul_q4(dtype, m, n, k, group, zero, scale32, out32):
     g = generator(m * n + k)
     x = (torch.randn((m, k), generator=g, device="cuda") + 0.5).to(DTYPE[dtype])
