@@ -56,6 +56,7 @@ typedef __bf16 ca_q;
 #define CA_PARTS ((CA_G + CA_GS - 1) / CA_GS)    // tiles that the heads of a group are cut into
 #define CA_HV (CA_HKV * CA_PARTS)
 #define CA_UK (CA_SHARE ? 64 : 32 * CA_WAVES)
+static_assert(0x7fff0000LL + 96 * CA_UK + 32 <= 0x7fffffff, "positions ahead of the last key of the longest request have 32 bits");
 #define CA_LAZY 6.0f
 #define CA_TINY 1.17549435e-38f               // the least normal number: scales below count as zero
 #define CA_SLOT (CA_ROWS * CA_D + 2 * CA_ROWS)   // floats of a partial result

@@ -507,7 +507,8 @@ def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, length
     if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
         raise ValueError("the table must be an int32 device tensor [B, W] with rows of neighbouring entries")
     batch, width = table.shape
-    if batch < 1 or width < 1 or width * page > 0x7FFFFF00 or tokens > 0x7FFFFF00 or tuple(lengths.shape) != (batch,):
+    # (positions have 32 bits in the kernel, which looks up the pages of up to 96 steps ahead)
+    if batch < 1 or width < 1 or width * page > 0x7FFF0000 or tokens > 0x7FFF0000 or tuple(lengths.shape) != (batch,):
         raise ValueError("lengths is [B] and table [B, W], neither B nor W being 0")
     if starts is None and tokens != batch:
         raise ValueError("without starts there is one row per request")
