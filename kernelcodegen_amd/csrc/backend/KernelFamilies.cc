@@ -1735,7 +1735,7 @@ bool emitCacheAttention(KernelSpec& s, std::string& src, KernelLaunchInfo& info,
   src = d.wrap(kTpl_cache_attention);
   info.name = s.name;
   info.grid[0] = (uint32_t)((join ? std::max<int64_t>(1, pieces - 1) : pieces) * hv);
-  if (join) info.grid[1] = (uint32_t)(blocks * dh / 16 / jt);
+  if (join) info.grid[1] = (uint32_t)ceilDiv(blocks * dh / 16, jt);
   info.block[0] = (uint32_t)(join ? 512 : 64 * waves);
   info.numArgs = join ? 2 : 16;
   return true;

@@ -222,6 +222,7 @@ struct CaEnd { int first, tokens, parts, slot; };      // rows, parts (0: nothin
 #define CA_ENDS (4 * CA_HV * CA_PIECES)                // floats of all of them, in front of the parts
 
 #if CA_JOIN
+static_assert(CA_JT == 8 || CA_BLOCKS * CA_NT % CA_JT == 0, "wavefronts that share columns meet at barriers");
 // A workgroup for every beginning of a share and CA_JT tiles of 16 rows and 16 columns of O; it has something to do where that is the first one
 // inside of a tile of rows, and adds up the parts of the tile.  8 / CA_JT wavefronts take every so many-th part of the same columns: four
 // in a decoding step, where a tile may have many parts; one, in a quarter of the workgroups, where tiles have 64 rows or more (1000 tokens
@@ -235,7 +236,7 @@ void CA_NAME(const float* __restrict__ part, ca_q* __restrict__ out) {
   if (e.parts == 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15;
   const int unit = wave % CA_JT, of16 = blockIdx.y * CA_JT + unit, rb = of16 / CA_NT, tt = of16 % CA_NT;
-  if (rb * 16 >= e.tokens * CA_GS) return;
+  if (rb >= CA_BLOCKS || rb * 16 >= e.tokens * CA_GS) return;      // (the last workgroup of a tile may have more wavefronts than there are columns)
   const int row = rb * 16 + n < e.tokens * CA_GS ? n : 0;                       // (rows that there are not were not written)
   const float* later = part + CA_ENDS + ((long long)id * 2 - 2) * CA_SLOT;       // part i > 0 is slot 0 of share id + i - 1
   const int at = CA_ROWS * CA_D + (rb * 16 + row) * 2, of = ((rb * CA_NT + tt) * 64 + lane - n + row) * 4;

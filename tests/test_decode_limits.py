@@ -61,3 +61,13 @@ def test_positions_ahead_of_the_last_key_stay_within_32_bits(monkeypatch, page):
         with pytest.raises(ValueError):
             attention(monkeypatch, 1, 1, width, page)
     attention(monkeypatch, 1, 1, 0x7FFF0000 // page, page)
+
+
+@pytest.mark.parametrize("waves", [1, 2, 4])
+@pytest.mark.parametrize("rb", [1, 2])
+def test_a_join_has_workgroups_for_all_columns(waves, rb):
+    for d in range(32, 257, 32):
+        params = dict(H=2, D=d, PAGE=16, G=4, F16=0, RB=rb, WAVES=waves, SHARE=1, QT=8 * d, QH=d, SCALE=0.1, STARTS=1)
+        params.update(KP=32 * d, KT=2 * d, KH=d, VP=32 * d, VT=2 * d, VH=d)
+        info = R.emit_kernel("cache_join", "kernel0", **params)[1]
+        assert info["grid"][1] * info["block"][0] // 64 >= rb * waves * d // 16
