@@ -12,13 +12,15 @@
 // operand of O^T = V^T P^T is read, when the eight keys of that product's lane are taken to be those that the lane has scores of.  V goes
 // through LDS rows that belong to the wavefront alone, from which transposing reads give a lane its eight keys of one column, and is
 // converted to IEEE half, exactly.  The probabilities are
-// rounded to IEEE half (11 bits, they lie in [0, 2^CA_LAZY]), whatever the type of q; for results in IEEE half, which that rounding would
+// rounded to IEEE half (11 bits, they lie in [0, 2^(CA_LAZY + CA_HEAD)]), whatever the type of q; for results in IEEE half, which that rounding would
 // make 1.4 times less exact than their own does, the rest of the rounding goes through a second product (CA_SPLIT) where rows are few
 // and the cache's bytes bound the launch.
 //
 // A page's vscale goes into the exponent: P' = 2^(s - m) vscale = 2^(s + log2 vscale - m'), with m' the running maximum of that
-// sum, so P' keeps its bits whatever the scales are; the sum of the probabilities takes P' / vscale as rounded, in fp32, so that a
-// rounding shifts weight between keys and does not scale the result (and two dot products replace four additions).
+// sum less CA_HEAD: half precision holds all bits of a P' down to 2^-23 of the largest, whatever the scales are.  Keys below add little to the
+// result, but where their page's vscale is the small one they may have most of the weight: the sum of the probabilities takes
+// P' / vscale before P' is rounded, in fp32.  (With the sum taken of the rounded P', pages with 2^-24 of another's scale did not count, and
+// results came out twice what they should be.  The additions in place of two dot products are not seen in the time.)
 //
 // Work: the keys of a tile are cut into units of CA_UK = 32 CA_WAVES, one step of each wavefront of a workgroup.  All units of all tiles of a head
 // stand in one line that is cut evenly between CA_PIECES workgroups (prefix sums of the units of each request, in closed form,
@@ -58,6 +60,7 @@ typedef __bf16 ca_q;
 #define CA_UK (CA_SHARE ? 64 : 32 * CA_WAVES)
 static_assert(0x7fff0000LL + 96 * CA_UK + 32 <= 0x7fffffff, "positions ahead of the last key of the longest request have 32 bits");
 #define CA_LAZY 6.0f
+#define CA_HEAD 9.0f
 #define CA_TINY 1.17549435e-38f               // the least normal number: scales below count as zero
 #define CA_SLOT (CA_ROWS * CA_D + 2 * CA_ROWS)   // floats of a partial result
 
@@ -196,6 +199,10 @@ __device__ __forceinline__ bool ca_locate(int piece, const int* __restrict__ len
   return true;
 }
 
+// The root of the factor that brings sums from one maximum to another: by two products with it, since a sum over pages with small scales is large
+// and may stay where the factor itself is below the least number.
+__device__ __forceinline__ float ca_root(float from, float to) { return __builtin_amdgcn_exp2f((from - to) * 0.5f); }
+
 __device__ __forceinline__ float ca_cross(float v, bool max) {      // over the four lanes that hold a row
   auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
   const unsigned a0 = a[0], a1 = a[1];       // (the bits of an element of a vector have to be copied out of it first)
@@ -247,9 +254,9 @@ void CA_NAME(const float* __restrict__ part, ca_q* __restrict__ out) {
     const float* p = later + ((long long)i * 2 + (i ? 0 : e.slot)) * CA_SLOT;
     const kcg_f32x4 x = *(const kcg_f32x4*)(p + of);
     const float pm = p[at], pl = p[at + 1], to = fmaxf(m, pm), ref = to == -__builtin_inff() ? 0.0f : to;
-    const float fa = __builtin_amdgcn_exp2f(m - ref), fb = __builtin_amdgcn_exp2f(pm - ref);
-    o = o * fa + x * fb;
-    l = l * fa + pl * fb;
+    const float fa = ca_root(m, ref), fb = ca_root(pm, ref);
+    o = o * (fa * fa) + x * (fb * fb);
+    l = l * fa * fa + pl * fb * fb;
     m = to;
   }
   if (CA_JT < 8) {
@@ -268,9 +275,9 @@ void CA_NAME(const float* __restrict__ part, ca_q* __restrict__ out) {
     l = 0.0f;
 #pragma unroll
     for (int w = unit; w < 8; w += CA_JT) {
-      const float f = __builtin_amdgcn_exp2f(ml[w][n][0] - ref);
-      o += red[w][lane] * f;
-      l += ml[w][n][1] * f;
+      const float f = ca_root(ml[w][n][0], ref);
+      o += red[w][lane] * (f * f);
+      l += ml[w][n][1] * f * f;
     }
   }
   ca_store(out, e.first, e.tokens, hv, rb, tt, o, l);
@@ -625,13 +632,13 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
               mx = fmaxf(mx, __builtin_fmaf(fmaxf(fmaxf(sc[rb][h][0], sc[rb][h][1]), fmaxf(sc[rb][h][2], sc[rb][h][3])), by[h], plus[h]));
             mx = ca_cross(mx, true);
             if (__any(mx > m[rb] + CA_LAZY)) {
-              const float to = fmaxf(m[rb], mx), f = to == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m[rb] - to);
+              const float to = fmaxf(m[rb], mx), f = to == -__builtin_inff() ? 1.0f : ca_root(m[rb], to);
               m[rb] = to;
-              l[rb] *= f;
+              l[rb] = l[rb] * f * f;
 #pragma unroll
-              for (int i = 0; i < CA_NT; ++i) acc[rb][i] *= f;
+              for (int i = 0; i < CA_NT; ++i) acc[rb][i] *= f * f;
             }
-            const float ref = m[rb] == -__builtin_inff() ? 0.0f : m[rb];
+            const float ref = m[rb] == -__builtin_inff() ? 0.0f : m[rb] - CA_HEAD;
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
               float p[4];
@@ -639,10 +646,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
               for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][h][r], by[h], plus[h] - ref));
               pf[rb][2 * h] = kcg_pack_f16x2(p[0], p[1]);
               pf[rb][2 * h + 1] = kcg_pack_f16x2(p[2], p[3]);
-              const kcg_f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
-              const float sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(kcg_f16x2, pf[rb][2 * h]), one,
-                                                       __builtin_amdgcn_fdot2(__builtin_bit_cast(kcg_f16x2, pf[rb][2 * h + 1]), one, 0.0f, false), false);
-              l[rb] = __builtin_fmaf(sum, iv[h], l[rb]);
+              l[rb] = __builtin_fmaf((p[0] + p[1]) + (p[2] + p[3]), iv[h], l[rb]);
             }
           }
         }
@@ -969,13 +973,13 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
                          fmaxf(fmaxf(sc[rb][1][0], sc[rb][1][1]), fmaxf(sc[rb][1][2], sc[rb][1][3])));
         mx = ca_cross(mx, true);
         if (__any(mx > m[rb] + CA_LAZY)) {
-          const float to = fmaxf(m[rb], mx), f = to == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m[rb] - to);
+          const float to = fmaxf(m[rb], mx), f = to == -__builtin_inff() ? 1.0f : ca_root(m[rb], to);
           m[rb] = to;
-          l[rb] *= f;
+          l[rb] = l[rb] * f * f;
 #pragma unroll
-          for (int i = 0; i < CA_NT; ++i) acc[rb][i] *= f;
+          for (int i = 0; i < CA_NT; ++i) acc[rb][i] *= f * f;
         }
-        const float ref = m[rb] == -__builtin_inff() ? 0.0f : m[rb];
+        const float ref = m[rb] == -__builtin_inff() ? 0.0f : m[rb] - CA_HEAD;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float p[4];
@@ -989,13 +993,8 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
             const kcg_f16x2 up = __builtin_bit_cast(kcg_f16x2, pf[rb][2 * h + j]);
             pl[rb][2 * h + j] = kcg_pack_f16x2(p[2 * j] - (float)up[0], p[2 * j + 1] - (float)up[1]);
           }
-          const float sum = (p[0] + p[1]) + (p[2] + p[3]);
-#else
-          const kcg_f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
-          const float sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(kcg_f16x2, pf[rb][2 * h]), one,
-                                                   __builtin_amdgcn_fdot2(__builtin_bit_cast(kcg_f16x2, pf[rb][2 * h + 1]), one, 0.0f, false), false);
 #endif
-          l[rb] = __builtin_fmaf(sum, iv[h], l[rb]);
+          l[rb] = __builtin_fmaf((p[0] + p[1]) + (p[2] + p[3]), iv[h], l[rb]);
         }
       }
       auto stage = [&]() __attribute__((always_inline)) {      // (a wavefront's own LDS accesses are carried out in order)
@@ -1133,8 +1132,9 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
       float sum = 0.0f, f[CA_WAVES];
 #pragma unroll
       for (int w = 0; w < CA_WAVES; ++w) {
-        f[w] = __builtin_amdgcn_exp2f(ml[w][at][0] - ref);
-        sum = __builtin_fmaf(ml[w][at][1], f[w], sum);
+        const float root = ca_root(ml[w][at][0], ref);
+        f[w] = root * root;
+        sum = __builtin_fmaf(ml[w][at][1] * root, root, sum);
       }
 #pragma unroll
       for (int j = 0; j < (CA_NT + CA_WAVES - 1) / CA_WAVES; ++j) {

@@ -5,9 +5,17 @@ import pytest
 import torch
 
 from kernelcodegen_amd import ops
-from test_gpu_decode_step import attention_case, close, ints, plain_attention
+from test_gpu_decode_step import DTYPE, HALF_ULP, attention_case, close, ints, laid_out, plain_attention
 
 pytestmark = pytest.mark.gpu
+
+
+def near(got, expected):
+    """As `close`, for values of any size: nothing is added but half the distance of the least numbers of IEEE half, 2^-25."""
+    want, mag = expected
+    tol = want.abs() * HALF_ULP[got.dtype] + mag * 1.25 * HALF_ULP[torch.float16] + (2.0 ** -25 if got.dtype == torch.float16 else 0.0)
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bool(bad.any()), (int(bad.sum()), float(((got.double() - want).abs() / tol).max()))
 
 
 def again(call):
@@ -30,3 +38,48 @@ def test_tiles_of_fewer_wavefronts_are_joined_whole(d, waves, rb):
     want = plain_attention(q, *caches, *scales, table, lengths, starts, d ** -0.5, 0.0, 0, None)
     keys, first = ints(lengths), ints(starts)
     close(again(lambda: ops.cache_attention(q, *caches, *scales, table, keys, first, SHARE=1, WHOLE=0, WAVES=waves, RB=rb, GRID=50)), want)
+
+
+# ---- scales far apart
+
+def far_apart(dtype, many, low, seed=11):
+    """Two requests whose pages have in turn a scale and 2^low of it; all are attended to."""
+    lengths, counts = ([400, 90], [70, 20]) if many else ([400, 90, 33, 3000], None)
+    q, caches, scales, table, starts = attention_case(seed, lengths, counts, 8, 2, 64, 16, "tokens", dtype, spread=0)
+    held = [table[b, :-(-n // 16)].long() for b, n in enumerate(lengths)]
+    return q, caches, scales, table, lengths, starts, held
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("low", [-11, -20, -24, -30, -60])
+@pytest.mark.parametrize("first", [0, 1])
+def test_pages_of_small_values_keep_their_weight(dtype, many, low, first):
+    q, caches, scales, table, lengths, starts, held = far_apart(dtype, many, low)
+    for pages in held:
+        scales[1][pages[first::2]] *= 2.0 ** low
+    got = ops.cache_attention(q, *caches, *scales, table, ints(lengths), None if starts is None else ints(starts))
+    near(got, plain_attention(q, *caches, *scales, table, lengths, starts, 0.125, 0.0, 0, None))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("count", [1, 40])
+@pytest.mark.parametrize("sink", [-11, 0])
+def test_many_keys_of_little_weight_beside_one_of_much(dtype, count, sink):
+    """One key has 2^15 to 2^17 times the weight of each of the others, whose page's scale is 2^-11 of its own or 2^11 times that."""
+    n, d = 40000, 32
+    caches = [laid_out(2500, 16, 1, d, "tokens") for _ in range(2)]
+    k, v = (c.view(torch.uint8) for c in caches)
+    k[0, 0, 0, 0] = 0x52                      # 10
+    g = torch.Generator(device="cuda").manual_seed(3)
+    v.copy_(((torch.rand((2500, 16, 1, d), generator=g, device="cuda") + 0.5) * 128).to(torch.float8_e4m3fn).view(torch.uint8))
+    scales = [torch.ones((2500, 1), device="cuda") for _ in range(2)]
+    scales[1][1:] = 2.0 ** -11
+    if sink:
+        scales[1] = 2.0 ** -11 / scales[1]
+    q = torch.zeros((count, 1, d), device="cuda", dtype=DTYPE[dtype])
+    q[:, 0, 0] = torch.linspace(1.04, 1.18, count, device="cuda") if count > 1 else 1.11
+    table = torch.arange(2500, device="cuda", dtype=torch.int32)[None]
+    starts = None if count == 1 else [0, count]
+    got = ops.cache_attention(q, *caches, *scales, table, ints([n]), None if starts is None else ints(starts), scale=1.0)
+    near(got, plain_attention(q, *caches, *scales, table, [n], starts, 1.0, 0.0, 0, None))
