@@ -62,6 +62,9 @@ static_assert(0x7fff0000LL + 96 * CA_UK + 32 <= 0x7fffffff, "positions ahead of 
 #define CA_LAZY 6.0f
 #define CA_HEAD 9.0f
 #define CA_TINY 1.17549435e-38f               // the least normal number: scales below count as zero
+// What the logarithm of a scale of zero counts as: the keys of its page, which have weight but add nothing, then leave the running maximum, and so
+// the bits of P', to those of pages with scales of 2^-50 and more; and up to 2^31 such keys leave their sum finite.
+#define CA_NOTHING -80.0f
 #define CA_SLOT (CA_ROWS * CA_D + 2 * CA_ROWS)   // floats of a partial result
 
 struct CaRequest { int length, count, first; };       // keys, rows, first row
@@ -527,7 +530,6 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
       int later = pagesOf(key + 16 * CA_UK), step = 0;
       load(key, 0, now);
       ready(now);
-      float lvk = 0.0f;              // logarithm of the last vscale that was not zero
 #pragma unroll 1
       while (true) {
         if (step == 0) {
@@ -543,8 +545,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
           lv[h] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, now.vs), 4 * step + h));
           const bool zero = lv[h] == -__builtin_inff();
           zeros |= zero;
-          if (zero) lv[h] = lvk;
-          lvk = lv[h];
+          if (zero) lv[h] = CA_NOTHING;
           iv[h] = __builtin_amdgcn_exp2f(-lv[h]);
         }
         unsigned char *kb = sh.k[count & 1], *vb = sh.v[count & 1];
@@ -913,7 +914,6 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
     const int key8 = n / 2 < 4 ? g * 4 + n / 2 : 16 + g * 4 + n / 2 - 4;
     const ca_lds vread = (ca_lds)vs + CA_VROW(key8) + (n & 1) * 8;
 
-    float lvk = 0.0f;              // logarithm of the last vscale that was not zero
     kcg_f32x4 sc[CA_RB][2];
     // `behind` is called when the registers of K are free
     auto scores = [&](auto behind) __attribute__((always_inline)) {
@@ -1082,8 +1082,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
           ks[h] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, now.ks), 2 * step + h));
           lv[h] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, now.vs), 2 * step + h));
           zero[h] = lv[h] == -__builtin_inff();
-          if (zero[h]) lv[h] = lvk;
-          lvk = lv[h];
+          if (zero[h]) lv[h] = CA_NOTHING;
           iv[h] = __builtin_amdgcn_exp2f(-lv[h]);
         }
         const bool more = key < last;

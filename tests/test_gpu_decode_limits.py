@@ -83,3 +83,53 @@ def test_many_keys_of_little_weight_beside_one_of_much(dtype, count, sink):
     starts = None if count == 1 else [0, count]
     got = ops.cache_attention(q, *caches, *scales, table, ints([n]), None if starts is None else ints(starts), scale=1.0)
     near(got, plain_attention(q, *caches, *scales, table, [n], starts, 1.0, 0.0, 0, None))
+
+
+# ---- pages of zeros
+
+@pytest.mark.parametrize("dtype,size", [("bf16", 0), ("bf16", -14), ("bf16", -30), ("bf16", -50), ("f16", 0), ("f16", -12)])
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("zeros", [[0], [0, 1, 2, 3], [1, 5], [2, 3, 4, 5, 6, 7, 8]])
+def test_pages_of_zeros_leave_small_values_their_bits(dtype, size, many, zeros):
+    """Pages of zeros stand first, or behind a page of large values that nobody attends to; V is of some size 2^size."""
+    q, caches, scales, table, lengths, starts, held = far_apart(dtype, many, 0, 12)
+    scales[1] *= 2.0 ** size
+    for pages in held:
+        scales[1][pages[[z for z in zeros if z < len(pages)]]] = 0.0
+    if 0 not in zeros:
+        # the request's first page: large values, and keys that the first head's queries point away from
+        for b, pages in enumerate(held):
+            scales[1][pages[0]] *= 2.0 ** 20
+            caches[0].view(torch.uint8)[pages[0]] = 0x78 + 0x80
+            scales[0][pages[0]] = 4.0
+        q.abs_()
+    got = ops.cache_attention(q, *caches, *scales, table, ints(lengths), None if starts is None else ints(starts))
+    near(got, plain_attention(q, *caches, *scales, table, lengths, starts, 0.125, 0.0, 0, None))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("count", [1, 40])
+def test_a_key_of_a_page_of_zeros_may_have_most_of_the_weight(dtype, count):
+    n, d = 40000, 32
+    caches = [laid_out(2500, 16, 1, d, "tokens") for _ in range(2)]
+    k, v = (c.view(torch.uint8) for c in caches)
+    k[0, 0, 0, 0] = 0x54                      # 12: 2^17 times the others' weight
+    g = torch.Generator(device="cuda").manual_seed(4)
+    v.copy_(((torch.rand((2500, 16, 1, d), generator=g, device="cuda") + 0.5) * 128).to(torch.float8_e4m3fn).view(torch.uint8))
+    scales = [torch.ones((2500, 1), device="cuda") for _ in range(2)]
+    scales[1].fill_(2.0 ** -8)
+    scales[1][0] = 0.0
+    q = torch.zeros((count, 1, d), device="cuda", dtype=DTYPE[dtype])
+    q[:, 0, 0] = 1.0
+    table = torch.arange(2500, device="cuda", dtype=torch.int32)[None]
+    starts = None if count == 1 else [0, count]
+    got = ops.cache_attention(q, *caches, *scales, table, ints([n]), None if starts is None else ints(starts), scale=1.0)
+    near(got, plain_attention(q, *caches, *scales, table, [n], starts, 1.0, 0.0, 0, None))
+
+
+@pytest.mark.parametrize("many", [False, True])
+def test_only_pages_of_zeros(many):
+    q, caches, scales, table, lengths, starts, held = far_apart("bf16", many, 0, 13)
+    scales[1].zero_()
+    got = ops.cache_attention(q, *caches, *scales, table, ints(lengths), None if starts is None else ints(starts))
+    assert not bool(got.any())
