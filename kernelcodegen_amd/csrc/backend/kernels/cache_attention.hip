@@ -107,28 +107,33 @@ __device__ __forceinline__ unsigned ca_floor_sum(unsigned n, unsigned a, unsigne
 
 __device__ __forceinline__ int ca_tokens(const CaRequest& r) { return r.count < CA_TOK ? (r.count > 0 ? r.count : 1) : CA_TOK; }
 __device__ __forceinline__ int ca_tiles(const CaRequest& r) { return r.count <= CA_TOK ? (r.count > 0 ? 1 : 0) : (r.count + CA_TOK - 1) / CA_TOK; }
-__device__ __forceinline__ int ca_base(const CaRequest& r) { return r.length > r.count ? r.length - r.count : 0; }
+// The key that a request's first row stands at; negative where it has more rows than keys.
+__device__ __forceinline__ int ca_base(const CaRequest& r) { return r.length - r.count; }
 __device__ __forceinline__ int ca_low(const CaRequest& r, int tile) {     // first unit of a tile
 #if CA_WINDOW
-  const int p = ca_base(r) + tile * ca_tokens(r) - CA_WINDOW + 1;
-  return p > 0 && r.length >= r.count ? p / CA_UK : 0;        // (rows before the first key: from the start)
+  const int p = ca_base(r) + tile * ca_tokens(r);
+  return p >= CA_WINDOW ? (p - CA_WINDOW + 1) / CA_UK : 0;
 #else
   return 0;
 #endif
 }
+// A tile whose rows all stand before the first key counts one unit, in which there is nothing to do.
 __device__ __forceinline__ int ca_units(const CaRequest& r, int tile) {
-  return (ca_base(r) + (tile + 1) * ca_tokens(r) + CA_UK - 1) / CA_UK - ca_low(r, tile);
+  const int whole = ca_base(r) + (tile + 1) * ca_tokens(r), end = whole < r.length ? whole : r.length;
+  return end > 0 ? (end + CA_UK - 1) / CA_UK - ca_low(r, tile) : 1;
 }
-// Units of the tiles before `tile`: every tile ends with its last token's position (the last tile of several counts as if it were whole).
+// Units of the tiles before `tile`: every tile ends with its last token's position, the last one of several with the last key.
 __device__ __forceinline__ int ca_before(const CaRequest& r, int tile) {
   if (tile <= 1) return tile == 0 ? 0 : ca_units(r, 0);
   const int p = ca_base(r), t = ca_tokens(r);
-  unsigned sum = ca_floor_sum(tile, t, p + t + CA_UK - 1, CA_UK);
+  const bool cut = tile == ca_tiles(r);
+  const int n = cut ? tile - 1 : tile, none = p < 0 ? -p / t : 0;       // (tiles before the first key)
+  unsigned sum = cut ? ca_units(r, n) : 0;
+  if (n <= none) return (int)sum + n;
+  sum += none + ca_floor_sum(n - none, t, p + (none + 1) * t + CA_UK - 1, CA_UK);
 #if CA_WINDOW
-  int skip = 0;                            // tiles whose window begins with the first key
-  if (r.length < r.count) skip = tile;
-  else if (p < CA_WINDOW) skip = (CA_WINDOW - 1 - p) / t + 1;
-  if (tile > skip) sum -= ca_floor_sum(tile - skip, t, p + skip * t - CA_WINDOW + 1, CA_UK);
+  const unsigned skip = p < CA_WINDOW ? (CA_WINDOW - 1u - p) / t + 1 : 0;       // tiles whose window begins with the first key
+  if ((unsigned)n > skip) sum -= ca_floor_sum(n - skip, t, p + skip * t - CA_WINDOW + 1, CA_UK);
 #endif
   return (int)sum;
 }

@@ -517,9 +517,6 @@ def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, length
     if slopes is not None and tuple(slopes.shape) != (heads,):
         raise ValueError("slopes is [heads]")
     group = heads // kv_heads
-    # the kernel counts pieces of 32 keys and more of all tiles of 16 rows and more in 32 bits
-    if (tokens * min(group, 64) // 16 + batch + 1) * (width * page // 32 + 2) >= 1 << 31:
-        raise ValueError("too many rows times keys for one launch")
     if not 0.0 <= cap < math.inf or window < 0:
         raise ValueError("cap and window must not be negative")
     params = dict(H=kv_heads, D=d, PAGE=page, G=group, F16=int(q.dtype == torch.float16), STARTS=int(starts is not None), CAP=cap, WINDOW=window,
@@ -530,6 +527,10 @@ def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, length
     params.update(cfg)
     blocks = params["RB"] * (params["WAVES"] if params["SHARE"] else 1)
     tiles = kv_heads * -(-group // (16 * blocks))         # of a token's heads
+    # the kernel counts the units of keys of all tiles in 32 bits
+    of, unit = 16 * blocks // min(group, 16 * blocks), 64 if params["SHARE"] else 32 * params["WAVES"]
+    if not params["WHOLE"] and (tokens // of + batch + 1) * ((width * page + of) // unit + 1) > 0x7FFF0000:
+        raise ValueError("too many rows times keys for one launch")
     kern = R.get_kernel("cache_attention", **params)
     if params["WHOLE"]:
         # with starts, every request's first tile and what the tokens fill behind it, however they are spread (also behind the last request)

@@ -1,8 +1,11 @@
 """What the operators of a decoding step refuse and how they keep to 32 bits, without a GPU."""
+import subprocess
+
 import pytest
 import torch
 
 from kernelcodegen_amd import ops, runtime as R
+from test_decode_step import ROOT
 
 
 class Operand:
@@ -71,3 +74,64 @@ def test_a_join_has_workgroups_for_all_columns(waves, rb):
         params.update(KP=32 * d, KT=2 * d, KH=d, VP=32 * d, VT=2 * d, VH=d)
         info = R.emit_kernel("cache_join", "kernel0", **params)[1]
         assert info["grid"][1] * info["block"][0] // 64 >= rb * waves * d // 16
+
+
+def test_units_of_all_tiles_have_32_bits(monkeypatch):
+    """9 heads to a kv head: a tile of 16 rows has one token, and there are as many tiles as tokens."""
+    forms = dict(heads=9, starts=True, SHARE=0, WHOLE=0, WAVES=1, RB=1)
+    for tokens, keys in ((60000, 1250000), (1, 0x7FFE0000)):
+        units = tokens * (keys // 32 - tokens // 64)              # about: of rows that are the last ones of a request
+        if units > 1 << 31:
+            with pytest.raises(ValueError):
+                attention(monkeypatch, tokens, 1, keys // 16, **forms)
+        else:
+            attention(monkeypatch, tokens, 1, keys // 16, **forms)
+    attention(monkeypatch, 6_200_000, 1, 4, starts=True)
+
+
+PADDED = r"""
+#include <cstdio>
+#define __device__
+#define __forceinline__ inline
+#define __restrict__
+%s
+// units of the tiles of a request, one after the other
+static long long counted(const CaRequest& r, long long& idle) {
+  long long sum = 0;
+  for (int i = 0; i < ca_tiles(r); ++i) {
+    const bool keys = r.length - r.count + (i + 1LL) * ca_tokens(r) > 0;
+    sum += ca_units(r, i);
+    if (!keys && ca_units(r, i) != 1) return -1;
+    idle += !keys;
+  }
+  return sum;
+}
+int main() {
+  // rows behind the last request, and more rows than keys: a tile that sees no key counts one unit, and the closed sums agree
+  const int lengths[] = {0, 1, 63, 64, 500, 6000}, counts[] = {1, 2, 63, 129, 700, 4096, 70000};
+  for (int length : lengths)
+    for (int count : counts) {
+      const CaRequest r = {length, count, 0};
+      long long idle = 0, sum = counted(r, idle);
+      if (sum < 0 || ca_before(r, ca_tiles(r)) != sum) { printf("%%d rows, %%d keys: %%d, counted %%lld\n", count, length, ca_before(r, ca_tiles(r)), sum); return 1; }
+      if (length == 0 && sum != ca_tiles(r)) { puts("rows without keys"); return 1; }
+    }
+  // padding to 2^31 rows stays within 32 bits
+  const CaRequest all = {0, 0x7fff0000, 0};
+  if (ca_before(all, ca_tiles(all)) != ca_tiles(all)) { puts("all"); return 1; }
+  return 0;
+}
+"""
+
+
+@pytest.mark.parametrize("window", [0, 1, 100, 0x7FFFFFFF])
+@pytest.mark.parametrize("rows,keys", [(1, 128), (4, 32), (12, 128), (64, 64), (128, 64)])
+def test_tiles_without_keys_count_one_unit(tmp_path, window, rows, keys):
+    text = open(ROOT + "/kernelcodegen_amd/csrc/backend/kernels/cache_attention.hip").read()
+    part = text[text.index("struct CaRequest"):text.index("// Request b; b == B")] + text[text.index("// sum of the whole parts"):text.index("// Sum over the lanes up to")]
+    source = tmp_path / "units.cc"
+    source.write_text("#define CA_WINDOW %d\n#define CA_TOK %d\n#define CA_UK %d\n" % (window, rows, keys) + PADDED % part)
+    exe = str(tmp_path / "units")
+    subprocess.run(["g++", "-O1", "-fsanitize=signed-integer-overflow", "-fno-sanitize-recover", "-o", exe, str(source)], check=True)
+    done = subprocess.run([exe], capture_output=True, text=True)
+    assert done.returncode == 0, done.stdout + done.stderr

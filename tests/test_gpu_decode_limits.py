@@ -133,3 +133,31 @@ def test_only_pages_of_zeros(many):
     scales[1].zero_()
     got = ops.cache_attention(q, *caches, *scales, table, ints(lengths), None if starts is None else ints(starts))
     assert not bool(got.any())
+
+
+# ---- rows that see no key
+
+def test_rows_behind_the_last_request_may_be_many():
+    """More rows than 32 bits could count the keys of, if these rows had any."""
+    tokens = 6_200_000
+    q = torch.ones((tokens, 1, 32), device="cuda", dtype=torch.bfloat16)
+    caches, scales = [laid_out(4, 16, 1, 32, "tokens") for _ in range(2)], [torch.ones((4, 1), device="cuda") for _ in range(2)]
+    for c in caches:
+        c.view(torch.uint8).fill_(0x38)
+    table, keys, starts = ints([[0, 1, 2, 3]]), ints([64]), ints([0, 3])
+    got = again(lambda: ops.cache_attention(q, *caches, *scales, table, keys, starts))
+    assert bool((got[:3] == 1).all()) and not bool(got[3:].any())
+
+
+@pytest.mark.parametrize("lengths,counts,pad,window", [([100, 40], [30, 1], 3000, 0), ([64], [2], 500, 0), ([10, 700], [900, 40], 20, 0), ([10, 700], [900, 40], 300, 50),
+                                                       ([5, 0, 300], [200, 7, 3], 100, 1000)])
+@pytest.mark.parametrize("kv_heads", [1, 4])
+def test_rows_without_keys_beside_others(lengths, counts, pad, window, kv_heads):
+    q, caches, scales, table, starts = attention_case(15, lengths, counts, 4, kv_heads, 64, 16, "tokens", "bf16")
+    q = torch.cat([q, torch.ones_like(q[:1]).expand(pad, -1, -1)])
+    want = plain_attention(q, *caches, *scales, table, lengths, starts, 0.125, 0.0, window, None)
+    keys, first = ints(lengths), ints(starts)
+    for form in ({}, dict(SHARE=0, WHOLE=0, RB=1, WAVES=4, GRID=7), dict(SHARE=0, WHOLE=1, RB=1, WAVES=2), dict(SHARE=1, WHOLE=0, RB=2, WAVES=4, GRID=64)):
+        got = again(lambda: ops.cache_attention(q, *caches, *scales, table, keys, first, window=window or None, **form))
+        close(got, want)
+        assert not bool(got[starts[-1]:].any())
