@@ -1,7 +1,7 @@
 // ---- new keys and values into a paged cache in 8 bits ----
 //   a = largest finite magnitude among the new rows of a page and head, need = the least power of two with 448 need >= a (0 for a = 0)
 //   scale = need where the page begins with these rows, else max(old scale, need); what the page holds is brought to it
-//   cache = e4m3(x / scale), to the nearest, ties to even; infinities become +-448, a NaN stays one
+//   cache = e4m3(x / scale), to the nearest, ties to even; infinities become +-448, or 0 where the scale is 0; a NaN stays one
 // A scale that is a power of two costs a floating format range but no precision, and a page whose scale has to grow is converted
 // without loss down to the format's least numbers.
 //
@@ -137,6 +137,10 @@ void CW_NAME(const cw_t* __restrict__ k, const cw_t* __restrict__ v, unsigned ch
       if (power) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = (float)raw[i] * inv;
+        if (scale == 0.0f) {         // (nothing finite but zeros)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = raw[i] != raw[i] ? f[i] : 0.0f;
+        }
       } else {
 #pragma unroll 1
         for (int i = 0; i < 8; ++i) f[i] = (float)raw[i] / scale;

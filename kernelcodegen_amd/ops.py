@@ -407,7 +407,7 @@ def cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots):
     k_scale, v_scale: fp32 [pages, heads]; slots: int64 [tokens], page * page_size + place in the page, a token with another slot (-1) is
     left out.  The tokens of a page stand together and in order, as page_slots gives them.  A page's scale is the least power of two by
     which its rows fit the format; where a page has earlier rows, these are converted when the scale has to grow.  A page whose
-    first row is written is taken to be new.  Infinities become the largest numbers that the scale allows."""
+    first row is written is taken to be new.  Infinities become the largest numbers that the scale allows: 0 where all else is 0."""
     key = ("cache_write", R.signature(k, v, k_cache, v_cache, k_scale, v_scale, slots))
     run = _bound.get(key)
     if run is None:

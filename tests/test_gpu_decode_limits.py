@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from kernelcodegen_amd import ops
-from test_gpu_decode_step import DTYPE, HALF_ULP, attention_case, close, ints, laid_out, plain_attention
+from test_gpu_decode_step import DTYPE, HALF_ULP, attention_case, close, ints, laid_out, plain_attention, same, values
 
 pytestmark = pytest.mark.gpu
 
@@ -161,3 +161,23 @@ def test_rows_without_keys_beside_others(lengths, counts, pad, window, kv_heads)
         got = again(lambda: ops.cache_attention(q, *caches, *scales, table, keys, first, window=window or None, **form))
         close(got, want)
         assert not bool(got[starts[-1]:].any())
+
+
+# ---- infinities and NaN among zeros
+
+@pytest.mark.parametrize("dtype", sorted(DTYPE))
+def test_infinities_among_zeros_count_as_zeros(dtype):
+    caches, scales = [laid_out(4, 16, 2, 64, "tokens") for _ in range(2)], [torch.full((4, 2), 7.0, device="cuda") for _ in range(2)]
+    x = torch.zeros((20, 2, 64), device="cuda", dtype=DTYPE[dtype])
+    x[3, 0, 5], x[18, 0, 6], x[4, 1, 7], x[19, 1, 0] = math.inf, -math.inf, math.nan, math.inf
+    at = torch.arange(20, device="cuda") + 16
+    ops.cache_write(x, x, *caches, *scales, at)
+    # all finite magnitudes are zeros, so the scales are; a NaN stays one
+    want = torch.zeros((64, 2, 64), device="cuda", dtype=torch.float64)
+    want[16:36][x.isnan()] = math.nan
+    assert scales[0][:, 0].tolist() == scales[1][:, 1].tolist() == [7, 0, 0, 7] and same(values(caches[0]).view(64, 2, 64), want)
+    back = ops.cache_read(caches[0], scales[0], at, torch.float32)
+    assert int(back.isnan().sum()) == 1 and bool(back[4, 1, 7].isnan()) and not bool(back.nan_to_num().any())
+    q = torch.ones((1, 2, 64), device="cuda", dtype=torch.float16)
+    got = ops.cache_attention(q, *caches, *scales, ints([[1, 2]]), ints([20]))
+    assert not bool(got[0, 0].any()) and bool(got[0, 1].isnan().all())
