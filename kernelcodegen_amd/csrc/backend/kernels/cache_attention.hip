@@ -557,14 +557,19 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
         // not every row of the tile sees every key of the step, or a scale is zero
         bool flagged = false;
         if (key + 64 > first + 1 || (CA_WINDOW && key < first + tokens - CA_WINDOW) || zeros) {
-          // V of keys that no row sees, which may be anything, and of pages whose scale is zero, counts as zero
+          // V of keys that no row sees, which may be anything, counts as zero, and so does that of pages whose scale is zero, but for NaN
           unsigned nan = 0;
 #pragma unroll
           for (int u = 0; u < CA_SL; ++u) {
             const float scale = __shfl(now.vs, step * 4 + of[u] / 16, 64);
-            if (key + of[u] < lo || key + of[u] >= hi || scale == -__builtin_inff()) v[u] = kcg_u32x4{0, 0, 0, 0};
+            const int page = __shfl(now.page, step * 4 + of[u] / 16, 64);
+            if (key + of[u] < lo || key + of[u] >= hi || page < 0) v[u] = kcg_u32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) nan |= ca_nan_bytes(v[u][i]);
+            for (int i = 0; i < 4; ++i) {
+              const unsigned bytes = ca_nan_bytes(v[u][i]);
+              if (scale == -__builtin_inff()) v[u][i] &= bytes * 0xffu;
+              nan |= bytes;
+            }
           }
           if (nan != 0) sh.nan[count & 3] = 1;
           __syncthreads();
@@ -1008,14 +1013,18 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
         __builtin_amdgcn_wave_barrier();
       };
       if (masked) {
-        // V of keys that no row sees, which may be anything, and of pages whose scale is zero, counts as zero
+        // V of keys that no row sees, which may be anything, counts as zero, and so does that of pages whose scale is zero, but for NaN
         unsigned nan = 0;
 #pragma unroll
         for (int u = 0; u < CA_VL; ++u) {
           const int key32 = (u * 64 + lane) / (CA_D / 16);
-          if (at + key32 < lo || at + key32 >= hi || (key32 < 16 ? zero[0] : zero[1])) v[u] = kcg_u32x4{0, 0, 0, 0};
+          if (at + key32 < lo || at + key32 >= hi || !(key32 < 16 ? there[0] : there[1])) v[u] = kcg_u32x4{0, 0, 0, 0};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) nan |= ca_nan_bytes(v[u][i]);
+          for (int i = 0; i < 4; ++i) {
+            const unsigned bytes = ca_nan_bytes(v[u][i]);
+            if (key32 < 16 ? zero[0] : zero[1]) v[u][i] &= bytes * 0xffu;
+            nan |= bytes;
+          }
         }
         if (__any(nan != 0)) {
           // NaN where some rows see the key and some may not: it goes to those that do, by a product of where V is NaN and who sees

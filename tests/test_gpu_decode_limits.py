@@ -181,3 +181,17 @@ def test_infinities_among_zeros_count_as_zeros(dtype):
     q = torch.ones((1, 2, 64), device="cuda", dtype=torch.float16)
     got = ops.cache_attention(q, *caches, *scales, ints([[1, 2]]), ints([20]))
     assert not bool(got[0, 0].any()) and bool(got[0, 1].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("many", [False, True])
+def test_nan_of_a_page_of_zeros_stays(dtype, many):
+    """What such a page holds times its scale is zero, or NaN where that is NaN, of K and of V."""
+    q, caches, scales, table, lengths, starts, held = far_apart(dtype, many, 0, 14)
+    scales[1][held[0][3]] = 0.0
+    v = caches[1].view(torch.uint8)
+    v[held[0][3]] &= 0x3F
+    v[held[0][3], 5, 1, 9] = 0x7F
+    got = ops.cache_attention(q, *caches, *scales, table, ints(lengths), None if starts is None else ints(starts))
+    rows = got[:70] if many else got[:1]
+    assert bool(rows[:, 4:, 9].isnan().all()) and int(got.isnan().sum()) == rows.shape[0] * 4
