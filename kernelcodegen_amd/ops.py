@@ -519,6 +519,8 @@ def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, length
     group = heads // kv_heads
     if not 0.0 <= cap < math.inf or window < 0:
         raise ValueError("cap and window must not be negative")
+    if window >= width * page:          # (none is left out; and a row's position less the window has 32 bits)
+        window = 0
     params = dict(H=kv_heads, D=d, PAGE=page, G=group, F16=int(q.dtype == torch.float16), STARTS=int(starts is not None), CAP=cap, WINDOW=window,
                   SLOPES=int(slopes is not None), SCALE=d ** -0.5 if scale is None else scale, KP=ks[0], KT=ks[1], KH=ks[2], VP=vs[0], VT=vs[1], VH=vs[2],
                   QT=qs[0], QH=qs[1], **_cache_attention_form(batch, tokens, kv_heads, group, d, width * page))
@@ -529,7 +531,7 @@ def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, length
     tiles = kv_heads * -(-group // (16 * blocks))         # of a token's heads
     # the kernel counts the units of keys of all tiles in 32 bits
     of, unit = 16 * blocks // min(group, 16 * blocks), 64 if params["SHARE"] else 32 * params["WAVES"]
-    if not params["WHOLE"] and (tokens // of + batch + 1) * ((width * page + of) // unit + 1) > 0x7FFF0000:
+    if (tokens // of + batch + 1) * ((width * page + of) // unit + 1) > 0x7FFF0000:
         raise ValueError("too many rows times keys for one launch")
     kern = R.get_kernel("cache_attention", **params)
     if params["WHOLE"]:

@@ -39,7 +39,7 @@ class Emitted(Exception):
     """A kernel is asked for: the arguments have passed."""
 
 
-def attention(monkeypatch, tokens, batch, width, page=16, heads=1, kv_heads=1, d=32, starts=False, **cfg):
+def attention(monkeypatch, tokens, batch, width, page=16, heads=1, kv_heads=1, d=32, starts=False, window=0, **cfg):
     """The parameters of the kernel that a call would launch."""
     def get_kernel(family, **params):
         raise Emitted(params)
@@ -49,7 +49,7 @@ def attention(monkeypatch, tokens, batch, width, page=16, heads=1, kv_heads=1, d
     i32 = torch.int32
     with pytest.raises(Emitted) as asked:
         ops._cache_attention_launch(Operand((tokens, heads, d), torch.bfloat16), *caches, *scales, Operand((batch, width), i32), Operand((batch,), i32),
-                                    Operand((batch + 1,), i32) if starts else None, None, 0.0, 0, None, cfg)
+                                    Operand((batch + 1,), i32) if starts else None, None, 0.0, window, None, cfg)
     return asked.value.args[0]
 
 
@@ -135,3 +135,14 @@ def test_tiles_without_keys_count_one_unit(tmp_path, window, rows, keys):
     subprocess.run(["g++", "-O1", "-fsanitize=signed-integer-overflow", "-fno-sanitize-recover", "-o", exe, str(source)], check=True)
     done = subprocess.run([exe], capture_output=True, text=True)
     assert done.returncode == 0, done.stdout + done.stderr
+
+
+def test_a_window_of_all_keys_is_none(monkeypatch):
+    """Positions of rows before the first key are negative: less a window, they have to stay within 32 bits."""
+    for window in (160, 1000, 0x7FFFFFFF, 1 << 40):
+        assert attention(monkeypatch, 30, 1, 10, starts=True, window=window)["WINDOW"] == 0
+    assert attention(monkeypatch, 30, 1, 10, starts=True, window=159)["WINDOW"] == 159
+    for tokens, keys in ((1 << 30, 1 << 30), (1 << 26, 1 << 20)):
+        for form in ({}, dict(WHOLE=1, SHARE=0, RB=1, WAVES=1)):
+            with pytest.raises(ValueError):
+                attention(monkeypatch, tokens, 1, keys // 16, starts=True, window=keys - 1, **form)

@@ -195,3 +195,12 @@ def test_nan_of_a_page_of_zeros_stays(dtype, many):
     got = ops.cache_attention(q, *caches, *scales, table, ints(lengths), None if starts is None else ints(starts))
     rows = got[:70] if many else got[:1]
     assert bool(rows[:, 4:, 9].isnan().all()) and int(got.isnan().sum()) == rows.shape[0] * 4
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 40])
+@pytest.mark.parametrize("lengths,counts", [([10], [30]), ([100, 7], [3, 90]), ([300, 64], [400, 70])])
+def test_a_window_of_all_keys_before_rows_without_keys(window, lengths, counts):
+    q, caches, scales, table, starts = attention_case(18, lengths, counts, 4, 2, 64, 16, "tokens", "bf16")
+    want = plain_attention(q, *caches, *scales, table, lengths, starts, 0.125, 0.0, 0, None)
+    for form in ({}, dict(SHARE=1, WHOLE=0, RB=1, WAVES=4), dict(SHARE=0, WHOLE=0, RB=1, WAVES=4), dict(SHARE=0, WHOLE=1, RB=1, WAVES=2)):
+        close(ops.cache_attention(q, *caches, *scales, table, ints(lengths), ints(starts), window=window, **form), want)
