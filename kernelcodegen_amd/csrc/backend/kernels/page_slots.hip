@@ -56,7 +56,6 @@ void PS_NAME(const int* __restrict__ lengths, const int* __restrict__ added, int
     if (blockIdx.x == 0 && b < B) {
       starts[b + 1] = tokens0 + s.tokens[threadIdx.x + 1];
       lengths_out[b] = len + add;
-      if (b == 0) starts[0] = 0;
     }
     // Which request of this round: the last whose sum before it is not over `i`.  Of eight parts at a time, since the reads of one step are
     // under way together: a round of 256 takes three.
@@ -97,5 +96,8 @@ void PS_NAME(const int* __restrict__ lengths, const int* __restrict__ added, int
     slots[i] = -1;
     positions[i] = -1;
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) used[0] = pages0 < F ? pages0 : F;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    starts[0] = 0;
+    used[0] = pages0 < F ? pages0 : F;
+  }
 }

@@ -204,3 +204,14 @@ def test_a_window_of_all_keys_before_rows_without_keys(window, lengths, counts):
     want = plain_attention(q, *caches, *scales, table, lengths, starts, 0.125, 0.0, 0, None)
     for form in ({}, dict(SHARE=1, WHOLE=0, RB=1, WAVES=4), dict(SHARE=0, WHOLE=0, RB=1, WAVES=4), dict(SHARE=0, WHOLE=1, RB=1, WAVES=2)):
         close(ops.cache_attention(q, *caches, *scales, table, ints(lengths), ints(starts), window=window, **form), want)
+
+
+# ---- page_slots
+
+def test_page_slots_of_no_requests():
+    none, table, free = ints([]), torch.zeros((0, 3), device="cuda", dtype=torch.int32), ints([7, 8])
+    for tokens in (0, 5, 3000):
+        for r in ops.page_slots(none, none, table, free, 16, tokens):
+            r.fill_(-9)
+        slots, positions, starts, lengths, used = ops.page_slots(none, none, table, free, 16, tokens)
+        assert starts.tolist() == [0] and used.tolist() == [0] and lengths.tolist() == [] and slots.tolist() == positions.tolist() == [-1] * tokens
