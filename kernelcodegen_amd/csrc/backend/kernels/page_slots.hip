@@ -7,7 +7,11 @@
 // list, the stores.
 // Measured: 64 requests of one token each 2.8 us (an empty launch 1.7), 200 of up to 700 7.
 // Parameters: PS_NAME, PS_BLOCK, PS_PAGE.
-struct PsSums { int pages[PS_BLOCK + 1], tokens[PS_BLOCK + 1], lengths[PS_BLOCK], waves[2][PS_BLOCK / 64]; };
+// Lengths, places and sums are counted without a sign, so that length + added may use all bits of a positive number, and a place is compared
+// with its table without one: sums that pass 32 bits give wrong slots, but no access out of range.
+struct PsSums { unsigned pages[PS_BLOCK + 1], tokens[PS_BLOCK + 1], lengths[PS_BLOCK], waves[2][PS_BLOCK / 64]; };
+
+__device__ __forceinline__ unsigned ps_pages(unsigned tokens) { return tokens / PS_PAGE + (tokens % PS_PAGE ? 1 : 0); }
 
 // Sum over the lanes up to and including this one.
 __device__ __forceinline__ int ps_scan(int v) {
@@ -27,24 +31,26 @@ void PS_NAME(const int* __restrict__ lengths, const int* __restrict__ added, int
              long long B_, long long T_, long long W_, long long table_row, long long F_, long long* __restrict__ slots,
              int* __restrict__ positions, int* __restrict__ starts, int* __restrict__ lengths_out, int* __restrict__ used) {
   __shared__ PsSums s;
-  const int B = (int)B_, T = (int)T_, W = (int)W_, F = (int)F_;
-  constexpr int page = PS_PAGE;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = blockIdx.x * PS_BLOCK + threadIdx.x, step = gridDim.x * PS_BLOCK;
-  int pages0 = 0, tokens0 = 0;                 // of the requests before this round's
+  const int B = (int)B_;
+  const unsigned T = (unsigned)T_, W = (unsigned)W_, F = F_ < 0x7fffffff ? (unsigned)F_ : 0x7fffffffu;
+  constexpr unsigned page = PS_PAGE;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const unsigned first = blockIdx.x * PS_BLOCK + threadIdx.x, step = gridDim.x * PS_BLOCK;
+  unsigned pages0 = 0, tokens0 = 0;            // of the requests before this round's
   for (int b0 = 0; b0 < B; b0 += PS_BLOCK) {
     const int b = b0 + threadIdx.x, n = B - b0 < PS_BLOCK ? B - b0 : PS_BLOCK;
-    int len = 0, add = 0;
+    unsigned len = 0, add = 0;
     if (b < B) {
       len = lengths[b] > 0 ? lengths[b] : 0;
       add = added[b] > 0 ? added[b] : 0;
     }
-    const int p = ps_scan((len + add + page - 1) / page - (len + page - 1) / page), t = ps_scan(add);
+    const unsigned p = ps_scan(ps_pages(len + add) - ps_pages(len)), t = ps_scan(add);
     if (lane == 63) { s.waves[0][wave] = p; s.waves[1][wave] = t; }
     __syncthreads();
-    int pb = 0, tb = 0;
+    unsigned pb = 0, tb = 0;
 #pragma unroll
     for (int w = 0; w < PS_BLOCK / 64 - 1; ++w) {
-      const int pw = s.waves[0][w], tw = s.waves[1][w];
+      const unsigned pw = s.waves[0][w], tw = s.waves[1][w];
       pb += w < wave ? pw : 0;
       tb += w < wave ? tw : 0;
     }
@@ -59,7 +65,7 @@ void PS_NAME(const int* __restrict__ lengths, const int* __restrict__ added, int
     }
     // Which request of this round: the last whose sum before it is not over `i`.  Of eight parts at a time, since the reads of one step are
     // under way together: a round of 256 takes three.
-    auto find = [&](const int* sums, int i) {
+    auto find = [&](const unsigned* sums, unsigned i) {
       int lo = 0;
 #pragma unroll
       for (int part = PS_BLOCK > 512 ? 512 : 64; part > 0; part /= 8) {
@@ -73,14 +79,18 @@ void PS_NAME(const int* __restrict__ lengths, const int* __restrict__ added, int
       return lo;
     };
     // page i off the list and token i: both numbers' loads, from some length where there is none, then the stores
-    const int pages = s.pages[n], tokens = s.tokens[n], most = pages > tokens ? pages : tokens;
-    for (int i = first; i < most; i += step) {
-      const int rp = find(s.pages, i), place = (s.lengths[rp] + page - 1) / page + i - s.pages[rp];
-      const bool put = i < pages && place < W && pages0 + i < F;
+    const unsigned pages = s.pages[n], tokens = s.tokens[n];
+    const unsigned freed = pages0 < F ? F - pages0 : 0, rows = tokens0 < T ? T - tokens0 : 0;        // what there is room for (below 2^31)
+    const unsigned some = pages < freed ? pages : freed, rest = tokens < rows ? tokens : rows, most = some > rest ? some : rest;
+    for (unsigned i = first; i < most; i += step) {
+      const int rp = find(s.pages, i);
+      const unsigned place = ps_pages(s.lengths[rp]) + i - s.pages[rp];
+      const bool put = i < some && place < W;
       const int fresh = *(put ? free_pages + pages0 + i : lengths);
-      const int r = find(s.tokens, i), have = s.lengths[r], at = have + i - s.tokens[r], before = (have + page - 1) / page, column = at / page;
-      const int k = pages0 + s.pages[r] + column - before;
-      const bool token = i < tokens && tokens0 + i < T, old = column < before, page_there = token && column < W && (old || k < F);
+      const int r = find(s.tokens, i);
+      const unsigned have = s.lengths[r], at = have + i - s.tokens[r], before = ps_pages(have), column = at / page;
+      const unsigned k = pages0 + s.pages[r] + column - before;
+      const bool token = i < rest, old = column < before, page_there = token && column < W && (old || k < F);
       const int id = *(!page_there ? lengths : old ? table + (long long)(b0 + r) * table_row + column : free_pages + k);
       if (put) table[(long long)(b0 + rp) * table_row + place] = fresh;
       if (token) {
@@ -88,11 +98,11 @@ void PS_NAME(const int* __restrict__ lengths, const int* __restrict__ added, int
         positions[tokens0 + i] = at;
       }
     }
-    pages0 += s.pages[n];
-    tokens0 += s.tokens[n];
+    pages0 += pages;
+    tokens0 += tokens;
     __syncthreads();
   }
-  for (int i = tokens0 + first; i < T; i += step) {
+  for (long long i = (long long)tokens0 + first; i < T; i += step) {
     slots[i] = -1;
     positions[i] = -1;
   }

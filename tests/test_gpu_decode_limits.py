@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from kernelcodegen_amd import ops
-from test_gpu_decode_step import DTYPE, HALF_ULP, attention_case, close, ints, laid_out, plain_attention, same, values
+from test_gpu_decode_step import DTYPE, HALF_ULP, attention_case, close, ints, laid_out, plain_attention, plain_pages, same, values
 
 pytestmark = pytest.mark.gpu
 
@@ -215,3 +215,24 @@ def test_page_slots_of_no_requests():
             r.fill_(-9)
         slots, positions, starts, lengths, used = ops.page_slots(none, none, table, free, 16, tokens)
         assert starts.tolist() == [0] and used.tolist() == [0] and lengths.tolist() == [] and slots.tolist() == positions.tolist() == [-1] * tokens
+
+
+@pytest.mark.parametrize("page", [2 ** 30, 2 ** 30 + 5, 2 ** 31 - 1])
+def test_page_slots_of_very_large_pages(page):
+    lengths, added, free = [0, 3, 2 ** 30, 2 ** 30 + 4], [2, 1, 3, 2], [9, 4, 5, 8]
+    table = [[-5, -5, -5], [6, -5, -5], [2, -5, -5], [3, 1, -5]]
+    want = plain_pages(lengths, added, table, free, page, 9)
+    at = ints(table)
+    got = ops.page_slots(ints(lengths), ints(added), at, ints(free), page, 9)
+    for g, w in zip(got, want):
+        assert g.tolist() == w
+    assert at.tolist() == want[5]
+
+
+def test_page_slots_of_the_largest_lengths():
+    lengths, added, page = [2 ** 31 - 9, 5], [8, 2], 2 ** 26
+    table = [list(range(32)), [40] + [-1] * 31]
+    want = plain_pages(lengths, added, table, [50], page, 12)
+    got = ops.page_slots(ints(lengths), ints(added), ints(table), ints([50]), page, 12)
+    for g, w in zip(got, want):
+        assert g.tolist() == w
