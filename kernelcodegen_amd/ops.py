@@ -608,6 +608,8 @@ def _matmul_q4_launch(x, w, scale, zero, out_dtype, cfg):
     if (x.data_ptr() | w.data_ptr()) % 16:
         raise ValueError("x and w must start on multiples of 16 bytes")
     rows = math.prod(x.shape[:-1])
+    if rows > 0x7FFFFF00:
+        raise ValueError("too many rows for one launch")
     if rows == 0:
         return None, None, 0
     if not cfg.keys() <= {"MB", "MR", "NT", "WN", "WK", "SPLIT"}:

@@ -146,3 +146,13 @@ def test_a_window_of_all_keys_is_none(monkeypatch):
         for form in ({}, dict(WHOLE=1, SHARE=0, RB=1, WAVES=1)):
             with pytest.raises(ValueError):
                 attention(monkeypatch, tokens, 1, keys // 16, starts=True, window=keys - 1, **form)
+
+
+def test_rows_of_a_4_bit_product_have_32_bits(monkeypatch):
+    def get_kernel(family, **params):
+        raise Emitted(params)
+    monkeypatch.setattr(R, "get_kernel", get_kernel)
+    w, scale = Operand((8, 16), torch.uint8), Operand((8, 1), torch.bfloat16)
+    for shape, refused in (((1 << 31, 32), True), ((1 << 16, 1 << 15, 32), True), ((0x7FFFFF01, 32), True), ((0x7FFFFF00, 32), False)):
+        with pytest.raises(ValueError if refused else Emitted):
+            ops._matmul_q4_launch(Operand(shape, torch.bfloat16), w, scale, None, None, {})
