@@ -519,6 +519,8 @@ def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, length
     group = heads // kv_heads
     if not 0.0 <= cap < math.inf or window < 0:
         raise ValueError("cap and window must not be negative")
+    if cap > 2.0 ** 40:                 # (scores up to 2^27 are what they are to fp32)
+        cap = 0.0
     if window >= width * page:          # (none is left out; and a row's position less the window has 32 bits)
         window = 0
     params = dict(H=kv_heads, D=d, PAGE=page, G=group, F16=int(q.dtype == torch.float16), STARTS=int(starts is not None), CAP=cap, WINDOW=window,

@@ -236,3 +236,15 @@ def test_page_slots_of_the_largest_lengths():
     got = ops.page_slots(ints(lengths), ints(added), ints(table), ints([50]), page, 12)
     for g, w in zip(got, want):
         assert g.tolist() == w
+
+
+# ---- scores
+
+@pytest.mark.parametrize("cap", [1e3, 1e5, 1e9, 1e38, 1e300])
+@pytest.mark.parametrize("count", [1, 40])
+def test_a_large_cap_leaves_scores_as_they_are(cap, count):
+    """A score's error: e4m3 sums and fp32 products 2^-17 of the largest sum |q k|, tanh 2^-22 of the score."""
+    lengths = [300]
+    q, caches, scales, table, starts = attention_case(16, lengths, None if count == 1 else [count], 4, 2, 64, 16, "tokens", "f16")
+    got = ops.cache_attention(q, *caches, *scales, table, ints(lengths), None if starts is None else ints(starts), cap=cap)
+    near(got, plain_attention(q, *caches, *scales, table, lengths, starts, 0.125, cap, 0, None))
