@@ -1728,7 +1728,7 @@ bool emitCacheAttention(KernelSpec& s, std::string& src, KernelLaunchInfo& info,
   d.add("CA_JOIN", join ? 1 : 0);
   d.add("CA_D", dh); d.add("CA_HKV", s.p["H"]); d.add("CA_G", g); d.add("CA_GS", gs); d.add("CA_PAGE", s.p["PAGE"]);
   d.add("CA_F16", s.p["F16"]); d.add("CA_RB", rb); d.add("CA_WAVES", waves); d.add("CA_SHARE", share ? 1 : 0); d.add("CA_PIECES", pieces); d.add("CA_WHOLE", wholeTiles ? 1 : 0); d.add("CA_MIN", least);
-  d.add("CA_OCC", occ); d.add("CA_SPLIT", s.p["F16"] && !share ? 1 : 0);
+  d.add("CA_OCC", occ); d.add("CA_SPLIT", s.get("SPLIT", s.p["F16"]) ? 1 : 0);
   d.add("CA_SCALE", floatLiteral(scale)); d.add("CA_CAP", floatLiteral(cap)); d.add("CA_HAS_CAP", cap > 0.0 ? 1 : 0);
   d.add("CA_WINDOW", window); d.add("CA_SLOPES", slopes ? 1 : 0); d.add("CA_STARTS", starts ? 1 : 0);
   for (auto key : {"KP", "KT", "KH", "VP", "VT", "VH", "QT", "QH"}) d.add(std::string("CA_") + key, std::to_string(s.p[key]) + "LL");

@@ -12,9 +12,10 @@
 // operand of O^T = V^T P^T is read, when the eight keys of that product's lane are taken to be those that the lane has scores of.  V goes
 // through LDS rows that belong to the wavefront alone, from which transposing reads give a lane its eight keys of one column, and is
 // converted to IEEE half, exactly.  The probabilities are
-// rounded to IEEE half (11 bits, they lie in [0, 2^(CA_LAZY + CA_HEAD)]), whatever the type of q; for results in IEEE half, which that rounding would
-// make 1.4 times less exact than their own does, the rest of the rounding goes through a second product (CA_SPLIT) where rows are few
-// and the cache's bytes bound the launch.
+// rounded to IEEE half (11 bits, they lie in [0, 2^(CA_LAZY + CA_HEAD)]), which leaves results in bfloat16, of 8 bits, about as exact as their own
+// rounding does.  Results in half precision it would make 1.4 times less exact: there the rest of the rounding goes through a second product
+// (CA_SPLIT), in every form, so that a row's bits do not go by the rows beside it.  Where the cache's bytes bound the launch that costs
+// nothing, where rows share keys a fifth (1500 rows of 32 heads behind 6000 keys: 251 us, 209 without).
 //
 // A page's vscale goes into the exponent: P' = 2^(s - m) vscale = 2^(s + log2 vscale - m'), with m' the running maximum of that
 // sum less CA_HEAD: half precision holds all bits of a P' down to 2^-23 of the largest, whatever the scales are.  Keys below add little to the
@@ -607,6 +608,9 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
 
         const bool work = mine && key <= pos1 && (!CA_WINDOW || key + 63 > pos0 - CA_WINDOW);
         unsigned pf[CA_RB][8];
+#if CA_SPLIT
+        unsigned pl[CA_RB][8];           // what the rounding of pf leaves
+#endif
         kcg_f32x4 sc[CA_RB][4];
         if (work) {
 #pragma unroll
@@ -668,6 +672,13 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
               for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][h][r], by[h], plus[h] - ref));
               pf[rb][2 * h] = kcg_pack_f16x2(p[0], p[1]);
               pf[rb][2 * h + 1] = kcg_pack_f16x2(p[2], p[3]);
+#if CA_SPLIT
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const kcg_f16x2 up = __builtin_bit_cast(kcg_f16x2, pf[rb][2 * h + j]);
+                pl[rb][2 * h + j] = kcg_pack_f16x2(__builtin_fmaf((float)up[0], -1.0f, p[2 * j]), __builtin_fmaf((float)up[1], -1.0f, p[2 * j + 1]));
+              }
+#endif
               l[rb] = __builtin_fmaf((p[0] + p[1]) + (p[2] + p[3]), iv[h], l[rb]);
             }
           }
@@ -708,6 +719,10 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
               for (int rb = 0; rb < CA_RB; ++rb) {
                 const kcg_u32x4 p = {pf[rb][4 * h], pf[rb][4 * h + 1], pf[rb][4 * h + 2], pf[rb][4 * h + 3]};
                 acc[rb][tt] = CA_MFMA16(vf, p, acc[rb][tt]);
+#if CA_SPLIT
+                const kcg_u32x4 q = {pl[rb][4 * h], pl[rb][4 * h + 1], pl[rb][4 * h + 2], pl[rb][4 * h + 3]};
+                acc[rb][tt] = CA_MFMA16(vf, q, acc[rb][tt]);
+#endif
               }
             }
         }
@@ -1012,7 +1027,7 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const kcg_f16x2 up = __builtin_bit_cast(kcg_f16x2, pf[rb][2 * h + j]);
-            pl[rb][2 * h + j] = kcg_pack_f16x2(p[2 * j] - (float)up[0], p[2 * j + 1] - (float)up[1]);
+            pl[rb][2 * h + j] = kcg_pack_f16x2(__builtin_fmaf((float)up[0], -1.0f, p[2 * j]), __builtin_fmaf((float)up[1], -1.0f, p[2 * j + 1]));
           }
 #endif
           l[rb] = __builtin_fmaf((p[0] + p[1]) + (p[2] + p[3]), iv[h], l[rb]);

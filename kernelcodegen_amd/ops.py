@@ -470,7 +470,8 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, table, lengths, start
       score = scale * q.k (scale: d^-0.5), then cap * tanh(score / cap), then + slopes[head] * (key's position - row's), slopes fp32
       [heads]; a row sees the keys up to its own position, of these the last `window`.
     Entries of the table behind a request's length have no effect; keys on pages that are not the cache's count as not there.  `cfg`
-    overrides kernel parameters (RB, SHARE, WAVES, WHOLE, GRID, LEAST, OCC)."""
+    overrides kernel parameters (RB, SHARE, WAVES, WHOLE, GRID, LEAST, OCC; SPLIT: whether probabilities keep what their
+    rounding to 11 bits leaves, by default for half precision)."""
     scale, cap, window = None if scale is None else float(scale), float(cap or 0.0), operator.index(window or 0)
     key = ("cache_attention", R.signature(q, k_cache, v_cache, k_scale, v_scale, table, lengths, starts, slopes), scale, cap, window)
     hit = None if cfg else _bound.get(key)
@@ -525,8 +526,8 @@ def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, length
         window = 0
     params = dict(H=kv_heads, D=d, PAGE=page, G=group, F16=int(q.dtype == torch.float16), STARTS=int(starts is not None), CAP=cap, WINDOW=window,
                   SLOPES=int(slopes is not None), SCALE=d ** -0.5 if scale is None else scale, KP=ks[0], KT=ks[1], KH=ks[2], VP=vs[0], VT=vs[1], VH=vs[2],
-                  QT=qs[0], QH=qs[1], **_cache_attention_form(batch, tokens, kv_heads, group, d, width * page))
-    if not cfg.keys() <= {"RB", "WAVES", "SHARE", "GRID", "LEAST", "OCC", "WHOLE"}:
+                  QT=qs[0], QH=qs[1], **_cache_attention_form(batch, tokens, kv_heads, group, d, width * page, q.dtype == torch.float16))
+    if not cfg.keys() <= {"RB", "WAVES", "SHARE", "GRID", "LEAST", "OCC", "WHOLE", "SPLIT"}:
         raise ValueError("unknown kernel parameters")
     params.update(cfg)
     blocks = params["RB"] * (params["WAVES"] if params["SHARE"] else 1)
@@ -547,7 +548,7 @@ def _cache_attention_launch(q, k_cache, v_cache, k_scale, v_scale, table, length
     return _into_last(kern.bind(), (tuple(q.shape), q.dtype)), join, floats
 
 
-def _cache_attention_form(batch, tokens, kv_heads, group, d, keys):
+def _cache_attention_form(batch, tokens, kv_heads, group, d, keys, half):
     """The tiles and who takes what of them; `keys`: what a request's row of the table has room for.
 
     A tile has 16 rows of a kv head, whose keys are split between the wavefronts of a workgroup.  Where the average request has more than 32
@@ -561,10 +562,11 @@ def _cache_attention_form(batch, tokens, kv_heads, group, d, keys):
       a tile each, 4096 tiles, of 16 keys: one wavefront 11.5, two 16.1, four 25.1;  512 keys: 55, 52, 56;  64 tiles, 512 keys: 14.7, 9.1, 6.8
       8 prompts of up to 300 behind up to 600 keys: shared keys with 16 rows a wavefront 41, 32 rows 49, keys split 58;  2 of 1000 behind 6000:
       202, 167, 195;  64 of up to 16 tokens behind 1000: 35, 54, 44
-      32 heads to one kv head: 8 of up to 32000 keys: keys split, 16 rows a tile 21.6, 32 rows 26.9, shared 26.2;  16 of 16000 of 256: 38, 61, 32"""
+      32 heads to one kv head: 8 of up to 32000 keys: keys split, 16 rows a tile 21.6, 32 rows 26.9, shared 26.2;  16 of 16000 of 256: 38, 61, 32
+      2 of 500 behind 4000, 8 heads of 256 to a kv head: half precision 16 rows a wavefront 172, 32 rows 212;  bfloat16, 32 rows: 138"""
     rows = group * max(1, -(-tokens // batch))
     share = int(rows > (32 if d <= 128 else 16))
-    blocks = 2 if share and rows * keys >= 1 << 21 else 1
+    blocks = 2 if share and rows * keys >= 1 << 21 and not (half and d > 128) else 1
     tiles = batch * kv_heads * -(-group // 16)
     whole = int(not share and (keys <= 512 or (keys <= 1024 and tiles >= 512)))
     waves = 4

@@ -248,3 +248,17 @@ def test_a_large_cap_leaves_scores_as_they_are(cap, count):
     q, caches, scales, table, starts = attention_case(16, lengths, None if count == 1 else [count], 4, 2, 64, 16, "tokens", "f16")
     got = ops.cache_attention(q, *caches, *scales, table, ints(lengths), None if starts is None else ints(starts), cap=cap)
     near(got, plain_attention(q, *caches, *scales, table, lengths, starts, 0.125, cap, 0, None))
+
+
+# ---- bits of the probabilities
+
+def test_rows_of_half_precision_have_the_same_bits_in_every_form():
+    """The probabilities' error is that of their sum's and scores' fp32 arithmetic, not 2^-11: by the root of the mean square over all results, half an ulp
+    of the results (2^-12 at most, 0.58 of it on average) and no more than a tenth beside it."""
+    lengths, counts = [2000], [200]
+    q, caches, scales, table, starts = attention_case(17, lengths, counts, 4, 1, 128, 16, "tokens", "f16", spread=0)
+    want, _ = plain_attention(q, *caches, *scales, table, lengths, starts, 128 ** -0.5, 0.0, 0, None)
+    rounded = (want.half().double() - want).norm()
+    for form in ({}, dict(SHARE=0, WHOLE=0, RB=1, WAVES=4), dict(SHARE=1, WHOLE=0, RB=1, WAVES=4), dict(SHARE=1, WHOLE=0, RB=2, WAVES=4)):
+        got = ops.cache_attention(q, *caches, *scales, table, ints(lengths), ints(starts), **form)
+        assert float((got.double() - want).norm() / rounded) < 1.1, form
