@@ -25,6 +25,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -57,9 +58,10 @@ int launch(const Launch* self, const uint64_t* slots) {
   return self->entry(self->handle, self->dims, stream, slots, self->pointers + self->scalars);
 }
 
-// A new tensor on `like`'s device: on the part without the dispatcher, which takes as long as the allocation itself.
+// A new tensor on `like`'s device: on the part without the dispatcher, which takes as long as the allocation itself, unless a mode
+// (torch.utils._python_dispatch) looks at what is called.
 at::Tensor fresh(const at::Tensor& like, at::IntArrayRef shape, at::ScalarType dtype) {
-  if (like.is_cuda()) return at::Tensor(at::detail::empty_cuda(shape, dtype, like.device(), std::nullopt));
+  if (like.is_cuda() && !c10::impl::dispatch_mode_enabled()) return at::Tensor(at::detail::empty_cuda(shape, dtype, like.device(), std::nullopt));
   return at::empty(shape, like.options().dtype(dtype).requires_grad(false));
 }
 

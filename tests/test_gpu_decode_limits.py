@@ -262,3 +262,26 @@ def test_rows_of_half_precision_have_the_same_bits_in_every_form():
     for form in ({}, dict(SHARE=0, WHOLE=0, RB=1, WAVES=4), dict(SHARE=1, WHOLE=0, RB=1, WAVES=4), dict(SHARE=1, WHOLE=0, RB=2, WAVES=4)):
         got = ops.cache_attention(q, *caches, *scales, table, ints(lengths), ints(starts), **form)
         assert float((got.double() - want).norm() / rounded) < 1.1, form
+
+
+# ---- dispatch modes
+
+def test_modes_that_look_at_allocations_see_the_results():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.names = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    a = torch.ones((64, 64), device="cuda", dtype=torch.bfloat16)
+    args = (ints([5]), ints([1]), ints([[3, 4]]), ints([9]))
+    for call in (lambda: ops.matmul(a, a), lambda: ops.page_slots(*args, 16, 1)):
+        call()
+        with Seen() as seen:
+            call()
+        assert any("empty" in name for name in seen.names)
