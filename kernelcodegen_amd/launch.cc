@@ -19,6 +19,7 @@
 //                                          parts of one allocation
 //   signature(tensor or None, ...)         what a kernel can depend on of its operands, as bytes: device, type, sizes, strides and how
 //                                          far each address is from a multiple of 16
+//   row_signature(tensor or None, ...)     the same without the last size and the strides before the last
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -289,8 +290,10 @@ PyObject* withResults(PyObject* me, PyObject* args) {
   END_HANDLE_TH_ERRORS
 }
 
-PyObject* signature(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
+// `rows`: without what a kernel takes as arguments of tensors whose rows it walks over, the length of a row and how far rows are apart.
+// Rows of one element or none are rows of neighbouring elements.
+template <bool rows>
+PyObject* signatureOf(PyObject* const* args, Py_ssize_t n) {
   // (a tensor of d dimensions takes 2 d + 2 numbers of 8 bytes)
   int64_t out[256];
   size_t at = 0;
@@ -313,11 +316,27 @@ PyObject* signature(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const auto device = t.device();
     out[at++] = d | (int64_t)t.scalar_type() << 8 | (int64_t)device.type() << 16 | (int64_t)(uint8_t)device.index() << 24 |
                 (int64_t)t.layout() << 32;
-    for (int64_t j = 0; j < d; ++j) out[at++] = t.size(j);
-    for (int64_t j = 0; j < d; ++j) out[at++] = t.stride(j);
+    if (rows) {
+      for (int64_t j = 0; j + 1 < d; ++j) out[at++] = t.size(j);
+      if (d) out[at++] = t.size(d - 1) > 1 ? t.stride(d - 1) : 1;
+    } else {
+      for (int64_t j = 0; j < d; ++j) out[at++] = t.size(j);
+      for (int64_t j = 0; j < d; ++j) out[at++] = t.stride(j);
+    }
     out[at++] = (int64_t)((uintptr_t)t.data_ptr() & 15);
   }
   return PyBytes_FromStringAndSize((const char*)out, (Py_ssize_t)(at * sizeof out[0]));
+}
+
+PyObject* signature(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  return signatureOf<false>(args, n);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* rowSignature(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  return signatureOf<true>(args, n);
   END_HANDLE_TH_ERRORS
 }
 
@@ -334,6 +353,7 @@ PyMethodDef methods[] = {{"result", withResult, METH_VARARGS, "result(shape, dty
                          {"results", withResults, METH_VARARGS, "results((shape, dtype), ...): a Launch that allocates and returns its last pointers' tensors"},
                          {nullptr, nullptr, 0, nullptr}};
 PyMethodDef functions[] = {{"signature", (PyCFunction)(void (*)(void))signature, METH_FASTCALL, "what a kernel can depend on of its operands"},
+                           {"row_signature", (PyCFunction)(void (*)(void))rowSignature, METH_FASTCALL, "the same without the rows' length and distance"},
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", "bound kernel launches on torch tensors", -1, functions};
 

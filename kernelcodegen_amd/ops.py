@@ -4,6 +4,7 @@ Shapes are static (baked into the kernel), like every kernel the generator
 emits."""
 import math
 import operator
+import threading
 
 import torch
 
@@ -18,8 +19,20 @@ def _need_cuda(*ts):
 
 # (operator, every property of the operands that the kernel depends on) -> the bound launch of that kernel.  Nothing in a
 # key or a value belongs to one tensor: shapes, types, options and whether the operands are aligned.  A call with kernel
-# parameters of its own (cfg) goes through get_kernel each time.
-_bound = {}
+# parameters of its own (cfg) goes through get_kernel each time.  The oldest entries of a program with ever new sizes are dropped; their
+# kernels stay loaded.
+class _Launches(dict):
+    MOST = 4096
+    _change = threading.Lock()
+
+    def __setitem__(self, key, launch):
+        with self._change:
+            while len(self) >= self.MOST and key not in self:
+                del self[next(iter(self))]
+            super().__setitem__(key, launch)
+
+
+_bound = _Launches()
 
 
 def _into(run, shape=None, dtype=None):
@@ -352,7 +365,7 @@ def page_slots(lengths, added, table, free, page_size, tokens):
     [B], number of pages taken int32 [1]): slot = page * page_size + place in the page, what cache_write takes; -1 for padding and for
     tokens that have no page, because `free` or the table is too short.  starts and the new lengths are what cache_attention takes."""
     page_size, tokens = operator.index(page_size), operator.index(tokens)
-    key = ("page_slots", R.signature(lengths, added, table, free), page_size, tokens)
+    key = ("page_slots", R.signature(lengths, added), R.row_signature(table, free), page_size, tokens)
     run = _bound.get(key)
     if run is None:
         _bound[key] = run = _page_slots_launch(lengths, added, table, free, page_size, tokens)

@@ -181,6 +181,18 @@ def signature(*tensors):
     return signature(*tensors)
 
 
+def _plain_row_signature(*tensors):
+    return tuple([None if t is None else (t.device, t.dtype, t.layout, t.shape[:-1], t.stride(-1) if t.dim() and t.shape[-1] > 1 else 1, t.dim(), t.data_ptr() & 15)
+                  for t in tensors])
+
+
+def row_signature(*tensors):
+    """signature() of operands whose rows' length and distance are arguments of the kernel, and left out."""
+    global row_signature
+    row_signature = importlib.import_module(__package__ + "._launch").row_signature if _native_launch() else _plain_row_signature
+    return row_signature(*tensors)
+
+
 class Kernel:
     def __init__(self, module, handle, info=None):
         self.module, self.handle, self.info = module, handle, info

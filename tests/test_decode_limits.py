@@ -156,3 +156,45 @@ def test_rows_of_a_4_bit_product_have_32_bits(monkeypatch):
     for shape, refused in (((1 << 31, 32), True), ((1 << 16, 1 << 15, 32), True), ((0x7FFFFF01, 32), True), ((0x7FFFFF00, 32), False)):
         with pytest.raises(ValueError if refused else Emitted):
             ops._matmul_q4_launch(Operand(shape, torch.bfloat16), w, scale, None, None, {})
+
+
+# ---- bound launches
+
+def test_the_number_of_free_pages_asks_for_no_other_launch(monkeypatch):
+    """The list of free pages and the table's width are another in every step of a loop that passes parts of tensors."""
+    made, got = [], []
+
+    def launch(*args):
+        made.append(args)
+        return lambda *a: got.append(a)
+    monkeypatch.setattr(ops, "_page_slots_launch", launch)
+    monkeypatch.setattr(ops, "_bound", {})
+    i32 = torch.int32
+    lengths, table, free = torch.zeros(3, dtype=i32), torch.zeros((3, 40), dtype=i32), torch.zeros(400, dtype=i32)
+    for used in range(0, 400, 4):
+        ops.page_slots(lengths, lengths, table[:, :1 + used // 20], free[used:], 16, 3)
+    assert len(made) == 1 and [(a[6], a[7], a[8]) for a in got] == [(1 + u // 20, 40, 400 - u) for u in range(0, 400, 4)]
+    # what is checked by the first call only is in the key
+    for other in (dict(free=free[::2]), dict(free=free.long()), dict(free=free[None]), dict(table=table[:, ::2]), dict(table=table[:2]), dict(table=table.long()),
+                  dict(lengths=lengths[:2]), dict(page_size=32), dict(tokens=4)):
+        before = len(made)
+        ops.page_slots(**{**dict(lengths=lengths, added=lengths, table=table, free=free, page_size=16, tokens=3), **other})
+        assert len(made) == before + 1, other
+
+
+@pytest.mark.parametrize("kind", ["plain", "native"])
+def test_signatures_of_rows(kind):
+    row_signature = R._plain_row_signature if kind == "plain" else __import__("kernelcodegen_amd._launch", fromlist=["x"]).row_signature
+    x = torch.zeros((4, 10))
+    assert row_signature(x, None) == row_signature(x[:, :3], None) == row_signature(torch.zeros((4, 20))[:, ::20], None) == row_signature(x[:, :0], None)
+    different = [row_signature(*t) for t in ((x,), (x[:3],), (x[:, ::2],), (x[0],), (x[:, 1:],), (x.int(),), (x[None],), (x, x), (x, None), (None,), (torch.zeros(()),))]
+    assert len(set(different)) == len(different)
+
+
+def test_bound_launches_are_no_more_than_some():
+    kept = type(ops._bound)()
+    for i in range(3 * kept.MOST):
+        kept[i] = -i
+    assert len(kept) == kept.MOST and kept.get(3 * kept.MOST - 1) == 1 - 3 * kept.MOST and kept.get(0) is None
+    kept[3 * kept.MOST - 5] = "again"
+    assert len(kept) == kept.MOST and kept.get(2 * kept.MOST) == -2 * kept.MOST
