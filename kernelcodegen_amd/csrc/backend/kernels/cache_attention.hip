@@ -573,15 +573,17 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
           unsigned nan = 0;
 #pragma unroll
           for (int u = 0; u < CA_SL; ++u) {
-            const float scale = __shfl(now.vs, step * 4 + of[u] / 16, 64);
-            const int page = __shfl(now.page, step * 4 + of[u] / 16, 64);
-            if (key + of[u] < lo || key + of[u] >= hi || page < 0) v[u] = kcg_u32x4{0, 0, 0, 0};
+            bool none = key + of[u] < lo || key + of[u] >= hi;
+            if (zeros) {
+              const float scale = __shfl(now.vs, step * 4 + of[u] / 16, 64);
+              none |= __shfl(now.page, step * 4 + of[u] / 16, 64) < 0;
+              if (scale == -__builtin_inff())
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const unsigned bytes = ca_nan_bytes(v[u][i]);
-              if (scale == -__builtin_inff()) v[u][i] &= bytes * 0xffu;
-              nan |= bytes;
+                for (int i = 0; i < 4; ++i) v[u][i] &= ca_nan_bytes(v[u][i]) * 0xffu;
             }
+            if (none) v[u] = kcg_u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) nan |= ca_nan_bytes(v[u][i]);
           }
           if (nan != 0) sh.nan[count & 3] = 1;
           __syncthreads();
@@ -1044,13 +1046,12 @@ void CA_NAME(const ca_q* __restrict__ q, const unsigned char* __restrict__ kc, c
 #pragma unroll
         for (int u = 0; u < CA_VL; ++u) {
           const int key32 = (u * 64 + lane) / (CA_D / 16);
+          if ((zero[0] || zero[1]) && (key32 < 16 ? zero[0] : zero[1]))
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[u][i] &= ca_nan_bytes(v[u][i]) * 0xffu;
           if (at + key32 < lo || at + key32 >= hi || !(key32 < 16 ? there[0] : there[1])) v[u] = kcg_u32x4{0, 0, 0, 0};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const unsigned bytes = ca_nan_bytes(v[u][i]);
-            if (key32 < 16 ? zero[0] : zero[1]) v[u][i] &= bytes * 0xffu;
-            nan |= bytes;
-          }
+          for (int i = 0; i < 4; ++i) nan |= ca_nan_bytes(v[u][i]);
         }
         if (__any(nan != 0)) {
           // NaN where some rows see the key and some may not: it goes to those that do, by a product of where V is NaN and who sees
