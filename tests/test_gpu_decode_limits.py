@@ -285,3 +285,15 @@ def test_modes_that_look_at_allocations_see_the_results():
         with Seen() as seen:
             call()
         assert any("empty" in name for name in seen.names)
+
+
+# ---- a step of prompts and single tokens
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_chunks_beside_single_tokens_and_padding(dtype):
+    lengths = [1 + 37 * i % 500 for i in range(60)] + [700, 300]
+    counts = [1] * 60 + [200, 130]
+    q, caches, scales, table, starts = attention_case(19, lengths, counts, 8, 2, 64, 16, "tokens", dtype)
+    q = torch.cat([q, torch.ones_like(q[:100])])
+    got = ops.cache_attention(q, *caches, *scales, table, ints(lengths), ints(starts))
+    close(got, plain_attention(q, *caches, *scales, table, lengths, starts, 0.125, 0.0, 0, None))
