@@ -62,6 +62,18 @@ def test_pages_of_small_values_keep_their_weight(dtype, many, low, first):
     near(got, plain_attention(q, *caches, *scales, table, lengths, starts, 0.125, 0.0, 0, None))
 
 
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("first", [0, 1])
+def test_scales_as_far_apart_as_they_may_be(many, first):
+    """A factor of 2^100, the least 2^-78."""
+    q, caches, scales, table, lengths, starts, held = far_apart("bf16", many, 0, 20)
+    for pages in held:
+        scales[1][pages] *= 2.0 ** 30
+        scales[1][pages[first::2]] *= 2.0 ** -100
+    got = ops.cache_attention(q, *caches, *scales, table, ints(lengths), None if starts is None else ints(starts))
+    near(got, plain_attention(q, *caches, *scales, table, lengths, starts, 0.125, 0.0, 0, None))
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("count", [1, 40])
 @pytest.mark.parametrize("sink", [-11, 0])
