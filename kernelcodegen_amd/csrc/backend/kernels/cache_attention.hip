@@ -416,7 +416,7 @@ __device__ __forceinline__ bool ca_begin(int id, int piece, float* __restrict__ 
 #if CA_SHARE
 // Many rows: every wavefront has 16 CA_RB rows of the tile of its own, and all of them work on the same 64 keys a step, which they bring into two
 // LDS buffers together; so a key is read once for 16 CA_RB CA_WAVES rows and nothing is added up between wavefronts.
-// Measured: 1500 tokens of 32 heads over 8 of 128, behind 2 requests of up to 6000 keys, 162 us with the join, 620 TFLOP/s as 16-bit products
+// Measured: 1500 tokens of 32 heads over 8 of 128, behind 2 requests of up to 6000 keys, 160 us with the join, 625 TFLOP/s as 16-bit products
 // would count; vector instructions are under way 55 % of the time (scores, exp2), matrix instructions 30 %.
 // V is converted on its way into LDS, once for all wavefronts, as far as LDS holds two such workgroups (D up to 128).
 #define CA_V16 (CA_D <= 128)

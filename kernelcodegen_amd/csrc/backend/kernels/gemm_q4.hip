@@ -18,8 +18,8 @@
 // their sums through LDS, and Q4_SPLIT workgroups split it again, whose fp32 results gemm_q4_join adds in order.
 // Where a group has 128 codes or more, product j of a step's half takes k = 32 g + 8 j .. + 7 for quarter g of the wavefront, 16 bytes
 // of codes as they come; smaller groups need products of 32 neighbouring k, so the quarters exchange dwords (four permlane swaps).
-// Measured: 1 row, N = K = 4096, bf16, groups of 128: 3.8 us (2.3 TB/s; reading as many bytes alone takes 3.0); 16 rows, N 11008, K 4096, half
-// precision with zeros: 8.6 us (2.8 TB/s; reading alone 5.1); 61 rows, N 4096, K 11008, groups of 64: 18.1 us with the join's 3.  One row is
+// Measured: 1 row, N = K = 4096, bf16, groups of 128: 3.8 to 4.4 us by the process (2 TB/s; reading as many bytes alone takes 3.0); 16 rows, N 11008, K 4096, half
+// precision with zeros: 8.6 us (2.8 TB/s; reading alone 5.1); 61 rows, N 4096, K 11008, groups of 64: 17.9 us with the join's 3.  One row is
 // bound by the launch and one trip to memory.  At 61 rows vector instructions are under way half of the time (codes to numbers, sums to results), LDS
 // accesses, of X by every wavefront's columns anew, 57 %, matrix products 20 %, each step's one after the other.  The sums of X taken by the
 // matrix product itself, with ones in the weights' place, cost this case 1.5 us.

@@ -5,10 +5,10 @@
 // Every workgroup takes the prefix sums of all requests (PS_BLOCK at a time) and then its share of the pages and tokens, each found in the
 // sums in LDS: a step of any shape is one launch.  Bound by what waits for one another: the lengths, the sums, the table or the
 // list, the stores.
-// Measured: 64 requests of one token each 2.8 us (an empty launch 1.7), 200 of up to 700 7.
-// Parameters: PS_NAME, PS_BLOCK, PS_PAGE.
+// Measured: 64 requests of one token each 2.8 us (an empty launch 1.7), 200 of up to 700 8.
 // Lengths, places and sums are counted without a sign, so that length + added may use all bits of a positive number, and a place is compared
 // with its table without one: sums that pass 32 bits give wrong slots, but no access out of range.
+// Parameters: PS_NAME, PS_BLOCK, PS_PAGE.
 struct PsSums { unsigned pages[PS_BLOCK + 1], tokens[PS_BLOCK + 1], lengths[PS_BLOCK], waves[2][PS_BLOCK / 64]; };
 
 __device__ __forceinline__ unsigned ps_pages(unsigned tokens) { return tokens / PS_PAGE + (tokens % PS_PAGE ? 1 : 0); }

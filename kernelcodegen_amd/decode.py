@@ -57,7 +57,7 @@ class Decoder:
 
     def step(self, tokens, added=None):
         """Takes the new tokens of all requests, int64 [T], those of a request beside one another: added[b] (int32 [B]) of request b, or
-        one of each.  Returns the scores of each request's next token, [B, vocab]."""
+        one of each.  Returns the scores of each request's next token, [B, vocab] (nothing of use for a request that gets none)."""
         rows = tokens.shape[0]
         slots, _, starts, lengths, used = ops.page_slots(self.lengths, self._one if added is None else added, self.table, self.free, self.page, rows)
         x = ops.gather(self.embedding, tokens).view(rows, -1)
