@@ -576,7 +576,7 @@ def _cache_attention_form(batch, tokens, kv_heads, group, d, keys, half):
       8 prompts of up to 300 behind up to 600 keys: shared keys with 16 rows a wavefront 41, 32 rows 49, keys split 58;  2 of 1000 behind 6000:
       202, 167, 195;  64 of up to 16 tokens behind 1000: 35, 54, 44
       32 heads to one kv head: 8 of up to 32000 keys: keys split, 16 rows a tile 21.6, 32 rows 26.9, shared 26.2;  16 of 16000 of 256: 38, 61, 32
-      2 of 500 behind 4000, 8 heads of 256 to a kv head: half precision 16 rows a wavefront 172, 32 rows 212;  bfloat16, 32 rows: 138"""
+      2 of 500 behind 4000, 8 heads of 256 to a kv head: half precision 16 rows a wavefront 140, 32 rows 212;  bfloat16, 32 rows: 138"""
     rows = group * max(1, -(-tokens // batch))
     share = int(rows > (32 if d <= 128 else 16))
     blocks = 2 if share and rows * keys >= 1 << 21 and not (half and d > 128) else 1
