@@ -1660,22 +1660,37 @@ bool emitPageSlots(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std:
   return true;
 }
 
+// cache_write, and cache_append, which turns keys and queries by their positions on the way.
 bool emitCacheWrite(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::string& err) {
+  const bool append = s.family == "cache_append";
   if (!cacheShape(s, {"KP", "KT", "KH", "VP", "VT", "VH"}, err)) return false;
   if (!whole(s, "F16", 0, 2, err) || !whole(s, "WIN", 1, 16, err)) return false;
   const int64_t esize = s.p["F16"] ? 2 : 4;
-  for (auto key : {"XKT", "XKH", "XVT", "XVH"})
-    if (!whole(s, key, 0, (int64_t)1 << 40, err)) return false;
-    else if (s.p[key] * esize % 16) { err = std::string("cache_write: ") + key + " must be a multiple of 16 bytes"; return false; }
+  auto rows = [&](std::initializer_list<const char*> strides) {
+    for (auto key : strides)
+      if (!whole(s, key, 0, (int64_t)1 << 40, err)) return false;
+      else if (s.p[key] * esize % 16) { err = s.family + ": " + key + " must be a multiple of 16 bytes"; return false; }
+    return true;
+  };
+  if (!rows({"XKT", "XKH", "XVT", "XVH"})) return false;
+  if (append) {
+    if (!rows({"XQT", "XQH"}) || !whole(s, "HQ", 1, 65536, err) || !whole(s, "R", 16, s.p["D"], err) || !whole(s, "QN", 1, 8, err)) return false;
+    if (s.p["R"] % 16) { err = "cache_append: R must be a multiple of 16"; return false; }
+  }
   Defines d;
   d.add("CW_NAME", s.name);
-  d.add("CW_T", std::string(typeName(s.p["F16"]))); d.add("CW_ESIZE", esize);
+  d.add("CW_T", std::string(typeName(s.p["F16"]))); d.add("CW_ESIZE", esize); d.add("CW_ROT", append ? 1 : 0);
   for (auto key : {"H", "D", "PAGE", "WIN"}) d.add(std::string("CW_") + key, s.p[key]);
   for (auto key : {"KP", "KT", "KH", "VP", "VT", "VH", "XKT", "XKH", "XVT", "XVH"}) d.add(std::string("CW_") + key, std::to_string(s.p[key]) + "LL");
+  if (append) {
+    d.add("CW_PAIRS", s.get("PAIRS", 0) ? 1 : 0);
+    for (auto key : {"R", "HQ", "QN"}) d.add(std::string("CW_") + key, s.p[key]);
+    for (auto key : {"XQT", "XQH"}) d.add(std::string("CW_") + key, std::to_string(s.p[key]) + "LL");
+  }
   src = d.wrap(kTpl_cache_write);
   info.name = s.name;
   info.block[0] = 256;
-  info.numArgs = 9;
+  info.numArgs = append ? 14 : 9;
   return true;
 }
 
@@ -1776,6 +1791,60 @@ bool emitGemmQ4(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::st
   return true;
 }
 
+// adapters_down and adapters_up, which takes what the first leaves: the same parameters.
+bool emitAdapters(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::string& err) {
+  const bool up = s.family == "adapters_up";
+  if (!whole(s, "N", 1, 0x7FFFFF00, err) || !whole(s, "K", 8, 0x7FFFFF00, err) || !whole(s, "RANK", 8, 256, err) || !whole(s, "F16", 0, 1, err)) return false;
+  for (auto key : {"K", "RANK"})
+    if (s.p[key] % 8) { err = s.family + ": " + key + " must be a multiple of 8"; return false; }
+  for (auto key : {"XT", "YT", "ZT"})
+    if (!whole(s, key, 0, (int64_t)1 << 40, err)) return false;
+  if (s.p["XT"] % 8) { err = s.family + ": XT must be a multiple of 16 bytes"; return false; }
+  const int64_t ks = s.get("KS", 1), slots = s.get("S", 1), ns = s.get("NS", 1);
+  if (ks < 1 || ks > 64 || slots < 1 || slots > 16 || ns < 1 || ns > 4096) { err = s.family + ": KS must be in [1,64], S in [1,16], NS in [1,4096]"; return false; }
+  const char* x = s.p["F16"] ? "_Float16" : "__bf16";
+  const bool y32 = s.get("Y_F32", 0) != 0, align = s.get("ALIGN", 0) != 0;
+  if (align && (s.p["YT"] * (y32 ? 4 : 2) % 16 || s.p["ZT"] * (y32 ? 4 : 2) % 16)) { err = s.family + ": ALIGN is for rows on multiples of 16 bytes"; return false; }
+  Defines d;
+  d.add("AD_NAME", s.name); d.add("AD_UP", up ? 1 : 0);
+  for (auto key : {"N", "K", "RANK", "F16"}) d.add(std::string("AD_") + key, s.p[key]);
+  for (auto key : {"XT", "YT", "ZT"}) d.add(std::string("AD_") + key, std::to_string(s.p[key]) + "LL");
+  d.add("AD_YTYPE", std::string(y32 ? "float" : x)); d.add("AD_ALIGN", align ? 1 : 0);
+  d.add("AD_SCALE", s.get("SCALES", 0) ? 1 : 0); d.add("AD_INPLACE", s.get("INPLACE", 0) ? 1 : 0);
+  d.add("AD_KS", ks); d.add("AD_S", slots); d.add("AD_NS", ns);
+  src = d.wrap(kTpl_adapters);
+  info.name = s.name;
+  info.block[0] = 256;
+  info.numArgs = up ? 8 : 6;
+  return true;
+}
+
+// token_logprobs, and logprobs_join, which finishes rows that several workgroups share: the same parameters.
+bool emitLogprobs(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::string& err) {
+  const bool join = s.family == "logprobs_join";
+  // (an index of a number or a segment has 32 bits; the segments of a row are in LDS)
+  if (!whole(s, "V", 1, 1 << 19, err) || !whole(s, "F16", 0, 2, err) || !whole(s, "TOP", 0, 32, err)) return false;
+  const int64_t v = s.p["V"], esize = s.p["F16"] ? 2 : 4;
+  if (s.p["TOP"] > v) { err = s.family + ": TOP must not be above V"; return false; }
+  if (!whole(s, "STRIDE", 0, (int64_t)1 << 40, err)) return false;
+  const int64_t parts = s.get("PARTS", 1), threads = s.get("THREADS", 512), u = s.get("U", esize == 2 ? 4 : 8);
+  if (parts < 1 || parts > 1024 || (join && parts == 1)) { err = s.family + ": PARTS must be in [1,1024], more than one to join"; return false; }
+  if (threads < 64 || threads > 1024 || threads % 64 || u < 1 || u > 16) { err = s.family + ": THREADS must be a multiple of 64 up to 1024, U in [1,16]"; return false; }
+  const bool shift = s.get("SHIFT", 0) != 0;
+  if (!shift && s.p["STRIDE"] * esize % 16) { err = s.family + ": rows off a multiple of 16 bytes need SHIFT"; return false; }
+  s.p["PARTS"] = parts; s.p["THREADS"] = threads; s.p["U"] = u;
+  Defines d;
+  d.add("LP_NAME", s.name);
+  d.add("LP_T", std::string(typeName(s.p["F16"]))); d.add("LP_ES", esize); d.add("LP_SHIFT", shift ? 1 : 0); d.add("LP_JOIN", join ? 1 : 0);
+  for (auto key : {"V", "TOP", "PARTS", "THREADS", "U"}) d.add(std::string("LP_") + key, s.p[key]);
+  d.add("LP_STRIDE", std::to_string(s.p["STRIDE"]) + "LL");
+  src = d.wrap(kTpl_token_logprobs);
+  info.name = s.name;
+  info.block[0] = (uint32_t)threads;
+  info.numArgs = join ? 8 : parts > 1 ? 2 : 6;
+  return true;
+}
+
 }  // namespace
 
 const std::string& prelude() {
@@ -1802,10 +1871,12 @@ bool emitKernel(KernelSpec& spec, std::string& src, KernelLaunchInfo& info, std:
   if (spec.family == "fmha_bf16") return emitFmhaBf16(spec, src, info, err);
   if (spec.family == "fmha_f32") return emitFmhaF32(spec, src, info, err);
   if (spec.family == "page_slots") return emitPageSlots(spec, src, info, err);
-  if (spec.family == "cache_write") return emitCacheWrite(spec, src, info, err);
+  if (spec.family == "cache_write" || spec.family == "cache_append") return emitCacheWrite(spec, src, info, err);
   if (spec.family == "cache_read") return emitCacheRead(spec, src, info, err);
   if (spec.family == "cache_attention" || spec.family == "cache_join") return emitCacheAttention(spec, src, info, err);
   if (spec.family == "gemm_q4" || spec.family == "gemm_q4_join") return emitGemmQ4(spec, src, info, err);
+  if (spec.family == "adapters_down" || spec.family == "adapters_up") return emitAdapters(spec, src, info, err);
+  if (spec.family == "token_logprobs" || spec.family == "logprobs_join") return emitLogprobs(spec, src, info, err);
   err = "unknown kernel family '" + spec.family + "'";
   return false;
 }

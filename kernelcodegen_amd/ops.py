@@ -431,6 +431,13 @@ def cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots):
 
 
 def _cache_write_launch(k, v, k_cache, v_cache, k_scale, v_scale, slots):
+    params = _cache_write_params(k, v, k_cache, v_cache, k_scale, v_scale, slots)
+    kern = R.get_kernel("cache_write", **params)
+    run = kern.bind(grid=(max(1, -(-2 * params["H"] * -(-slots.shape[0] // params["WIN"]) // 4)),))
+    return run if hasattr(run, "results") else lambda *a: run(*[x.data_ptr() if isinstance(x, torch.Tensor) else x for x in a])
+
+
+def _cache_write_params(k, v, k_cache, v_cache, k_scale, v_scale, slots):
     _on_device(k, v, k_cache, v_cache)
     _vectors(torch.int64, slots)
     _vectors(torch.float32, k_scale, v_scale)
@@ -444,10 +451,47 @@ def _cache_write_launch(k, v, k_cache, v_cache, k_scale, v_scale, slots):
     # tokens of a wavefront, which takes the pages they lead one after the other: us for tokens of a page each and of whole pages (8 heads of 128)
     # 128 tokens: one 3.5 and 4, four 5.2 and 3.3;  512: one 6.2 and 8.2, four 6.8 and 4.1, sixteen 15 and 3.6;  9000 of whole pages: 58, 29, 12.5
     win = 1 if tokens <= 128 else 4 if tokens <= 2048 else 16
-    kern = R.get_kernel("cache_write", H=heads, D=d, PAGE=k_cache.shape[1], F16=_STORAGE[k.dtype], WIN=win, KP=ks[0], KT=ks[1], KH=ks[2],
-                        VP=vs[0], VT=vs[1], VH=vs[2], XKT=xk[0], XKH=xk[1], XVT=xv[0], XVH=xv[1])
-    run = kern.bind(grid=(max(1, -(-2 * heads * -(-tokens // win) // 4)),))
-    return run if hasattr(run, "results") else lambda *a: run(*[x.data_ptr() if isinstance(x, torch.Tensor) else x for x in a])
+    return dict(H=heads, D=d, PAGE=k_cache.shape[1], F16=_STORAGE[k.dtype], WIN=win, KP=ks[0], KT=ks[1], KH=ks[2],
+                VP=vs[0], VT=vs[1], VH=vs[2], XKT=xk[0], XKH=xk[1], XVT=xv[0], XVH=xv[1])
+
+
+def cache_append(q, k, v, k_cache, v_cache, k_scale, v_scale, slots, positions, rotation, interleaved=False):
+    """cache_write of keys that are turned by their positions on the way, and the queries turned the same way.
+
+    k, v, the caches, scales and slots as for cache_write; q: [tokens, query heads, d] of k's type; positions: int32 [tokens], as page_slots
+    gives them; rotation: fp32 [P, R], row p the cosines of position p's R / 2 angles, then their sines, R a multiple of 16 up to d.  The first R numbers of
+    a head are R / 2 pairs (x, y) that become (x cos - y sin, y cos + x sin): numbers i and i + R / 2, or 2 i and 2 i + 1 (interleaved).
+    Returns the turned queries, contiguous, in q's type.  A row without a position (-1) is left unturned, padding for instance; a position behind the
+    table's last makes the numbers that it would turn NaN.  A key's 8 bits, and its page's scale, are those of the formula in 64 bits."""
+    interleaved = bool(interleaved)
+    key = ("cache_append", R.signature(q, k, v, k_cache, v_cache, k_scale, v_scale, slots, positions, rotation), interleaved)
+    run = _bound.get(key)
+    if run is None:
+        _bound[key] = run = _cache_append_launch(q, k, v, k_cache, v_cache, k_scale, v_scale, slots, positions, rotation, interleaved)
+    tokens = slots.shape[0]
+    if not tokens:
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
+    return run(k, v, k_cache, v_cache, k_scale, v_scale, slots, tokens, k_cache.shape[0], q, positions, rotation, rotation.shape[0])
+
+
+def _cache_append_launch(q, k, v, k_cache, v_cache, k_scale, v_scale, slots, positions, rotation, interleaved):
+    params = _cache_write_params(k, v, k_cache, v_cache, k_scale, v_scale, slots)
+    _on_device(q)
+    _vectors(torch.int32, positions)
+    _vectors(torch.float32, rotation)
+    xq = _row_strides(q, k_cache, (k.dtype,))
+    tokens, heads, d = q.shape
+    if tokens != slots.shape[0] or tuple(positions.shape) != (tokens,) or not heads:
+        raise ValueError("queries and positions are those of the keys' tokens")
+    if rotation.dim() != 2 or rotation.shape[0] < 1 or rotation.shape[1] % 16 or not 16 <= rotation.shape[1] <= d or rotation.data_ptr() % 16:
+        raise ValueError("rotation is [P, R] on a multiple of 16 bytes, R a multiple of 16 up to the head dimension")
+    # passes of a token's query heads for one reading of its angles
+    passes = 1 if tokens <= 128 else 4
+    kern = R.get_kernel("cache_append", R=rotation.shape[1], PAIRS=int(interleaved), HQ=heads, QN=passes, XQT=xq[0], XQH=xq[1], **params)
+    waves = 2 * params["H"] * -(-tokens // params["WIN"]) + tokens * -(-heads // (passes * (64 // (d // 8))))
+    if waves > 0x7FFFFFFF:
+        raise ValueError("too many tokens for one launch")
+    return _into_last(kern.bind(grid=(max(1, -(-waves // 4)),)), (tuple(q.shape), q.dtype))
 
 
 def cache_read(cache, scale, slots, dtype=torch.bfloat16):
@@ -671,3 +715,143 @@ def _matmul_q4_form(rows, n, k, group):
     steps = -(-k // 256) // form["WK"]
     form["SPLIT"] = max(1, min(256 // workgroups, steps, 64)) if form["WN"] > 1 and steps >= 4 else 1
     return form
+
+
+def add_adapters(y, x, a, b, which, scale=None, inplace=False, **cfg):
+    """The low-rank adapters of many requests beside a projection that they share: y[t] + scale[r] * b[r] (a[r] x[t]), r = which[t].
+
+    y: [tokens, N], what the shared projection gives, of x's type or fp32; x: [tokens, K], IEEE half or bfloat16; a: [adapters, rank, K] and b: [adapters, N,
+    rank], of x's type and contiguous; which: int32 [tokens], in any order, each adapter for any number of tokens; scale: fp32 [adapters], None for 1.
+    Rank and K are multiples of 8, the rank up to 256 (a smaller one is filled up with zeros).  Rows of x and y may lie apart.  Returns a
+    contiguous tensor of y's type, or y itself (inplace); a token whose adapter is none of them (-1) keeps its row of y.  Sums are
+    fp32, a[r] x[t] enters the second product with 16 bits or more, and the sum with y is rounded once.  `cfg` overrides kernel parameters (KS, S, NS)."""
+    inplace = bool(inplace)
+    key = ("add_adapters", R.signature(y, x, a, b, which, scale), inplace)
+    hit = None if cfg else _bound.get(key)
+    if hit is None:
+        hit = _add_adapters_launch(y, x, a, b, which, scale, inplace, cfg)
+        if not cfg:
+            _bound[key] = hit
+    down, up = hit
+    tokens, adapters = which.shape[0], a.shape[0]
+    if down is None:
+        return y if inplace else torch.empty_like(y, memory_format=torch.contiguous_format)
+    part = down(x, a, which, tokens, adapters)
+    if not inplace:
+        return up(part, y, b, which, 0 if scale is None else scale, tokens, adapters)
+    up(part.data_ptr(), y.data_ptr(), b.data_ptr(), which.data_ptr(), 0 if scale is None else scale.data_ptr(), tokens, adapters, y.data_ptr())
+    return y
+
+
+def _add_adapters_launch(y, x, a, b, which, scale, inplace, cfg):
+    _on_device(y, x)
+    _need_cuda(a, b)
+    _vectors(torch.int32, which)
+    if scale is not None:
+        _vectors(torch.float32, scale)
+    if x.dtype not in (torch.float16, torch.bfloat16) or a.dtype != x.dtype or b.dtype != x.dtype or y.dtype not in (x.dtype, torch.float32):
+        raise ValueError("x, a and b are IEEE half or bfloat16, y has their type or is fp32")
+    if y.dim() != 2 or x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
+        raise ValueError("y is [tokens, N], x [tokens, K], a [adapters, rank, K], b [adapters, N, rank]")
+    (tokens, n), k, (adapters, rank) = y.shape, x.shape[1], a.shape[:2]
+    if x.shape[0] != tokens or tuple(which.shape) != (tokens,) or a.shape[2] != k or tuple(b.shape) != (adapters, n, rank):
+        raise ValueError("y is [tokens, N], x [tokens, K], a [adapters, rank, K], b [adapters, N, rank], which [tokens]")
+    if adapters < 1 or adapters > 0x7FFFFFFF or rank % 8 or not 8 <= rank <= 256 or k % 8 or not 8 <= k <= 0x7FFFFF00 or not 1 <= n <= 0x7FFFFF00:
+        raise ValueError("rank and K are multiples of 8, the rank up to 256, and there is an adapter")
+    if scale is not None and tuple(scale.shape) != (adapters,):
+        raise ValueError("scale is [adapters]")
+    if x.stride(1) != 1 or (y.stride(1) != 1 and n > 1):
+        raise ValueError("the numbers of a row must lie beside one another")
+    if (x.data_ptr() | a.data_ptr() | b.data_ptr()) % 16 or x.stride(0) % 8:
+        raise ValueError("rows of x, a and b must start on multiples of 16 bytes")
+    if inplace and tokens > 1 and y.stride(0) < n:
+        raise ValueError("rows of y must not overlap")
+    if tokens > 0x7FFFFF00:
+        raise ValueError("too many tokens for one launch")
+    if not cfg.keys() <= {"KS", "S", "NS"}:
+        raise ValueError("unknown kernel parameters")
+    if not tokens:
+        return None, None
+    yt = y.stride(0) if tokens > 1 else 0
+    zt, size = yt if inplace else n, y.element_size()
+    params = dict(N=n, K=k, RANK=rank, F16=int(x.dtype == torch.float16), Y_F32=int(y.dtype == torch.float32), XT=x.stride(0) if tokens > 1 else 0, YT=yt, ZT=zt,
+                  ALIGN=int((y.data_ptr() | yt * size | zt * size) % 16 == 0), SCALES=int(scale is not None), INPLACE=int(inplace),
+                  **{**_add_adapters_form(tokens, adapters, n, k, rank), **cfg})
+    tiles = -(-tokens // 16) * params["S"]
+    if tiles * max(params["KS"], params["NS"]) > 0x7FFFFFFF:
+        raise ValueError("too many tokens for one launch")
+    down = R.get_kernel("adapters_down", **params).bind(grid=(tiles * params["KS"],))
+    up = R.get_kernel("adapters_up", **params).bind(grid=(tiles * params["NS"],))
+    return _into_last(down, ((params["KS"], tokens, rank), torch.float32)), up if inplace else _into_last(up, ((tokens, n), y.dtype))
+
+
+def _add_adapters_form(tokens, adapters, n, k, rank):
+    """Workgroups for the adapters of a tile of 16 tokens (S), for parts of k (KS) and of the columns (NS)."""
+    tiles = -(-tokens // 16)
+    slots = min(16, tokens, adapters) if tiles <= 16 else 1
+    ks = max(1, min(8, 512 // (tiles * slots), k // 512))
+    ns = max(1, min(-(-n // 256), 1024 // (tiles * slots)))
+    return dict(S=slots, KS=ks, NS=ns)
+
+
+def token_logprobs(logits, tokens, top=0, **cfg):
+    """Log probabilities of given tokens under the softmax of their rows of logits, with each row's entropy and likeliest tokens.
+
+    logits: [rows, V], fp32, IEEE half or bfloat16, neighbouring along V (rows may lie apart), V up to 2^19; tokens: int64 [rows]; top: 0 to 32, up to V.
+    Returns (logprob fp32 [rows], entropy fp32 [rows], logprobs of the likeliest fp32 [rows, top], which they are int64 [rows, top]), the likeliest
+    first, of equal ones the lowest.  A token that is none of the V has the log probability -inf, as one whose logit is -inf.  In a row of
+    nothing but -inf all have it, and the entropy is 0; a NaN or +inf in a row makes its numbers NaN, and a NaN counts as -inf among the likeliest.
+    `cfg` overrides kernel parameters (PARTS, THREADS, U)."""
+    top = operator.index(top)
+    key = ("token_logprobs", R.signature(logits, tokens), top)
+    hit = None if cfg else _bound.get(key)
+    if hit is None:
+        hit = _token_logprobs_launch(logits, tokens, top, cfg)
+        if not cfg:
+            _bound[key] = hit
+    run, join = hit
+    if run is None:
+        return _no_rows(logits, top)
+    return run(logits, tokens) if join is None else join(run(logits), logits, tokens, logits.shape[0])
+
+
+def _no_rows(logits, top):
+    device = logits.device
+    return (torch.empty(0, device=device), torch.empty(0, device=device), torch.empty((0, top), device=device),
+            torch.empty((0, top), dtype=torch.int64, device=device))
+
+
+def _token_logprobs_launch(logits, tokens, top, cfg):
+    _on_device(logits)
+    _vectors(torch.int64, tokens)
+    if logits.dim() != 2 or logits.dtype not in _STORAGE or tuple(tokens.shape) != (logits.shape[0],):
+        raise ValueError("logits are [rows, V] in fp32, IEEE half or bfloat16, tokens [rows]")
+    rows, v = logits.shape
+    if not 1 <= v <= 1 << 19 or not 0 <= top <= min(32, v):
+        raise ValueError("a row has 1 to 2^19 logits, and up to 32 of them are asked for")
+    if v > 1 and logits.stride(1) != 1:
+        raise ValueError("the logits of a row must lie beside one another")
+    if not cfg.keys() <= {"PARTS", "THREADS", "U"}:
+        raise ValueError("unknown kernel parameters")
+    if not rows:
+        return None, None
+    stride, size = logits.stride(0) if rows > 1 else 0, logits.element_size()
+    params = dict(V=v, F16=_STORAGE[logits.dtype], TOP=top, STRIDE=stride, SHIFT=int((stride * size | logits.data_ptr()) % 16 != 0),
+                  **{**_token_logprobs_form(rows, v * size), **cfg})
+    parts = params["PARTS"]
+    if rows * parts > 0x7FFFFFFF:
+        raise ValueError("too many rows for one launch")
+    kern = R.get_kernel("token_logprobs", **params)
+    results = ((rows,), torch.float32), ((rows,), torch.float32), ((rows, top), torch.float32), ((rows, top), torch.int64)
+    if parts == 1:
+        return _into_last(kern.bind(grid=(rows,)), *results), None
+    vectors = -(-v * size // 16) + params["SHIFT"]
+    floats = rows * (3 * parts + (4 * -(-vectors // 64) if top else 0))
+    join = R.get_kernel("logprobs_join", **{**params, "THREADS": 256}).bind(grid=(rows,))
+    return _into_last(kern.bind(grid=(rows * parts,)), ((floats,), torch.float32)), _into_last(join, *results)
+
+
+def _token_logprobs_form(rows, bytes_):
+    """Workgroups of a row."""
+    parts = 1 if rows >= 256 else max(1, min(-(-512 // rows), bytes_ // 16384))
+    return dict(PARTS=parts, THREADS=512 if parts == 1 else 256)
