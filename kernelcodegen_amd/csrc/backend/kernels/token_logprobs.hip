@@ -25,7 +25,7 @@ typedef LP_T lp_t;
 #define LP_LOW (-3.402823466e38f)
 #define LP_LOG2E 1.4426950408889634f
 typedef lp_t lp_vec __attribute__((ext_vector_type(LP_VW)));
-typedef unsigned long long lp_key;
+typedef double lp_key;
 
 struct LpSum {
   float m, s, u;
@@ -37,36 +37,39 @@ __device__ __forceinline__ LpSum lp_add(LpSum a, LpSum b) {
 }
 // Elements of a row that lie in front of its first aligned vector's begin, as a number of that vector's elements.
 __device__ __forceinline__ int lp_offset(const lp_t* x) { return LP_SHIFT ? (int)((size_t)x / LP_ES % LP_VW) : 0; }
-__device__ __forceinline__ void lp_load(const lp_t* __restrict__ x, int at, float (&v)[LP_VW]) {
-  if (at >= 0 && at + LP_VW <= LP_V) {
-    const lp_vec raw = *(const lp_vec*)(x + at);
+// A vector of which parts may lie outside of the row: these are -inf.  (All loads are unconditional: one behind a branch would be waited for there.)
+__device__ __forceinline__ void lp_edge(const lp_t* __restrict__ x, int at, float (&v)[LP_VW]) {
+  lp_t raw[LP_VW];
 #pragma unroll
-    for (int i = 0; i < LP_VW; ++i) v[i] = (float)raw[i];
-  } else {
+  for (int i = 0; i < LP_VW; ++i) raw[i] = x[at + i < 0 ? 0 : at + i < LP_V ? at + i : LP_V - 1];
 #pragma unroll
-    for (int i = 0; i < LP_VW; ++i) v[i] = at + i >= 0 && at + i < LP_V ? (float)x[at + i] : -__builtin_inff();
-  }
+  for (int i = 0; i < LP_VW; ++i) v[i] = at + i >= 0 && at + i < LP_V ? (float)raw[i] : -__builtin_inff();
 }
 
 #if !LP_JOIN
-// The sums of blocks [first, end) of a row for the whole workgroup's threads; the segments' largest numbers.
-__device__ __forceinline__ LpSum lp_scan(const lp_t* __restrict__ x, int first, int end, float* segments) {
+// The sums of blocks [first, end) of a row, those of each wavefront; the segments' largest numbers.
+__device__ __forceinline__ void lp_scan(const lp_t* __restrict__ x, int first, int end, LpSum* sums, float* segments) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, o = lp_offset(x);
   LpSum a = {LP_LOW, 0.0f, 0.0f};
+  // Blocks that lie within the row are under way while those before them are counted; in the place of others the row's first whole vector is read.
+  lp_vec next[LP_U];
+  auto inside = [&](int b) { return LP_V >= 2 * LP_VW && b < end && b * (64 * LP_VW) >= o && (b + 1) * (64 * LP_VW) - o <= LP_V; };
+  auto fetch = [&](int b) {
+    if (LP_V < 2 * LP_VW) return;
+#pragma unroll
+    for (int j = 0; j < LP_U; ++j) next[j] = *(const lp_vec*)(x + (inside(b + j) ? (b + j) * (64 * LP_VW) - o + lane * LP_VW : (LP_VW - o) % LP_VW));
+  };
+  fetch(first + wave * LP_U);
   for (int b = first + wave * LP_U; b < end; b += LP_WAVES * LP_U) {
     float v[LP_U][LP_VW], top[LP_U], most = a.m;
-    if (b + LP_U <= end && b * (64 * LP_VW) >= o && (b + LP_U) * (64 * LP_VW) - o <= LP_V) {
-      lp_vec raw[LP_U];
 #pragma unroll
-      for (int j = 0; j < LP_U; ++j) raw[j] = *(const lp_vec*)(x + ((b + j) * 64 + lane) * LP_VW - o);
+    for (int j = 0; j < LP_U; ++j) {
+      const bool edge = b + j < end && !inside(b + j);
 #pragma unroll
-      for (int j = 0; j < LP_U; ++j)
-#pragma unroll
-        for (int i = 0; i < LP_VW; ++i) v[j][i] = (float)raw[j][i];
-    } else {
-#pragma unroll
-      for (int j = 0; j < LP_U; ++j) lp_load(x, b + j < end ? ((b + j) * 64 + lane) * LP_VW - o : LP_V, v[j]);
+      for (int i = 0; i < LP_VW; ++i) v[j][i] = b + j < end && LP_V >= 2 * LP_VW ? (float)next[j][i] : -__builtin_inff();
+      if (edge) lp_edge(x, ((b + j) * 64 + lane) * LP_VW - o, v[j]);
     }
+    fetch(b + LP_WAVES * LP_U);
 #pragma unroll
     for (int j = 0; j < LP_U; ++j) {
       top[j] = v[j][0];
@@ -102,118 +105,212 @@ __device__ __forceinline__ LpSum lp_scan(const lp_t* __restrict__ x, int first, 
   }
 #pragma unroll
   for (int by = 32; by > 0; by >>= 1) a = lp_add(a, {__shfl_xor(a.m, by, 64), __shfl_xor(a.s, by, 64), __shfl_xor(a.u, by, 64)});
-  __shared__ LpSum sums[LP_WAVES];
   if (lane == 0) sums[wave] = a;
   __syncthreads();
-  a = sums[0];
-#pragma unroll
-  for (int w = 1; w < LP_WAVES; ++w) a = lp_add(a, sums[w]);
-  return a;
 }
 #endif
+template <int N> __device__ __forceinline__ LpSum lp_total(const LpSum* parts) {
+  LpSum a = {parts[0].m, 0.0f, 0.0f};
+#pragma unroll 16
+  for (int i = 1; i < N; ++i) a.m = fmaxf(a.m, parts[i].m);
+#pragma unroll 16
+  for (int i = 0; i < N; ++i) {
+    const float d = parts[i].m - a.m, f = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+    a.s += f * parts[i].s;
+    a.u += f * (parts[i].u + fmaxf(d, -1e30f) * parts[i].s);
+  }
+  return a;
+}
 
 #if LP_PARTS == 1 || LP_JOIN
 #if LP_TOP
-#define LP_Q1 ((LP_SEGMENTS + LP_THREADS - 1) / LP_THREADS)                      // segments of a thread
-#define LP_Q2 ((LP_TOP * 16 + LP_THREADS - 1) / LP_THREADS)                      // and vectors, when they are read again
-#define LP_MOST (LP_Q1 > LP_Q2 * LP_VW ? LP_Q1 : LP_Q2 * LP_VW)
+// A value and an index below 2^19 as a number from 1 to 2, whose order is the values' and for equal ones the indices' backwards (comparing two of
+// these takes one instruction of the ordinary rate); 0 is none.
 __device__ __forceinline__ lp_key lp_order(float x, int index) {
   x = x != x ? -__builtin_inff() : x == 0.0f ? 0.0f : x;
   const unsigned b = __builtin_bit_cast(unsigned, x), up = b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
-  return (lp_key)up << 32 | (0xffffffffu - (unsigned)index);
+  return __builtin_bit_cast(double, 0x3ff0000000000000ULL | (unsigned long long)up << 19 | (0x7ffffu - (unsigned)index));
 }
 __device__ __forceinline__ float lp_value(lp_key k) {
-  const unsigned up = (unsigned)(k >> 32);
+  const unsigned up = (unsigned)(__builtin_bit_cast(unsigned long long, k) >> 19);
   return __builtin_bit_cast(float, up ^ (up >> 31 ? 0x80000000u : 0xffffffffu));
 }
-__device__ __forceinline__ int lp_index(lp_key k) { return (int)(0xffffffffu - (unsigned)k); }
+__device__ __forceinline__ int lp_index(lp_key k) { return 0x7ffff - (int)(__builtin_bit_cast(unsigned long long, k) & 0x7ffff); }
+#define LP_LIST 256                                                              // keys that are counted out against one another
+#define LP_E1 ((LP_SEGMENTS + LP_THREADS - 1) / LP_THREADS)                      // segments of a thread
+#define LP_E2 ((LP_TOP * 16 + LP_THREADS - 1) / LP_THREADS)                      // and vectors, when they are read again
 struct LpPick {
-  lp_key best[LP_THREADS], bound[LP_WAVES], near[LP_WAVES * LP_TOP], list[LP_TOP * LP_MOST], found[LP_TOP], last;
+  lp_key list[2][LP_LIST + 32], found[2][LP_TOP], wave[2][LP_WAVES];
+  __attribute__((aligned(16))) float best[LP_THREADS / 2];
+  float bound[LP_WAVES];
   int many[2];
 };
-__device__ __forceinline__ int lp_rank(const lp_key* list, int n, lp_key k) {
-  int r = 0;
-#pragma unroll 8
-  for (int i = 0; i < n; ++i) r += list[i] > k;
-  return r;
+#define LP_DPP(old, v, control, rows) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, v), control, rows, 0xf, false))
+#define LP_SWAP(v, control) __builtin_amdgcn_update_dpp(0, v, control, 0xf, 0xf, true)       // (quad_perm 1 0 3 2 is 0xb1, 2 3 0 1 is 0x4e)
+// What LP_TOP of the workgroup's numbers reach (or all): of a wavefront's 32 pairs of lanes the LP_TOP-th largest, and of these the largest.
+__device__ __forceinline__ float lp_bound(LpPick& p, float best) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const float most = __builtin_inff(), pair = fmaxf(best, __builtin_bit_cast(float, LP_SWAP(__builtin_bit_cast(int, best), 0xb1)));
+  p.best[threadIdx.x / 2] = pair;
+  __builtin_amdgcn_wave_barrier();        // (a wavefront's own accesses to LDS are carried out in order)
+  int r = 0;                               // pairs above this one; its lanes look at half of them each
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const kcg_f32x4 other = *(const kcg_f32x4*)(p.best + wave * 32 + lane % 2 * 16 + i * 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r += other[e] > pair;
+  }
+  r += LP_SWAP(r, 0xb1);
+  float v = r < LP_TOP ? pair : most;
+  v = fminf(v, LP_DPP(most, v, 0x111, 0xf));        // row_shr 1, 2, 4, 8, then a row's last lane into the next row, the second row's into the others
+  v = fminf(v, LP_DPP(most, v, 0x112, 0xf));
+  v = fminf(v, LP_DPP(most, v, 0x114, 0xf));
+  v = fminf(v, LP_DPP(most, v, 0x118, 0xf));
+  v = fminf(v, LP_DPP(most, v, 0x142, 0xa));
+  v = fminf(v, LP_DPP(most, v, 0x143, 0xc));
+  if (lane == 63) p.bound[wave] = v;
+  __syncthreads();
+  float bound = -most;
+#pragma unroll
+  for (int w = 0; w < LP_WAVES; ++w) bound = fmaxf(bound, p.bound[w]);
+  return bound;
 }
-// The LP_TOP largest of all threads' keys, or all where they are fewer, in order, into p.found; keys of 0 are none.
-template <int Q> __device__ __forceinline__ void lp_pick(const lp_key (&keys)[Q], LpPick& p) {
-  const int wave = threadIdx.x >> 6;
-  lp_key best = keys[0];
+// The LP_TOP largest of the threads' numbers v[q] that are there (index(q) from 0 on) and not below the bound, by value and index, into p.found[turn]; all where
+// they are fewer.  LP_TOP of the numbers (or all) reach the bound.  p.list and p.found are zeros before, p.many too.
+template <int E, class Index> __device__ __forceinline__ void lp_pick(LpPick& p, int turn, const float (&v)[E], float bound, Index index) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  unsigned long long mask[E];
+  int total = 0, at = 0;
 #pragma unroll
-  for (int q = 1; q < Q; ++q) best = keys[q] > best ? keys[q] : best;
-  p.best[threadIdx.x] = best;
-  if (threadIdx.x < LP_WAVES) p.bound[threadIdx.x] = 0;
-  if (threadIdx.x < LP_TOP) p.found[threadIdx.x] = 0;
-  if (threadIdx.x == 0) p.many[0] = p.many[1] = 0, p.last = 0;
-  __syncthreads();
-  if (best && lp_rank(p.best + wave * 64, 64, best) == LP_TOP - 1) p.bound[wave] = best;
-  __syncthreads();
-  lp_key bound = p.bound[0];
+  for (int q = 0; q < E; ++q) {
+    mask[q] = __ballot(index(q) >= 0 && v[q] >= bound);
+    total += __builtin_popcountll(mask[q]);
+  }
+  if (total) {
+    if (lane == 0) at = atomicAdd(&p.many[turn], total);
+    at = __builtin_amdgcn_readfirstlane(at);
 #pragma unroll
-  for (int w = 1; w < LP_WAVES; ++w) bound = p.bound[w] > bound ? p.bound[w] : bound;
-  const bool near = best && best >= bound;          // LP_TOP threads of a wavefront or fewer
-  if (near) p.near[atomicAdd(&p.many[0], 1)] = best;
-  __syncthreads();
-  bool mine = false;
-  if (near) {
-    const int r = lp_rank(p.near, p.many[0], best);
-    mine = r < LP_TOP;
-    if (r == LP_TOP - 1) p.last = best;
+    for (int q = 0; q < E; ++q) {
+      const int mine = at + __builtin_amdgcn_mbcnt_hi((unsigned)(mask[q] >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask[q], 0));
+      if ((mask[q] >> lane & 1) && mine < LP_LIST) p.list[turn][mine] = lp_order(v[q], index(q));
+      at += __builtin_popcountll(mask[q]);
+    }
   }
   __syncthreads();
-  if (mine) {
+  const int n = p.many[turn];
+  if (n <= LP_LIST) {
+    // four lanes count how many are above one of them
+#pragma unroll 1
+    for (int i = threadIdx.x / 4; i < n; i += LP_THREADS / 4) {
+      const lp_key k = p.list[turn][i];
+      int r = 0;
+#pragma unroll 1
+      for (int j = 0; j < n; j += 32) {
+        lp_key other[8];
 #pragma unroll
-    for (int q = 0; q < Q; ++q)
-      if (keys[q] && keys[q] >= p.last) p.list[atomicAdd(&p.many[1], 1)] = keys[q];
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.many[1]; i += LP_THREADS) {
-    const int r = lp_rank(p.list, p.many[1], p.list[i]);
-    if (r < LP_TOP) p.found[r] = p.list[i];
+        for (int e = 0; e < 8; ++e) other[e] = p.list[turn][j + e * 4 + lane % 4];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r += other[e] > k;
+      }
+      r += LP_SWAP(r, 0xb1);
+      r += LP_SWAP(r, 0x4e);
+      if (r < LP_TOP && lane % 4 == 0) p.found[turn][r] = k;
+    }
+  } else {
+    // many equal ones, or the largest ones all in few threads: one after the other
+    lp_key last = 2.0;
+#pragma unroll 1
+    for (int t = 0; t < LP_TOP; ++t) {
+      lp_key best = 0.0;
+#pragma unroll
+      for (int q = 0; q < E; ++q) {
+        const lp_key k = index(q) >= 0 ? lp_order(v[q], index(q)) : 0.0;
+        best = k < last ? fmax(best, k) : best;
+      }
+#pragma unroll
+      for (int by = 32; by > 0; by >>= 1) best = fmax(best, __shfl_xor(best, by, 64));
+      if (lane == 0) p.wave[t & 1][wave] = best;
+      __syncthreads();
+      last = 0.0;
+#pragma unroll
+      for (int w = 0; w < LP_WAVES; ++w) last = fmax(last, p.wave[t & 1][w]);
+      if (threadIdx.x == 0) p.found[turn][t] = last;
+    }
   }
   __syncthreads();
 }
 #endif
-__device__ __forceinline__ void lp_finish(const lp_t* __restrict__ x, long long row, LpSum a, const float* segments, const long long* __restrict__ tokens,
-                                          float* __restrict__ logprob, float* __restrict__ entropy, float* __restrict__ values, long long* __restrict__ indices) {
-  const float none = -__builtin_inff(), ln = logf(a.s);
-  if (threadIdx.x == 0) {
-    const long long t = tokens[row];
-    const float v = t >= 0 && t < LP_V ? (float)x[t] : none, h = ln - a.u / a.s;
-    logprob[row] = a.s == 0.0f ? none : v - a.m - ln;
-    entropy[row] = a.s == 0.0f || h < 0.0f ? 0.0f : h;
-  }
+// `sums`: gives the row's sums.
+template <class Sums> __device__ __forceinline__ void lp_finish(const lp_t* __restrict__ x, long long row, Sums sums, const float* segments,
+                                                                const long long* __restrict__ tokens, float* __restrict__ logprob, float* __restrict__ entropy,
+                                                                float* __restrict__ values, long long* __restrict__ indices) {
+  const float none = -__builtin_inff();
+  const long long token = tokens[row];
+  const float given = token >= 0 && token < LP_V ? (float)x[token] : none;
 #if LP_TOP
   __shared__ LpPick p;
   const int o = lp_offset(x), count = ((LP_V + o + LP_VW - 1) / LP_VW + 15) / 16;          // segments of this row
-  lp_key one[LP_Q1];
+  float v[LP_E1], best = none;
 #pragma unroll
-  for (int q = 0; q < LP_Q1; ++q) {
+  for (int q = 0; q < LP_E1; ++q) {
     const int i = q * LP_THREADS + threadIdx.x;
-    one[q] = i < count ? lp_order(segments[i], i) : 0;
+    v[q] = segments[i < count ? i : 0];
+    v[q] = i < count && v[q] == v[q] ? v[q] : none;
+    best = fmaxf(best, v[q]);
   }
-  lp_pick(one, p);
-  lp_key two[LP_Q2 * LP_VW];
+  for (int i = threadIdx.x; i < 2 * (LP_LIST + 32); i += LP_THREADS) p.list[0][i] = 0.0;
+  if (threadIdx.x < 2 * LP_TOP) p.found[0][threadIdx.x] = 0.0;
+  if (threadIdx.x < 2) p.many[threadIdx.x] = 0;
+  lp_pick(p, 0, v, lp_bound(p, best), [&](int q) {
+    const int i = q * LP_THREADS + (int)threadIdx.x;
+    return i < count ? i : -1;
+  });
+  // their numbers
+  int at[LP_E2];
+  lp_vec raw[LP_E2];
 #pragma unroll
-  for (int q = 0; q < LP_Q2; ++q) {
+  for (int q = 0; q < LP_E2; ++q) {
     const int i = q * LP_THREADS + threadIdx.x;
-    const lp_key segment = i < LP_TOP * 16 ? p.found[i / 16] : 0;
-    const int at = segment ? (lp_index(segment) * 16 + i % 16) * LP_VW - o : LP_V;
-    float v[LP_VW];
-    lp_load(x, at, v);
-#pragma unroll
-    for (int j = 0; j < LP_VW; ++j) two[q * LP_VW + j] = at + j >= 0 && at + j < LP_V ? lp_order(v[j], at + j) : 0;
+    const lp_key k = i < LP_TOP * 16 ? p.found[0][i < LP_TOP * 16 ? i / 16 : 0] : 0.0;
+    at[q] = k > 0.0 ? (lp_index(k) * 16 + i % 16) * LP_VW - o : LP_V;
+    if (LP_V >= 2 * LP_VW) raw[q] = *(const lp_vec*)(x + (at[q] >= 0 && at[q] + LP_VW <= LP_V ? at[q] : (LP_VW - o) % LP_VW));
   }
-  __syncthreads();
-  lp_pick(two, p);
+  const LpSum a = sums();
+  const float ln = logf(a.s);
+  float w[LP_E2 * LP_VW];
+  best = none;
+#pragma unroll
+  for (int q = 0; q < LP_E2; ++q) {
+    float e[LP_VW];
+#pragma unroll
+    for (int j = 0; j < LP_VW; ++j) e[j] = LP_V >= 2 * LP_VW ? (float)raw[q][j] : none;
+    if (at[q] < LP_V && (LP_V < 2 * LP_VW || at[q] < 0 || at[q] + LP_VW > LP_V)) lp_edge(x, at[q], e);
+#pragma unroll
+    for (int j = 0; j < LP_VW; ++j) {
+      w[q * LP_VW + j] = e[j] == e[j] ? e[j] : none;
+      best = fmaxf(best, at[q] < LP_V ? w[q * LP_VW + j] : none);
+    }
+  }
+  // LP_TOP segments have one each that reaches the least of their largest ones; where there are not as many segments, a bound is found as for them
+  const float bound = LP_V >= LP_TOP * 16 * LP_VW ? lp_value(p.found[0][LP_TOP - 1]) : lp_bound(p, best);
+  lp_pick(p, 1, w, bound, [&](int q) {
+    const int i = at[q / LP_VW] + q % LP_VW;
+    return i < LP_V ? i : -1;                          // (or in front of the row)
+  });
   if (threadIdx.x < LP_TOP) {
-    const lp_key k = p.found[threadIdx.x];
+    const lp_key k = p.found[1][threadIdx.x];
     values[row * LP_TOP + threadIdx.x] = a.s == 0.0f ? none : lp_value(k) - a.m - ln;
     indices[row * LP_TOP + threadIdx.x] = lp_index(k);
   }
+#else
+  const LpSum a = sums();
+  const float ln = logf(a.s);
 #endif
+  if (threadIdx.x == 0) {
+    const float h = ln - a.u / a.s;
+    logprob[row] = a.s == 0.0f ? none : given - a.m - ln;
+    entropy[row] = a.s == 0.0f || h < 0.0f ? 0.0f : h;
+  }
 }
 #endif
 
@@ -223,31 +320,26 @@ void LP_NAME(const float* __restrict__ part, const lp_t* __restrict__ logits, co
              float* __restrict__ entropy, float* __restrict__ values, long long* __restrict__ indices) {
   const long long row = blockIdx.x;
   const float* mine = part + row * (LP_PARTS * 3 + (LP_TOP ? LP_SEGMENTS : 0));
-  LpSum a = {mine[0], mine[1], mine[2]};
-#pragma unroll 4
-  for (int i = 1; i < LP_PARTS; ++i) a = lp_add(a, {mine[3 * i], mine[3 * i + 1], mine[3 * i + 2]});
-  lp_finish(logits + row * LP_STRIDE, row, a, mine + LP_PARTS * 3, tokens, logprob, entropy, values, indices);
+  lp_finish(logits + row * LP_STRIDE, row, [&] { return lp_total<LP_PARTS>((const LpSum*)mine); }, mine + LP_PARTS * 3, tokens, logprob, entropy, values, indices);
 #elif LP_PARTS > 1
 void LP_NAME(const lp_t* __restrict__ logits, float* __restrict__ part) {
+  __shared__ LpSum sums[LP_WAVES];
   const long long row = blockIdx.x / LP_PARTS;
   const int i = blockIdx.x % LP_PARTS, first = i * LP_SHARE, end = first + LP_SHARE < LP_BLOCKS ? first + LP_SHARE : LP_BLOCKS;
   float* mine = part + row * (LP_PARTS * 3 + (LP_TOP ? LP_SEGMENTS : 0));
-  const LpSum a = lp_scan(logits + row * LP_STRIDE, first, end, mine + LP_PARTS * 3);
-  if (threadIdx.x == 0) {
-    mine[3 * i] = a.m;
-    mine[3 * i + 1] = a.s;
-    mine[3 * i + 2] = a.u;
-  }
+  lp_scan(logits + row * LP_STRIDE, first, end, sums, mine + LP_PARTS * 3);
+  if (threadIdx.x == 0) ((LpSum*)mine)[i] = lp_total<LP_WAVES>(sums);
 #else
 void LP_NAME(const lp_t* __restrict__ logits, const long long* __restrict__ tokens, float* __restrict__ logprob, float* __restrict__ entropy,
              float* __restrict__ values, long long* __restrict__ indices) {
+  __shared__ LpSum sums[LP_WAVES];
 #if LP_TOP
   __shared__ float segments[LP_SEGMENTS];
 #else
   float* segments = nullptr;
 #endif
   const long long row = blockIdx.x;
-  const LpSum a = lp_scan(logits + row * LP_STRIDE, 0, LP_BLOCKS, segments);
-  lp_finish(logits + row * LP_STRIDE, row, a, segments, tokens, logprob, entropy, values, indices);
+  lp_scan(logits + row * LP_STRIDE, 0, LP_BLOCKS, sums, segments);
+  lp_finish(logits + row * LP_STRIDE, row, [&] { return lp_total<LP_WAVES>(sums); }, segments, tokens, logprob, entropy, values, indices);
 #endif
 }

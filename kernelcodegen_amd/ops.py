@@ -837,7 +837,7 @@ def _token_logprobs_launch(logits, tokens, top, cfg):
         return None, None
     stride, size = logits.stride(0) if rows > 1 else 0, logits.element_size()
     params = dict(V=v, F16=_STORAGE[logits.dtype], TOP=top, STRIDE=stride, SHIFT=int((stride * size | logits.data_ptr()) % 16 != 0),
-                  **{**_token_logprobs_form(rows, v * size), **cfg})
+                  **{**_token_logprobs_form(rows, v * size, top), **cfg})
     parts = params["PARTS"]
     if rows * parts > 0x7FFFFFFF:
         raise ValueError("too many rows for one launch")
@@ -847,11 +847,18 @@ def _token_logprobs_launch(logits, tokens, top, cfg):
         return _into_last(kern.bind(grid=(rows,)), *results), None
     vectors = -(-v * size // 16) + params["SHIFT"]
     floats = rows * (3 * parts + (4 * -(-vectors // 64) if top else 0))
-    join = R.get_kernel("logprobs_join", **{**params, "THREADS": 256}).bind(grid=(rows,))
+    join = R.get_kernel("logprobs_join", **{**params, "THREADS": 512}).bind(grid=(rows,))
     return _into_last(kern.bind(grid=(rows * parts,)), ((floats,), torch.float32)), _into_last(join, *results)
 
 
-def _token_logprobs_form(rows, bytes_):
-    """Workgroups of a row."""
-    parts = 1 if rows >= 256 else max(1, min(-(-512 // rows), bytes_ // 16384))
-    return dict(PARTS=parts, THREADS=512 if parts == 1 else 256)
+def _token_logprobs_form(rows, bytes_, top):
+    """Workgroups of a row, their threads, and vectors that a lane has under way.
+
+    Fewer rows than units are cut into about 1024 parts of 8 KiB or more, and a second launch finishes them.  More have a workgroup each,
+    which is the smaller the more of them wait for their alternatives beside others that read.  Measured, in us, both launches:
+      1 row of 32000, bf16, top 5: 8 parts 7.4, 4 parts 7.5, one workgroup 7.8;  64 of 128000, fp32, top 20: 16 parts 16.6, 8 parts 18.9, one workgroup 24
+      500 of 50021, half, top 10: a workgroup of 256 threads each 19.5, of 512 19.3, 2 parts 20.7
+      2000 of 32000, bf16, top 20: of 512 threads 42, 256 40, 128 37.3;  top 5: 256 35.5, 128 33.1;  top 0: 512 28.2, 256 29.5"""
+    if rows < 256 and bytes_ >= 16384:
+        return dict(PARTS=min(-(-1024 // rows), bytes_ // 8192), THREADS=256, U=2)
+    return dict(PARTS=1, THREADS=512 if top == 0 else 128 if rows >= 1024 and bytes_ <= 1 << 18 else 256, U=2)
