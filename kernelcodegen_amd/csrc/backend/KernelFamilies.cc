@@ -1802,14 +1802,20 @@ bool emitAdapters(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::
   if (s.p["XT"] % 8) { err = s.family + ": XT must be a multiple of 16 bytes"; return false; }
   const int64_t ks = s.get("KS", 1), slots = s.get("S", 1), ns = s.get("NS", 1);
   if (ks < 1 || ks > 64 || slots < 1 || slots > 16 || ns < 1 || ns > 4096) { err = s.family + ": KS must be in [1,64], S in [1,16], NS in [1,4096]"; return false; }
+  // 16 TS tokens a tile, of the second launch 16 UT: registers hold TS times the rank's results, LDS the columns of 4 / UT wavefronts
+  const int64_t ts = s.get(up ? "UT" : "TS", 1), jt = ceilDiv(s.p["RANK"], 16);
+  if ((ts != 1 && ts != 2 && ts != 4) || (up ? (4 / ts) * s.p["RANK"] > 256 : ts * jt > 16)) {
+    err = s.family + (up ? ": UT must be 1, 2 or 4, and 4 / UT times the rank up to 256" : ": TS must be 1, 2 or 4, and TS times the rank up to 256");
+    return false;
+  }
   const char* x = s.p["F16"] ? "_Float16" : "__bf16";
   const bool y32 = s.get("Y_F32", 0) != 0, align = s.get("ALIGN", 0) != 0;
-  if (align && (s.p["YT"] * (y32 ? 4 : 2) % 16 || s.p["ZT"] * (y32 ? 4 : 2) % 16)) { err = s.family + ": ALIGN is for rows on multiples of 16 bytes"; return false; }
+  if (align && (s.p["N"] < (y32 ? 4 : 8) || s.p["YT"] * (y32 ? 4 : 2) % 16 || s.p["ZT"] * (y32 ? 4 : 2) % 16)) { err = s.family + ": ALIGN is for rows on multiples of 16 bytes"; return false; }
   Defines d;
   d.add("AD_NAME", s.name); d.add("AD_UP", up ? 1 : 0);
   for (auto key : {"N", "K", "RANK", "F16"}) d.add(std::string("AD_") + key, s.p[key]);
   for (auto key : {"XT", "YT", "ZT"}) d.add(std::string("AD_") + key, std::to_string(s.p[key]) + "LL");
-  d.add("AD_YTYPE", std::string(y32 ? "float" : x)); d.add("AD_ALIGN", align ? 1 : 0);
+  d.add("AD_YTYPE", std::string(y32 ? "float" : x)); d.add("AD_YSIZE", y32 ? 4 : 2); d.add("AD_TS", ts); d.add("AD_DEPTH", ts + jt <= 4 ? 2 : 1); d.add("AD_ALIGN", align ? 1 : 0);
   d.add("AD_SCALE", s.get("SCALES", 0) ? 1 : 0); d.add("AD_INPLACE", s.get("INPLACE", 0) ? 1 : 0);
   d.add("AD_KS", ks); d.add("AD_S", slots); d.add("AD_NS", ns);
   src = d.wrap(kTpl_adapters);

@@ -3,13 +3,14 @@
 // A row whose adapter is none of the AD_ADAPTERS is Y's.  X, A and B in 16 bits, Y and Z in 16 or 32.
 //
 // Two launches, since every column needs all of h: adapters_down leaves h in fp32, in AD_KS parts of k; adapters_up adds the parts in order.
-// Tokens come in any order, and a step's requests may have an adapter each or share one.  A tile is 16 tokens as they stand; each adapter that
+// Tokens come in any order, and a step's requests may have an adapter each or share one.  A tile is 16 AD_TS tokens as they stand (of either launch its own AD_TS); each adapter that
 // occurs in it (found by comparing lanes) is multiplied with the whole tile, and of the result only its own tokens are kept: rows of a
 // matrix product do not touch one another.  A prompt's tiles have one adapter; a decoding step's have up to 16, which AD_S workgroups share.
 // h is not rounded to 16 bits: it enters the second product as the sum of two 16-bit numbers, which the matrix instruction takes as 2 AD_RANK
 // values of k with B's columns twice.  In half precision h is brought below 2^15 by a power of two of its row.
-// Parameters: AD_NAME, AD_UP (this is adapters_up), AD_F16, AD_RANK, AD_K, AD_N, AD_XT, AD_YT, AD_ZT (strides of rows, elements), AD_YTYPE, AD_ALIGN (rows
-// of Y and Z start on multiples of 16 bytes), AD_SCALE (0: no scales), AD_INPLACE, AD_KS, AD_S, AD_NS (workgroups along N).
+// Both products have the tokens as their columns, so that a lane has four neighbouring numbers of one token in each result.
+// Parameters: AD_NAME, AD_UP (this is adapters_up), AD_F16, AD_RANK, AD_K, AD_N, AD_XT, AD_YT, AD_ZT (strides of rows, elements), AD_YTYPE, AD_YSIZE, AD_ALIGN (rows
+// of Y and Z start on multiples of 16 bytes), AD_SCALE (0: no scales), AD_INPLACE, AD_TS, AD_KS, AD_S, AD_NS (workgroups along N).
 typedef _Float16 ad_f16x8 __attribute__((ext_vector_type(8)));
 #if AD_F16
 typedef _Float16 ad_x;
@@ -19,17 +20,19 @@ typedef __bf16 ad_x;
 #define AD_MFMA(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(kcg_bf16x8, a), __builtin_bit_cast(kcg_bf16x8, b), c, 0, 0, 0)
 #endif
 typedef ad_x ad_v __attribute__((ext_vector_type(8)));
+typedef unsigned long long ad_mask;
 #define AD_JT ((AD_RANK + 15) / 16)                // tiles of the rank
+#define AD_TILE (16 * AD_TS)
 
-// Calls each(r, mask of the tile's tokens) for the adapters of a tile that are this workgroup's.
-template <class Each> __device__ __forceinline__ unsigned ad_adapters(const int* __restrict__ which, long long t0, long long T, long long adapters, int slot, Each each) {
+// Calls each(r, mask of the tile's tokens) for the adapters of a tile that are this workgroup's; returns the mask of the tokens that have one.
+template <class Each> __device__ __forceinline__ ad_mask ad_adapters(const int* __restrict__ which, long long t0, long long T, long long adapters, int slot, Each each) {
   const int lane = threadIdx.x & 63;
-  int mine = lane < 16 && t0 + lane < T ? which[t0 + lane] : -1;
-  const unsigned with = (unsigned)__ballot(mine >= 0 && mine < adapters);
-  unsigned todo = with;
+  const int mine = lane < AD_TILE && t0 + lane < T ? which[t0 + lane] : -1;
+  const ad_mask with = __ballot(mine >= 0 && mine < adapters);
+  ad_mask todo = with;
   for (int n = 0; todo; ++n) {
-    const int r = __builtin_amdgcn_readlane(mine, __builtin_ctz(todo));
-    const unsigned same = (unsigned)__ballot(mine == r);
+    const int r = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
+    const ad_mask same = __ballot(mine == r);
     todo &= ~same;
     if (n % AD_S == slot) each(r, same);
   }
@@ -37,143 +40,251 @@ template <class Each> __device__ __forceinline__ unsigned ad_adapters(const int*
 }
 
 #if !AD_UP
+// A wavefront has its own part of k and brings it in whole lines, 64 k of eight rows a load: through LDS rows of its own, 16 bytes apart from a multiple
+// of 128, from where a lane takes the chunks that the product wants (chunk l / 16 of row l % 16; straight from memory, neighbouring lanes touch
+// different lines).
+#define AD_STEPS ((AD_K + 63) / 64)
+#define AD_SHARE ((AD_STEPS + 4 * AD_KS - 1) / (4 * AD_KS))       // of a wavefront
+#define AD_ROWS (16 * (AD_TS + AD_JT))                            // of X, then of A
+#define AD_PITCH 144
 extern "C" __global__ __launch_bounds__(256)
 void AD_NAME(const ad_x* __restrict__ X, const ad_x* __restrict__ A, const int* __restrict__ which, long long T, long long adapters, float* __restrict__ part) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int ks = blockIdx.x % AD_KS, slot = blockIdx.x / AD_KS % AD_S;
-  const long long t0 = (long long)(blockIdx.x / (AD_KS * AD_S)) * 16;
-  __shared__ kcg_f32x4 red[4][AD_JT][64];
-  const long long t = t0 + i < T ? t0 + i : T - 1;
-  ad_adapters(which, t0, T, adapters, slot, [&](int r, unsigned same) {
-    kcg_f32x4 acc[AD_JT];
+  const long long t0 = (long long)(blockIdx.x / (AD_KS * AD_S)) * AD_TILE;
+  union Shared {
+    __attribute__((aligned(16))) unsigned char rows[4][AD_ROWS * AD_PITCH];
+    kcg_f32x4 red[4][AD_TS * AD_JT][64];
+  };
+  __shared__ Shared sh;
+  unsigned char* mine = sh.rows[wave];
+  const ad_x* x[AD_TS * 2];
 #pragma unroll
-    for (int j = 0; j < AD_JT; ++j) acc[j] = kcg_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const ad_x* x = X + t * AD_XT;
+  for (int c = 0; c < AD_TS * 2; ++c) {
+    const long long t = t0 + c * 8 + lane / 8;
+    x[c] = X + (t < T ? t : T - 1) * AD_XT;
+  }
+  const int first = (ks * 4 + wave) * AD_SHARE, end = first + AD_SHARE < AD_STEPS ? first + AD_SHARE : AD_STEPS;
+  ad_adapters(which, t0, T, adapters, slot, [&](int r, ad_mask same) {
+    kcg_f32x4 acc[AD_TS][AD_JT];
+#pragma unroll
+    for (int t = 0; t < AD_TS; ++t)
+#pragma unroll
+      for (int j = 0; j < AD_JT; ++j) acc[t][j] = kcg_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const ad_x* a = A + (long long)r * AD_RANK * AD_K;
-    for (int s = ks * 4 + wave; s < (AD_K + 31) / 32; s += AD_KS * 4) {
-      const int k = s * 32 + g * 8;
-      const bool in = AD_K % 32 == 0 || k < AD_K;
-      kcg_u32x4 b = *(const kcg_u32x4*)(x + (in ? k : 0));
-      if (!in) b = kcg_u32x4{0, 0, 0, 0};
+    kcg_u32x4 next[AD_DEPTH][AD_ROWS / 8];
+    auto fetch = [&](int s, kcg_u32x4 (&to)[AD_ROWS / 8]) {
+      int k = (s < AD_STEPS ? s : 0) * 64 + lane % 8 * 8;
+      if (AD_K % 64) k = k < AD_K ? k : 0;
 #pragma unroll
-      for (int j = 0; j < AD_JT; ++j) {
-        const int row = j * 16 + i < AD_RANK ? j * 16 + i : AD_RANK - 1;
-        kcg_u32x4 w = *(const kcg_u32x4*)(a + (long long)row * AD_K + (in ? k : 0));
-        if (!in) w = kcg_u32x4{0, 0, 0, 0};
-        acc[j] = AD_MFMA(w, b, acc[j]);
+      for (int c = 0; c < AD_TS * 2; ++c) to[c] = *(const kcg_u32x4*)(x[c] + k);
+#pragma unroll
+      for (int c = 0; c < AD_JT * 2; ++c) {
+        const int row = c * 8 + lane / 8;
+        to[AD_TS * 2 + c] = *(const kcg_u32x4*)(a + (AD_RANK % 16 && row >= AD_RANK ? AD_RANK - 1 : row) * (long long)AD_K + k);
+      }
+    };
+#pragma unroll
+    for (int d = 0; d < AD_DEPTH; ++d) fetch(first + d, next[d]);
+#pragma unroll 1
+    for (int s0 = first; s0 < end; s0 += AD_DEPTH) {
+#pragma unroll
+      for (int d = 0; d < AD_DEPTH; ++d) {
+        const int s = s0 + d;
+        // (k behind the last, and steps that are another wavefront's, take part as zeros)
+        const bool in = s < end && (AD_K % 64 == 0 || s * 64 + lane % 8 * 8 < AD_K);
+#pragma unroll
+        for (int c = 0; c < AD_ROWS / 8; ++c)
+          *(kcg_u32x4*)(mine + (c * 8 + lane / 8) * AD_PITCH + lane % 8 * 16) = in ? next[d][c] : kcg_u32x4{0, 0, 0, 0};
+        fetch(s + AD_DEPTH, next[d]);
+        __builtin_amdgcn_wave_barrier();        // (a wavefront's own accesses to LDS are carried out in order)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          kcg_u32x4 b[AD_TS];
+#pragma unroll
+          for (int t = 0; t < AD_TS; ++t) b[t] = *(const kcg_u32x4*)(mine + (t * 16 + i) * AD_PITCH + (h * 4 + g) * 16);
+#pragma unroll
+          for (int j = 0; j < AD_JT; ++j) {
+            const kcg_u32x4 w = *(const kcg_u32x4*)(mine + ((AD_TS + j) * 16 + i) * AD_PITCH + (h * 4 + g) * 16);
+#pragma unroll
+            for (int t = 0; t < AD_TS; ++t) acc[t][j] = AD_MFMA(w, b[t], acc[t][j]);
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
       }
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < AD_JT; ++j) red[wave][j][lane] = acc[j];
+    for (int t = 0; t < AD_TS; ++t)
+#pragma unroll
+      for (int j = 0; j < AD_JT; ++j) sh.red[wave][t * AD_JT + j][lane] = acc[t][j];
     __syncthreads();
-    for (int j = wave; j < AD_JT; j += 4) {
-      const kcg_f32x4 sum = red[0][j][lane] + red[1][j][lane] + red[2][j][lane] + red[3][j][lane];
-      const int at = j * 16 + g * 4;
-      if ((same >> i & 1) && at < AD_RANK) *(kcg_f32x4*)(part + ((long long)ks * T + t) * AD_RANK + at) = sum;
+    for (int u = wave; u < AD_TS * AD_JT; u += 4) {
+      const kcg_f32x4 sum = sh.red[0][u][lane] + sh.red[1][u][lane] + sh.red[2][u][lane] + sh.red[3][u][lane];
+      const int row = u / AD_JT * 16 + i, at = u % AD_JT * 16 + g * 4;
+      if ((same >> row & 1) && at < AD_RANK) *(kcg_f32x4*)(part + ((long long)ks * T + t0 + row) * AD_RANK + at) = sum;
     }
+    __syncthreads();
   });
 }
 #else
 typedef AD_YTYPE ad_y;
-typedef ad_y ad_y4 __attribute__((ext_vector_type(4)));
+#define AD_C (16 / AD_YSIZE)                       // columns of a lane, which lie beside one another: 16 bytes
+#define AD_COLS (16 * AD_C)                        // and of a wavefront
+typedef ad_y ad_yv __attribute__((ext_vector_type(AD_C)));
 #define AD_CHUNKS (AD_RANK / 8)
 #define AD_STEPS ((2 * AD_CHUNKS + 3) / 4)         // products: both halves of h
+#define AD_HALF (AD_CHUNKS % 4 == 0 ? AD_STEPS / 2 : AD_STEPS)    // of which so many have other columns of B
+#define AD_GROUPS (4 / AD_TS)                       // wavefronts beside one another along N; AD_TS of them have 16 tokens each
+#define AD_STEP (AD_GROUPS * AD_COLS)              // columns of a workgroup
+#define AD_PITCH (AD_CHUNKS % 2 ? AD_RANK * 2 : AD_RANK * 2 + 16)  // of a row of B in LDS: an odd number of 16 bytes
+#define AD_LOADS ((AD_STEP * AD_CHUNKS + 255) / 256)
 
-// Adds to 16 columns of a row.
-__device__ __forceinline__ void ad_put(const ad_y* __restrict__ y, ad_y* __restrict__ z, int n, const kcg_f32x4 (&add)[4]) {
-  if (AD_ALIGN && n + 16 <= AD_N) {
-    ad_y4 v[4];
+// Columns n to n + AD_C of a row.
+__device__ __forceinline__ ad_yv ad_get(const ad_y* y, int n) {
+  if (AD_ALIGN) return *(const ad_yv*)(y + (n + AD_C <= AD_N ? n : 0));
+  ad_yv v;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = *(const ad_y4*)(y + n + q * 4);
+  for (int e = 0; e < AD_C; ++e) v[e] = y[n + e < AD_N ? n + e : AD_N - 1];
+  return v;
+}
+__device__ __forceinline__ void ad_put(const ad_y* y, ad_y* z, int n, ad_yv v, const float (&add)[AD_C]) {
+  if (AD_ALIGN && n + AD_C <= AD_N) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[q][e] = (ad_y)((float)v[q][e] + add[q][e]);
-      *(ad_y4*)(z + n + q * 4) = v[q];
-    }
+    for (int e = 0; e < AD_C; ++e) v[e] = (ad_y)((float)v[e] + add[e]);
+    *(ad_yv*)(z + n) = v;
   } else {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + q * 4 + e < AD_N) z[n + q * 4 + e] = (ad_y)((float)y[n + q * 4 + e] + add[q][e]);
+    for (int e = 0; e < AD_C; ++e)
+      if (n + e < AD_N) z[n + e] = (ad_y)((float)(AD_ALIGN ? y[n + e] : v[e]) + add[e]);
   }
 }
 
+// A wavefront takes AD_COLS columns of 16 tokens at a time: lane l gets columns (l % 16) AD_C on of tokens 4 (l / 16) to 4 (l / 16) + 3, whole lines of Y with
+// its neighbours, when the columns of product q are every AD_C-th from q on.  B comes for the whole workgroup, in whole lines, and goes through LDS,
+// rows put into the order in which the products take them; the next columns' B and Y are under way meanwhile.
 extern "C" __global__ __launch_bounds__(256)
 void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restrict__ B, const int* __restrict__ which, const float* __restrict__ scale, long long T,
              long long adapters, ad_y* Z) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int sub = wave % AD_TS, group = wave / AD_TS;
   const int ns = blockIdx.x % AD_NS, slot = blockIdx.x / AD_NS % AD_S;
-  const long long t0 = (long long)(blockIdx.x / (AD_NS * AD_S)) * 16;
-  const long long t = t0 + i < T ? t0 + i : T - 1;
-  const ad_y* y = Y + t * AD_YT;
-  ad_y* z = Z + t * AD_ZT;
-  const unsigned with = ad_adapters(which, t0, T, adapters, slot, [&](int r, unsigned same) {
-    float h[AD_STEPS][8], most = 0.0f;
+  const long long t0 = (long long)(blockIdx.x / (AD_NS * AD_S)) * AD_TILE, tw = t0 + sub * 16;
+  __shared__ __attribute__((aligned(16))) unsigned char rows[AD_STEP * AD_PITCH];
+  long long row[4];
 #pragma unroll
-    for (int s = 0; s < AD_STEPS; ++s) {
-      const int c = (s * 4 + g) % AD_CHUNKS * 8;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) h[s][e] = 0.0f;
-#pragma unroll
-      for (int p = 0; p < AD_KS; ++p) {
-        const kcg_f32x4* at = (const kcg_f32x4*)(part + ((long long)p * T + t) * AD_RANK + c);
-        const kcg_f32x4 one = at[0], two = at[1];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) h[s][e] += one[e], h[s][4 + e] += two[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) most = fmaxf(most, __builtin_fabsf(h[s][e]));
-    }
-    float up = 1.0f, down = 1.0f;
-    if (AD_F16) {
-      most = fmaxf(most, __shfl_xor(most, 16, 64));
-      most = fmaxf(most, __shfl_xor(most, 32, 64));
-      int e = (int)(__builtin_bit_cast(unsigned, most) >> 23) - 127;
-      e = e < -100 ? -100 : e > 126 ? 126 : e;
-      up = __builtin_bit_cast(float, (unsigned)(127 + 14 - e) << 23);
-      down = __builtin_bit_cast(float, (unsigned)(127 - 14 + e) << 23);
-    }
-    kcg_u32x4 f[AD_STEPS];
-#pragma unroll
-    for (int s = 0; s < AD_STEPS; ++s) {
-      const int q = s * 4 + g;
-      ad_v v;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = h[s][e] * up;
-        const ad_x high = (ad_x)a;
-        const float left = a - (float)high;
-        v[e] = q < AD_CHUNKS ? high : q < 2 * AD_CHUNKS && left - left == 0.0f ? (ad_x)left : (ad_x)0.0f;
-      }
-      f[s] = __builtin_bit_cast(kcg_u32x4, v);
-    }
-    const float by = (AD_SCALE ? scale[r] : 1.0f) * down;
+  for (int e = 0; e < 4; ++e) row[e] = tw + g * 4 + e < T ? tw + g * 4 + e : T - 1;
+  const ad_mask with = ad_adapters(which, t0, T, adapters, slot, [&](int r, ad_mask same) {
     const ad_x* b = B + (long long)r * AD_N * AD_RANK;
-    for (int nb = (ns * 4 + wave) * 64; nb < AD_N; nb += AD_NS * 256) {
-      kcg_f32x4 acc[4];
+    const unsigned mine = (unsigned)(same >> (sub * 16)) & 0xffffu;
+    kcg_u32x4 w[AD_LOADS];
+    ad_yv v[4];
+    auto fetch = [&](int nb) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int n = nb + (i >> 2) * 16 + q * 4 + (i & 3);
-        const ad_x* row = b + (long long)(n < AD_N ? n : AD_N - 1) * AD_RANK;
-        acc[q] = kcg_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int s = 0; s < AD_STEPS; ++s) {
-          const int c = s * 4 + g;
-          kcg_u32x4 w = *(const kcg_u32x4*)(row + c % AD_CHUNKS * 8);
-          if (c >= 2 * AD_CHUNKS) w = kcg_u32x4{0, 0, 0, 0};
-          acc[q] = AD_MFMA(w, f[s], acc[q]);
-        }
-        acc[q] *= by;
+      for (int c = 0; c < AD_LOADS; ++c) {
+        const int u = c * 256 + threadIdx.x, n = nb + u / AD_CHUNKS;
+        w[c] = *(const kcg_u32x4*)(b + (n < AD_N ? (long long)n * AD_RANK + u % AD_CHUNKS * 8 : 0));
       }
-      if (same >> i & 1) ad_put(y, z, nb + g * 16, acc);
+      if (mine) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = ad_get(Y + row[e] * AD_YT, nb + group * AD_COLS + i * AD_C);
+      }
+    };
+    fetch(ns * AD_STEP);
+    // h of this wavefront's tokens in two numbers of 16 bits
+    kcg_u32x4 f[AD_STEPS];
+    kcg_f32x4 times = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (mine) {
+      const long long t = tw + i < T ? tw + i : T - 1;
+      float h[AD_STEPS][8], most = 0.0f;
+#pragma unroll
+      for (int s = 0; s < AD_STEPS; ++s) {
+        const int c = (s * 4 + g) % AD_CHUNKS * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[s][e] = 0.0f;
+#pragma unroll
+        for (int p = 0; p < AD_KS; ++p) {
+          const kcg_f32x4* at = (const kcg_f32x4*)(part + ((long long)p * T + t) * AD_RANK + c);
+          const kcg_f32x4 one = at[0], two = at[1];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) h[s][e] += one[e], h[s][4 + e] += two[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, __builtin_fabsf(h[s][e]));
+      }
+      float up = 1.0f, down = AD_SCALE ? scale[r] : 1.0f;
+      if (AD_F16) {
+        most = fmaxf(most, __shfl_xor(most, 16, 64));
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        int e = (int)(__builtin_bit_cast(unsigned, most) >> 23) - 127;
+        e = e < -100 ? -100 : e > 126 ? 126 : e;
+        up = __builtin_bit_cast(float, (unsigned)(127 + 14 - e) << 23);
+        down *= __builtin_bit_cast(float, (unsigned)(127 - 14 + e) << 23);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) times[e] = AD_F16 ? __shfl(down, g * 4 + e, 64) : down;
+#pragma unroll
+      for (int s = 0; s < AD_STEPS; ++s) {
+        const int q = s * 4 + g;
+        ad_v o;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float a = h[s][e] * up;
+          const ad_x high = (ad_x)a;
+          const float left = a - (float)high;
+          o[e] = q < AD_CHUNKS ? high : q < 2 * AD_CHUNKS && left - left == 0.0f ? (ad_x)left : (ad_x)0.0f;
+        }
+        f[s] = __builtin_bit_cast(kcg_u32x4, o);
+      }
     }
+#pragma unroll 1
+    for (int nb = ns * AD_STEP; nb < AD_N; nb += AD_NS * AD_STEP) {
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < AD_LOADS; ++c) {
+        const int u = c * 256 + threadIdx.x, n = u / AD_CHUNKS;       // row n % AD_C of lane n / AD_C % 16 in product n % AD_C
+        if (AD_STEP * AD_CHUNKS % 256 == 0 || n < AD_STEP)
+          *(kcg_u32x4*)(rows + (n / AD_COLS * AD_COLS + n % AD_C * 16 + n % AD_COLS / AD_C) * AD_PITCH + u % AD_CHUNKS * 16) = w[c];
+      }
+      ad_yv now[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) now[e] = v[e];
+      __syncthreads();
+      if (nb + AD_NS * AD_STEP < AD_N) fetch(nb + AD_NS * AD_STEP);
+      if (mine) {
+        kcg_f32x4 acc[AD_C];
+#pragma unroll
+        for (int q = 0; q < AD_C; ++q) {
+          const unsigned char* at = rows + (group * AD_COLS + q * 16 + i) * AD_PITCH;
+          acc[q] = kcg_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          kcg_u32x4 c[AD_HALF];
+#pragma unroll
+          for (int s = 0; s < AD_HALF; ++s) {
+            c[s] = *(const kcg_u32x4*)(at + (s * 4 + g) % AD_CHUNKS * 16);
+            if (s * 4 + 3 >= 2 * AD_CHUNKS && s * 4 + g >= 2 * AD_CHUNKS) c[s] = kcg_u32x4{0, 0, 0, 0};        // (k behind both halves)
+          }
+#pragma unroll
+          for (int s = 0; s < AD_STEPS; ++s) acc[q] = AD_MFMA(f[s], c[s % AD_HALF], acc[q]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float add[AD_C];
+#pragma unroll
+          for (int q = 0; q < AD_C; ++q) add[q] = times[e] * acc[q][e];
+          if (mine >> (g * 4 + e) & 1) ad_put(Y + row[e] * AD_YT, Z + row[e] * AD_ZT, nb + group * AD_COLS + i * AD_C, now[e], add);
+        }
+      }
+    }
+    __syncthreads();
   });
-  if (!AD_INPLACE && slot == 0 && !(with >> i & 1) && t0 + i < T) {
-    const kcg_f32x4 none[4] = {};
-    for (int nb = (ns * 4 + wave) * 64; nb < AD_N; nb += AD_NS * 256) ad_put(y, z, nb + g * 16, none);
+  if (!AD_INPLACE && slot == 0) {
+#pragma unroll 1
+    for (int e = 0; e < 4; ++e) {
+      if ((with >> (sub * 16 + g * 4 + e) & 1) || tw + g * 4 + e >= T) continue;
+      const float none[AD_C] = {};
+      for (int n = ns * AD_STEP + group * AD_COLS + i * AD_C; n < AD_N; n += AD_NS * AD_STEP)
+        ad_put(Y + row[e] * AD_YT, Z + row[e] * AD_ZT, n, ad_get(Y + row[e] * AD_YT, n), none);
+    }
   }
 }
 #endif

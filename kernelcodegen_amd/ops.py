@@ -724,7 +724,7 @@ def add_adapters(y, x, a, b, which, scale=None, inplace=False, **cfg):
     rank], of x's type and contiguous; which: int32 [tokens], in any order, each adapter for any number of tokens; scale: fp32 [adapters], None for 1.
     Rank and K are multiples of 8, the rank up to 256 (a smaller one is filled up with zeros).  Rows of x and y may lie apart.  Returns a
     contiguous tensor of y's type, or y itself (inplace); a token whose adapter is none of them (-1) keeps its row of y.  Sums are
-    fp32, a[r] x[t] enters the second product with 16 bits or more, and the sum with y is rounded once.  `cfg` overrides kernel parameters (KS, S, NS)."""
+    fp32, a[r] x[t] enters the second product with 16 bits or more, and the sum with y is rounded once.  `cfg` overrides kernel parameters (TS, UT, KS, S, NS)."""
     inplace = bool(inplace)
     key = ("add_adapters", R.signature(y, x, a, b, which, scale), inplace)
     hit = None if cfg else _bound.get(key)
@@ -768,30 +768,39 @@ def _add_adapters_launch(y, x, a, b, which, scale, inplace, cfg):
         raise ValueError("rows of y must not overlap")
     if tokens > 0x7FFFFF00:
         raise ValueError("too many tokens for one launch")
-    if not cfg.keys() <= {"KS", "S", "NS"}:
+    if not cfg.keys() <= {"TS", "UT", "KS", "S", "NS"}:
         raise ValueError("unknown kernel parameters")
     if not tokens:
         return None, None
     yt = y.stride(0) if tokens > 1 else 0
     zt, size = yt if inplace else n, y.element_size()
     params = dict(N=n, K=k, RANK=rank, F16=int(x.dtype == torch.float16), Y_F32=int(y.dtype == torch.float32), XT=x.stride(0) if tokens > 1 else 0, YT=yt, ZT=zt,
-                  ALIGN=int((y.data_ptr() | yt * size | zt * size) % 16 == 0), SCALES=int(scale is not None), INPLACE=int(inplace),
-                  **{**_add_adapters_form(tokens, adapters, n, k, rank), **cfg})
-    tiles = -(-tokens // 16) * params["S"]
-    if tiles * max(params["KS"], params["NS"]) > 0x7FFFFFFF:
+                  ALIGN=int(n * size >= 16 and (y.data_ptr() | yt * size | zt * size) % 16 == 0), SCALES=int(scale is not None), INPLACE=int(inplace),
+                  **{**_add_adapters_form(tokens, adapters, n, k, rank, 256 // size), **cfg})
+    grids = [-(-tokens // (16 * params[tile])) * params["S"] * params[by] for tile, by in (("TS", "KS"), ("UT", "NS"))]
+    if max(grids) > 0x7FFFFFFF:
         raise ValueError("too many tokens for one launch")
-    down = R.get_kernel("adapters_down", **params).bind(grid=(tiles * params["KS"],))
-    up = R.get_kernel("adapters_up", **params).bind(grid=(tiles * params["NS"],))
+    down, up = (R.get_kernel(family, **params).bind(grid=(grid,)) for family, grid in zip(("adapters_down", "adapters_up"), grids))
     return _into_last(down, ((params["KS"], tokens, rank), torch.float32)), up if inplace else _into_last(up, ((tokens, n), y.dtype))
 
 
-def _add_adapters_form(tokens, adapters, n, k, rank):
-    """Workgroups for the adapters of a tile of 16 tokens (S), for parts of k (KS) and of the columns (NS)."""
-    tiles = -(-tokens // 16)
-    slots = min(16, tokens, adapters) if tiles <= 16 else 1
-    ks = max(1, min(8, 512 // (tiles * slots), k // 512))
-    ns = max(1, min(-(-n // 256), 1024 // (tiles * slots)))
-    return dict(S=slots, KS=ks, NS=ns)
+def _add_adapters_form(tokens, adapters, n, k, rank, columns):
+    """Tokens of a tile (16 TS, and 16 UT in the second launch), workgroups for a tile's adapters (S), for parts of k (KS) and of the columns (NS).
+
+    Up to 1024 tokens may be a decoding step's, with an adapter each: tiles of 16, whose adapters several workgroups share out.  More are prompts'.
+    Parts of k fill the part in the first launch and are read by all workgroups of the second.  Measured, in us, first and second launch:
+      64 tokens, 40 adapters of rank 16, N = K = 4096: k in 4 parts 4.9 and 5.8, in 8 4.2 and 7.2;  4 workgroups along N instead of 8: 6.2
+      5000 tokens, rank 64: 16 a tile, k in 2 parts 12.5 and 20.2, in one 20 and 17.1;  64 a tile, in 4 parts 15.6 and 26;  32 workgroups along N
+      (one pass each) 17.1, 8: 18.7;  16 tokens a tile in the second launch 41, 32 tokens 32, 64 27
+      2600 tokens, rank 32, K 4096, N 11008, fp32: k in 2 parts 13 and 47.7, in one 17.2 and 46.9;  43 workgroups along N 48.6, 172 62, 8 86"""
+    ts = 2 if tokens > 1024 and 64 < rank <= 128 else 1
+    ut = 4 if tokens > 1024 or rank > 128 else 2 if rank > 64 else 1
+    tiles, wide = -(-tokens // (16 * ts)), -(-tokens // (16 * ut))
+    slots = min(16 if tiles <= 16 else 4, tokens, adapters) if tokens <= 1024 else 1
+    ks = max(1, min(8, (256 if tokens <= 1024 else 768) // (tiles * slots), k // 512))
+    blocks = -(-n // (columns * 4 // ut))
+    each = max(1, blocks * wide * slots // 2048)
+    return dict(TS=ts, UT=ut, S=slots, KS=ks, NS=-(-blocks // each))
 
 
 def token_logprobs(logits, tokens, top=0, **cfg):

@@ -233,6 +233,18 @@ def test_add_adapters_of_rows_that_lie_apart(dtype, inplace):
         assert torch.equal(all_y, kept)
 
 
+@pytest.mark.parametrize("dtype,out", [("bf16", "bf16"), ("f16", "f32")])
+@pytest.mark.parametrize("ts,ut,rank", [(1, 1, 16), (2, 2, 8), (4, 4, 24), (4, 1, 64), (2, 2, 128), (4, 2, 16), (1, 4, 256), (1, 1, 40)])
+@pytest.mark.parametrize("form", [dict(KS=1, S=1, NS=1), dict(KS=5, S=3, NS=2), dict(KS=8, S=16, NS=7)])
+def test_add_adapters_forms(dtype, out, ts, ut, rank, form):
+    """Tiles whose adapters are shared out between workgroups, or one workgroup's; parts of k, the last of which are empty."""
+    y, x, a, b, which, scale = adapters_case(ts + rank, 150, 328, 1032, rank, 9, dtype, out)
+    which[40:120] = 4
+    check_adapters(ops.add_adapters(y, x, a, b, which, scale, TS=ts, UT=ut, **form), y, x, a, b, which, scale)
+    got = ops.add_adapters(y.clone(), x, a, b, which, None, inplace=True, TS=ts, UT=ut, **form)
+    check_adapters(got, y, x, a, b, which, None)
+
+
 def test_add_adapters_keeps_what_half_precision_would_lose():
     """x a of 2^20 and of 2^-30, which half precision holds no numbers for."""
     for spread, b_spread in ((2.0 ** 13, 2.0 ** -14), (2.0 ** -12, 1.0)):
@@ -405,7 +417,7 @@ def test_refusals():
              dict(x=x[:, :56]), dict(x=x[:2]), dict(a=a[:1]), dict(b=b[:1]), dict(b=b[:, :39]), dict(a=a[:0], b=b[:0], scale=scale[:0]), dict(which=which.long()), dict(which=which[:2]),
              dict(which=which.cpu()), dict(scale=scale[:1]), dict(scale=scale.half()), dict(scale=scale.cpu()), dict(x=x.cpu()), dict(a=a.cpu()), dict(y=y.cpu()), dict(a=a[:, :4], b=b[..., :4]),
              dict(a=a[:, :4].contiguous(), b=b[..., :4].contiguous()), dict(a=a.transpose(1, 2)), dict(x=x[:, :36].contiguous(), a=a[..., :36].contiguous()), dict(x=x.t().contiguous().t()),
-             dict(y=y.t().contiguous().t()), dict(x=torch.ones(200, device="cuda", dtype=torch.half)[4:196].view(3, 64)), dict(y=y[:1].expand(3, 40), inplace=True), dict(KS=65), dict(PARTS=2), dict(S=0)])
+             dict(y=y.t().contiguous().t()), dict(x=torch.ones(200, device="cuda", dtype=torch.half)[4:196].view(3, 64)), dict(y=y[:1].expand(3, 40), inplace=True), dict(KS=65), dict(PARTS=2), dict(S=0), dict(TS=3)])
     logits, tokens = torch.ones((3, 50), device="cuda"), ints([1, 2, 3], torch.int64)
     refused(ops.token_logprobs, dict(logits=logits, tokens=tokens, top=3),
             [dict(logits=logits.double()), dict(logits=logits.cpu()), dict(logits=logits[0]), dict(logits=logits[:2]), dict(logits=logits[:, :0], top=0), dict(logits=logits.t().contiguous().t()),
