@@ -17,7 +17,8 @@
 //   neighbours (CW_PAIRS):                   (x_2i, x_2i+1) -> the same
 // with c and s of row `position` of the table.  What becomes of a key jumps where 8 bits do, so it has to be the formula's: the two products
 // are exact in fp64 and their sum is rounded there once; on the way to fp32 what is cut off leaves its trace in the last bit (rounding to odd), so the
-// rounding to 8 bits is that of the 53-bit number, and so is the comparison with 448 that gives the scale.  Wavefronts behind those of the cache take
+// rounding to 8 bits is that of the 53-bit number, and so is the comparison with 448 that gives the scale.  Queries, whose results have 16 or 32
+// bits, are summed in fp32 (all of it in fp64: 7200 tokens of 32 query heads 79 us, this way 50).  Wavefronts behind those of the cache take
 // a token's queries, CW_QN passes of CW_RPP heads for one reading of c and s.
 // Measured, 8 heads of 128: 64 tokens of a page each 2.9 us (an empty launch 1.7); 9000 tokens of whole pages, half precision, 12.5 us, 4.4 TB/s.
 // Parameters: CW_NAME, CW_H, CW_D, CW_PAGE, CW_T (input type), CW_ESIZE, CW_WIN, strides as in cache_attention: CW_KP .. CW_VH (bytes), CW_XKT
@@ -84,26 +85,28 @@ __device__ __forceinline__ CwTurn cw_turn(const float* __restrict__ table, int p
   }
   return w;
 }
-// To fp32: to odd, where another rounding follows, or to the nearest.
-template <bool ODD> __device__ __forceinline__ float cw_round(double v) {
-  if (!ODD) return (float)v;
+// To fp32, to odd.
+__device__ __forceinline__ float cw_odd(double v) {
   const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
   const unsigned low = (unsigned)b, cut = (low & 0xe0000000u) | ((low & 0x1fffffffu) ? 0x20000000u : 0u);
   return (float)__builtin_bit_cast(double, (b & 0xffffffff00000000ULL) | cut);
 }
-// x: the chunk; y: its partner.
-template <bool ODD> __device__ __forceinline__ void cw_apply(const CwTurn& w, const cw_x8& x, const cw_x8& y, int c, float (&f)[8]) {
+// The chunk x, whose partner is y, turned: with a sum in fp64 and rounded to odd (KEY), or in fp32.
+template <bool KEY> __device__ __forceinline__ void cw_apply(const CwTurn& w, const cw_x8& x, const cw_x8& y, int c, float (&f)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    double v;
-    if (CW_PAIRS) {
-      const double co = w.t[0][i / 2], si = w.t[2][i / 2], a = (float)x[i], b = (float)x[i ^ 1];
-      v = a * co + (i & 1 ? b * si : -(b * si));
+    const float co = w.t[CW_PAIRS ? 0 : i / 4][CW_PAIRS ? i / 2 : i % 4], si = w.t[CW_PAIRS ? 2 : 2 + i / 4][CW_PAIRS ? i / 2 : i % 4];
+    const float a = (float)x[i], b = (float)(CW_PAIRS ? x[i ^ 1] : y[i]);
+    const bool first = CW_PAIRS ? i % 2 == 0 : c < CW_HALF;
+    float v;
+    if (KEY) {
+      const double p = (double)b * si;
+      v = cw_odd((double)a * co + (first ? -p : p));
     } else {
-      const double co = w.t[i / 4][i % 4], si = w.t[2 + i / 4][i % 4], a = (float)x[i], b = (float)y[i];
-      v = a * co + (c < CW_HALF ? -(b * si) : b * si);
+      const float p = b * si;
+      v = __builtin_fmaf(a, co, first ? -p : p);
     }
-    f[i] = w.turned ? w.lost ? __builtin_nanf("") : cw_round<ODD>(v) : (float)x[i];
+    f[i] = w.turned ? w.lost ? __builtin_nanf("") : v : a;
   }
 }
 #endif
@@ -141,7 +144,7 @@ void CW_NAME(const cw_t* __restrict__ k, const cw_t* __restrict__ v, unsigned ch
     for (int j = 0; j < CW_QN; ++j) {
       const int h = h0 + j * CW_RPP;
       float f[8];
-      cw_apply<CW_ESIZE == 2>(w, a[j], b[CW_PAIRS ? 0 : j], c, f);
+      cw_apply<false>(w, a[j], b[CW_PAIRS ? 0 : j], c, f);
       cw_x8 o;
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] = (cw_t)f[i];
@@ -206,8 +209,11 @@ void CW_NAME(const cw_t* __restrict__ k, const cw_t* __restrict__ v, unsigned ch
       if (values) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) held[j][i] = (float)raws[j][i];
-      } else {
+      } else if (j == 0 || j * CW_RPP < run) {
         cw_apply<true>(turns[j], raws[j], others[j], c, held[j]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) held[j][i] = 0.0f;
       }
     // a row that registers do not hold
     auto again = [&](int r, float (&f)[8]) {
