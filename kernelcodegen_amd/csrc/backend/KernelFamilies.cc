@@ -1810,12 +1810,12 @@ bool emitAdapters(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::
   }
   const char* x = s.p["F16"] ? "_Float16" : "__bf16";
   const bool y32 = s.get("Y_F32", 0) != 0, align = s.get("ALIGN", 0) != 0;
-  if (align && (s.p["N"] < (y32 ? 4 : 8) || s.p["YT"] * (y32 ? 4 : 2) % 16 || s.p["ZT"] * (y32 ? 4 : 2) % 16)) { err = s.family + ": ALIGN is for rows on multiples of 16 bytes"; return false; }
+  if (align && (s.p["YT"] * (y32 ? 4 : 2) % 16 || s.p["ZT"] * (y32 ? 4 : 2) % 16)) { err = s.family + ": ALIGN is for rows on multiples of 16 bytes"; return false; }
   Defines d;
   d.add("AD_NAME", s.name); d.add("AD_UP", up ? 1 : 0);
   for (auto key : {"N", "K", "RANK", "F16"}) d.add(std::string("AD_") + key, s.p[key]);
   for (auto key : {"XT", "YT", "ZT"}) d.add(std::string("AD_") + key, std::to_string(s.p[key]) + "LL");
-  d.add("AD_YTYPE", std::string(y32 ? "float" : x)); d.add("AD_YSIZE", y32 ? 4 : 2); d.add("AD_TS", ts); d.add("AD_DEPTH", ts + jt <= 4 ? 2 : 1); d.add("AD_ALIGN", align ? 1 : 0);
+  d.add("AD_YTYPE", std::string(y32 ? "float" : x)); d.add("AD_YSIZE", y32 ? 4 : 2); d.add("AD_PIECES", y32 && !s.p["F16"] ? 3 : 2); d.add("AD_TS", ts); d.add("AD_DEPTH", ts + jt <= 4 ? 2 : 1); d.add("AD_ALIGN", align ? 1 : 0);
   d.add("AD_SCALE", s.get("SCALES", 0) ? 1 : 0); d.add("AD_INPLACE", s.get("INPLACE", 0) ? 1 : 0);
   d.add("AD_KS", ks); d.add("AD_S", slots); d.add("AD_NS", ns);
   src = d.wrap(kTpl_adapters);

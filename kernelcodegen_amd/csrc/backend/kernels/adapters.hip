@@ -5,11 +5,13 @@
 // Two launches, since every column needs all of h: adapters_down leaves h in fp32, in AD_KS parts of k; adapters_up adds the parts in order.
 // Tokens come in any order, and a step's requests may have an adapter each or share one.  A tile is 16 AD_TS tokens as they stand (of either launch its own AD_TS); each adapter that
 // occurs in it (found by comparing lanes) is multiplied with the whole tile, and of the result only its own tokens are kept: rows of a
-// matrix product do not touch one another.  A prompt's tiles have one adapter; a decoding step's have up to 16, which AD_S workgroups share.
-// h is not rounded to 16 bits: it enters the second product as the sum of two 16-bit numbers, which the matrix instruction takes as 2 AD_RANK
-// values of k with B's columns twice.  In half precision h is brought below 2^15 by a power of two of its row.
+// matrix product do not touch one another.  A prompt's tiles have one adapter; a decoding step's have up to 16, which AD_S workgroups share; those
+// that find none are the last of the launch.
+// h is not rounded to 16 bits: it enters the second product as the sum of AD_PIECES 16-bit numbers, which the matrix instruction takes as AD_PIECES AD_RANK
+// values of k with B's columns as often.  Two of half precision have 22 bits; two of bfloat16 have 16, enough for results in it, and three
+// have all of fp32's, for results in that.  In half precision h is brought below 2^15 by a power of two of its row.
 // Both products have the tokens as their columns, so that a lane has four neighbouring numbers of one token in each result.
-// Parameters: AD_NAME, AD_UP (this is adapters_up), AD_F16, AD_RANK, AD_K, AD_N, AD_XT, AD_YT, AD_ZT (strides of rows, elements), AD_YTYPE, AD_YSIZE, AD_ALIGN (rows
+// Parameters: AD_NAME, AD_UP (this is adapters_up), AD_F16, AD_PIECES, AD_RANK, AD_K, AD_N, AD_XT, AD_YT, AD_ZT (strides of rows, elements), AD_YTYPE, AD_YSIZE, AD_ALIGN (rows
 // of Y and Z start on multiples of 16 bytes), AD_SCALE (0: no scales), AD_INPLACE, AD_TS, AD_KS, AD_S, AD_NS (workgroups along N).
 typedef _Float16 ad_f16x8 __attribute__((ext_vector_type(8)));
 #if AD_F16
@@ -29,13 +31,29 @@ template <class Each> __device__ __forceinline__ ad_mask ad_adapters(const int* 
   const int lane = threadIdx.x & 63;
   const int mine = lane < AD_TILE && t0 + lane < T ? which[t0 + lane] : -1;
   const ad_mask with = __ballot(mine >= 0 && mine < adapters);
-  ad_mask todo = with;
-  for (int n = 0; todo; ++n) {
+#if AD_S > 1
+  // tokens that are the first ones with their adapter: lane by lane further away compared
+  int other = mine;
+  bool again = false;
+#pragma unroll
+  for (int d = 1; d < AD_TILE; ++d) {
+    other = __builtin_amdgcn_update_dpp(-1, other, 0x138, 0xf, 0xf, false);        // wave_shr 1
+    again |= other == mine;
+  }
+  const ad_mask first = __ballot(!again) & with;
+  const int turn = __builtin_amdgcn_mbcnt_hi((unsigned)(first >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)first, 0));
+  for (int n = slot; n < __builtin_popcountll(first); n += AD_S) {
+    const int r = __builtin_amdgcn_readlane(mine, __builtin_ctzll(__ballot(turn == n) & first));
+    each(r, __ballot(mine == r));
+  }
+#else
+  for (ad_mask todo = with; todo;) {
     const int r = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
     const ad_mask same = __ballot(mine == r);
     todo &= ~same;
-    if (n % AD_S == slot) each(r, same);
+    each(r, same);
   }
+#endif
   return with;
 }
 
@@ -50,8 +68,8 @@ template <class Each> __device__ __forceinline__ ad_mask ad_adapters(const int* 
 extern "C" __global__ __launch_bounds__(256)
 void AD_NAME(const ad_x* __restrict__ X, const ad_x* __restrict__ A, const int* __restrict__ which, long long T, long long adapters, float* __restrict__ part) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-  const int ks = blockIdx.x % AD_KS, slot = blockIdx.x / AD_KS % AD_S;
-  const long long t0 = (long long)(blockIdx.x / (AD_KS * AD_S)) * AD_TILE;
+  const int tiles = (int)((T + AD_TILE - 1) / AD_TILE), ks = blockIdx.x % AD_KS, slot = blockIdx.x / AD_KS / tiles;
+  const long long t0 = (long long)(blockIdx.x / AD_KS % tiles) * AD_TILE;
   union Shared {
     __attribute__((aligned(16))) unsigned char rows[4][AD_ROWS * AD_PITCH];
     kcg_f32x4 red[4][AD_TS * AD_JT][64];
@@ -132,31 +150,38 @@ typedef AD_YTYPE ad_y;
 #define AD_C (16 / AD_YSIZE)                       // columns of a lane, which lie beside one another: 16 bytes
 #define AD_COLS (16 * AD_C)                        // and of a wavefront
 typedef ad_y ad_yv __attribute__((ext_vector_type(AD_C)));
+#if AD_ALIGN
+typedef ad_yv ad_mem;
+#else
+typedef ad_y ad_mem __attribute__((ext_vector_type(AD_C), aligned(AD_YSIZE)));     // (rows may start anywhere)
+#endif
 #define AD_CHUNKS (AD_RANK / 8)
-#define AD_STEPS ((2 * AD_CHUNKS + 3) / 4)         // products: both halves of h
-#define AD_HALF (AD_CHUNKS % 4 == 0 ? AD_STEPS / 2 : AD_STEPS)    // of which so many have other columns of B
+#define AD_STEPS ((AD_PIECES * AD_CHUNKS + 3) / 4)  // products: all numbers that h is the sum of
+#define AD_OWN (AD_CHUNKS % 4 == 0 ? AD_CHUNKS / 4 : AD_STEPS)    // of which so many have other columns of B
 #define AD_GROUPS (4 / AD_TS)                       // wavefronts beside one another along N; AD_TS of them have 16 tokens each
 #define AD_STEP (AD_GROUPS * AD_COLS)              // columns of a workgroup
 #define AD_PITCH (AD_CHUNKS % 2 ? AD_RANK * 2 : AD_RANK * 2 + 16)  // of a row of B in LDS: an odd number of 16 bytes
 #define AD_LOADS ((AD_STEP * AD_CHUNKS + 255) / 256)
 
-// Columns n to n + AD_C of a row.
+// Columns n to n + AD_C of a row; elements of a vector that passes the row's end come one by one, all of them before any is put.
 __device__ __forceinline__ ad_yv ad_get(const ad_y* y, int n) {
-  if (AD_ALIGN) return *(const ad_yv*)(y + (n + AD_C <= AD_N ? n : 0));
-  ad_yv v;
+  ad_yv v = {};
+  if (AD_N >= AD_C) v = *(const ad_mem*)(y + (n + AD_C <= AD_N ? n : 0));
+  if (AD_N % AD_C && n < AD_N && n + AD_C > AD_N) {
 #pragma unroll
-  for (int e = 0; e < AD_C; ++e) v[e] = y[n + e < AD_N ? n + e : AD_N - 1];
+    for (int e = 0; e < AD_C; ++e) v[e] = y[n + e < AD_N ? n + e : AD_N - 1];
+  }
   return v;
 }
-__device__ __forceinline__ void ad_put(const ad_y* y, ad_y* z, int n, ad_yv v, const float (&add)[AD_C]) {
-  if (AD_ALIGN && n + AD_C <= AD_N) {
+__device__ __forceinline__ void ad_put(ad_y* z, int n, ad_yv v, const float (&add)[AD_C]) {
 #pragma unroll
-    for (int e = 0; e < AD_C; ++e) v[e] = (ad_y)((float)v[e] + add[e]);
-    *(ad_yv*)(z + n) = v;
+  for (int e = 0; e < AD_C; ++e) v[e] = (ad_y)((float)v[e] + add[e]);
+  if (n + AD_C <= AD_N) {
+    *(ad_mem*)(z + n) = v;
   } else {
 #pragma unroll
     for (int e = 0; e < AD_C; ++e)
-      if (n + e < AD_N) z[n + e] = (ad_y)((float)(AD_ALIGN ? y[n + e] : v[e]) + add[e]);
+      if (n + e < AD_N) z[n + e] = v[e];
   }
 }
 
@@ -168,8 +193,8 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
              long long adapters, ad_y* Z) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int sub = wave % AD_TS, group = wave / AD_TS;
-  const int ns = blockIdx.x % AD_NS, slot = blockIdx.x / AD_NS % AD_S;
-  const long long t0 = (long long)(blockIdx.x / (AD_NS * AD_S)) * AD_TILE, tw = t0 + sub * 16;
+  const int tiles = (int)((T + AD_TILE - 1) / AD_TILE), ns = blockIdx.x % AD_NS, slot = blockIdx.x / AD_NS / tiles;
+  const long long t0 = (long long)(blockIdx.x / AD_NS % tiles) * AD_TILE, tw = t0 + sub * 16;
   __shared__ __attribute__((aligned(16))) unsigned char rows[AD_STEP * AD_PITCH];
   long long row[4];
 #pragma unroll
@@ -191,7 +216,7 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
       }
     };
     fetch(ns * AD_STEP);
-    // h of this wavefront's tokens in two numbers of 16 bits
+    // h of this wavefront's tokens in numbers of 16 bits
     kcg_u32x4 f[AD_STEPS];
     kcg_f32x4 times = {0.0f, 0.0f, 0.0f, 0.0f};
     if (mine) {
@@ -231,8 +256,9 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
         for (int e = 0; e < 8; ++e) {
           const float a = h[s][e] * up;
           const ad_x high = (ad_x)a;
-          const float left = a - (float)high;
-          o[e] = q < AD_CHUNKS ? high : q < 2 * AD_CHUNKS && left - left == 0.0f ? (ad_x)left : (ad_x)0.0f;
+          const float left = a - (float)high;          // (nothing is left of an infinity)
+          const ad_x next = left - left == 0.0f ? (ad_x)left : (ad_x)0.0f, last = AD_PIECES > 2 && left - left == 0.0f ? (ad_x)(left - (float)next) : (ad_x)0.0f;
+          o[e] = q < AD_CHUNKS ? high : q < 2 * AD_CHUNKS ? next : q < AD_PIECES * AD_CHUNKS ? last : (ad_x)0.0f;
         }
         f[s] = __builtin_bit_cast(kcg_u32x4, o);
       }
@@ -257,21 +283,21 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
         for (int q = 0; q < AD_C; ++q) {
           const unsigned char* at = rows + (group * AD_COLS + q * 16 + i) * AD_PITCH;
           acc[q] = kcg_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-          kcg_u32x4 c[AD_HALF];
+          kcg_u32x4 c[AD_OWN];
 #pragma unroll
-          for (int s = 0; s < AD_HALF; ++s) {
+          for (int s = 0; s < AD_OWN; ++s) {
             c[s] = *(const kcg_u32x4*)(at + (s * 4 + g) % AD_CHUNKS * 16);
-            if (s * 4 + 3 >= 2 * AD_CHUNKS && s * 4 + g >= 2 * AD_CHUNKS) c[s] = kcg_u32x4{0, 0, 0, 0};        // (k behind both halves)
+            if (s * 4 + 3 >= AD_PIECES * AD_CHUNKS && s * 4 + g >= AD_PIECES * AD_CHUNKS) c[s] = kcg_u32x4{0, 0, 0, 0};        // (k behind all of them)
           }
 #pragma unroll
-          for (int s = 0; s < AD_STEPS; ++s) acc[q] = AD_MFMA(f[s], c[s % AD_HALF], acc[q]);
+          for (int s = 0; s < AD_STEPS; ++s) acc[q] = AD_MFMA(f[s], c[s % AD_OWN], acc[q]);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float add[AD_C];
 #pragma unroll
           for (int q = 0; q < AD_C; ++q) add[q] = times[e] * acc[q][e];
-          if (mine >> (g * 4 + e) & 1) ad_put(Y + row[e] * AD_YT, Z + row[e] * AD_ZT, nb + group * AD_COLS + i * AD_C, now[e], add);
+          if (mine >> (g * 4 + e) & 1) ad_put(Z + row[e] * AD_ZT, nb + group * AD_COLS + i * AD_C, now[e], add);
         }
       }
     }
@@ -283,7 +309,7 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
       if ((with >> (sub * 16 + g * 4 + e) & 1) || tw + g * 4 + e >= T) continue;
       const float none[AD_C] = {};
       for (int n = ns * AD_STEP + group * AD_COLS + i * AD_C; n < AD_N; n += AD_NS * AD_STEP)
-        ad_put(Y + row[e] * AD_YT, Z + row[e] * AD_ZT, n, ad_get(Y + row[e] * AD_YT, n), none);
+        ad_put(Z + row[e] * AD_ZT, n, ad_get(Y + row[e] * AD_YT, n), none);
     }
   }
 }

@@ -775,7 +775,7 @@ def _add_adapters_launch(y, x, a, b, which, scale, inplace, cfg):
     yt = y.stride(0) if tokens > 1 else 0
     zt, size = yt if inplace else n, y.element_size()
     params = dict(N=n, K=k, RANK=rank, F16=int(x.dtype == torch.float16), Y_F32=int(y.dtype == torch.float32), XT=x.stride(0) if tokens > 1 else 0, YT=yt, ZT=zt,
-                  ALIGN=int(n * size >= 16 and (y.data_ptr() | yt * size | zt * size) % 16 == 0), SCALES=int(scale is not None), INPLACE=int(inplace),
+                  ALIGN=int((y.data_ptr() | yt * size | zt * size) % 16 == 0), SCALES=int(scale is not None), INPLACE=int(inplace),
                   **{**_add_adapters_form(tokens, adapters, n, k, rank, 256 // size), **cfg})
     grids = [-(-tokens // (16 * params[tile])) * params["S"] * params[by] for tile, by in (("TS", "KS"), ("UT", "NS"))]
     if max(grids) > 0x7FFFFFFF:
@@ -787,17 +787,19 @@ def _add_adapters_launch(y, x, a, b, which, scale, inplace, cfg):
 def _add_adapters_form(tokens, adapters, n, k, rank, columns):
     """Tokens of a tile (16 TS, and 16 UT in the second launch), workgroups for a tile's adapters (S), for parts of k (KS) and of the columns (NS).
 
-    Up to 1024 tokens may be a decoding step's, with an adapter each: tiles of 16, whose adapters several workgroups share out.  More are prompts'.
+    Up to 1024 tokens may be a decoding step's, with an adapter each: tiles of 16, whose adapters up to 16 workgroups share out.  More are prompts'.
     Parts of k fill the part in the first launch and are read by all workgroups of the second.  Measured, in us, first and second launch:
-      64 tokens, 40 adapters of rank 16, N = K = 4096: k in 4 parts 4.9 and 5.8, in 8 4.2 and 7.2;  4 workgroups along N instead of 8: 6.2
-      5000 tokens, rank 64: 16 a tile, k in 2 parts 12.5 and 20.2, in one 20 and 17.1;  64 a tile, in 4 parts 15.6 and 26;  32 workgroups along N
+      64 tokens, 40 adapters of rank 16, N = K = 4096: k in 4 parts 4.5 and 5.6, in 8 4.1 and 6.6;  32 tokens a tile in the second launch 8.6, 64 15.9
+      128 tokens, 64 adapters of rank 64, N 11008: 32 tokens a tile 36, 16 39 (LDS for four wavefronts' columns);  300 tokens with one adapter: 6.5, 12.7
+      512 tokens, 64 adapters of rank 16: 16 workgroups for a tile's adapters 11.5 and 17.0, 4 16.6 and 15.2;  840 tokens in 20 runs: 7.9 and 7.1, 7.7 and 7.1
+      5000 tokens, rank 64: k in 2 parts 12.5 and 20.2, in one 20 and 17.1;  64 tokens a tile in the first launch, in 4 parts 15.6 and 26;  32 workgroups along N
       (one pass each) 17.1, 8: 18.7;  16 tokens a tile in the second launch 41, 32 tokens 32, 64 27
       2600 tokens, rank 32, K 4096, N 11008, fp32: k in 2 parts 13 and 47.7, in one 17.2 and 46.9;  43 workgroups along N 48.6, 172 62, 8 86"""
     ts = 2 if tokens > 1024 and 64 < rank <= 128 else 1
-    ut = 4 if tokens > 1024 or rank > 128 else 2 if rank > 64 else 1
+    ut = 4 if tokens > 1024 or rank > 128 else 2 if rank > 16 else 1
     tiles, wide = -(-tokens // (16 * ts)), -(-tokens // (16 * ut))
-    slots = min(16 if tiles <= 16 else 4, tokens, adapters) if tokens <= 1024 else 1
-    ks = max(1, min(8, (256 if tokens <= 1024 else 768) // (tiles * slots), k // 512))
+    slots = min(16, tokens, adapters) if tokens <= 1024 else 1
+    ks = max(1, min(8, 256 // (min(tiles, 16) * slots) if tokens <= 1024 else 768 // tiles, k // 512))
     blocks = -(-n // (columns * 4 // ut))
     each = max(1, blocks * wide * slots // 2048)
     return dict(TS=ts, UT=ut, S=slots, KS=ks, NS=-(-blocks // each))
@@ -863,11 +865,12 @@ def _token_logprobs_launch(logits, tokens, top, cfg):
 def _token_logprobs_form(rows, bytes_, top):
     """Workgroups of a row, their threads, and vectors that a lane has under way.
 
-    Fewer rows than units are cut into about 1024 parts of 8 KiB or more, and a second launch finishes them.  More have a workgroup each,
+    Fewer long rows than units are cut into about 1024 parts of 8 KiB or more, and a second launch finishes them.  Others have a workgroup each,
     which is the smaller the more of them wait for their alternatives beside others that read.  Measured, in us, both launches:
-      1 row of 32000, bf16, top 5: 8 parts 7.4, 4 parts 7.5, one workgroup 7.8;  64 of 128000, fp32, top 20: 16 parts 16.6, 8 parts 18.9, one workgroup 24
+      16 rows, bf16, top 5: of 16000 a workgroup each 7.2, parts 9.1;  32000: 8.8 and 9.3;  64000: 11.2 and 9.2;  128000: 16.8 and 11.1
+      200 rows: of 32000 9.3 and 12.7;  64000: 12.3 and 15.1;  128000: 18.3 and 19.1;  64 of 128000, fp32, top 20: 16 parts 16.6, 8 parts 18.9, whole 24
       500 of 50021, half, top 10: a workgroup of 256 threads each 19.5, of 512 19.3, 2 parts 20.7
-      2000 of 32000, bf16, top 20: of 512 threads 42, 256 40, 128 37.3;  top 5: 256 35.5, 128 33.1;  top 0: 512 28.2, 256 29.5"""
-    if rows < 256 and bytes_ >= 16384:
+      2000 of 32000, bf16, top 20: of 512 threads 42, 256 40, 128 37.3;  top 5: 256 35.5, 128 33.1;  top 0: 512 28.5, 256 30"""
+    if rows < 256 and bytes_ > (98304 if rows < 64 else 196608):
         return dict(PARTS=min(-(-1024 // rows), bytes_ // 8192), THREADS=256, U=2)
-    return dict(PARTS=1, THREADS=512 if top == 0 else 128 if rows >= 1024 and bytes_ <= 1 << 18 else 256, U=2)
+    return dict(PARTS=1, THREADS=512 if top == 0 or rows < 256 else 128 if rows >= 1024 and bytes_ <= 1 << 18 else 256, U=2)
