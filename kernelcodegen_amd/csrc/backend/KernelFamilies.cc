@@ -1794,14 +1794,14 @@ bool emitGemmQ4(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::st
 // adapters_down and adapters_up, which takes what the first leaves: the same parameters.
 bool emitAdapters(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::string& err) {
   const bool up = s.family == "adapters_up";
-  if (!whole(s, "N", 1, 0x7FFFFF00, err) || !whole(s, "K", 8, 0x7FFFFF00, err) || !whole(s, "RANK", 8, 256, err) || !whole(s, "F16", 0, 1, err)) return false;
+  if (!whole(s, "N", 1, 0x3FFFFF00, err) || !whole(s, "K", 8, 0x3FFFFF00, err) || !whole(s, "RANK", 8, 256, err) || !whole(s, "F16", 0, 1, err)) return false;
   for (auto key : {"K", "RANK"})
     if (s.p[key] % 8) { err = s.family + ": " + key + " must be a multiple of 8"; return false; }
   for (auto key : {"XT", "YT", "ZT"})
     if (!whole(s, key, 0, (int64_t)1 << 40, err)) return false;
   if (s.p["XT"] % 8) { err = s.family + ": XT must be a multiple of 16 bytes"; return false; }
-  const int64_t ks = s.get("KS", 1), slots = s.get("S", 1), ns = s.get("NS", 1);
-  if (ks < 1 || ks > 64 || slots < 1 || slots > 16 || ns < 1 || ns > 4096) { err = s.family + ": KS must be in [1,64], S in [1,16], NS in [1,4096]"; return false; }
+  const int64_t ks = s.get("KS", 1);
+  if (ks < 1 || ks > 64) { err = s.family + ": KS must be in [1,64]"; return false; }
   // 16 TS tokens a tile, of the second launch 16 UT: registers hold TS times the rank's results, LDS the columns of 4 / UT wavefronts
   const int64_t ts = s.get(up ? "UT" : "TS", 1), jt = ceilDiv(s.p["RANK"], 16);
   if ((ts != 1 && ts != 2 && ts != 4) || (up ? (4 / ts) * s.p["RANK"] > 256 : ts * jt > 16)) {
@@ -1817,11 +1817,11 @@ bool emitAdapters(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::
   for (auto key : {"XT", "YT", "ZT"}) d.add(std::string("AD_") + key, std::to_string(s.p[key]) + "LL");
   d.add("AD_YTYPE", std::string(y32 ? "float" : x)); d.add("AD_YSIZE", y32 ? 4 : 2); d.add("AD_PIECES", y32 && !s.p["F16"] ? 3 : 2); d.add("AD_TS", ts); d.add("AD_DEPTH", ts + jt <= 4 ? 2 : 1); d.add("AD_ALIGN", align ? 1 : 0);
   d.add("AD_SCALE", s.get("SCALES", 0) ? 1 : 0); d.add("AD_INPLACE", s.get("INPLACE", 0) ? 1 : 0);
-  d.add("AD_KS", ks); d.add("AD_S", slots); d.add("AD_NS", ns);
+  d.add("AD_KS", ks); d.add("AD_MANY", s.get("MANY", 0) ? 1 : 0);
   src = d.wrap(kTpl_adapters);
   info.name = s.name;
   info.block[0] = 256;
-  info.numArgs = up ? 8 : 6;
+  info.numArgs = up ? 10 : 7;
   return true;
 }
 
@@ -1833,21 +1833,22 @@ bool emitLogprobs(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::
   const int64_t v = s.p["V"], esize = s.p["F16"] ? 2 : 4;
   if (s.p["TOP"] > v) { err = s.family + ": TOP must not be above V"; return false; }
   if (!whole(s, "STRIDE", 0, (int64_t)1 << 40, err)) return false;
-  const int64_t parts = s.get("PARTS", 1), threads = s.get("THREADS", 512), u = s.get("U", esize == 2 ? 4 : 8);
-  if (parts < 1 || parts > 1024 || (join && parts == 1)) { err = s.family + ": PARTS must be in [1,1024], more than one to join"; return false; }
+  const int64_t threads = s.get("THREADS", 512), u = s.get("U", 2);
+  const bool split = join || s.get("SPLIT", 0) != 0;
   if (threads < 64 || threads > 1024 || threads % 64 || u < 1 || u > 16) { err = s.family + ": THREADS must be a multiple of 64 up to 1024, U in [1,16]"; return false; }
   const bool shift = s.get("SHIFT", 0) != 0;
   if (!shift && s.p["STRIDE"] * esize % 16) { err = s.family + ": rows off a multiple of 16 bytes need SHIFT"; return false; }
-  s.p["PARTS"] = parts; s.p["THREADS"] = threads; s.p["U"] = u;
+  s.p["THREADS"] = threads; s.p["U"] = u;
   Defines d;
   d.add("LP_NAME", s.name);
   d.add("LP_T", std::string(typeName(s.p["F16"]))); d.add("LP_ES", esize); d.add("LP_SHIFT", shift ? 1 : 0); d.add("LP_JOIN", join ? 1 : 0);
-  for (auto key : {"V", "TOP", "PARTS", "THREADS", "U"}) d.add(std::string("LP_") + key, s.p[key]);
+  d.add("LP_SPLIT", split ? 1 : 0);
+  for (auto key : {"V", "TOP", "THREADS", "U"}) d.add(std::string("LP_") + key, s.p[key]);
   d.add("LP_STRIDE", std::to_string(s.p["STRIDE"]) + "LL");
   src = d.wrap(kTpl_token_logprobs);
   info.name = s.name;
   info.block[0] = (uint32_t)threads;
-  info.numArgs = join ? 8 : parts > 1 ? 2 : 6;
+  info.numArgs = join ? 8 : split ? 3 : 6;
   return true;
 }
 

@@ -5,14 +5,15 @@
 // Two launches, since every column needs all of h: adapters_down leaves h in fp32, in AD_KS parts of k; adapters_up adds the parts in order.
 // Tokens come in any order, and a step's requests may have an adapter each or share one.  A tile is 16 AD_TS tokens as they stand (of either launch its own AD_TS); each adapter that
 // occurs in it (found by comparing lanes) is multiplied with the whole tile, and of the result only its own tokens are kept: rows of a
-// matrix product do not touch one another.  A prompt's tiles have one adapter; a decoding step's have up to 16, which AD_S workgroups share; those
+// matrix product do not touch one another.  A prompt's tiles have one adapter; a decoding step's have up to 16, which workgroups share; those
 // that find none are the last of the launch.
 // h is not rounded to 16 bits: it enters the second product as the sum of AD_PIECES 16-bit numbers, which the matrix instruction takes as AD_PIECES AD_RANK
 // values of k with B's columns as often.  Two of half precision have 22 bits; two of bfloat16 have 16, enough for results in it, and three
 // have all of fp32's, for results in that.  In half precision h is brought below 2^15 by a power of two of its row.
 // Both products have the tokens as their columns, so that a lane has four neighbouring numbers of one token in each result.
 // Parameters: AD_NAME, AD_UP (this is adapters_up), AD_F16, AD_PIECES, AD_RANK, AD_K, AD_N, AD_XT, AD_YT, AD_ZT (strides of rows, elements), AD_YTYPE, AD_YSIZE, AD_ALIGN (rows
-// of Y and Z start on multiples of 16 bytes), AD_SCALE (0: no scales), AD_INPLACE, AD_TS, AD_KS, AD_S, AD_NS (workgroups along N).
+// of Y and Z start on multiples of 16 bytes), AD_SCALE (0: no scales), AD_INPLACE, AD_TS, AD_KS, AD_MANY (a
+// tile's adapters are shared out; between how many workgroups, and how many there are along N, are arguments).
 typedef _Float16 ad_f16x8 __attribute__((ext_vector_type(8)));
 #if AD_F16
 typedef _Float16 ad_x;
@@ -27,11 +28,11 @@ typedef unsigned long long ad_mask;
 #define AD_TILE (16 * AD_TS)
 
 // Calls each(r, mask of the tile's tokens) for the adapters of a tile that are this workgroup's; returns the mask of the tokens that have one.
-template <class Each> __device__ __forceinline__ ad_mask ad_adapters(const int* __restrict__ which, long long t0, long long T, long long adapters, int slot, Each each) {
+template <class Each> __device__ __forceinline__ ad_mask ad_adapters(const int* __restrict__ which, long long t0, long long T, long long adapters, int slot, int slots, Each each) {
   const int lane = threadIdx.x & 63;
   const int mine = lane < AD_TILE && t0 + lane < T ? which[t0 + lane] : -1;
   const ad_mask with = __ballot(mine >= 0 && mine < adapters);
-#if AD_S > 1
+#if AD_MANY
   // tokens that are the first ones with their adapter: lane by lane further away compared
   int other = mine;
   bool again = false;
@@ -42,7 +43,7 @@ template <class Each> __device__ __forceinline__ ad_mask ad_adapters(const int* 
   }
   const ad_mask first = __ballot(!again) & with;
   const int turn = __builtin_amdgcn_mbcnt_hi((unsigned)(first >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)first, 0));
-  for (int n = slot; n < __builtin_popcountll(first); n += AD_S) {
+  for (int n = slot; n < __builtin_popcountll(first); n += slots) {
     const int r = __builtin_amdgcn_readlane(mine, __builtin_ctzll(__ballot(turn == n) & first));
     each(r, __ballot(mine == r));
   }
@@ -66,9 +67,11 @@ template <class Each> __device__ __forceinline__ ad_mask ad_adapters(const int* 
 #define AD_ROWS (16 * (AD_TS + AD_JT))                            // of X, then of A
 #define AD_PITCH 144
 extern "C" __global__ __launch_bounds__(256)
-void AD_NAME(const ad_x* __restrict__ X, const ad_x* __restrict__ A, const int* __restrict__ which, long long T, long long adapters, float* __restrict__ part) {
+void AD_NAME(const ad_x* __restrict__ X, const ad_x* __restrict__ A, const int* __restrict__ which, long long T, long long adapters, long long slots,
+             float* __restrict__ part) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-  const int tiles = (int)((T + AD_TILE - 1) / AD_TILE), ks = blockIdx.x % AD_KS, slot = blockIdx.x / AD_KS / tiles;
+  const unsigned tiles = (unsigned)((T + AD_TILE - 1) / AD_TILE);
+  const int ks = blockIdx.x % AD_KS, slot = blockIdx.x / AD_KS / tiles;
   const long long t0 = (long long)(blockIdx.x / AD_KS % tiles) * AD_TILE;
   union Shared {
     __attribute__((aligned(16))) unsigned char rows[4][AD_ROWS * AD_PITCH];
@@ -83,7 +86,7 @@ void AD_NAME(const ad_x* __restrict__ X, const ad_x* __restrict__ A, const int* 
     x[c] = X + (t < T ? t : T - 1) * AD_XT;
   }
   const int first = (ks * 4 + wave) * AD_SHARE, end = first + AD_SHARE < AD_STEPS ? first + AD_SHARE : AD_STEPS;
-  ad_adapters(which, t0, T, adapters, slot, [&](int r, ad_mask same) {
+  ad_adapters(which, t0, T, adapters, slot, (int)slots, [&](int r, ad_mask same) {
     kcg_f32x4 acc[AD_TS][AD_JT];
 #pragma unroll
     for (int t = 0; t < AD_TS; ++t)
@@ -190,16 +193,17 @@ __device__ __forceinline__ void ad_put(ad_y* z, int n, ad_yv v, const float (&ad
 // rows put into the order in which the products take them; the next columns' B and Y are under way meanwhile.
 extern "C" __global__ __launch_bounds__(256)
 void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restrict__ B, const int* __restrict__ which, const float* __restrict__ scale, long long T,
-             long long adapters, ad_y* Z) {
+             long long adapters, long long slots, long long NS_, ad_y* Z) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int sub = wave % AD_TS, group = wave / AD_TS;
-  const int tiles = (int)((T + AD_TILE - 1) / AD_TILE), ns = blockIdx.x % AD_NS, slot = blockIdx.x / AD_NS / tiles;
-  const long long t0 = (long long)(blockIdx.x / AD_NS % tiles) * AD_TILE, tw = t0 + sub * 16;
+  const unsigned NS = (unsigned)NS_, tiles = (unsigned)((T + AD_TILE - 1) / AD_TILE);
+  const int ns = blockIdx.x % NS, slot = blockIdx.x / NS / tiles;
+  const long long t0 = (long long)(blockIdx.x / NS % tiles) * AD_TILE, tw = t0 + sub * 16, step = (long long)NS * AD_STEP;
   __shared__ __attribute__((aligned(16))) unsigned char rows[AD_STEP * AD_PITCH];
   long long row[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) row[e] = tw + g * 4 + e < T ? tw + g * 4 + e : T - 1;
-  const ad_mask with = ad_adapters(which, t0, T, adapters, slot, [&](int r, ad_mask same) {
+  const ad_mask with = ad_adapters(which, t0, T, adapters, slot, (int)slots, [&](int r, ad_mask same) {
     const ad_x* b = B + (long long)r * AD_N * AD_RANK;
     const unsigned mine = (unsigned)(same >> (sub * 16)) & 0xffffu;
     kcg_u32x4 w[AD_LOADS];
@@ -264,7 +268,7 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
       }
     }
 #pragma unroll 1
-    for (int nb = ns * AD_STEP; nb < AD_N; nb += AD_NS * AD_STEP) {
+    for (int nb = ns * AD_STEP; nb < AD_N; nb += NS * AD_STEP) {
       __syncthreads();
 #pragma unroll
       for (int c = 0; c < AD_LOADS; ++c) {
@@ -276,7 +280,7 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
 #pragma unroll
       for (int e = 0; e < 4; ++e) now[e] = v[e];
       __syncthreads();
-      if (nb + AD_NS * AD_STEP < AD_N) fetch(nb + AD_NS * AD_STEP);
+      if (nb + step < AD_N) fetch(nb + (int)step);
       if (mine) {
         kcg_f32x4 acc[AD_C];
 #pragma unroll
@@ -308,7 +312,7 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
     for (int e = 0; e < 4; ++e) {
       if ((with >> (sub * 16 + g * 4 + e) & 1) || tw + g * 4 + e >= T) continue;
       const float none[AD_C] = {};
-      for (int n = ns * AD_STEP + group * AD_COLS + i * AD_C; n < AD_N; n += AD_NS * AD_STEP)
+      for (int n = ns * AD_STEP + group * AD_COLS + i * AD_C; n < AD_N; n += NS * AD_STEP)
         ad_put(Z + row[e] * AD_ZT, n, ad_get(Y + row[e] * AD_YT, n), none);
     }
   }

@@ -12,15 +12,14 @@
 // Both times the largest of N keys are found the same way: the key holds value and index, so no two are equal; each thread takes its best one, of
 // those of a wavefront the k-th is a bound, what reaches the highest bound is counted out against one another.
 // Vectors are the aligned ones of memory, the first and the last of a row maybe with elements outside of it, which are left out.
-// A row is a workgroup, or LP_PARTS of them, whose sums and segments logprobs_join (LP_JOIN) finishes.
+// A row is a workgroup, or several parts (LP_SPLIT; how many is an argument), whose sums and segments logprobs_join (LP_JOIN) finishes.
 // Parameters: LP_NAME, LP_V, LP_T, LP_ES (element bytes), LP_STRIDE (of rows, elements), LP_SHIFT (rows may start off a multiple of 16 bytes), LP_TOP,
-// LP_PARTS, LP_THREADS, LP_U, LP_JOIN.
+// LP_SPLIT, LP_THREADS, LP_U, LP_JOIN.
 typedef LP_T lp_t;
 #define LP_VW (16 / LP_ES)
 #define LP_VECTORS ((LP_V + (LP_SHIFT ? LP_VW - 1 : 0) + LP_VW - 1) / LP_VW)     // at most
 #define LP_BLOCKS ((LP_VECTORS + 63) / 64)
 #define LP_SEGMENTS (LP_BLOCKS * 4)
-#define LP_SHARE ((LP_BLOCKS + LP_PARTS - 1) / LP_PARTS)                         // blocks of a part
 #define LP_WAVES (LP_THREADS / 64)
 #define LP_LOW (-3.402823466e38f)
 #define LP_LOG2E 1.4426950408889634f
@@ -109,12 +108,12 @@ __device__ __forceinline__ void lp_scan(const lp_t* __restrict__ x, int first, i
   __syncthreads();
 }
 #endif
-template <int N> __device__ __forceinline__ LpSum lp_total(const LpSum* parts) {
+__device__ __forceinline__ LpSum lp_total(const LpSum* parts, int n) {
   LpSum a = {parts[0].m, 0.0f, 0.0f};
-#pragma unroll 16
-  for (int i = 1; i < N; ++i) a.m = fmaxf(a.m, parts[i].m);
-#pragma unroll 16
-  for (int i = 0; i < N; ++i) {
+#pragma unroll 8
+  for (int i = 1; i < n; ++i) a.m = fmaxf(a.m, parts[i].m);
+#pragma unroll 8
+  for (int i = 0; i < n; ++i) {
     const float d = parts[i].m - a.m, f = __builtin_amdgcn_exp2f(d * LP_LOG2E);
     a.s += f * parts[i].s;
     a.u += f * (parts[i].u + fmaxf(d, -1e30f) * parts[i].s);
@@ -122,7 +121,7 @@ template <int N> __device__ __forceinline__ LpSum lp_total(const LpSum* parts) {
   return a;
 }
 
-#if LP_PARTS == 1 || LP_JOIN
+#if !LP_SPLIT || LP_JOIN
 #if LP_TOP
 // A value and an index below 2^19 as a number from 1 to 2, whose order is the values' and for equal ones the indices' backwards (comparing two of
 // these takes one instruction of the ordinary rate); 0 is none.
@@ -316,19 +315,19 @@ template <class Sums> __device__ __forceinline__ void lp_finish(const lp_t* __re
 
 extern "C" __global__ __launch_bounds__(LP_THREADS)
 #if LP_JOIN
-void LP_NAME(const float* __restrict__ part, const lp_t* __restrict__ logits, const long long* __restrict__ tokens, long long rows, float* __restrict__ logprob,
+void LP_NAME(const float* __restrict__ part, const lp_t* __restrict__ logits, const long long* __restrict__ tokens, long long parts, float* __restrict__ logprob,
              float* __restrict__ entropy, float* __restrict__ values, long long* __restrict__ indices) {
   const long long row = blockIdx.x;
-  const float* mine = part + row * (LP_PARTS * 3 + (LP_TOP ? LP_SEGMENTS : 0));
-  lp_finish(logits + row * LP_STRIDE, row, [&] { return lp_total<LP_PARTS>((const LpSum*)mine); }, mine + LP_PARTS * 3, tokens, logprob, entropy, values, indices);
-#elif LP_PARTS > 1
-void LP_NAME(const lp_t* __restrict__ logits, float* __restrict__ part) {
+  const float* mine = part + row * (parts * 3 + (LP_TOP ? LP_SEGMENTS : 0));
+  lp_finish(logits + row * LP_STRIDE, row, [&] { return lp_total((const LpSum*)mine, (int)parts); }, mine + parts * 3, tokens, logprob, entropy, values, indices);
+#elif LP_SPLIT
+void LP_NAME(const lp_t* __restrict__ logits, long long parts, float* __restrict__ part) {
   __shared__ LpSum sums[LP_WAVES];
-  const long long row = blockIdx.x / LP_PARTS;
-  const int i = blockIdx.x % LP_PARTS, first = i * LP_SHARE, end = first + LP_SHARE < LP_BLOCKS ? first + LP_SHARE : LP_BLOCKS;
-  float* mine = part + row * (LP_PARTS * 3 + (LP_TOP ? LP_SEGMENTS : 0));
-  lp_scan(logits + row * LP_STRIDE, first, end, sums, mine + LP_PARTS * 3);
-  if (threadIdx.x == 0) ((LpSum*)mine)[i] = lp_total<LP_WAVES>(sums);
+  const unsigned n = (unsigned)parts, row = blockIdx.x / n, i = blockIdx.x % n, share = (LP_BLOCKS + n - 1) / n;
+  const int first = (int)(i * share), end = first + (int)share < LP_BLOCKS ? first + (int)share : LP_BLOCKS;
+  float* mine = part + row * (parts * 3 + (LP_TOP ? LP_SEGMENTS : 0));
+  lp_scan(logits + row * LP_STRIDE, first, end, sums, mine + parts * 3);
+  if (threadIdx.x == 0) ((LpSum*)mine)[i] = lp_total(sums, LP_WAVES);
 #else
 void LP_NAME(const lp_t* __restrict__ logits, const long long* __restrict__ tokens, float* __restrict__ logprob, float* __restrict__ entropy,
              float* __restrict__ values, long long* __restrict__ indices) {
@@ -340,6 +339,6 @@ void LP_NAME(const lp_t* __restrict__ logits, const long long* __restrict__ toke
 #endif
   const long long row = blockIdx.x;
   lp_scan(logits + row * LP_STRIDE, 0, LP_BLOCKS, sums, segments);
-  lp_finish(logits + row * LP_STRIDE, row, [&] { return lp_total<LP_WAVES>(sums); }, segments, tokens, logprob, entropy, values, indices);
+  lp_finish(logits + row * LP_STRIDE, row, [&] { return lp_total(sums, LP_WAVES); }, segments, tokens, logprob, entropy, values, indices);
 #endif
 }

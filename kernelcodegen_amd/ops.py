@@ -732,14 +732,14 @@ def add_adapters(y, x, a, b, which, scale=None, inplace=False, **cfg):
         hit = _add_adapters_launch(y, x, a, b, which, scale, inplace, cfg)
         if not cfg:
             _bound[key] = hit
-    down, up = hit
+    down, up, slots, across = hit
     tokens, adapters = which.shape[0], a.shape[0]
     if down is None:
         return y if inplace else torch.empty_like(y, memory_format=torch.contiguous_format)
-    part = down(x, a, which, tokens, adapters)
+    part = down(x, a, which, tokens, adapters, slots)
     if not inplace:
-        return up(part, y, b, which, 0 if scale is None else scale, tokens, adapters)
-    up(part.data_ptr(), y.data_ptr(), b.data_ptr(), which.data_ptr(), 0 if scale is None else scale.data_ptr(), tokens, adapters, y.data_ptr())
+        return up(part, y, b, which, 0 if scale is None else scale, tokens, adapters, slots, across)
+    up(part.data_ptr(), y.data_ptr(), b.data_ptr(), which.data_ptr(), 0 if scale is None else scale.data_ptr(), tokens, adapters, slots, across, y.data_ptr())
     return y
 
 
@@ -756,8 +756,8 @@ def _add_adapters_launch(y, x, a, b, which, scale, inplace, cfg):
     (tokens, n), k, (adapters, rank) = y.shape, x.shape[1], a.shape[:2]
     if x.shape[0] != tokens or tuple(which.shape) != (tokens,) or a.shape[2] != k or tuple(b.shape) != (adapters, n, rank):
         raise ValueError("y is [tokens, N], x [tokens, K], a [adapters, rank, K], b [adapters, N, rank], which [tokens]")
-    if adapters < 1 or adapters > 0x7FFFFFFF or rank % 8 or not 8 <= rank <= 256 or k % 8 or not 8 <= k <= 0x7FFFFF00 or not 1 <= n <= 0x7FFFFF00:
-        raise ValueError("rank and K are multiples of 8, the rank up to 256, and there is an adapter")
+    if adapters < 1 or adapters > 0x7FFFFFFF or rank % 8 or not 8 <= rank <= 256 or k % 8 or not 8 <= k <= 0x3FFFFF00 or not 1 <= n <= 0x3FFFFF00:
+        raise ValueError("rank and K are multiples of 8, the rank up to 256, K and N below 2^30, and there is an adapter")
     if scale is not None and tuple(scale.shape) != (adapters,):
         raise ValueError("scale is [adapters]")
     if x.stride(1) != 1 or (y.stride(1) != 1 and n > 1):
@@ -771,17 +771,21 @@ def _add_adapters_launch(y, x, a, b, which, scale, inplace, cfg):
     if not cfg.keys() <= {"TS", "UT", "KS", "S", "NS"}:
         raise ValueError("unknown kernel parameters")
     if not tokens:
-        return None, None
+        return None, None, 0, 0
     yt = y.stride(0) if tokens > 1 else 0
     zt, size = yt if inplace else n, y.element_size()
     params = dict(N=n, K=k, RANK=rank, F16=int(x.dtype == torch.float16), Y_F32=int(y.dtype == torch.float32), XT=x.stride(0) if tokens > 1 else 0, YT=yt, ZT=zt,
                   ALIGN=int((y.data_ptr() | yt * size | zt * size) % 16 == 0), SCALES=int(scale is not None), INPLACE=int(inplace),
                   **{**_add_adapters_form(tokens, adapters, n, k, rank, 256 // size), **cfg})
-    grids = [-(-tokens // (16 * params[tile])) * params["S"] * params[by] for tile, by in (("TS", "KS"), ("UT", "NS"))]
+    slots, across = params.pop("S"), min(params.pop("NS"), -(-n * size // 256))
+    params["MANY"] = int(slots > 1)
+    if slots < 1 or across < 1:
+        raise ValueError("bad kernel parameters")
+    grids = [-(-tokens // (16 * max(1, params[tile]))) * slots * by for tile, by in (("TS", params["KS"]), ("UT", across))]
     if max(grids) > 0x7FFFFFFF:
         raise ValueError("too many tokens for one launch")
     down, up = (R.get_kernel(family, **params).bind(grid=(grid,)) for family, grid in zip(("adapters_down", "adapters_up"), grids))
-    return _into_last(down, ((params["KS"], tokens, rank), torch.float32)), up if inplace else _into_last(up, ((tokens, n), y.dtype))
+    return _into_last(down, ((params["KS"], tokens, rank), torch.float32)), up if inplace else _into_last(up, ((tokens, n), y.dtype)), slots, across
 
 
 def _add_adapters_form(tokens, adapters, n, k, rank, columns):
@@ -800,6 +804,7 @@ def _add_adapters_form(tokens, adapters, n, k, rank, columns):
     tiles, wide = -(-tokens // (16 * ts)), -(-tokens // (16 * ut))
     slots = min(16, tokens, adapters) if tokens <= 1024 else 1
     ks = max(1, min(8, 256 // (min(tiles, 16) * slots) if tokens <= 1024 else 768 // tiles, k // 512))
+    ks = 1 << ks.bit_length() - 1            # (a kernel for each)
     blocks = -(-n // (columns * 4 // ut))
     each = max(1, blocks * wide * slots // 2048)
     return dict(TS=ts, UT=ut, S=slots, KS=ks, NS=-(-blocks // each))
@@ -820,10 +825,10 @@ def token_logprobs(logits, tokens, top=0, **cfg):
         hit = _token_logprobs_launch(logits, tokens, top, cfg)
         if not cfg:
             _bound[key] = hit
-    run, join = hit
+    run, join, parts = hit
     if run is None:
         return _no_rows(logits, top)
-    return run(logits, tokens) if join is None else join(run(logits), logits, tokens, logits.shape[0])
+    return run(logits, tokens) if join is None else join(run(logits, parts), logits, tokens, parts)
 
 
 def _no_rows(logits, top):
@@ -845,21 +850,23 @@ def _token_logprobs_launch(logits, tokens, top, cfg):
     if not cfg.keys() <= {"PARTS", "THREADS", "U"}:
         raise ValueError("unknown kernel parameters")
     if not rows:
-        return None, None
+        return None, None, 1
     stride, size = logits.stride(0) if rows > 1 else 0, logits.element_size()
     params = dict(V=v, F16=_STORAGE[logits.dtype], TOP=top, STRIDE=stride, SHIFT=int((stride * size | logits.data_ptr()) % 16 != 0),
                   **{**_token_logprobs_form(rows, v * size, top), **cfg})
-    parts = params["PARTS"]
+    parts = params.pop("PARTS")
+    if not 1 <= parts <= 1024:
+        raise ValueError("a row has 1 to 1024 parts")
     if rows * parts > 0x7FFFFFFF:
         raise ValueError("too many rows for one launch")
-    kern = R.get_kernel("token_logprobs", **params)
+    kern = R.get_kernel("token_logprobs", SPLIT=int(parts > 1), **params)
     results = ((rows,), torch.float32), ((rows,), torch.float32), ((rows, top), torch.float32), ((rows, top), torch.int64)
     if parts == 1:
-        return _into_last(kern.bind(grid=(rows,)), *results), None
+        return _into_last(kern.bind(grid=(rows,)), *results), None, 1
     vectors = -(-v * size // 16) + params["SHIFT"]
     floats = rows * (3 * parts + (4 * -(-vectors // 64) if top else 0))
     join = R.get_kernel("logprobs_join", **{**params, "THREADS": 512}).bind(grid=(rows,))
-    return _into_last(kern.bind(grid=(rows * parts,)), ((floats,), torch.float32)), _into_last(join, *results)
+    return _into_last(kern.bind(grid=(rows * parts,)), ((floats,), torch.float32)), _into_last(join, *results), parts
 
 
 def _token_logprobs_form(rows, bytes_, top):
@@ -872,5 +879,5 @@ def _token_logprobs_form(rows, bytes_, top):
       500 of 50021, half, top 10: a workgroup of 256 threads each 19.5, of 512 19.3, 2 parts 20.7
       2000 of 32000, bf16, top 20: of 512 threads 42, 256 40, 128 37.3;  top 5: 256 35.5, 128 33.1;  top 0: 512 28.5, 256 30"""
     if rows < 256 and bytes_ > (98304 if rows < 64 else 196608):
-        return dict(PARTS=min(-(-1024 // rows), bytes_ // 8192), THREADS=256, U=2)
+        return dict(PARTS=min(-(-1024 // rows), bytes_ // 8192, 64), THREADS=256, U=2)
     return dict(PARTS=1, THREADS=512 if top == 0 or rows < 256 else 128 if rows >= 1024 and bytes_ <= 1 << 18 else 256, U=2)

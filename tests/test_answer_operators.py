@@ -11,10 +11,10 @@ ADAPT = dict(N=1000, K=4096, RANK=16, F16=0, Y_F32=0, XT=4096, YT=1000, ZT=1000,
 LOGPROBS = dict(V=32000, F16=2, TOP=5, STRIDE=32000)
 GOOD = [("cache_append", dict(cache(d), **{**APPEND, "R": r, "F16": f16, "WIN": win, "PAIRS": pairs}), 14)
         for d, r, f16, win, pairs in ((128, 128, 2, 1, 0), (96, 96, 0, 16, 1), (256, 32, 1, 4, 0), (32, 16, 2, 16, 1), (224, 224, 0, 1, 0), (160, 80, 1, 16, 0))]
-GOOD += [(family, dict(ADAPT, **more), 8 if family.endswith("up") else 6) for family in ("adapters_down", "adapters_up")
-         for more in (dict(), dict(RANK=8, F16=1, Y_F32=1, SCALES=1, S=16, KS=8), dict(RANK=256, K=264, NS=4, UT=4), dict(RANK=64, TS=4, UT=4, KS=2), dict(RANK=128, TS=2, UT=2, Y_F32=1, F16=1), dict(RANK=24, N=77, YT=77, ZT=77, ALIGN=0, INPLACE=1), dict(N=4))]
+GOOD += [(family, dict(ADAPT, **more), 10 if family.endswith("up") else 7) for family in ("adapters_down", "adapters_up")
+         for more in (dict(), dict(RANK=8, F16=1, Y_F32=1, SCALES=1, MANY=1, KS=8), dict(RANK=256, K=264, UT=4, MANY=1), dict(RANK=64, TS=4, UT=4, KS=2), dict(RANK=128, TS=2, UT=2, Y_F32=1, F16=1), dict(RANK=24, N=77, YT=77, ZT=77, ALIGN=0, INPLACE=1), dict(N=4))]
 GOOD += [("token_logprobs", dict(LOGPROBS, **more), 6) for more in (dict(), dict(TOP=0, F16=1), dict(F16=0, TOP=32), dict(V=1, TOP=1, STRIDE=0), dict(V=1 << 19, F16=0, STRIDE=1 << 19), dict(V=50021, STRIDE=50021, SHIFT=1))]
-GOOD += [("token_logprobs", dict(LOGPROBS, PARTS=16, THREADS=256), 2), ("logprobs_join", dict(LOGPROBS, PARTS=16, THREADS=256), 8)]
+GOOD += [("token_logprobs", dict(LOGPROBS, SPLIT=1, THREADS=256), 3), ("logprobs_join", dict(LOGPROBS, THREADS=256), 8)]
 
 
 @pytest.mark.parametrize("family,params,nargs", GOOD)
@@ -30,10 +30,10 @@ def test_every_form_compiles_for_gfx950(family, params, nargs):
     ("cache_append", dict(cache(64), **WRITE)), ("cache_append", dict(cache(48), **APPEND)),
     ("adapters_up", dict(ADAPT, RANK=4)), ("adapters_up", dict(ADAPT, RANK=20)), ("adapters_up", dict(ADAPT, RANK=264)), ("adapters_down", dict(ADAPT, K=4)), ("adapters_down", dict(ADAPT, K=100)),
     ("adapters_down", dict(ADAPT, XT=100)), ("adapters_up", dict(ADAPT, YT=1004)), ("adapters_up", dict(ADAPT, F16=2)), ("adapters_up", dict(ADAPT, N=0)), ("adapters_down", dict(ADAPT, KS=65)),
-    ("adapters_down", dict(ADAPT, S=17)), ("adapters_up", dict(ADAPT, NS=0)), ("adapters_up", dict(ADAPT, UT=3)), ("adapters_down", dict(ADAPT, TS=4, RANK=72)), ("adapters_up", dict(ADAPT, UT=1, RANK=72)),
+    ("adapters_up", dict(ADAPT, UT=3)), ("adapters_down", dict(ADAPT, TS=4, RANK=72)), ("adapters_up", dict(ADAPT, UT=1, RANK=72)),
     ("token_logprobs", dict(LOGPROBS, V=0)), ("token_logprobs", dict(LOGPROBS, V=(1 << 19) + 1)), ("token_logprobs", dict(LOGPROBS, TOP=33)), ("token_logprobs", dict(LOGPROBS, V=4, STRIDE=8)),
-    ("token_logprobs", dict(LOGPROBS, F16=3)), ("token_logprobs", dict(LOGPROBS, STRIDE=32001)), ("token_logprobs", dict(LOGPROBS, THREADS=100)), ("token_logprobs", dict(LOGPROBS, PARTS=0)),
-    ("token_logprobs", dict(LOGPROBS, U=17)), ("logprobs_join", dict(LOGPROBS, PARTS=1)), ("token_logprobs", dict(LOGPROBS, STRIDE=-8))])
+    ("token_logprobs", dict(LOGPROBS, F16=3)), ("token_logprobs", dict(LOGPROBS, STRIDE=32001)), ("token_logprobs", dict(LOGPROBS, THREADS=100)),
+    ("token_logprobs", dict(LOGPROBS, U=17)), ("token_logprobs", dict(LOGPROBS, STRIDE=-8))])
 def test_bad_parameters_are_refused(family, params):
     with pytest.raises(_lib.KcgError):
         R.emit_kernel(family, "kernel0", **params)
