@@ -13,7 +13,8 @@
 // Both products have the tokens as their columns, so that a lane has four neighbouring numbers of one token in each result.
 // Parameters: AD_NAME, AD_UP (this is adapters_up), AD_F16, AD_PIECES, AD_RANK, AD_K, AD_N, AD_XT, AD_YT, AD_ZT (strides of rows, elements), AD_YTYPE, AD_YSIZE, AD_ALIGN (rows
 // of Y and Z start on multiples of 16 bytes), AD_SCALE (0: no scales), AD_INPLACE, AD_TS, AD_KS, AD_MANY (a
-// tile's adapters are shared out; between how many workgroups, and how many there are along N, are arguments).
+// tile's adapters are shared out; between how many workgroups, and how many there are along N, are arguments), AD_ONCE (there are as
+// many along N as have columns: each has one pass).
 typedef _Float16 ad_f16x8 __attribute__((ext_vector_type(8)));
 #if AD_F16
 typedef _Float16 ad_x;
@@ -280,7 +281,7 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
 #pragma unroll
       for (int e = 0; e < 4; ++e) now[e] = v[e];
       __syncthreads();
-      if (nb + step < AD_N) fetch(nb + (int)step);
+      if (!AD_ONCE && nb + step < AD_N) fetch(nb + (int)step);
       if (mine) {
         kcg_f32x4 acc[AD_C];
 #pragma unroll
@@ -304,6 +305,7 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
           if (mine >> (g * 4 + e) & 1) ad_put(Z + row[e] * AD_ZT, nb + group * AD_COLS + i * AD_C, now[e], add);
         }
       }
+      if (AD_ONCE) break;
     }
     __syncthreads();
   });

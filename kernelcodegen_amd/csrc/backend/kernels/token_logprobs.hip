@@ -34,6 +34,12 @@ __device__ __forceinline__ LpSum lp_add(LpSum a, LpSum b) {
   // (a difference that is no longer finite belongs to a factor of 0)
   return {m, fa * a.s + fb * b.s, fa * (a.u + fmaxf(a.m - m, -1e30f) * a.s) + fb * (b.u + fmaxf(b.m - m, -1e30f) * b.s)};
 }
+// Of all lanes.
+__device__ __forceinline__ LpSum lp_all(LpSum a) {
+#pragma unroll
+  for (int by = 32; by > 0; by >>= 1) a = lp_add(a, {__shfl_xor(a.m, by, 64), __shfl_xor(a.s, by, 64), __shfl_xor(a.u, by, 64)});
+  return a;
+}
 // Elements of a row that lie in front of its first aligned vector's begin, as a number of that vector's elements.
 __device__ __forceinline__ int lp_offset(const lp_t* x) { return LP_SHIFT ? (int)((size_t)x / LP_ES % LP_VW) : 0; }
 // A vector of which parts may lie outside of the row: these are -inf.  (All loads are unconditional: one behind a branch would be waited for there.)
@@ -102,21 +108,21 @@ __device__ __forceinline__ void lp_scan(const lp_t* __restrict__ x, int first, i
     }
 #endif
   }
-#pragma unroll
-  for (int by = 32; by > 0; by >>= 1) a = lp_add(a, {__shfl_xor(a.m, by, 64), __shfl_xor(a.s, by, 64), __shfl_xor(a.u, by, 64)});
+  a = lp_all(a);
   if (lane == 0) sums[wave] = a;
   __syncthreads();
 }
 #endif
-__device__ __forceinline__ LpSum lp_total(const LpSum* parts, int n) {
-  LpSum a = {parts[0].m, 0.0f, 0.0f};
-#pragma unroll 8
-  for (int i = 1; i < n; ++i) a.m = fmaxf(a.m, parts[i].m);
-#pragma unroll 8
-  for (int i = 0; i < n; ++i) {
-    const float d = parts[i].m - a.m, f = __builtin_amdgcn_exp2f(d * LP_LOG2E);
-    a.s += f * parts[i].s;
-    a.u += f * (parts[i].u + fmaxf(d, -1e30f) * parts[i].s);
+// Of all wavefronts.
+__device__ __forceinline__ LpSum lp_total(const LpSum* sums) {
+  LpSum a = {sums[0].m, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 1; i < LP_WAVES; ++i) a.m = fmaxf(a.m, sums[i].m);
+#pragma unroll
+  for (int i = 0; i < LP_WAVES; ++i) {
+    const float d = sums[i].m - a.m, f = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+    a.s += f * sums[i].s;
+    a.u += f * (sums[i].u + fmaxf(d, -1e30f) * sums[i].s);
   }
   return a;
 }
@@ -141,12 +147,25 @@ __device__ __forceinline__ int lp_index(lp_key k) { return 0x7ffff - (int)(__bui
 struct LpPick {
   lp_key list[2][LP_LIST + 32], found[2][LP_TOP], wave[2][LP_WAVES];
   __attribute__((aligned(16))) float best[LP_THREADS / 2];
-  float bound[LP_WAVES];
+  float bound[LP_WAVES], share[LP_WAVES];
   int many[2];
 };
 #define LP_DPP(old, v, control, rows) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, v), control, rows, 0xf, false))
 #define LP_SWAP(v, control) __builtin_amdgcn_update_dpp(0, v, control, 0xf, 0xf, true)       // (quad_perm 1 0 3 2 is 0xb1, 2 3 0 1 is 0x4e)
-// What LP_TOP of the workgroup's numbers reach (or all): of a wavefront's 32 pairs of lanes the LP_TOP-th largest, and of these the largest.
+// Least of the lanes' numbers, in lane 63.
+__device__ __forceinline__ float lp_least(float v) {
+  const float most = __builtin_inff();
+  v = fminf(v, LP_DPP(most, v, 0x111, 0xf));        // row_shr 1, 2, 4, 8, then a row's last lane into the next row, the second row's into the others
+  v = fminf(v, LP_DPP(most, v, 0x112, 0xf));
+  v = fminf(v, LP_DPP(most, v, 0x114, 0xf));
+  v = fminf(v, LP_DPP(most, v, 0x118, 0xf));
+  v = fminf(v, LP_DPP(most, v, 0x142, 0xa));
+  return fminf(v, LP_DPP(most, v, 0x143, 0xc));
+}
+// What LP_TOP of the workgroup's numbers reach (or all).  Of each wavefront's 32 pairs of lanes the LP_TOP-th largest is such a bound, the largest of these
+// too; and so is the least of the wavefronts' LP_SHARE-th largest, which reach LP_TOP together: closer where the numbers are spread evenly (of 2000
+// numbers 20 wanted, 8 wavefronts: about 40 reach it, 100 the first).
+#define LP_SHARE ((LP_TOP + LP_WAVES - 1) / LP_WAVES)
 __device__ __forceinline__ float lp_bound(LpPick& p, float best) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const float most = __builtin_inff(), pair = fmaxf(best, __builtin_bit_cast(float, LP_SWAP(__builtin_bit_cast(int, best), 0xb1)));
@@ -160,19 +179,19 @@ __device__ __forceinline__ float lp_bound(LpPick& p, float best) {
     for (int e = 0; e < 4; ++e) r += other[e] > pair;
   }
   r += LP_SWAP(r, 0xb1);
-  float v = r < LP_TOP ? pair : most;
-  v = fminf(v, LP_DPP(most, v, 0x111, 0xf));        // row_shr 1, 2, 4, 8, then a row's last lane into the next row, the second row's into the others
-  v = fminf(v, LP_DPP(most, v, 0x112, 0xf));
-  v = fminf(v, LP_DPP(most, v, 0x114, 0xf));
-  v = fminf(v, LP_DPP(most, v, 0x118, 0xf));
-  v = fminf(v, LP_DPP(most, v, 0x142, 0xa));
-  v = fminf(v, LP_DPP(most, v, 0x143, 0xc));
-  if (lane == 63) p.bound[wave] = v;
+  const float all = lp_least(r < LP_TOP ? pair : most), share = lp_least(r < LP_SHARE ? pair : most);
+  if (lane == 63) {
+    p.bound[wave] = all;
+    p.share[wave] = share;
+  }
   __syncthreads();
-  float bound = -most;
+  float bound = -most, together = most;
 #pragma unroll
-  for (int w = 0; w < LP_WAVES; ++w) bound = fmaxf(bound, p.bound[w]);
-  return bound;
+  for (int w = 0; w < LP_WAVES; ++w) {
+    bound = fmaxf(bound, p.bound[w]);
+    together = fminf(together, p.share[w]);
+  }
+  return fmaxf(bound, together);
 }
 // The LP_TOP largest of the threads' numbers v[q] that are there (index(q) from 0 on) and not below the bound, by value and index, into p.found[turn]; all where
 // they are fewer.  LP_TOP of the numbers (or all) reach the bound.  p.list and p.found are zeros before, p.many too.
@@ -319,7 +338,13 @@ void LP_NAME(const float* __restrict__ part, const lp_t* __restrict__ logits, co
              float* __restrict__ entropy, float* __restrict__ values, long long* __restrict__ indices) {
   const long long row = blockIdx.x;
   const float* mine = part + row * (parts * 3 + (LP_TOP ? LP_SEGMENTS : 0));
-  lp_finish(logits + row * LP_STRIDE, row, [&] { return lp_total((const LpSum*)mine, (int)parts); }, mine + parts * 3, tokens, logprob, entropy, values, indices);
+  auto sums = [&] {
+    // (each lane a part, or several)
+    LpSum a = {LP_LOW, 0.0f, 0.0f};
+    for (int i = threadIdx.x & 63; i < (int)parts; i += 64) a = lp_add(a, ((const LpSum*)mine)[i]);
+    return lp_all(a);
+  };
+  lp_finish(logits + row * LP_STRIDE, row, sums, mine + parts * 3, tokens, logprob, entropy, values, indices);
 #elif LP_SPLIT
 void LP_NAME(const lp_t* __restrict__ logits, long long parts, float* __restrict__ part) {
   __shared__ LpSum sums[LP_WAVES];
@@ -327,7 +352,7 @@ void LP_NAME(const lp_t* __restrict__ logits, long long parts, float* __restrict
   const int first = (int)(i * share), end = first + (int)share < LP_BLOCKS ? first + (int)share : LP_BLOCKS;
   float* mine = part + row * (parts * 3 + (LP_TOP ? LP_SEGMENTS : 0));
   lp_scan(logits + row * LP_STRIDE, first, end, sums, mine + parts * 3);
-  if (threadIdx.x == 0) ((LpSum*)mine)[i] = lp_total(sums, LP_WAVES);
+  if (threadIdx.x == 0) ((LpSum*)mine)[i] = lp_total(sums);
 #else
 void LP_NAME(const lp_t* __restrict__ logits, const long long* __restrict__ tokens, float* __restrict__ logprob, float* __restrict__ entropy,
              float* __restrict__ values, long long* __restrict__ indices) {
@@ -339,6 +364,6 @@ void LP_NAME(const lp_t* __restrict__ logits, const long long* __restrict__ toke
 #endif
   const long long row = blockIdx.x;
   lp_scan(logits + row * LP_STRIDE, 0, LP_BLOCKS, sums, segments);
-  lp_finish(logits + row * LP_STRIDE, row, [&] { return lp_total(sums, LP_WAVES); }, segments, tokens, logprob, entropy, values, indices);
+  lp_finish(logits + row * LP_STRIDE, row, [&] { return lp_total(sums); }, segments, tokens, logprob, entropy, values, indices);
 #endif
 }

@@ -777,11 +777,13 @@ def _add_adapters_launch(y, x, a, b, which, scale, inplace, cfg):
     params = dict(N=n, K=k, RANK=rank, F16=int(x.dtype == torch.float16), Y_F32=int(y.dtype == torch.float32), XT=x.stride(0) if tokens > 1 else 0, YT=yt, ZT=zt,
                   ALIGN=int((y.data_ptr() | yt * size | zt * size) % 16 == 0), SCALES=int(scale is not None), INPLACE=int(inplace),
                   **{**_add_adapters_form(tokens, adapters, n, k, rank, 256 // size), **cfg})
-    slots, across = params.pop("S"), min(params.pop("NS"), -(-n * size // 256))
-    params["MANY"] = int(slots > 1)
-    if slots < 1 or across < 1:
+    slots, across = params.pop("S"), params.pop("NS")
+    if slots < 1 or across < 1 or params["UT"] not in (1, 2, 4) or params["TS"] not in (1, 2, 4):
         raise ValueError("bad kernel parameters")
-    grids = [-(-tokens // (16 * max(1, params[tile]))) * slots * by for tile, by in (("TS", params["KS"]), ("UT", across))]
+    passes = -(-n // (256 // size * 4 // params["UT"]))
+    across = min(across, passes)
+    params.update(MANY=int(slots > 1), ONCE=int(across == passes))
+    grids = [-(-tokens // (16 * params[tile])) * slots * by for tile, by in (("TS", params["KS"]), ("UT", across))]
     if max(grids) > 0x7FFFFFFF:
         raise ValueError("too many tokens for one launch")
     down, up = (R.get_kernel(family, **params).bind(grid=(grid,)) for family, grid in zip(("adapters_down", "adapters_up"), grids))
