@@ -462,7 +462,8 @@ def cache_append(q, k, v, k_cache, v_cache, k_scale, v_scale, slots, positions, 
     gives them; rotation: fp32 [P, R], row p the cosines of position p's R / 2 angles, then their sines, R a multiple of 16 up to d.  The first R numbers of
     a head are R / 2 pairs (x, y) that become (x cos - y sin, y cos + x sin): numbers i and i + R / 2, or 2 i and 2 i + 1 (interleaved).
     Returns the turned queries, contiguous, in q's type.  A row without a position (-1) is left unturned, padding for instance; a position behind the
-    table's last makes the numbers that it would turn NaN.  A key's 8 bits, and its page's scale, are those of the formula in 64 bits."""
+    table's last makes the numbers that it would turn NaN.  A key's 8 bits, and its page's scale, are those of the formula in 64 bits (for numbers from
+    2^-126 on; one that grows beyond fp32's range counts as an infinity)."""
     interleaved = bool(interleaved)
     key = ("cache_append", R.signature(q, k, v, k_cache, v_cache, k_scale, v_scale, slots, positions, rotation), interleaved)
     run = _bound.get(key)

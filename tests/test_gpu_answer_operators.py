@@ -135,6 +135,24 @@ def test_cache_append_of_infinities_and_zeros():
     check_append(q, k, v, caches, scales, slots, [5, 6, 7, 8], angles(10, 32), False)
 
 
+def test_cache_append_offsets_beyond_32_bits():
+    """Pages behind 2^31 bytes of the cache, and rows of queries, keys and values that lie 2^29 numbers apart."""
+    page, heads, d, pages = 16, 8, 256, 70000
+    caches, scales = [torch.zeros((pages, page, heads, d), device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2)], [torch.zeros((pages, heads), device="cuda") for _ in range(2)]
+    far = torch.empty((6, 1 << 29), device="cuda", dtype=torch.bfloat16)
+    rows = far[:, :(4 + 2 * heads) * d].view(6, 4 + 2 * heads, d)
+    rows.copy_(torch.randn(rows.shape, generator=generator(4), device="cuda"))
+    q, k, v = rows.split((4, heads, heads), 1)
+    slots, where, table = [page * 7 + page - 1, page * 7 + 1, page * 5, page * 5 + 1, page * 5 + 2, -1], ints([3, 900, 0, 1, 2, 5]), angles(1000, 64)
+    at = ints(slots, torch.int64)
+    want_q, want_k = turned(q, where, table, False), turned(k, where, table, False)
+    want = [plain_write(x, c[-8:], s[-8:], at, page) for x, c, s in ((want_k, caches[0], scales[0]), (v, caches[1], scales[1]))]
+    got = ops.cache_append(q, k, v, *caches, *scales, torch.where(at < 0, at, at + (pages - 8) * page), where, table)
+    assert bool(((got.double() - want_q).abs() <= 2.0 ** -8 * want_q.abs() + 2.0 ** -20).all())       # (half a step, and the sums' 2^-23 of numbers below 8)
+    for c, s, (w, ws) in zip(caches, scales, want):
+        assert torch.equal(s[-8:].double(), ws) and same(values(c[-8:]), w) and not bool(s[:-8].any()) and not bool(c[:-8].view(torch.uint8).any())
+
+
 def test_cache_append_then_attention_sees_distances_only():
     """Rotated queries and keys: scores go by the distance, so a prompt moved along the positions has the same answers."""
     d, page, tokens = 64, 16, 40
@@ -276,6 +294,14 @@ def test_add_adapters_offsets_beyond_32_bits():
     check_adapters(got, y, x, small_a, small_b, ints([0, 1, -1]), None)
 
 
+def test_add_adapters_to_what_it_reads():
+    """In place, x the same tensor as y."""
+    _, x, a, b, which, scale = adapters_case(3, 50, 512, 512, 16, 5, "f16", "f16")
+    want = ops.add_adapters(x, x, a, b, which, scale)
+    y = x.clone()
+    assert ops.add_adapters(y, y, a, b, which, scale, inplace=True) is y and torch.equal(y, want)
+
+
 # ---- token_logprobs ----
 
 def check_logprobs(got, logits, tokens, top, terms=600):
@@ -389,6 +415,15 @@ def test_token_logprobs_of_rows_that_lie_apart_and_are_alike():
 
 
 # ---- what is refused, other streams, nothing to do ----
+
+@pytest.mark.parametrize("parts", [1, 3])
+def test_token_logprobs_offsets_beyond_32_bits(parts):
+    far = torch.empty((4, (1 << 30) + 5), device="cuda", dtype=torch.bfloat16)
+    logits = far[:, :20011]
+    logits.copy_(torch.randn(logits.shape, generator=generator(9), device="cuda") * 3)
+    tokens = ints([0, 20010, 7, 20011], torch.int64)
+    check_logprobs(ops.token_logprobs(logits, tokens, 6, PARTS=parts), logits, tokens, 6)
+
 
 def refused(call, good, bads):
     call(**good)
