@@ -141,11 +141,11 @@ __device__ __forceinline__ float lp_value(lp_key k) {
   return __builtin_bit_cast(float, up ^ (up >> 31 ? 0x80000000u : 0xffffffffu));
 }
 __device__ __forceinline__ int lp_index(lp_key k) { return 0x7ffff - (int)(__builtin_bit_cast(unsigned long long, k) & 0x7ffff); }
-#define LP_LIST 256                                                              // keys that are counted out against one another
+#define LP_LIST (LP_WAVES * LP_TOP > 256 ? LP_WAVES * LP_TOP : 256)               // keys that are counted out against one another
 #define LP_E1 ((LP_SEGMENTS + LP_THREADS - 1) / LP_THREADS)                      // segments of a thread
 #define LP_E2 ((LP_TOP * 16 + LP_THREADS - 1) / LP_THREADS)                      // and vectors, when they are read again
 struct LpPick {
-  lp_key list[2][LP_LIST + 32], found[2][LP_TOP], wave[2][LP_WAVES];
+  lp_key list[2][LP_LIST + 32], found[2][LP_TOP];
   __attribute__((aligned(16))) float best[LP_THREADS / 2];
   float bound[LP_WAVES], share[LP_WAVES];
   int many[2];
@@ -161,6 +161,23 @@ __device__ __forceinline__ float lp_least(float v) {
   v = fminf(v, LP_DPP(most, v, 0x118, 0xf));
   v = fminf(v, LP_DPP(most, v, 0x142, 0xa));
   return fminf(v, LP_DPP(most, v, 0x143, 0xc));
+}
+// The largest of the lanes' numbers, of their keys (first by the upper half).
+__device__ __forceinline__ unsigned lp_most(unsigned v) {
+#define LP_MAX(control, rows) { const unsigned o = __builtin_amdgcn_update_dpp(0, (int)v, control, rows, 0xf, false); v = v > o ? v : o; }
+  LP_MAX(0x111, 0xf)
+  LP_MAX(0x112, 0xf)
+  LP_MAX(0x114, 0xf)
+  LP_MAX(0x118, 0xf)
+  LP_MAX(0x142, 0xa)
+  LP_MAX(0x143, 0xc)
+#undef LP_MAX
+  return __builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ lp_key lp_most(lp_key v) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+  const unsigned high = lp_most((unsigned)(b >> 32)), low = lp_most((unsigned)(b >> 32) == high ? (unsigned)b : 0u);
+  return __builtin_bit_cast(double, (unsigned long long)high << 32 | low);
 }
 // What LP_TOP of the workgroup's numbers reach (or all).  Of each wavefront's 32 pairs of lanes the LP_TOP-th largest is such a bound, the largest of these
 // too; and so is the least of the wavefronts' LP_SHARE-th largest, which reach LP_TOP together: closer where the numbers are spread evenly (of 2000
@@ -215,27 +232,10 @@ template <int E, class Index> __device__ __forceinline__ void lp_pick(LpPick& p,
     }
   }
   __syncthreads();
-  const int n = p.many[turn];
-  if (n <= LP_LIST) {
-    // four lanes count how many are above one of them
-#pragma unroll 1
-    for (int i = threadIdx.x / 4; i < n; i += LP_THREADS / 4) {
-      const lp_key k = p.list[turn][i];
-      int r = 0;
-#pragma unroll 1
-      for (int j = 0; j < n; j += 32) {
-        lp_key other[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) other[e] = p.list[turn][j + e * 4 + lane % 4];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) r += other[e] > k;
-      }
-      r += LP_SWAP(r, 0xb1);
-      r += LP_SWAP(r, 0x4e);
-      if (r < LP_TOP && lane % 4 == 0) p.found[turn][r] = k;
-    }
-  } else {
-    // many equal ones, or the largest ones all in few threads: one after the other
+  int n = p.many[turn];
+  if (n > LP_LIST) {
+    // many equal ones (of masked numbers, say), or the largest ones all in few threads: each wavefront's, one after the other
+    n = LP_WAVES * LP_TOP;
     lp_key last = 2.0;
 #pragma unroll 1
     for (int t = 0; t < LP_TOP; ++t) {
@@ -243,17 +243,30 @@ template <int E, class Index> __device__ __forceinline__ void lp_pick(LpPick& p,
 #pragma unroll
       for (int q = 0; q < E; ++q) {
         const lp_key k = index(q) >= 0 ? lp_order(v[q], index(q)) : 0.0;
-        best = k < last ? fmax(best, k) : best;
+        best = k < last && k > best ? k : best;
       }
-#pragma unroll
-      for (int by = 32; by > 0; by >>= 1) best = fmax(best, __shfl_xor(best, by, 64));
-      if (lane == 0) p.wave[t & 1][wave] = best;
-      __syncthreads();
-      last = 0.0;
-#pragma unroll
-      for (int w = 0; w < LP_WAVES; ++w) last = fmax(last, p.wave[t & 1][w]);
-      if (threadIdx.x == 0) p.found[turn][t] = last;
+      last = lp_most(best);
+      if (lane == 0) p.list[turn][wave * LP_TOP + t] = last;
     }
+    for (int i = n + threadIdx.x; i < LP_LIST + 32; i += LP_THREADS) p.list[turn][i] = 0.0;
+    __syncthreads();
+  }
+  // four lanes count how many are above one of them
+#pragma unroll 1
+  for (int i = threadIdx.x / 4; i < n; i += LP_THREADS / 4) {
+    const lp_key k = p.list[turn][i];
+    int r = 0;
+#pragma unroll 1
+    for (int j = 0; j < n; j += 32) {
+      lp_key other[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) other[e] = p.list[turn][j + e * 4 + lane % 4];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r += other[e] > k;
+    }
+    r += LP_SWAP(r, 0xb1);
+    r += LP_SWAP(r, 0x4e);
+    if (r < LP_TOP && lane % 4 == 0) p.found[turn][r] = k;
   }
   __syncthreads();
 }
