@@ -34,11 +34,24 @@ __device__ __forceinline__ LpSum lp_add(LpSum a, LpSum b) {
   // (a difference that is no longer finite belongs to a factor of 0)
   return {m, fa * a.s + fb * b.s, fa * (a.u + fmaxf(a.m - m, -1e30f) * a.s) + fb * (b.u + fmaxf(b.m - m, -1e30f) * b.s)};
 }
+#define LP_DPP(old, v, control, rows) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, v), control, rows, 0xf, false))
+// row_shr 1, 2, 4, 8, then a row's last lane into the next row, the second row's into the others: lane 63 has what is of all lanes
+#define LP_LANES(STEP) STEP(0x111, 0xf) STEP(0x112, 0xf) STEP(0x114, 0xf) STEP(0x118, 0xf) STEP(0x142, 0xa) STEP(0x143, 0xc)
+__device__ __forceinline__ float lp_last(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63)); }
 // Of all lanes.
 __device__ __forceinline__ LpSum lp_all(LpSum a) {
-#pragma unroll
-  for (int by = 32; by > 0; by >>= 1) a = lp_add(a, {__shfl_xor(a.m, by, 64), __shfl_xor(a.s, by, 64), __shfl_xor(a.u, by, 64)});
-  return a;
+  float m = a.m, s, u;
+#define LP_STEP(control, rows) m = fmaxf(m, LP_DPP(LP_LOW, m, control, rows));
+  LP_LANES(LP_STEP)
+#undef LP_STEP
+  m = lp_last(m);
+  const float d = a.m - m, f = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+  s = f * a.s;
+  u = f * (a.u + fmaxf(d, -1e30f) * a.s);
+#define LP_STEP(control, rows) s += LP_DPP(0.0f, s, control, rows); u += LP_DPP(0.0f, u, control, rows);
+  LP_LANES(LP_STEP)
+#undef LP_STEP
+  return {m, lp_last(s), lp_last(u)};
 }
 // Elements of a row that lie in front of its first aligned vector's begin, as a number of that vector's elements.
 __device__ __forceinline__ int lp_offset(const lp_t* x) { return LP_SHIFT ? (int)((size_t)x / LP_ES % LP_VW) : 0; }
@@ -69,10 +82,15 @@ __device__ __forceinline__ void lp_scan(const lp_t* __restrict__ x, int first, i
     float v[LP_U][LP_VW], top[LP_U], most = a.m;
 #pragma unroll
     for (int j = 0; j < LP_U; ++j) {
-      const bool edge = b + j < end && !inside(b + j);
 #pragma unroll
-      for (int i = 0; i < LP_VW; ++i) v[j][i] = b + j < end && LP_V >= 2 * LP_VW ? (float)next[j][i] : -__builtin_inff();
-      if (edge) lp_edge(x, ((b + j) * 64 + lane) * LP_VW - o, v[j]);
+      for (int i = 0; i < LP_VW; ++i) v[j][i] = LP_V >= 2 * LP_VW ? (float)next[j][i] : -__builtin_inff();
+      if (b + j >= end) {
+        asm volatile("");        // (a branch, not a choice for each number)
+#pragma unroll
+        for (int i = 0; i < LP_VW; ++i) v[j][i] = -__builtin_inff();
+      } else if (!inside(b + j)) {
+        lp_edge(x, ((b + j) * 64 + lane) * LP_VW - o, v[j]);
+      }
     }
     fetch(b + LP_WAVES * LP_U);
 #pragma unroll
@@ -150,28 +168,19 @@ struct LpPick {
   float bound[LP_WAVES], share[LP_WAVES];
   int many[2];
 };
-#define LP_DPP(old, v, control, rows) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, v), control, rows, 0xf, false))
 #define LP_SWAP(v, control) __builtin_amdgcn_update_dpp(0, v, control, 0xf, 0xf, true)       // (quad_perm 1 0 3 2 is 0xb1, 2 3 0 1 is 0x4e)
 // Least of the lanes' numbers, in lane 63.
 __device__ __forceinline__ float lp_least(float v) {
-  const float most = __builtin_inff();
-  v = fminf(v, LP_DPP(most, v, 0x111, 0xf));        // row_shr 1, 2, 4, 8, then a row's last lane into the next row, the second row's into the others
-  v = fminf(v, LP_DPP(most, v, 0x112, 0xf));
-  v = fminf(v, LP_DPP(most, v, 0x114, 0xf));
-  v = fminf(v, LP_DPP(most, v, 0x118, 0xf));
-  v = fminf(v, LP_DPP(most, v, 0x142, 0xa));
-  return fminf(v, LP_DPP(most, v, 0x143, 0xc));
+#define LP_STEP(control, rows) v = fminf(v, LP_DPP(__builtin_inff(), v, control, rows));
+  LP_LANES(LP_STEP)
+#undef LP_STEP
+  return v;
 }
 // The largest of the lanes' numbers, of their keys (first by the upper half).
 __device__ __forceinline__ unsigned lp_most(unsigned v) {
-#define LP_MAX(control, rows) { const unsigned o = __builtin_amdgcn_update_dpp(0, (int)v, control, rows, 0xf, false); v = v > o ? v : o; }
-  LP_MAX(0x111, 0xf)
-  LP_MAX(0x112, 0xf)
-  LP_MAX(0x114, 0xf)
-  LP_MAX(0x118, 0xf)
-  LP_MAX(0x142, 0xa)
-  LP_MAX(0x143, 0xc)
-#undef LP_MAX
+#define LP_STEP(control, rows) { const unsigned o = __builtin_amdgcn_update_dpp(0, (int)v, control, rows, 0xf, false); v = v > o ? v : o; }
+  LP_LANES(LP_STEP)
+#undef LP_STEP
   return __builtin_amdgcn_readlane((int)v, 63);
 }
 __device__ __forceinline__ lp_key lp_most(lp_key v) {
@@ -306,8 +315,12 @@ template <class Sums> __device__ __forceinline__ void lp_finish(const lp_t* __re
     at[q] = k > 0.0 ? (lp_index(k) * 16 + i % 16) * LP_VW - o : LP_V;
     if (LP_V >= 2 * LP_VW) raw[q] = *(const lp_vec*)(x + (at[q] >= 0 && at[q] + LP_VW <= LP_V ? at[q] : (LP_VW - o) % LP_VW));
   }
-  const LpSum a = sums();
-  const float ln = logf(a.s);
+  LpSum a = {};
+  float ln = 0.0f;
+  if (__builtin_amdgcn_readfirstlane(threadIdx.x) < 64) {        // (the first wavefront, which gives the results)
+    a = sums();
+    ln = logf(a.s);
+  }
   float w[LP_E2 * LP_VW];
   best = none;
 #pragma unroll
@@ -334,6 +347,7 @@ template <class Sums> __device__ __forceinline__ void lp_finish(const lp_t* __re
     indices[row * LP_TOP + threadIdx.x] = lp_index(k);
   }
 #else
+  if (__builtin_amdgcn_readfirstlane(threadIdx.x) >= 64) return;
   const LpSum a = sums();
   const float ln = logf(a.s);
 #endif
