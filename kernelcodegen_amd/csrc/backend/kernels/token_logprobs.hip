@@ -6,6 +6,8 @@
 //
 // One pass over the row.  Each lane keeps m, s and u of what it has seen and brings s and u to a new maximum once for LP_U vectors:
 //   s' = s e^(m - m'),  u' = (u + (m - m') s) e^(m - m')
+// What a vector adds takes one instruction before its exponent: t = x log2 e - c with c = m log2 e rounded; what c lacks of it is known and divided out behind
+// all of them.  From |m| = 2^30 on that would pass the exponent's range, and numbers that differ lie 64 or more apart: any other factor than log2 e does.
 // m begins at the least finite number, not at -inf, so that x - m is never inf - inf for x = -inf.
 // The alternatives need no second pass: the pass leaves the largest number of each segment of 16 vectors (a DPP row of lanes), and the LP_TOP
 // largest numbers lie in the LP_TOP segments with the largest ones (ties to the lower segment, whose numbers come first), which are read again.
@@ -23,6 +25,7 @@ typedef LP_T lp_t;
 #define LP_WAVES (LP_THREADS / 64)
 #define LP_LOW (-3.402823466e38f)
 #define LP_LOG2E 1.4426950408889634f
+#define LP_LN2 0.6931471805599453f
 typedef lp_t lp_vec __attribute__((ext_vector_type(LP_VW)));
 typedef double lp_key;
 
@@ -101,17 +104,30 @@ __device__ __forceinline__ void lp_scan(const lp_t* __restrict__ x, int first, i
       most = fmaxf(most, top[j]);
     }
     const float change = a.m - most, factor = __builtin_amdgcn_exp2f(change * LP_LOG2E);
-    a.u = factor * (a.u + fmaxf(change, -1e30f) * a.s);
-    a.s *= factor;
-    a.m = most;
+    const bool far = __builtin_fabsf(most) >= 1073741824.0f;
+    const float by = far ? 1.0f : LP_LOG2E, c = most * by, rest = __builtin_fmaf(most, by, -c), back = __builtin_amdgcn_exp2f(-rest);
+    float s = 0.0f, u = 0.0f;
 #pragma unroll
     for (int j = 0; j < LP_U; ++j)
 #pragma unroll
       for (int i = 0; i < LP_VW; ++i) {
-        const float d = v[j][i] - most, e = __builtin_amdgcn_exp2f(d * LP_LOG2E);
-        a.s += e;
-        a.u = __builtin_fmaf(fmaxf(d, -1e30f), e, a.u);          // (-inf times 0)
+        const float t = __builtin_fmaf(v[j][i], by, -c), e = __builtin_amdgcn_exp2f(t);
+        s += e;
+        u = __builtin_fmaf(t, e, u);
       }
+    if (__ballot(u != u)) {                   // (-inf times 0, mostly)
+      u = 0.0f;
+#pragma unroll
+      for (int j = 0; j < LP_U; ++j)
+#pragma unroll
+        for (int i = 0; i < LP_VW; ++i) {
+          const float t = __builtin_fmaf(v[j][i], by, -c);
+          u = __builtin_fmaf(fmaxf(t, -1e30f), __builtin_amdgcn_exp2f(t), u);
+        }
+    }
+    a.u = __builtin_fmaf(factor, a.u + fmaxf(change, -1e30f) * a.s, (u - rest * s) * (back * LP_LN2));
+    a.s = __builtin_fmaf(factor, a.s, s * back);
+    a.m = most;
 #if LP_TOP
 #pragma unroll
     for (int j = 0; j < LP_U; ++j) {

@@ -403,6 +403,22 @@ def test_token_logprobs_of_masks_infinities_and_nan(dtype, parts):
     check_logprobs(ops.token_logprobs(logits, tokens, 12, PARTS=parts), logits, tokens, 12)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_token_logprobs_of_large_numbers(dtype):
+    """Rows around numbers of any size and sign, which are apart by single steps of the type, a few, or as usual."""
+    g = generator(12)
+    around = [3.0, 1e3, 1e6, 2.0 ** 23, 2.0 ** 29, 2.0 ** 30 * (1 - 2.0 ** -24), 2.0 ** 30, 2.0 ** 31, 1e12, 1e38, 3e38]
+    at = torch.tensor(around + [-x for x in around], device="cuda").to(DTYPE[dtype])
+    step = torch.frexp(at.float()).exponent - (24 if dtype == "f32" else 8)
+    n = torch.randint(-9, 10, (len(at), 5003), generator=g, device="cuda")
+    logits = torch.cat([(at.double()[:, None] + n * m * torch.exp2(step.double())[:, None]) for m in (1, 7, 300)] + [at.double()[:, None] + n.double()]).to(DTYPE[dtype])
+    tokens = torch.randint(0, 5003, (len(logits),), generator=g, device="cuda")
+    for parts in (1, 3):
+        check_logprobs(ops.token_logprobs(logits, tokens, 4, PARTS=parts), logits, tokens, 4)
+    logits[:, ::3] = -math.inf
+    check_logprobs(ops.token_logprobs(logits, tokens, 4), logits, tokens, 4)
+
+
 def test_token_logprobs_of_rows_that_lie_apart_and_are_alike():
     wide = torch.randn((20, 6000), generator=generator(1), device="cuda").half()
     tokens = torch.arange(10, device="cuda") * 17
