@@ -18,7 +18,7 @@
 // with c and s of row `position` of the table.  What becomes of a key jumps where 8 bits do, so it has to be the formula's: the two products
 // are exact in fp64 and their sum is rounded there once; on the way to fp32 what is cut off leaves its trace in the last bit (rounding to odd), so the
 // rounding to 8 bits is that of the 53-bit number, and so is the comparison with 448 that gives the scale.  Queries, whose results have 16 or 32
-// bits, are summed in fp32 (all of it in fp64: 7200 tokens of 32 query heads 79 us, this way 50).  Wavefronts behind those of the cache take
+// bits, are summed in fp32 (all of it in fp64: 10240 tokens of 32 query heads, 8 others, 79 us, this way 43, 5.4 TB/s).  Wavefronts behind those of the cache take
 // a token's queries, CW_QN passes of CW_RPP heads for one reading of c and s.
 // Measured, 8 heads of 128: 64 tokens of a page each 2.9 us (an empty launch 1.7); 9000 tokens of whole pages, half precision, 12.5 us, 4.4 TB/s.
 // Parameters: CW_NAME, CW_H, CW_D, CW_PAGE, CW_T (input type), CW_ESIZE, CW_WIN, strides as in cache_attention: CW_KP .. CW_VH (bytes), CW_XKT

@@ -856,7 +856,7 @@ def _token_logprobs_launch(logits, tokens, top, cfg):
         return None, None, 1
     stride, size = logits.stride(0) if rows > 1 else 0, logits.element_size()
     params = dict(V=v, F16=_STORAGE[logits.dtype], TOP=top, STRIDE=stride, SHIFT=int((stride * size | logits.data_ptr()) % 16 != 0),
-                  **{**_token_logprobs_form(rows, v * size, top), **cfg})
+                  **{**_token_logprobs_form(rows, v * size), **cfg})
     parts = params.pop("PARTS")
     if not 1 <= parts <= 1024:
         raise ValueError("a row has 1 to 1024 parts")
@@ -872,15 +872,16 @@ def _token_logprobs_launch(logits, tokens, top, cfg):
     return _into_last(kern.bind(grid=(rows * parts,)), ((floats,), torch.float32)), _into_last(join, *results), parts
 
 
-def _token_logprobs_form(rows, bytes_, top):
+def _token_logprobs_form(rows, bytes_):
     """Workgroups of a row, their threads, and vectors that a lane has under way.
 
     Fewer long rows than units are cut into about 1024 parts of 8 KiB or more, and a second launch finishes them.  Others have a workgroup each,
-    which is the smaller the more of them wait for their alternatives beside others that read.  Measured, in us, both launches:
-      16 rows, bf16, top 5: of 16000 a workgroup each 7.2, parts 9.1;  32000: 8.8 and 9.3;  64000: 11.2 and 9.2;  128000: 16.8 and 11.1
-      200 rows: of 32000 9.3 and 12.7;  64000: 12.3 and 15.1;  128000: 18.3 and 19.1;  64 of 128000, fp32, top 20: 16 parts 16.6, 8 parts 18.9, whole 24
-      500 of 50021, half, top 10: a workgroup of 256 threads each 19.5, of 512 19.3, 2 parts 20.7
-      2000 of 32000, bf16, top 20: of 512 threads 42, 256 40, 128 37.3;  top 5: 256 35.5, 128 33.1;  top 0: 512 28.5, 256 30"""
+    which is the smaller the more of them wait for their sums and alternatives beside others that read.  Measured, in us, both launches:
+      16 of 64000, bf16: a workgroup each 6.4, parts 5.6, with 5 alternatives 10 and 8.5;  200 of 32000: 5.6 and 7.8, 8.6 and 10.9
+      64 of 128000, fp32: whole 13.6 (1024 threads), in 16 parts 10.8, in 8 of 512 threads 10.5;  with 20 alternatives 18.9, 14.4, 14.2
+      500 of 50021, half: of 512 threads 12.7, 256 15.0, in 2 parts 15.1;  with 10 alternatives 17.3, 17.8, 20.3
+      700 of 1500, fp32, 5 alternatives: of 512 threads 6.8, 256 5.9;  5000 of 4096, bf16: 512 14.8, 256 11.6, 128 12.1;  with 5 alternatives 31, 21, 18.6
+      2000 of 32000, bf16: of 512 threads 29.2, 256 29.7, 128 27.1;  with 20 alternatives 39.8, 37.7, 34.8"""
     if rows < 256 and bytes_ > (98304 if rows < 64 else 196608):
         return dict(PARTS=min(-(-1024 // rows), bytes_ // 8192, 64), THREADS=256, U=2)
-    return dict(PARTS=1, THREADS=512 if top == 0 or rows < 256 else 128 if rows >= 1024 and bytes_ <= 1 << 18 else 256, U=2)
+    return dict(PARTS=1, THREADS=128 if rows >= 1024 and bytes_ <= 1 << 18 else 256 if rows >= 256 and bytes_ <= 32768 else 512, U=2)
