@@ -77,7 +77,7 @@ __device__ __forceinline__ void lp_scan(const lp_t* __restrict__ x, int first, i
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, o = lp_offset(x);
   LpSum a = {LP_LOW, 0.0f, 0.0f};
   // Blocks that lie within the row are under way while those before them are counted; in the place of others the row's first whole vector is read.
-  lp_vec next[LP_U];
+  lp_vec next[LP_U] = {};
   auto inside = [&](int b) { return LP_V >= 2 * LP_VW && b < end && b * (64 * LP_VW) >= o && (b + 1) * (64 * LP_VW) - o <= LP_V; };
   auto fetch = [&](int b) {
     if (LP_V < 2 * LP_VW) return;
@@ -87,19 +87,24 @@ __device__ __forceinline__ void lp_scan(const lp_t* __restrict__ x, int first, i
   fetch(first + wave * LP_U);
   for (int b = first + wave * LP_U; b < end; b += LP_WAVES * LP_U) {
     float v[LP_U][LP_VW], top[LP_U], most = a.m;
+    bool whole = true;
 #pragma unroll
-    for (int j = 0; j < LP_U; ++j) {
+    for (int j = 0; j < LP_U; ++j) whole = whole && inside(b + j);
+    if (whole) {
 #pragma unroll
-      for (int i = 0; i < LP_VW; ++i) v[j][i] = LP_V >= 2 * LP_VW ? (float)next[j][i] : -__builtin_inff();
-      if (b + j >= end) {
-        asm volatile("");        // (a branch, not a choice for each number)
+      for (int j = 0; j < LP_U; ++j)
 #pragma unroll
-        for (int i = 0; i < LP_VW; ++i) v[j][i] = -__builtin_inff();
-      } else if (!inside(b + j)) {
-        lp_edge(x, ((b + j) * 64 + lane) * LP_VW - o, v[j]);
+        for (int i = 0; i < LP_VW; ++i) v[j][i] = (float)next[j][i];
+    } else {
+#pragma unroll
+      for (int j = 0; j < LP_U; ++j) {
+#pragma unroll
+        for (int i = 0; i < LP_VW; ++i) v[j][i] = inside(b + j) ? (float)next[j][i] : -__builtin_inff();
+        if (b + j < end && !inside(b + j)) lp_edge(x, ((b + j) * 64 + lane) * LP_VW - o, v[j]);
       }
     }
     fetch(b + LP_WAVES * LP_U);
+    asm volatile("" ::: "memory");        // (else the loads would be put where the next iteration begins)
 #pragma unroll
     for (int j = 0; j < LP_U; ++j) {
       top[j] = v[j][0];
