@@ -236,13 +236,18 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
         const int c = (s * 4 + g) % AD_CHUNKS * 8;
 #pragma unroll
         for (int e = 0; e < 8; ++e) h[s][e] = 0.0f;
+        kcg_f32x4 parts[AD_KS][2];
 #pragma unroll
         for (int p = 0; p < AD_KS; ++p) {
           const kcg_f32x4* at = (const kcg_f32x4*)(part + ((long long)p * T + t) * AD_RANK + c);
-          const kcg_f32x4 one = at[0], two = at[1];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) h[s][e] += one[e], h[s][4 + e] += two[e];
+          parts[p][0] = at[0];
+          parts[p][1] = at[1];
         }
+        __builtin_amdgcn_sched_barrier(0);        // (all on their way before the first is waited for)
+#pragma unroll
+        for (int p = 0; p < AD_KS; ++p)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) h[s][e] += parts[p][e / 4][e % 4];
 #pragma unroll
         for (int e = 0; e < 8; ++e) most = fmaxf(most, __builtin_fabsf(h[s][e]));
       }
