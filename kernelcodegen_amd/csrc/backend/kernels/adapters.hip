@@ -32,36 +32,48 @@ typedef unsigned long long ad_mask;
 #define AD_JT ((AD_RANK + 15) / 16)                // tiles of the rank
 #define AD_TILE (16 * AD_TS)
 
-// Calls each(r, mask of the tile's tokens) for the adapters of a tile that are this workgroup's; returns the mask of the tokens that have one.
-template <class Each> __device__ __forceinline__ ad_mask ad_adapters(const int* __restrict__ which, long long t0, long long T, long long adapters, int slot, int slots, Each each) {
-  const int lane = threadIdx.x & 63;
-  const int mine = lane < AD_TILE && t0 + lane < T ? which[t0 + lane] : -1;
-  const ad_mask with = __ballot(mine >= 0 && mine < adapters);
+// The adapters of a tile that are this workgroup's, one after the other; `with`: the tile's tokens that have one.
+struct AdTurns {
+  int mine;
+  ad_mask with, todo;
 #if AD_MANY
-  // tokens that are the first ones with their adapter: lane by lane further away compared
-  int other = mine;
-  bool again = false;
-#pragma unroll
-  for (int d = 1; d < AD_TILE; ++d) {
-    other = __builtin_amdgcn_update_dpp(-1, other, 0x138, 0xf, 0xf, false);        // wave_shr 1
-    again |= other == mine;
-  }
-  const ad_mask first = __ballot(!again) & with;
-  const int turn = __builtin_amdgcn_mbcnt_hi((unsigned)(first >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)first, 0));
-  for (int n = slot; n < __builtin_popcountll(first); n += slots) {
-    const int r = __builtin_amdgcn_readlane(mine, __builtin_ctzll(__ballot(turn == n) & first));
-    each(r, __ballot(mine == r));
-  }
-#else
-  for (ad_mask todo = with; todo;) {
-    const int r = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
-    const ad_mask same = __ballot(mine == r);
-    todo &= ~same;
-    each(r, same);
-  }
+  int turn, n, slots;
 #endif
-  return with;
-}
+  __device__ __forceinline__ AdTurns(const int* __restrict__ which, long long t0, long long T, long long adapters, int slot, int slots_) {
+    const int lane = threadIdx.x & 63;
+    mine = lane < AD_TILE && t0 + lane < T ? which[t0 + lane] : -1;
+    todo = with = __ballot(mine >= 0 && mine < adapters);
+#if AD_MANY
+    // tokens that are the first ones with their adapter: lane by lane further away compared
+    int other = mine;
+    bool again = false;
+#pragma unroll
+    for (int d = 1; d < AD_TILE; ++d) {
+      other = __builtin_amdgcn_update_dpp(-1, other, 0x138, 0xf, 0xf, false);        // wave_shr 1
+      again |= other == mine;
+    }
+    todo &= __ballot(!again);
+    turn = __builtin_amdgcn_mbcnt_hi((unsigned)(todo >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)todo, 0));
+    n = slot;
+    slots = slots_;
+#endif
+  }
+  // The next one's number and its tokens.
+  __device__ __forceinline__ bool next(int& r, ad_mask& same) {
+#if AD_MANY
+    if (n >= __builtin_popcountll(todo)) return false;
+    r = __builtin_amdgcn_readlane(mine, __builtin_ctzll(__ballot(turn == n) & todo));
+    same = __ballot(mine == r);
+    n += slots;
+#else
+    if (!todo) return false;
+    r = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
+    same = __ballot(mine == r);
+    todo &= ~same;
+#endif
+    return true;
+  }
+};
 
 #if !AD_UP
 // A wavefront has its own part of k and brings it in whole lines, 64 k of eight rows a load: through LDS rows of its own, 16 bytes apart from a multiple
@@ -91,7 +103,10 @@ void AD_NAME(const ad_x* __restrict__ X, const ad_x* __restrict__ A, const int* 
     x[c] = X + (t < T ? t : T - 1) * AD_XT;
   }
   const int first = (ks * 4 + wave) * AD_SHARE, end = first + AD_SHARE < AD_STEPS ? first + AD_SHARE : AD_STEPS;
-  ad_adapters(which, t0, T, adapters, slot, (int)slots, [&](int r, ad_mask same) {
+  AdTurns turns(which, t0, T, adapters, slot, (int)slots);
+  int r;
+  ad_mask same;
+  while (turns.next(r, same)) {
     kcg_f32x4 acc[AD_TS][AD_JT];
 #pragma unroll
     for (int t = 0; t < AD_TS; ++t)
@@ -151,7 +166,7 @@ void AD_NAME(const ad_x* __restrict__ X, const ad_x* __restrict__ A, const int* 
       if ((same >> row & 1) && at < AD_RANK) *(kcg_f32x4*)(part + ((long long)ks * T + t0 + row) * AD_RANK + at) = sum;
     }
     __syncthreads();
-  });
+  }
 }
 #else
 typedef AD_YTYPE ad_y;
@@ -168,13 +183,14 @@ typedef ad_y ad_mem __attribute__((ext_vector_type(AD_C), aligned(AD_YSIZE)));  
 #define AD_OWN (AD_CHUNKS % 4 == 0 ? AD_CHUNKS / 4 : AD_STEPS)    // of which so many have other columns of B
 #define AD_GROUPS (4 / AD_TS)                       // wavefronts beside one another along N; AD_TS of them have 16 tokens each
 #define AD_STEP (AD_GROUPS * AD_COLS)              // columns of a workgroup
+#define AD_EVEN (AD_N % AD_STEP == 0)               // no column is behind the last
 #define AD_PITCH (AD_CHUNKS % 2 ? AD_RANK * 2 : AD_RANK * 2 + 16)  // of a row of B in LDS: an odd number of 16 bytes
 #define AD_LOADS ((AD_STEP * AD_CHUNKS + 255) / 256)
 
 // Columns n to n + AD_C of a row; elements of a vector that passes the row's end come one by one, all of them before any is put.
 __device__ __forceinline__ ad_yv ad_get(const ad_y* y, int n) {
   ad_yv v = {};
-  if (AD_N >= AD_C) v = *(const ad_mem*)(y + (n + AD_C <= AD_N ? n : 0));
+  if (AD_N >= AD_C) v = *(const ad_mem*)(y + (AD_EVEN || n + AD_C <= AD_N ? n : 0));
   if (AD_N % AD_C && n < AD_N && n + AD_C > AD_N) {
 #pragma unroll
     for (int e = 0; e < AD_C; ++e) v[e] = y[n + e < AD_N ? n + e : AD_N - 1];
@@ -184,9 +200,9 @@ __device__ __forceinline__ ad_yv ad_get(const ad_y* y, int n) {
 __device__ __forceinline__ void ad_put(ad_y* z, int n, ad_yv v, const float (&add)[AD_C]) {
 #pragma unroll
   for (int e = 0; e < AD_C; ++e) v[e] = (ad_y)((float)v[e] + add[e]);
-  if (n + AD_C <= AD_N) {
+  if (AD_EVEN || n + AD_C <= AD_N) {
     *(ad_mem*)(z + n) = v;
-  } else {
+  } else if (AD_N % AD_C) {
 #pragma unroll
     for (int e = 0; e < AD_C; ++e)
       if (n + e < AD_N) z[n + e] = v[e];
@@ -208,75 +224,86 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
   long long row[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) row[e] = tw + g * 4 + e < T ? tw + g * 4 + e : T - 1;
-  const ad_mask with = ad_adapters(which, t0, T, adapters, slot, (int)slots, [&](int r, ad_mask same) {
+  AdTurns turns(which, t0, T, adapters, slot, (int)slots);
+  int r;
+  ad_mask same;
+  kcg_u32x4 w[AD_LOADS], f[AD_STEPS];
+  ad_yv v[4];
+  float back = 1.0f, factor = 1.0f;
+  // B of an adapter's columns from nb on, and its scale; Y of them
+  auto fetch = [&](int r, int nb) {
     const ad_x* b = B + (long long)r * AD_N * AD_RANK;
-    const unsigned mine = (unsigned)(same >> (sub * 16)) & 0xffffu;
-    kcg_u32x4 w[AD_LOADS];
-    ad_yv v[4];
-    auto fetch = [&](int nb) {
 #pragma unroll
-      for (int c = 0; c < AD_LOADS; ++c) {
-        const int u = c * 256 + threadIdx.x, n = nb + u / AD_CHUNKS;
-        w[c] = *(const kcg_u32x4*)(b + (n < AD_N ? (long long)n * AD_RANK + u % AD_CHUNKS * 8 : 0));
-      }
-      if (mine) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = ad_get(Y + row[e] * AD_YT, nb + group * AD_COLS + i * AD_C);
-      }
-    };
-    fetch(ns * AD_STEP);
-    // h of this wavefront's tokens in numbers of 16 bits
-    kcg_u32x4 f[AD_STEPS];
-    kcg_f32x4 times = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (mine) {
-      const long long t = tw + i < T ? tw + i : T - 1;
-      float h[AD_STEPS][8], most = 0.0f;
-#pragma unroll
-      for (int s = 0; s < AD_STEPS; ++s) {
-        const int c = (s * 4 + g) % AD_CHUNKS * 8;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) h[s][e] = 0.0f;
-        kcg_f32x4 parts[AD_KS][2];
-#pragma unroll
-        for (int p = 0; p < AD_KS; ++p) {
-          const kcg_f32x4* at = (const kcg_f32x4*)(part + ((long long)p * T + t) * AD_RANK + c);
-          parts[p][0] = at[0];
-          parts[p][1] = at[1];
-        }
-        __builtin_amdgcn_sched_barrier(0);        // (all on their way before the first is waited for)
-#pragma unroll
-        for (int p = 0; p < AD_KS; ++p)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) h[s][e] += parts[p][e / 4][e % 4];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) most = fmaxf(most, __builtin_fabsf(h[s][e]));
-      }
-      float up = 1.0f, down = AD_SCALE ? scale[r] : 1.0f;
-      if (AD_F16) {
-        most = fmaxf(most, __shfl_xor(most, 16, 64));
-        most = fmaxf(most, __shfl_xor(most, 32, 64));
-        int e = (int)(__builtin_bit_cast(unsigned, most) >> 23) - 127;
-        e = e < -100 ? -100 : e > 126 ? 126 : e;
-        up = __builtin_bit_cast(float, (unsigned)(127 + 14 - e) << 23);
-        down *= __builtin_bit_cast(float, (unsigned)(127 - 14 + e) << 23);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) times[e] = AD_F16 ? __shfl(down, g * 4 + e, 64) : down;
-#pragma unroll
-      for (int s = 0; s < AD_STEPS; ++s) {
-        const int q = s * 4 + g;
-        ad_v o;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float a = h[s][e] * up;
-          const ad_x high = (ad_x)a;
-          const float left = a - (float)high;          // (nothing is left of an infinity)
-          const ad_x next = left - left == 0.0f ? (ad_x)left : (ad_x)0.0f, last = AD_PIECES > 2 && left - left == 0.0f ? (ad_x)(left - (float)next) : (ad_x)0.0f;
-          o[e] = q < AD_CHUNKS ? high : q < 2 * AD_CHUNKS ? next : q < AD_PIECES * AD_CHUNKS ? last : (ad_x)0.0f;
-        }
-        f[s] = __builtin_bit_cast(kcg_u32x4, o);
-      }
+    for (int c = 0; c < AD_LOADS; ++c) {
+      const int u = c * 256 + threadIdx.x, n = nb + u / AD_CHUNKS;
+      w[c] = *(const kcg_u32x4*)(b + (AD_EVEN || n < AD_N ? (long long)n * AD_RANK + u % AD_CHUNKS * 8 : 0));
     }
+    if (AD_SCALE) factor = scale[r];
+  };
+  auto fetch_y = [&](int nb) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = ad_get(Y + row[e] * AD_YT, nb + group * AD_COLS + i * AD_C);
+  };
+  bool more = turns.next(r, same);
+  if (more) {
+    fetch(r, ns * AD_STEP);
+    fetch_y(ns * AD_STEP);
+    // h of this wavefront's tokens in numbers of 16 bits
+    const long long t = tw + i < T ? tw + i : T - 1;
+    float h[AD_STEPS][8], most = 0.0f;
+#pragma unroll
+    for (int s = 0; s < AD_STEPS; ++s) {
+      const int c = (s * 4 + g) % AD_CHUNKS * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[s][e] = 0.0f;
+      kcg_f32x4 parts[AD_KS][2];
+#pragma unroll
+      for (int p = 0; p < AD_KS; ++p) {
+        const kcg_f32x4* at = (const kcg_f32x4*)(part + ((long long)p * T + t) * AD_RANK + c);
+        parts[p][0] = at[0];
+        parts[p][1] = at[1];
+      }
+      __builtin_amdgcn_sched_barrier(0);        // (all on their way before the first is waited for)
+#pragma unroll
+      for (int p = 0; p < AD_KS; ++p)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[s][e] += parts[p][e / 4][e % 4];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, __builtin_fabsf(h[s][e]));
+    }
+    float up = 1.0f;
+    if (AD_F16) {
+      most = fmaxf(most, __shfl_xor(most, 16, 64));
+      most = fmaxf(most, __shfl_xor(most, 32, 64));
+      int e = (int)(__builtin_bit_cast(unsigned, most) >> 23) - 127;
+      e = e < -100 ? -100 : e > 126 ? 126 : e;
+      up = __builtin_bit_cast(float, (unsigned)(127 + 14 - e) << 23);
+      back = __builtin_bit_cast(float, (unsigned)(127 - 14 + e) << 23);
+    }
+#pragma unroll
+    for (int s = 0; s < AD_STEPS; ++s) {
+      const int q = s * 4 + g;
+      ad_v o;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = h[s][e] * up;
+        const ad_x high = (ad_x)a;
+        const float left = a - (float)high;          // (nothing is left of an infinity)
+        const ad_x next = left - left == 0.0f ? (ad_x)left : (ad_x)0.0f, last = AD_PIECES > 2 && left - left == 0.0f ? (ad_x)(left - (float)next) : (ad_x)0.0f;
+        o[e] = q < AD_CHUNKS ? high : q < 2 * AD_CHUNKS ? next : q < AD_PIECES * AD_CHUNKS ? last : (ad_x)0.0f;
+      }
+      f[s] = __builtin_bit_cast(kcg_u32x4, o);
+    }
+  }
+#pragma unroll 1
+  while (more) {
+    const unsigned mine = (unsigned)(same >> (sub * 16)) & 0xffffu;
+    const float down = factor * back;
+    kcg_f32x4 times;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) times[e] = AD_F16 ? __shfl(down, g * 4 + e, 64) : down;
+    int following = 0;
+    more = turns.next(following, same);
 #pragma unroll 1
     for (int nb = ns * AD_STEP; nb < AD_N; nb += NS * AD_STEP) {
       __syncthreads();
@@ -290,7 +317,14 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
 #pragma unroll
       for (int e = 0; e < 4; ++e) now[e] = v[e];
       __syncthreads();
-      if (!AD_ONCE && nb + step < AD_N) fetch(nb + (int)step);
+      // the next columns, or the next adapter's first
+      if (!AD_ONCE && nb + step < AD_N) {
+        fetch(r, nb + (int)step);
+        fetch_y(nb + (int)step);
+      } else if (more) {
+        fetch(following, ns * AD_STEP);
+        if (!AD_ONCE) fetch_y(ns * AD_STEP);
+      }
       if (mine) {
         kcg_f32x4 acc[AD_C];
 #pragma unroll
@@ -316,12 +350,12 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
       }
       if (AD_ONCE) break;
     }
-    __syncthreads();
-  });
+    r = following;
+  }
   if (!AD_INPLACE && slot == 0) {
 #pragma unroll 1
     for (int e = 0; e < 4; ++e) {
-      if ((with >> (sub * 16 + g * 4 + e) & 1) || tw + g * 4 + e >= T) continue;
+      if ((turns.with >> (sub * 16 + g * 4 + e) & 1) || tw + g * 4 + e >= T) continue;
       const float none[AD_C] = {};
       for (int n = ns * AD_STEP + group * AD_COLS + i * AD_C; n < AD_N; n += NS * AD_STEP)
         ad_put(Z + row[e] * AD_ZT, n, ad_get(Y + row[e] * AD_YT, n), none);

@@ -794,22 +794,23 @@ def _add_adapters_launch(y, x, a, b, which, scale, inplace, cfg):
 def _add_adapters_form(tokens, adapters, n, k, rank, columns):
     """Tokens of a tile (16 TS, and 16 UT in the second launch), workgroups for a tile's adapters (S), for parts of k (KS) and of the columns (NS).
 
-    Up to 1024 tokens may be a decoding step's, with an adapter each: tiles of 16, whose adapters up to 16 workgroups share out.  More are prompts'.
-    Parts of k fill the part in the first launch and are read by all workgroups of the second.  Measured, in us, first and second launch:
-      64 tokens, 40 adapters of rank 16, N = K = 4096: k in 4 parts 4.5 and 5.6, in 8 4.1 and 6.6;  32 tokens a tile in the second launch 8.6, 64 15.9
+    Up to 1024 tokens may be a decoding step's, with an adapter each: tiles of 16, whose adapters up to 16 workgroups share out, 8 where the second launch
+    has many more than fill the part.  More tokens are prompts'.  Parts of k fill the part in the first launch and are read by all workgroups
+    of the second.  Measured, in us, first and second launch, or both:
+      64 tokens, 40 adapters of rank 16, N = K = 4096: k in 4 parts 4.8 and 5.4, in 8 4.1 and 6.6;  8 workgroups for a tile's adapters 11.9, 16 9.8
       128 tokens, 64 adapters of rank 64, N 11008: 32 tokens a tile 36, 16 39 (LDS for four wavefronts' columns);  300 tokens with one adapter: 6.5, 12.7
-      512 tokens, 64 adapters of rank 16: 16 workgroups for a tile's adapters 11.5 and 17.0, 4 16.6 and 15.2;  840 tokens in 20 runs: 7.9 and 7.1, 7.7 and 7.1
+      512 tokens, 64 adapters of rank 16: 16 workgroups for a tile's adapters 27.4, 8 27.8, 4 37;  1000 tokens: 57, 52, 54;  700 of rank 64, N 11008: 206, 175
+      those that share a tile's adapters with all columns' workgroups 57, fewer that have several passes 64;  840 tokens in 20 runs: 13.2 and 14.3
       5000 tokens, rank 64: k in 2 parts 12.5 and 20.2, in one 20 and 17.1;  64 tokens a tile in the first launch, in 4 parts 15.6 and 26;  32 workgroups along N
-      (one pass each) 17.1, 8: 18.7;  16 tokens a tile in the second launch 41, 32 tokens 32, 64 27
+      (one pass each) 17.1, 8: 18.7;  16 tokens a tile in the second launch 41, 32 tokens 36 (both launches), 64 32
       2600 tokens, rank 32, K 4096, N 11008, fp32: k in 2 parts 13 and 47.7, in one 17.2 and 46.9;  43 workgroups along N 48.6, 172 62, 8 86"""
     ts = 2 if tokens > 1024 and 64 < rank <= 128 else 1
     ut = 4 if tokens > 1024 or rank > 128 else 2 if rank > 16 else 1
-    tiles, wide = -(-tokens // (16 * ts)), -(-tokens // (16 * ut))
-    slots = min(16, tokens, adapters) if tokens <= 1024 else 1
+    tiles, wide, blocks = -(-tokens // (16 * ts)), -(-tokens // (16 * ut)), -(-n // (columns * 4 // ut))
+    slots = min(8 if wide * blocks > 384 else 16, tokens, adapters) if tokens <= 1024 else 1
     ks = max(1, min(8, 256 // (min(tiles, 16) * slots) if tokens <= 1024 else 768 // tiles, k // 512))
     ks = 1 << ks.bit_length() - 1            # (a kernel for each)
-    blocks = -(-n // (columns * 4 // ut))
-    each = max(1, blocks * wide * slots // 2048)
+    each = max(1, blocks * wide // 2048) if slots == 1 else 1
     return dict(TS=ts, UT=ut, S=slots, KS=ks, NS=-(-blocks // each))
 
 
