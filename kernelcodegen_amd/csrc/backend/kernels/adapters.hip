@@ -3,22 +3,22 @@
 // A row whose adapter is none of the AD_ADAPTERS is Y's.  X, A and B in 16 bits, Y and Z in 16 or 32.
 //
 // Two launches, since every column needs all of h: adapters_down leaves h in fp32, in AD_KS parts of k; adapters_up adds the parts in order.
-// Tokens come in any order, and a step's requests may have an adapter each or share one.  A tile is 16 AD_TS tokens as they stand (of either launch its own AD_TS); each adapter that
-// occurs in it (found by comparing lanes) is multiplied with the whole tile, and of the result only its own tokens are kept: rows of a
-// matrix product do not touch one another.  A prompt's tiles have one adapter; a decoding step's have up to 16, which workgroups share; those
-// that find none are the last of the launch.
+// Tokens come in any order, and a step's requests may have an adapter each or share one.  A tile is 16 AD_TS tokens as they stand (of either launch its
+// own AD_TS); each adapter that occurs in it (found by comparing lanes) is multiplied with the whole tile, and of the result only its own tokens
+// are kept: rows of a matrix product do not touch one another.  A prompt's tiles have one adapter; a decoding step's have up to 16, which
+// workgroups share; those that find none are the last of the launch.
 // h is not rounded to 16 bits: it enters the second product as the sum of AD_PIECES 16-bit numbers, which the matrix instruction takes as AD_PIECES AD_RANK
 // values of k with B's columns as often.  Two of half precision have 22 bits; two of bfloat16 have 16, enough for results in it, and three
 // have all of fp32's, for results in that.  In half precision h is brought below 2^15 by a power of two of its row.
 // Both products have the tokens as their columns, so that a lane has four neighbouring numbers of one token in each result.
-// Reading and writing bound prompts: 5000 tokens, rank 64, K = N = 4096 in bfloat16 13 us (X, 3.1 TB/s, LDS under way 42 % of the time) and 22 (Y and Z, 3.7
-// TB/s); 2600 tokens, rank 32, N = 11008 in fp32 11.5 and 50 (4.6 TB/s).  Of few tokens each launch is a chain: which adapter, its numbers, a sum over
-// wavefronts, the store: one token 2.8 and 4.6 us, 64 tokens with 40 adapters between them 4.7 and 5.4.  Both in one launch, in which a workgroup has all
-// of h for its columns, gain 1 us for a tile alone (6.8) and lose from there on (64 tokens: 11.1).
-// Parameters: AD_NAME, AD_UP (this is adapters_up), AD_F16, AD_PIECES, AD_RANK, AD_K, AD_N, AD_XT, AD_YT, AD_ZT (strides of rows, elements), AD_YTYPE, AD_YSIZE, AD_ALIGN (rows
-// of Y and Z start on multiples of 16 bytes), AD_SCALE (0: no scales), AD_INPLACE, AD_TS, AD_KS, AD_MANY (a
-// tile's adapters are shared out; between how many workgroups, and how many there are along N, are arguments), AD_ONCE (there are as
-// many along N as have columns: each has one pass).
+// Reading and writing bound prompts: 5000 tokens, rank 64, K = N = 4096 in bfloat16 13 us (X, 3.1 TB/s, LDS under way 40 % of the time) and 22 (Y and Z, 3.7
+// TB/s); 2600 tokens, rank 32, N = 11008 in fp32 11.4 and 51 (4.5 TB/s).  Of few tokens each launch is a chain: which adapter, its numbers, a sum over
+// wavefronts, the store: one token 2.8 and 4.0 us, 64 tokens with 40 adapters between them 4.8 and 5.4.  Both in one launch, in which a workgroup has all
+// of h for its columns, take as long for a tile alone (6.8) and lose from there on (64 tokens: 11.1).
+// Parameters: AD_NAME, AD_UP (this is adapters_up), AD_F16, AD_PIECES, AD_RANK, AD_K, AD_N, AD_XT, AD_YT, AD_ZT (strides of rows, elements), AD_YTYPE,
+// AD_YSIZE, AD_ALIGN (rows of Y and Z start on multiples of 16 bytes), AD_SCALE (0: no scales), AD_INPLACE, AD_TS, AD_KS, AD_MANY (a tile's adapters are
+// shared out; between how many workgroups, and how many there are along N, are arguments), AD_ONCE (there are as many along N as have columns:
+// each has one pass).
 typedef _Float16 ad_f16x8 __attribute__((ext_vector_type(8)));
 #if AD_F16
 typedef _Float16 ad_x;
@@ -211,7 +211,7 @@ __device__ __forceinline__ void ad_put(ad_y* z, int n, ad_yv v, const float (&ad
 
 // A wavefront takes AD_COLS columns of 16 tokens at a time: lane l gets columns (l % 16) AD_C on of tokens 4 (l / 16) to 4 (l / 16) + 3, whole lines of Y with
 // its neighbours, when the columns of product q are every AD_C-th from q on.  B comes for the whole workgroup, in whole lines, and goes through LDS,
-// rows put into the order in which the products take them; the next columns' B and Y are under way meanwhile.
+// rows put into the order in which the products take them; the next columns' B and Y, or the next adapter's, are under way meanwhile.
 extern "C" __global__ __launch_bounds__(256)
 void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restrict__ B, const int* __restrict__ which, const float* __restrict__ scale, long long T,
              long long adapters, long long slots, long long NS_, ad_y* Z) {
