@@ -11,9 +11,9 @@
 // values of k with B's columns as often.  Two of half precision have 22 bits; two of bfloat16 have 16, enough for results in it, and three
 // have all of fp32's, for results in that.  In half precision h is brought below 2^15 by a power of two of its row.
 // Both products have the tokens as their columns, so that a lane has four neighbouring numbers of one token in each result.
-// Reading and writing bound prompts: 5000 tokens, rank 64, K = N = 4096 in bfloat16 13 us (X, 3.1 TB/s, LDS under way 40 % of the time) and 22 (Y and Z, 3.7
+// Reading and writing bound prompts: 5000 tokens, rank 64, K = N = 4096 in bfloat16 13 us (X, 3.1 TB/s, LDS under way 40 % of the time) and 21 (Y and Z, 3.9
 // TB/s); 2600 tokens, rank 32, N = 11008 in fp32 11.4 and 51 (4.5 TB/s).  Of few tokens each launch is a chain: which adapter, its numbers, a sum over
-// wavefronts, the store: one token 2.8 and 4.0 us, 64 tokens with 40 adapters between them 4.8 and 5.4.  Both in one launch, in which a workgroup has all
+// wavefronts, the store: one token 2.9 and 4.0 us, 64 tokens with 40 adapters between them 4.8 and 5.5.  Both in one launch, in which a workgroup has all
 // of h for its columns, take as long for a tile alone (6.8) and lose from there on (64 tokens: 11.1).
 // Parameters: AD_NAME, AD_UP (this is adapters_up), AD_F16, AD_PIECES, AD_RANK, AD_K, AD_N, AD_XT, AD_YT, AD_ZT (strides of rows, elements), AD_YTYPE,
 // AD_YSIZE, AD_ALIGN (rows of Y and Z start on multiples of 16 bytes), AD_SCALE (0: no scales), AD_INPLACE, AD_TS, AD_KS, AD_MANY (a tile's adapters are
