@@ -262,6 +262,17 @@ def test_add_adapters_forms(dtype, out, ts, ut, rank, form):
     check_adapters(got, y, x, a, b, which, None)
 
 
+@pytest.mark.parametrize("n", [2048, 2003])
+@pytest.mark.parametrize("form", [dict(S=1, NS=1), dict(S=1, NS=100), dict(S=3, NS=2), dict(UT=4, S=1, NS=3), dict(UT=2, S=2, NS=100)])
+def test_add_adapters_in_place_by_passes_and_turns(n, form):
+    """Tiles of many adapters, one after the other and in several passes over the columns, write what they read."""
+    y, x, a, b, which, scale = adapters_case(n, 150, n, 264, 24, 11, "bf16", "bf16")
+    want = ops.add_adapters(y, x, a, b, which, scale)
+    assert ops.add_adapters(y, x, a, b, which, scale, inplace=True, KS=1, TS=1, **form) is y
+    check_adapters(want, *adapters_case(n, 150, n, 264, 24, 11, "bf16", "bf16"))
+    assert torch.equal(y, want)
+
+
 def test_add_adapters_keeps_what_half_precision_would_lose():
     """x a of 2^20 and of 2^-30, which half precision holds no numbers for."""
     for spread, b_spread in ((2.0 ** 13, 2.0 ** -14), (2.0 ** -12, 1.0)):
