@@ -1815,7 +1815,7 @@ bool emitAdapters(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::
   d.add("AD_NAME", s.name); d.add("AD_UP", up ? 1 : 0);
   for (auto key : {"N", "K", "RANK", "F16"}) d.add(std::string("AD_") + key, s.p[key]);
   for (auto key : {"XT", "YT", "ZT"}) d.add(std::string("AD_") + key, std::to_string(s.p[key]) + "LL");
-  d.add("AD_YTYPE", std::string(y32 ? "float" : x)); d.add("AD_YSIZE", y32 ? 4 : 2); d.add("AD_PIECES", y32 && !s.p["F16"] ? 3 : 2); d.add("AD_TS", ts); d.add("AD_DEPTH", ts + jt <= 4 ? 2 : 1); d.add("AD_ALIGN", align ? 1 : 0);
+  d.add("AD_YTYPE", std::string(y32 ? "float" : x)); d.add("AD_YSIZE", y32 ? 4 : 2); d.add("AD_PIECES", s.p["F16"] ? 2 : 3); d.add("AD_TS", ts); d.add("AD_DEPTH", ts + jt <= 4 ? 2 : 1); d.add("AD_ALIGN", align ? 1 : 0);
   d.add("AD_SCALE", s.get("SCALES", 0) ? 1 : 0); d.add("AD_INPLACE", s.get("INPLACE", 0) ? 1 : 0);
   d.add("AD_KS", ks); d.add("AD_MANY", s.get("MANY", 0) ? 1 : 0); d.add("AD_ONCE", s.get("ONCE", 0) ? 1 : 0);
   src = d.wrap(kTpl_adapters);

@@ -8,8 +8,9 @@
 // are kept: rows of a matrix product do not touch one another.  A prompt's tiles have one adapter; a decoding step's have up to 16, which
 // workgroups share; those that find none are the last of the launch.
 // h is not rounded to 16 bits: it enters the second product as the sum of AD_PIECES 16-bit numbers, which the matrix instruction takes as AD_PIECES AD_RANK
-// values of k with B's columns as often.  Two of half precision have 22 bits; two of bfloat16 have 16, enough for results in it, and three
-// have all of fp32's, for results in that.  In half precision h is brought below 2^15 by a power of two of its row.
+// values of k with B's columns as often.  Two of half precision have 22 bits, three of bfloat16 all of fp32's 24.  (Two of bfloat16 have 16: of 262144 results in
+// bfloat16, 64 tokens with 40 adapters, 295 were not the nearest to the formula, of the formula in fp32 53, of this 24; 9.3 and 9.5 us.)  In half precision h is brought below 2^15 by
+// a power of two of its row.
 // Both products have the tokens as their columns, so that a lane has four neighbouring numbers of one token in each result.
 // Reading and writing bound prompts: 5000 tokens, rank 64, K = N = 4096 in bfloat16 13 us (X, 3.1 TB/s, LDS under way 40 % of the time) and 21 (Y and Z, 3.9
 // TB/s); 2600 tokens, rank 32, N = 11008 in fp32 11.4 and 51 (4.5 TB/s).  Of few tokens each launch is a chain: which adapter, its numbers, a sum over

@@ -725,7 +725,7 @@ def add_adapters(y, x, a, b, which, scale=None, inplace=False, **cfg):
     rank], of x's type and contiguous; which: int32 [tokens], in any order, each adapter for any number of tokens; scale: fp32 [adapters], None for 1.
     Rank and K are multiples of 8, the rank up to 256 (a smaller one is filled up with zeros).  Rows of x and y may lie apart.  Returns a
     contiguous tensor of y's type, or y itself (inplace); a token whose adapter is none of them (-1) keeps its row of y.  Sums are
-    fp32, a[r] x[t] enters the second product with 16 bits or more, and the sum with y is rounded once.  `cfg` overrides kernel parameters (TS, UT, KS, S, NS)."""
+    fp32, a[r] x[t] enters the second product with 22 bits or more, and the sum with y is rounded once.  `cfg` overrides kernel parameters (TS, UT, KS, S, NS)."""
     inplace = bool(inplace)
     key = ("add_adapters", R.signature(y, x, a, b, which, scale), inplace)
     hit = None if cfg else _bound.get(key)
