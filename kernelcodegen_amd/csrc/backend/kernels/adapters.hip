@@ -187,6 +187,7 @@ typedef ad_y ad_mem __attribute__((ext_vector_type(AD_C), aligned(AD_YSIZE)));  
 #define AD_EVEN (AD_N % AD_STEP == 0)               // no column is behind the last
 #define AD_PITCH (AD_CHUNKS % 2 ? AD_RANK * 2 : AD_RANK * 2 + 16)  // of a row of B in LDS: an odd number of 16 bytes
 #define AD_LOADS ((AD_STEP * AD_CHUNKS + 255) / 256)
+#define AD_INSIDE (AD_EVEN && AD_STEP * AD_CHUNKS % 256 == 0)      // nor is a load's, whose lanes may pass the step's columns
 
 // Columns n to n + AD_C of a row; elements of a vector that passes the row's end come one by one, all of them before any is put.
 __device__ __forceinline__ ad_yv ad_get(const ad_y* y, int n) {
@@ -237,7 +238,7 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
 #pragma unroll
     for (int c = 0; c < AD_LOADS; ++c) {
       const int u = c * 256 + threadIdx.x, n = nb + u / AD_CHUNKS;
-      w[c] = *(const kcg_u32x4*)(b + (AD_EVEN || n < AD_N ? (long long)n * AD_RANK + u % AD_CHUNKS * 8 : 0));
+      w[c] = *(const kcg_u32x4*)(b + (AD_INSIDE || n < AD_N ? (long long)n * AD_RANK + u % AD_CHUNKS * 8 : 0));
     }
     if (AD_SCALE) factor = scale[r];
   };

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from kernelcodegen_amd import ops
+from test_gpu_answer_operators import adapters_case, check_adapters
 from test_gpu_decode_step import DTYPE, generator, ints
 
 pytestmark = pytest.mark.gpu
@@ -27,3 +28,21 @@ def test_adapters_h_enters_the_second_product_whole(dtype, out, tokens, n, rank)
     want = (y.double() + sum(values)[:, j]).to(DTYPE[out])
     assert torch.equal(ops.add_adapters(y, x, a, b, which), want)
     assert torch.equal(ops.add_adapters(y * 0.25, x, a, b, which, scale * 0.25), want * 0.25)
+
+
+# ---- add_adapters: more than 1024 tokens ----
+
+@pytest.mark.parametrize("dtype,out,tokens,n,k,rank,runs", [
+    ("bf16", "bf16", 1025, 1280, 264, 8, False), ("f16", "f32", 1025, 1280, 264, 16, False), ("bf16", "f32", 2600, 6400, 1032, 8, True), ("bf16", "bf16", 2600, 1003, 2048, 64, True),
+    ("f16", "f16", 1300, 1280, 520, 64, False), ("bf16", "bf16", 1100, 1024, 520, 128, True), ("f16", "f32", 1100, 1003, 520, 128, False), ("bf16", "f32", 1025, 640, 264, 256, False),
+    ("f16", "f16", 1100, 1024, 264, 24, True)])
+def test_adapters_of_more_than_a_thousand_tokens(dtype, out, tokens, n, k, rank, runs):
+    """The forms that the rule takes for prompts: other tiles, parts of k by the rank, one pass over the columns and (6400 of fp32) several; columns that are a whole
+    number of a workgroup's and others; runs of one adapter, and several in each tile."""
+    y, x, a, b, which, scale = adapters_case(tokens + rank, tokens, n, k, rank, 7, dtype, out)
+    if runs:
+        which = which.sort().values.contiguous()
+    got = ops.add_adapters(y, x, a, b, which, scale)
+    for at in (slice(None, 70), slice(tokens // 2 - 9, None, 29), slice(-40, None)):
+        check_adapters(got, y, x, a, b, which, scale, at)
+    assert ops.add_adapters(y, x, a, b, which, scale, inplace=True) is y and torch.equal(y, got)
