@@ -211,6 +211,25 @@ __device__ __forceinline__ void ad_put(ad_y* z, int n, ad_yv v, const float (&ad
   }
 }
 
+// a as the sum of AD_PIECES 16-bit numbers of its sign, none of them 0 unless a is (or, in half precision, below 2^-23): an infinity of B times all of them
+// is one, as times a.  Each is cut off, so that what is left has a's sign; where nothing is left, or nothing finite, halves do.
+__device__ __forceinline__ void ad_split(float a, float (&p)[3]) {
+#if AD_F16
+  p[0] = (float)__builtin_amdgcn_cvt_pkrtz(a, a)[0];
+  p[0] = (ad_x)(a - p[0]) == (ad_x)0.0f ? (float)(ad_x)(a * 0.5f) : p[0];
+  p[1] = a - a == 0.0f ? a - p[0] : a;
+#else
+  auto cut = [](float v) { return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, v) & 0xffff0000u); };
+  p[0] = cut(a);
+  const float left = a - p[0], half = a * 0.5f, mine = __builtin_fabsf(left) > 0.0f ? left : half;
+  p[0] = __builtin_fabsf(left) > 0.0f ? p[0] : half;
+  p[1] = cut(mine);
+  const float rest = mine - p[1], quarter = mine * 0.5f;
+  p[1] = __builtin_fabsf(rest) > 0.0f ? p[1] : quarter;
+  p[2] = __builtin_fabsf(rest) > 0.0f ? rest : quarter;
+#endif
+}
+
 // A wavefront takes AD_COLS columns of 16 tokens at a time: lane l gets columns (l % 16) AD_C on of tokens 4 (l / 16) to 4 (l / 16) + 3, whole lines of Y with
 // its neighbours, when the columns of product q are every AD_C-th from q on.  B comes for the whole workgroup, in whole lines, and goes through LDS,
 // rows put into the order in which the products take them; the next columns' B and Y, or the next adapter's, are under way meanwhile.
@@ -252,9 +271,9 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
     fetch_y(ns * AD_STEP);
     // h of this wavefront's tokens in numbers of 16 bits
     const long long t = tw + i < T ? tw + i : T - 1;
-    float h[AD_STEPS][8], most = 0.0f;
+    float h[AD_OWN][8], most = 0.0f;
 #pragma unroll
-    for (int s = 0; s < AD_STEPS; ++s) {
+    for (int s = 0; s < AD_OWN; ++s) {
       const int c = (s * 4 + g) % AD_CHUNKS * 8;
 #pragma unroll
       for (int e = 0; e < 8; ++e) h[s][e] = 0.0f;
@@ -283,18 +302,19 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
       back = __builtin_bit_cast(float, (unsigned)(127 - 14 + e) << 23);
     }
 #pragma unroll
-    for (int s = 0; s < AD_STEPS; ++s) {
+    for (int s = 0; s < AD_OWN; ++s) {
       const int q = s * 4 + g;
-      ad_v o;
+      ad_v p[AD_PIECES];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float a = h[s][e] * up;
-        const ad_x high = (ad_x)a;
-        const float left = a - (float)high;          // (nothing is left of an infinity)
-        const ad_x next = left - left == 0.0f ? (ad_x)left : (ad_x)0.0f, last = AD_PIECES > 2 && left - left == 0.0f ? (ad_x)(left - (float)next) : (ad_x)0.0f;
-        o[e] = q < AD_CHUNKS ? high : q < 2 * AD_CHUNKS ? next : q < AD_PIECES * AD_CHUNKS ? last : (ad_x)0.0f;
+        float of[3];
+        ad_split(AD_F16 ? h[s][e] * up : h[s][e], of);
+        if (AD_CHUNKS % 4) of[0] = q < AD_CHUNKS ? of[0] : q < 2 * AD_CHUNKS ? of[1] : q < AD_PIECES * AD_CHUNKS ? of[AD_PIECES - 1] : 0.0f;
+#pragma unroll
+        for (int n = 0; n < AD_PIECES; ++n) p[n][e] = (ad_x)of[n];
       }
-      f[s] = __builtin_bit_cast(kcg_u32x4, o);
+#pragma unroll
+      for (int n = 0; n < AD_STEPS / AD_OWN; ++n) f[n * AD_OWN + s] = __builtin_bit_cast(kcg_u32x4, p[n]);
     }
   }
 #pragma unroll 1

@@ -1,4 +1,6 @@
 """Adapters at the limits of their arithmetic, against the formulas in 64 bits."""
+import math
+
 import pytest
 import torch
 
@@ -28,6 +30,30 @@ def test_adapters_h_enters_the_second_product_whole(dtype, out, tokens, n, rank)
     want = (y.double() + sum(values)[:, j]).to(DTYPE[out])
     assert torch.equal(ops.add_adapters(y, x, a, b, which), want)
     assert torch.equal(ops.add_adapters(y * 0.25, x, a, b, which, scale * 0.25), want * 0.25)
+
+
+# ---- add_adapters: special values ----
+
+@pytest.mark.parametrize("dtype,out", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "f32"), ("f16", "f32")])
+@pytest.mark.parametrize("n,rank", [(200, 16), (101, 24), (333, 64), (70, 256)])
+def test_adapters_of_infinite_numbers(dtype, out, n, rank):
+    """An infinity in b, or in a, makes infinities of what it meets, as in the formula, not NaN; other columns, tokens and adapters have none of it."""
+    y, x, a, b, which, scale = adapters_case(n, 40, n, 64, rank, 3, dtype, out)
+    which[:] = torch.arange(40, device="cuda") % 4 - 1
+    x[4:10] = torch.nn.functional.one_hot(torch.arange(6, device="cuda"), 64)          # x a that 16 bits hold
+    scale[1] = -1.5
+    good = ops.add_adapters(y, x, a, b, which, scale)
+    b[0, 3, 5], b[0, 17, 1], b[0, n - 1, rank - 1], b[0, 9, 0], b[0, 9, 7], b[1, 3, 2], b[1, 5, 4], b[2, 6, 1] = math.inf, -math.inf, math.inf, math.inf, math.inf, -math.inf, math.nan, -math.inf
+    a[2, 1, 7] = math.inf
+    got = ops.add_adapters(y, x, a, b, which, scale)
+    want = y.double()
+    for r in range(3):
+        mine = which == r
+        h = x[mine].double() @ a[r].double().t()
+        want[mine] += float(scale[r]) * (h[:, None, :] * b[r].double()[None]).sum(-1)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[got.isinf()].double(), want[want.isinf()]) and torch.equal(got.isinf(), want.isinf())
+    fine = want.isfinite()
+    assert torch.equal(got[fine], good[fine]) and bool(want[which >= 0].isinf().any())
 
 
 # ---- add_adapters: more than 1024 tokens ----
