@@ -199,9 +199,7 @@ __device__ __forceinline__ ad_yv ad_get(const ad_y* y, int n) {
   }
   return v;
 }
-__device__ __forceinline__ void ad_put(ad_y* z, int n, ad_yv v, const float (&add)[AD_C]) {
-#pragma unroll
-  for (int e = 0; e < AD_C; ++e) v[e] = (ad_y)((float)v[e] + add[e]);
+__device__ __forceinline__ void ad_put(ad_y* z, int n, ad_yv v) {
   if (AD_EVEN || n + AD_C <= AD_N) {
     *(ad_mem*)(z + n) = v;
   } else if (AD_N % AD_C) {
@@ -364,10 +362,10 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float add[AD_C];
+          ad_yv sum;
 #pragma unroll
-          for (int q = 0; q < AD_C; ++q) add[q] = times[e] * acc[q][e];
-          if (mine >> (g * 4 + e) & 1) ad_put(Z + row[e] * AD_ZT, nb + group * AD_COLS + i * AD_C, now[e], add);
+          for (int q = 0; q < AD_C; ++q) sum[q] = (ad_y)((float)now[e][q] + times[e] * acc[q][e]);
+          if (mine >> (g * 4 + e) & 1) ad_put(Z + row[e] * AD_ZT, nb + group * AD_COLS + i * AD_C, sum);
         }
       }
       if (AD_ONCE) break;
@@ -378,9 +376,8 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
 #pragma unroll 1
     for (int e = 0; e < 4; ++e) {
       if ((turns.with >> (sub * 16 + g * 4 + e) & 1) || tw + g * 4 + e >= T) continue;
-      const float none[AD_C] = {};
       for (int n = ns * AD_STEP + group * AD_COLS + i * AD_C; n < AD_N; n += NS * AD_STEP)
-        ad_put(Z + row[e] * AD_ZT, n, ad_get(Y + row[e] * AD_YT, n), none);
+        ad_put(Z + row[e] * AD_ZT, n, ad_get(Y + row[e] * AD_YT, n));
     }
   }
 }

@@ -56,6 +56,19 @@ def test_adapters_of_infinite_numbers(dtype, out, n, rank):
     assert torch.equal(got[fine], good[fine]) and bool(want[which >= 0].isinf().any())
 
 
+@pytest.mark.parametrize("dtype", sorted(DTYPE))
+@pytest.mark.parametrize("tokens,n", [(3, 100), (90, 101), (40, 3), (1100, 200)])
+def test_adapters_rows_without_one_keep_their_bits(dtype, tokens, n):
+    y, x, a, b, which, scale = adapters_case(tokens, tokens, n, 64, 16, 3, "f16" if dtype == "f16" else "bf16", dtype)
+    whole = torch.int32 if dtype == "f32" else torch.int16
+    y.view(whole).random_(torch.iinfo(whole).min, torch.iinfo(whole).max, generator=generator(2))          # NaN of any kind, the least numbers
+    y[::2, ::3] = -0.0
+    which[tokens // 2:] = -1
+    for inplace in (False, True):
+        got = ops.add_adapters(y.clone(), x, a, b, which, scale, inplace=inplace)
+        assert torch.equal(got.view(whole)[which < 0], y.view(whole)[which < 0])
+
+
 # ---- add_adapters: more than 1024 tokens ----
 
 @pytest.mark.parametrize("dtype,out,tokens,n,k,rank,runs", [
