@@ -1791,15 +1791,16 @@ bool emitGemmQ4(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::st
   return true;
 }
 
-// adapters_down and adapters_up, which takes what the first leaves: the same parameters.
+// adapters_down, and adapters_up, which takes what the first leaves.  Each has the parameters that it depends on, so that projections of other columns share the first.
 bool emitAdapters(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::string& err) {
   const bool up = s.family == "adapters_up";
-  if (!whole(s, "N", 1, 0x3FFFFF00, err) || !whole(s, "K", 8, 0x3FFFFF00, err) || !whole(s, "RANK", 8, 256, err) || !whole(s, "F16", 0, 1, err)) return false;
+  if (!whole(s, "RANK", 8, 256, err) || !whole(s, "F16", 0, 1, err) || !whole(s, up ? "N" : "K", up ? 1 : 8, 0x3FFFFF00, err)) return false;
   for (auto key : {"K", "RANK"})
-    if (s.p[key] % 8) { err = s.family + ": " + key + " must be a multiple of 8"; return false; }
-  for (auto key : {"XT", "YT", "ZT"})
+    if (s.get(key, 0) % 8) { err = s.family + ": " + key + " must be a multiple of 8"; return false; }
+  const std::vector<const char*> strides = up ? std::vector<const char*>{"YT", "ZT"} : std::vector<const char*>{"XT"};
+  for (auto key : strides)
     if (!whole(s, key, 0, (int64_t)1 << 40, err)) return false;
-  if (s.p["XT"] % 8) { err = s.family + ": XT must be a multiple of 16 bytes"; return false; }
+  if (!up && s.p["XT"] % 8) { err = s.family + ": XT must be a multiple of 16 bytes"; return false; }
   const int64_t ks = s.get("KS", 1);
   if (ks < 1 || ks > 64) { err = s.family + ": KS must be in [1,64]"; return false; }
   // 16 TS tokens a tile, of the second launch 16 UT: registers hold TS times the rank's results, LDS the columns of 4 / UT wavefronts
@@ -1808,16 +1809,19 @@ bool emitAdapters(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::
     err = s.family + (up ? ": UT must be 1, 2 or 4, and 4 / UT times the rank up to 256" : ": TS must be 1, 2 or 4, and TS times the rank up to 256");
     return false;
   }
-  const char* x = s.p["F16"] ? "_Float16" : "__bf16";
-  const bool y32 = s.get("Y_F32", 0) != 0, align = s.get("ALIGN", 0) != 0;
-  if (align && (s.p["YT"] * (y32 ? 4 : 2) % 16 || s.p["ZT"] * (y32 ? 4 : 2) % 16)) { err = s.family + ": ALIGN is for rows on multiples of 16 bytes"; return false; }
   Defines d;
   d.add("AD_NAME", s.name); d.add("AD_UP", up ? 1 : 0);
-  for (auto key : {"N", "K", "RANK", "F16"}) d.add(std::string("AD_") + key, s.p[key]);
-  for (auto key : {"XT", "YT", "ZT"}) d.add(std::string("AD_") + key, std::to_string(s.p[key]) + "LL");
-  d.add("AD_YTYPE", std::string(y32 ? "float" : x)); d.add("AD_YSIZE", y32 ? 4 : 2); d.add("AD_PIECES", s.p["F16"] ? 2 : 3); d.add("AD_TS", ts); d.add("AD_DEPTH", ts + jt <= 4 ? 2 : 1); d.add("AD_ALIGN", align ? 1 : 0);
-  d.add("AD_SCALE", s.get("SCALES", 0) ? 1 : 0); d.add("AD_INPLACE", s.get("INPLACE", 0) ? 1 : 0);
-  d.add("AD_KS", ks); d.add("AD_MANY", s.get("MANY", 0) ? 1 : 0); d.add("AD_ONCE", s.get("ONCE", 0) ? 1 : 0);
+  for (auto key : {up ? "N" : "K", "RANK", "F16"}) d.add(std::string("AD_") + key, s.p[key]);
+  for (auto key : strides) d.add(std::string("AD_") + key, std::to_string(s.p[key]) + "LL");
+  d.add("AD_TS", ts); d.add("AD_KS", ks); d.add("AD_MANY", s.get("MANY", 0) ? 1 : 0);
+  if (up) {
+    const bool y32 = s.get("Y_F32", 0) != 0, align = s.get("ALIGN", 0) != 0;
+    if (align && (s.p["YT"] * (y32 ? 4 : 2) % 16 || s.p["ZT"] * (y32 ? 4 : 2) % 16)) { err = s.family + ": ALIGN is for rows on multiples of 16 bytes"; return false; }
+    d.add("AD_YTYPE", std::string(y32 ? "float" : s.p["F16"] ? "_Float16" : "__bf16")); d.add("AD_YSIZE", y32 ? 4 : 2); d.add("AD_PIECES", s.p["F16"] ? 2 : 3);
+    d.add("AD_ALIGN", align ? 1 : 0); d.add("AD_SCALE", s.get("SCALES", 0) ? 1 : 0); d.add("AD_INPLACE", s.get("INPLACE", 0) ? 1 : 0); d.add("AD_ONCE", s.get("ONCE", 0) ? 1 : 0);
+  } else {
+    d.add("AD_DEPTH", ts + jt <= 4 ? 2 : 1);
+  }
   src = d.wrap(kTpl_adapters);
   info.name = s.name;
   info.block[0] = 256;

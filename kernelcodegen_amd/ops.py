@@ -775,20 +775,20 @@ def _add_adapters_launch(y, x, a, b, which, scale, inplace, cfg):
         return None, None, 0, 0
     yt = y.stride(0) if tokens > 1 else 0
     zt, size = yt if inplace else n, y.element_size()
-    params = dict(N=n, K=k, RANK=rank, F16=int(x.dtype == torch.float16), Y_F32=int(y.dtype == torch.float32), XT=x.stride(0) if tokens > 1 else 0, YT=yt, ZT=zt,
-                  ALIGN=int((y.data_ptr() | yt * size | zt * size) % 16 == 0), SCALES=int(scale is not None), INPLACE=int(inplace),
-                  **{**_add_adapters_form(tokens, adapters, n, k, rank, 256 // size), **cfg})
-    slots, across = params.pop("S"), params.pop("NS")
-    if slots < 1 or across < 1 or params["UT"] not in (1, 2, 4) or params["TS"] not in (1, 2, 4):
+    form = {**_add_adapters_form(tokens, adapters, n, k, rank, 256 // size), **cfg}
+    slots, across = form["S"], form["NS"]
+    if slots < 1 or across < 1 or form["UT"] not in (1, 2, 4) or form["TS"] not in (1, 2, 4):
         raise ValueError("bad kernel parameters")
-    passes = -(-n // (256 // size * 4 // params["UT"]))
+    passes = -(-n // (256 // size * 4 // form["UT"]))
     across = min(across, passes)
-    params.update(MANY=int(slots > 1), ONCE=int(across == passes))
-    grids = [-(-tokens // (16 * params[tile])) * slots * by for tile, by in (("TS", params["KS"]), ("UT", across))]
+    grids = [-(-tokens // (16 * form[tile])) * slots * by for tile, by in (("TS", form["KS"]), ("UT", across))]
     if max(grids) > 0x7FFFFFFF:
         raise ValueError("too many tokens for one launch")
-    down, up = (R.get_kernel(family, **params).bind(grid=(grid,)) for family, grid in zip(("adapters_down", "adapters_up"), grids))
-    return _into_last(down, ((params["KS"], tokens, rank), torch.float32)), up if inplace else _into_last(up, ((tokens, n), y.dtype)), slots, across
+    both = dict(RANK=rank, F16=int(x.dtype == torch.float16), KS=form["KS"], MANY=int(slots > 1))
+    down = R.get_kernel("adapters_down", K=k, XT=x.stride(0) if tokens > 1 else 0, TS=form["TS"], **both).bind(grid=(grids[0],))
+    up = R.get_kernel("adapters_up", N=n, YT=yt, ZT=zt, Y_F32=int(y.dtype == torch.float32), ALIGN=int((y.data_ptr() | yt * size | zt * size) % 16 == 0), UT=form["UT"],
+                      SCALES=int(scale is not None), INPLACE=int(inplace), ONCE=int(across == passes), **both).bind(grid=(grids[1],))
+    return _into_last(down, ((form["KS"], tokens, rank), torch.float32)), up if inplace else _into_last(up, ((tokens, n), y.dtype)), slots, across
 
 
 def _add_adapters_form(tokens, adapters, n, k, rank, columns):

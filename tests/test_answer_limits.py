@@ -2,7 +2,10 @@
 import re
 import subprocess
 
-from kernelcodegen_amd import runtime as R
+import torch
+
+from kernelcodegen_amd import ops, runtime as R
+from test_decode_limits import Operand
 
 
 def test_adapters_read_no_column_behind_the_last(tmp_path):
@@ -38,3 +41,36 @@ def test_adapters_read_no_column_behind_the_last(tmp_path):
     (tmp_path / "reads.cc").write_text("\n".join(source))
     subprocess.check_call(["g++", "-O1", "-w", "-o", str(tmp_path / "reads"), str(tmp_path / "reads.cc")])
     assert len(names) > 800 and subprocess.check_output([str(tmp_path / "reads")], text=True) == ""
+
+
+def asked_kernels(monkeypatch, tokens, n, k=256, rank=16, adapters=4, inplace=False, f32=False, **cfg):
+    """(family, parameters) of the kernels that a call of add_adapters asks for."""
+    asked = []
+
+    class Kernel:
+        def bind(self, grid):
+            return lambda *values: None
+
+    def get_kernel(family, **params):
+        asked.append((family, params))
+        return Kernel()
+    monkeypatch.setattr(R, "get_kernel", get_kernel)
+    bf16, i32 = torch.bfloat16, torch.int32
+    ops._add_adapters_launch(Operand((tokens, n), torch.float32 if f32 else bf16), Operand((tokens, k), bf16), Operand((adapters, rank, k), bf16),
+                             Operand((adapters, n, rank), bf16), Operand((tokens,), i32), Operand((adapters,), torch.float32), inplace, cfg)
+    return asked
+
+
+def test_adapters_kernels_have_only_the_parameters_that_they_depend_on(monkeypatch):
+    """Projections that share what they read share the first launch's kernel; the second's does not depend on k."""
+    first = [asked_kernels(monkeypatch, 40, n, inplace=inplace, f32=f32)[0] for n, inplace, f32 in ((512, False, False), (1000, False, False), (512, True, False), (512, False, True))]
+    assert all(kernel == first[0] for kernel in first) and first[0][0] == "adapters_down"
+    second = [asked_kernels(monkeypatch, 40, 512, k)[1] for k in (256, 264, 504)]
+    assert all(kernel == second[0] for kernel in second) and second[0][0] == "adapters_up"
+    for family, params in (first[0], second[0]):
+        text = R.emit_kernel(family, "kernel0", **params)[0]
+        for key in params:
+            with_other = R.emit_kernel(family, "kernel0", **{**params, key: {"K": 1024, "XT": 1024, "N": 1024, "YT": 1024, "ZT": 1024, "RANK": 32, "KS": 2, "TS": 2, "UT": 2}.get(key, 1 - params[key])})[0]
+            assert with_other != text, key
+        others = dict(N=77, K=512, XT=512, YT=72, ZT=64, Y_F32=1, SCALES=0, INPLACE=1, ONCE=0, TS=4, UT=4)
+        assert R.emit_kernel(family, "kernel0", **{**others, **params})[0] == text
