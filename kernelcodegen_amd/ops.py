@@ -356,6 +356,13 @@ def _vectors(dtype, *ts):
             raise ValueError("expected contiguous device tensors of type %s" % dtype)
 
 
+def _grid(workgroups, threads, of):
+    """The grid of a launch along one dimension: it takes fewer than 2^32 threads."""
+    if workgroups * threads > 0xFFFFFFFF:
+        raise ValueError("too many %s for one launch" % of)
+    return (workgroups,)
+
+
 def page_slots(lengths, added, table, free, page_size, tokens):
     """Page tables and slots of one step's tokens, on the device alone.
 
@@ -488,11 +495,10 @@ def _cache_append_launch(q, k, v, k_cache, v_cache, k_scale, v_scale, slots, pos
         raise ValueError("rotation is [P, R] on a multiple of 16 bytes, R a multiple of 16 up to the head dimension")
     # passes of a token's query heads for one reading of its angles
     passes = 1 if tokens <= 128 else 4
-    kern = R.get_kernel("cache_append", R=rotation.shape[1], PAIRS=int(interleaved), HQ=heads, QN=passes, XQT=xq[0], XQH=xq[1], **params)
     waves = 2 * params["H"] * -(-tokens // params["WIN"]) + tokens * -(-heads // (passes * (64 // (d // 8))))
-    if waves > 0x7FFFFFFF:
-        raise ValueError("too many tokens for one launch")
-    return _into_last(kern.bind(grid=(max(1, -(-waves // 4)),)), (tuple(q.shape), q.dtype))
+    grid = _grid(max(1, -(-waves // 4)), 256, "tokens")
+    kern = R.get_kernel("cache_append", R=rotation.shape[1], PAIRS=int(interleaved), HQ=heads, QN=passes, XQT=xq[0], XQH=xq[1], **params)
+    return _into_last(kern.bind(grid=grid), (tuple(q.shape), q.dtype))
 
 
 def cache_read(cache, scale, slots, dtype=torch.bfloat16):
@@ -767,8 +773,6 @@ def _add_adapters_launch(y, x, a, b, which, scale, inplace, cfg):
         raise ValueError("rows of x, a and b must start on multiples of 16 bytes")
     if inplace and tokens > 1 and y.stride(0) < n:
         raise ValueError("rows of y must not overlap")
-    if tokens > 0x7FFFFF00:
-        raise ValueError("too many tokens for one launch")
     if not cfg.keys() <= {"TS", "UT", "KS", "S", "NS"}:
         raise ValueError("unknown kernel parameters")
     if not tokens:
@@ -781,13 +785,11 @@ def _add_adapters_launch(y, x, a, b, which, scale, inplace, cfg):
         raise ValueError("bad kernel parameters")
     passes = -(-n // (256 // size * 4 // form["UT"]))
     across = min(across, passes)
-    grids = [-(-tokens // (16 * form[tile])) * slots * by for tile, by in (("TS", form["KS"]), ("UT", across))]
-    if max(grids) > 0x7FFFFFFF:
-        raise ValueError("too many tokens for one launch")
+    grids = [_grid(-(-tokens // (16 * form[tile])) * slots * by, 256, "tokens") for tile, by in (("TS", form["KS"]), ("UT", across))]
     both = dict(RANK=rank, F16=int(x.dtype == torch.float16), KS=form["KS"], MANY=int(slots > 1))
-    down = R.get_kernel("adapters_down", K=k, XT=x.stride(0) if tokens > 1 else 0, TS=form["TS"], **both).bind(grid=(grids[0],))
+    down = R.get_kernel("adapters_down", K=k, XT=x.stride(0) if tokens > 1 else 0, TS=form["TS"], **both).bind(grid=grids[0])
     up = R.get_kernel("adapters_up", N=n, YT=yt, ZT=zt, Y_F32=int(y.dtype == torch.float32), ALIGN=int((y.data_ptr() | yt * size | zt * size) % 16 == 0), UT=form["UT"],
-                      SCALES=int(scale is not None), INPLACE=int(inplace), ONCE=int(across == passes), **both).bind(grid=(grids[1],))
+                      SCALES=int(scale is not None), INPLACE=int(inplace), ONCE=int(across == passes), **both).bind(grid=grids[1])
     return _into_last(down, ((form["KS"], tokens, rank), torch.float32)), up if inplace else _into_last(up, ((tokens, n), y.dtype)), slots, across
 
 
@@ -863,16 +865,15 @@ def _token_logprobs_launch(logits, tokens, top, cfg):
     parts = params.pop("PARTS")
     if not 1 <= parts <= 1024:
         raise ValueError("a row has 1 to 1024 parts")
-    if rows * parts > 0x7FFFFFFF:
-        raise ValueError("too many rows for one launch")
+    grid = _grid(rows * parts, params["THREADS"], "rows")
     kern = R.get_kernel("token_logprobs", SPLIT=int(parts > 1), **params)
     results = ((rows,), torch.float32), ((rows,), torch.float32), ((rows, top), torch.float32), ((rows, top), torch.int64)
     if parts == 1:
-        return _into_last(kern.bind(grid=(rows,)), *results), None, 1
+        return _into_last(kern.bind(grid=grid), *results), None, 1
     vectors = -(-v * size // 16) + params["SHIFT"]
     floats = rows * (3 * parts + (4 * -(-vectors // 64) if top else 0))
-    join = R.get_kernel("logprobs_join", **{**params, "THREADS": 512}).bind(grid=(rows,))
-    return _into_last(kern.bind(grid=(rows * parts,)), ((floats,), torch.float32)), _into_last(join, *results), parts
+    join = R.get_kernel("logprobs_join", **{**params, "THREADS": 512}).bind(grid=_grid(rows, 512, "rows"))
+    return _into_last(kern.bind(grid=grid), ((floats,), torch.float32)), _into_last(join, *results), parts
 
 
 def _token_logprobs_form(rows, bytes_):

@@ -2,10 +2,11 @@
 import re
 import subprocess
 
+import pytest
 import torch
 
 from kernelcodegen_amd import ops, runtime as R
-from test_decode_limits import Operand
+from test_decode_limits import Emitted, Operand
 
 
 def test_adapters_read_no_column_behind_the_last(tmp_path):
@@ -74,3 +75,31 @@ def test_adapters_kernels_have_only_the_parameters_that_they_depend_on(monkeypat
             assert with_other != text, key
         others = dict(N=77, K=512, XT=512, YT=72, ZT=64, Y_F32=1, SCALES=0, INPLACE=1, ONCE=0, TS=4, UT=4)
         assert R.emit_kernel(family, "kernel0", **{**others, **params})[0] == text
+
+
+def refused_from(monkeypatch, launch, first):
+    """`launch(n)` asks for a kernel below `first` and is refused from there on."""
+    def get_kernel(family, **params):
+        raise Emitted(params)
+    monkeypatch.setattr(R, "get_kernel", get_kernel)
+    with pytest.raises(Emitted):
+        launch(first - 1)
+    for n in (first, 4 * first, 1 << 33):
+        with pytest.raises(ValueError):
+            launch(n)
+
+
+def test_a_launch_has_fewer_than_2_to_the_32_threads(monkeypatch):
+    bf16, f32, i32, i64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
+    for v, threads in ((8, 128), (1 << 18, 512)):            # (a row's workgroup)
+        refused_from(monkeypatch, lambda rows: ops._token_logprobs_launch(Operand((rows, v), bf16), Operand((rows,), i64), 0, {}), (1 << 32) // threads)
+    refused_from(monkeypatch, lambda rows: ops._token_logprobs_launch(Operand((rows, 4096), f32), Operand((rows,), i64), 5, dict(PARTS=4, THREADS=256)), 1 << 22)
+    # the first launch has a workgroup of 256 for 16 tokens; the second, here, one for 64 tokens and 128 columns
+    adapters = lambda n: lambda tokens: ops._add_adapters_launch(Operand((tokens, n), bf16), Operand((tokens, 8), bf16), Operand((2, 8, 8), bf16), Operand((2, n, 8), bf16),
+                                                                 Operand((tokens,), i32), None, False, dict(NS=16))
+    refused_from(monkeypatch, adapters(8), (1 << 28) - 15)
+    refused_from(monkeypatch, adapters(2048), (1 << 26) - 63)
+    cache, scale = Operand((4, 16, 8, 64), torch.float8_e4m3fn), Operand((4, 8), f32)
+    # a wavefront for 16 tokens and a head of the keys or values, and for 32 heads of a token's queries
+    refused_from(monkeypatch, lambda tokens: ops._cache_append_launch(Operand((tokens, 32, 64), bf16), Operand((tokens, 8, 64), bf16), Operand((tokens, 8, 64), bf16), cache, cache,
+                                                                      scale, scale, Operand((tokens,), i64), Operand((tokens,), i32), Operand((100, 64), f32), False), (1 << 25) - 15)
