@@ -102,4 +102,4 @@ def test_a_launch_has_fewer_than_2_to_the_32_threads(monkeypatch):
     cache, scale = Operand((4, 16, 8, 64), torch.float8_e4m3fn), Operand((4, 8), f32)
     # a wavefront for 16 tokens and a head of the keys or values, and for 32 heads of a token's queries
     refused_from(monkeypatch, lambda tokens: ops._cache_append_launch(Operand((tokens, 32, 64), bf16), Operand((tokens, 8, 64), bf16), Operand((tokens, 8, 64), bf16), cache, cache,
-                                                                      scale, scale, Operand((tokens,), i64), Operand((tokens,), i32), Operand((100, 64), f32), False), (1 << 25) - 15)
+                                                                      scale, scale, Operand((tokens,), i64), Operand((tokens,), i32), Operand((100, 64), f32), False), (1 << 25) - 3)
