@@ -17,9 +17,11 @@
 //   neighbours (CW_PAIRS):                   (x_2i, x_2i+1) -> the same
 // with c and s of row `position` of the table.  What becomes of a key jumps where 8 bits do, so it has to be the formula's: the two products
 // are exact in fp64 and their sum is rounded there once; on the way to fp32 what is cut off leaves its trace in the last bit (rounding to odd), so the
-// rounding to 8 bits is that of the 53-bit number, and so is the comparison with 448 that gives the scale.  Queries, whose results have 16 or 32
-// bits, are summed in fp32 (all of it in fp64: 10240 tokens of 32 query heads, 8 others, 79 us, this way 43, 5.4 TB/s).  Wavefronts behind those of the cache take
-// a token's queries, CW_QN passes of CW_RPP heads for one reading of c and s.
+// rounding to 8 bits is that of the 53-bit number, and so is the comparison with 448 that gives the scale.  Queries in fp32
+// are summed in fp64 as well and rounded once (7206 tokens of 32 query heads, 8 others, 64 us, summed in fp32 68); those of 16 bits in fp32, whose two roundings
+// are 2^-12 and less of their last (in half precision 43 us, all of it in fp64 79).  Wavefronts behind those of the cache take a token's queries, CW_QN
+// passes of CW_RPP heads for one reading of c and s.
+// Half precision moves 163 MB in these 43 us, 3.7 TB/s: the turns in fp64 of the keys and their 128 registers bound it, not memory (fp32: 310 MB, 4.8 TB/s).
 // Measured, 8 heads of 128: 64 tokens of a page each 2.9 us (an empty launch 1.7); 9000 tokens of whole pages, half precision, 12.5 us, 4.4 TB/s.
 // Parameters: CW_NAME, CW_H, CW_D, CW_PAGE, CW_T (input type), CW_ESIZE, CW_WIN, strides as in cache_attention: CW_KP .. CW_VH (bytes), CW_XKT
 // CW_XKH CW_XVT CW_XVH (of k and v, elements); CW_ROT, and with it CW_R, CW_PAIRS, CW_HQ (heads of q), CW_QN, CW_XQT CW_XQH.
@@ -91,7 +93,7 @@ __device__ __forceinline__ float cw_odd(double v) {
   const unsigned low = (unsigned)b, cut = (low & 0xe0000000u) | ((low & 0x1fffffffu) ? 0x20000000u : 0u);
   return (float)__builtin_bit_cast(double, (b & 0xffffffff00000000ULL) | cut);
 }
-// The chunk x, whose partner is y, turned: with a sum in fp64 and rounded to odd (KEY), or in fp32.
+// The chunk x, whose partner is y, turned: with a sum in fp64, rounded to odd (KEY) or to the nearest, or for 16 bits in fp32.
 template <bool KEY> __device__ __forceinline__ void cw_apply(const CwTurn& w, const cw_x8& x, const cw_x8& y, int c, float (&f)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -99,9 +101,9 @@ template <bool KEY> __device__ __forceinline__ void cw_apply(const CwTurn& w, co
     const float a = (float)x[i], b = (float)(CW_PAIRS ? x[i ^ 1] : y[i]);
     const bool first = CW_PAIRS ? i % 2 == 0 : c < CW_HALF;
     float v;
-    if (KEY) {
-      const double p = (double)b * si;
-      v = cw_odd((double)a * co + (first ? -p : p));
+    if (KEY || CW_ESIZE > 2) {
+      const double p = (double)b * si, sum = (double)a * co + (first ? -p : p);
+      v = KEY ? cw_odd(sum) : (float)sum;
     } else {
       const float p = b * si;
       v = __builtin_fmaf(a, co, first ? -p : p);

@@ -1,11 +1,11 @@
-"""Adapters at the limits of their arithmetic, against the formulas in 64 bits."""
+"""Rotation into the cache and adapters at the limits of their arithmetic and of their forms, against the formulas in 64 bits."""
 import math
 
 import pytest
 import torch
 
 from kernelcodegen_amd import ops
-from test_gpu_answer_operators import adapters_case, check_adapters
+from test_gpu_answer_operators import adapters_case, angles, append_case, check_adapters, turned
 from test_gpu_decode_step import DTYPE, generator, ints
 
 pytestmark = pytest.mark.gpu
@@ -85,3 +85,17 @@ def test_adapters_of_more_than_a_thousand_tokens(dtype, out, tokens, n, k, rank,
     for at in (slice(None, 70), slice(tokens // 2 - 9, None, 29), slice(-40, None)):
         check_adapters(got, y, x, a, b, which, scale, at)
     assert ops.add_adapters(y, x, a, b, which, scale, inplace=True) is y and torch.equal(y, got)
+
+
+# ---- cache_append ----
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("tokens,heads,d,rotated", [(1, 12, 64, 32), (140, 32, 128, 128), (20, 3, 96, 96)])
+def test_queries_in_fp32_are_rounded_once(interleaved, tokens, heads, d, rotated):
+    """Products of fp32 numbers are exact in 64 bits, so the formula's sum there, rounded to fp32, is one number."""
+    slots = [16 + i for i in range(tokens)]
+    (q, k, v), caches, scales = append_case(tokens + d, slots, heads, 2, d, 16, "tokens", "f32", 12)
+    positions = ints([(37 * i) % 500 for i in range(tokens)])
+    table = angles(500, rotated)
+    got = ops.cache_append(q, k, v, *caches, *scales, ints(slots, torch.int64), positions, table, interleaved=interleaved)
+    assert torch.equal(got, turned(q, positions, table, interleaved).float())
