@@ -1,11 +1,11 @@
-"""Rotation into the cache and adapters at the limits of their arithmetic and of their forms, against the formulas in 64 bits."""
+"""Rotation into the cache, adapters and log probabilities at the limits of their arithmetic and of their forms, against the formulas in 64 bits."""
 import math
 
 import pytest
 import torch
 
 from kernelcodegen_amd import ops
-from test_gpu_answer_operators import adapters_case, angles, append_case, check_adapters, turned
+from test_gpu_answer_operators import adapters_case, angles, append_case, check_adapters, check_logprobs, turned
 from test_gpu_decode_step import DTYPE, generator, ints
 
 pytestmark = pytest.mark.gpu
@@ -99,3 +99,43 @@ def test_queries_in_fp32_are_rounded_once(interleaved, tokens, heads, d, rotated
     table = angles(500, rotated)
     got = ops.cache_append(q, k, v, *caches, *scales, ints(slots, torch.int64), positions, table, interleaved=interleaved)
     assert torch.equal(got, turned(q, positions, table, interleaved).float())
+
+
+def test_append_writes_the_same_in_a_graph_and_on_another_stream():
+    """The cache and its scales, put back before each call, with other keys, values and positions in the same places."""
+    slots = list(range(16, 60))
+    (q, k, v), caches, scales = append_case(5, slots, 4, 2, 64, 16, "tokens", "bf16", 5)
+    at, where, table = ints(slots, torch.int64), ints([i + 3 for i in range(44)]), angles(100, 64)
+    held = [c.view(torch.uint8) for c in caches] + scales
+    old = [h.clone() for h in held]
+
+    def restore():
+        for h, o in zip(held, old):
+            h.copy_(o)
+
+    def append():
+        return ops.cache_append(q, k, v, *caches, *scales, at, where, table)
+
+    def what(call):
+        restore()
+        return [t.clone() for t in (call(), *held)]
+    first, side = what(append), torch.cuda.Stream()
+    assert not any(torch.equal(h, o) for h, o in zip(held, old))
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = what(append)
+    side.synchronize()
+    assert all(torch.equal(g, w) for g, w in zip(got, first))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        recorded = append()
+    for i in range(4):
+        q.copy_(torch.randn(q.shape, generator=generator(i), device="cuda"))
+        k.copy_(torch.randn(k.shape, generator=generator(i + 9), device="cuda") * 4.0 ** i)
+        v.copy_(torch.randn(v.shape, generator=generator(i + 19), device="cuda") * 0.25 ** i)
+        where.add_(7)
+        want = what(append)
+        recorded.zero_()
+        got = what(lambda: graph.replay() or recorded)
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want)) and not torch.equal(got[0], first[0])
