@@ -139,3 +139,19 @@ def test_append_writes_the_same_in_a_graph_and_on_another_stream():
         got = what(lambda: graph.replay() or recorded)
         torch.cuda.synchronize()
         assert all(torch.equal(g, w) for g, w in zip(got, want)) and not torch.equal(got[0], first[0])
+
+
+# ---- token_logprobs: more rows than two for each unit ----
+
+@pytest.mark.parametrize("dtype,rows,v,top", [("bf16", 1024, 5003, 32), ("f32", 1500, 801, 5), ("bf16", 1030, 32000, 0), ("f16", 1100, 20011, 20)])
+def test_log_probabilities_of_more_than_a_thousand_rows(dtype, rows, v, top):
+    """The workgroups that the rule takes from 1024 rows on; rows with few numbers left, none, an infinity or a NaN among the others."""
+    g = generator(rows)
+    logits = (torch.randn((rows, v), generator=g, device="cuda") * 3).to(DTYPE[dtype])
+    tokens = torch.randint(-1, v + 1, (rows,), generator=g, device="cuda")
+    logits[3::50, 40:] = -math.inf
+    logits[7::90] = -math.inf
+    logits[8::91, v // 2], logits[9::92, v - 1], logits[10::93, 5:] = math.inf, math.nan, logits[10, 0]
+    check_logprobs(ops.token_logprobs(logits, tokens, top), logits, tokens, top)
+    x = logits[:, 3:v - 2]
+    check_logprobs(ops.token_logprobs(x, tokens - 4, min(top, 7)), x, tokens - 4, min(top, 7))
