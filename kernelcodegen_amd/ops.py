@@ -797,10 +797,13 @@ def _add_adapters_form(tokens, adapters, n, k, rank, columns):
     """Tokens of a tile (16 TS, and 16 UT in the second launch), workgroups for a tile's adapters (S), for parts of k (KS) and of the columns (NS).
 
     Up to 1024 tokens may be a decoding step's, with an adapter each: tiles of 16, whose adapters up to 16 workgroups share out, 8 where the second launch
-    has many more than fill the part.  More tokens are prompts'.  Parts of k fill the part in the first launch and are read by all workgroups
-    of the second, the more the higher the rank.  Measured, in us, first and second launch, or both:
-      N = K = 4096, 8 tokens, 8 adapters: of rank 128 k in 2 parts 19, 4 16.6, 8 16.9;  64 of 64: 38, 41, 57, of rank 32 13.2, 13.2;  1250 tokens, rank 32: 16.5, 15.3,
-      20.2, rank 64: 21.7, 23.3, 31, in one 29;  2000 of rank 128: 45, 48, 75
+    has many more than fill the part.  More tokens are prompts'.  Parts of k fill the part in the first launch, the shorter the longer k is, and are read by all workgroups
+    of the second, the more the higher the rank and the more columns: from rank 64 on two, not four, where workgroups of the first times n are 64 k or more.
+    Measured, in us, first and second launch, or both:
+      N = K = 4096, 8 tokens, 8 adapters: of rank 128 k in 2 parts 19, 4 16.7, 8 16.9, rank 64 12.1, 11.0;  64 of 64: 38, 41, rank 64 19.7, 21.7, rank 32 13.2, 13.2
+      1250 tokens, rank 32: 16.5, 15.3, 20.2;  4 runs of rank 64, 1100 tokens: k in one 29.6, 2 parts 22.4, 4 21.5;  1900: 31.8, 25.0, 25.1, rank 128 57, 43.4, 42.8
+      N 11008, K 4096, rank 64, 128 tokens of 3 adapters: 2 parts 19.0, 4 19.4;  48 of 48: 32, 33;  4 runs, 1900 tokens: 36.6, 40.9
+      N 4096, K 11008, the same: 21.4, 16.2;  31, 26;  40.2, 35.2;  rank 128: 32, 26;  65, 56;  73, 58
       64 tokens, 40 adapters of rank 16: k in 4 parts 4.8 and 5.4, in 8 4.1 and 6.6;  8 workgroups for a tile's adapters 11.9, 16 9.8
       128 tokens, 64 adapters of rank 64, N 11008: 32 tokens a tile 36, 16 39 (LDS for four wavefronts' columns);  300 tokens with one adapter: 6.5, 12.7
       512 tokens, 64 adapters of rank 16: 16 workgroups for a tile's adapters 27.4, 8 27.8, 4 37;  1000 tokens: 57, 52, 54;  700 of rank 64, N 11008: 206, 175
@@ -812,7 +815,7 @@ def _add_adapters_form(tokens, adapters, n, k, rank, columns):
     ut = 4 if tokens > 1024 or rank > 128 else 2 if rank > 16 else 1
     tiles, wide, blocks = -(-tokens // (16 * ts)), -(-tokens // (16 * ut)), -(-n // (columns * 4 // ut))
     slots = min(8 if wide * blocks > 384 else 16, tokens, adapters) if tokens <= 1024 else 1
-    ks = max(1, min(2 if rank >= 64 and tiles * slots >= 60 else 4, 256 // (min(tiles, 16) * slots) if tokens <= 1024 else 768 // tiles, k // 512))
+    ks = max(1, min(2 if rank >= 64 and tiles * slots * n >= 64 * k else 4, 256 // (min(tiles, 16) * slots) if tokens <= 1024 else 768 // tiles, k // 512))
     ks = 1 << ks.bit_length() - 1            # (a kernel for each)
     each = max(1, blocks * wide // 2048) if slots == 1 else 1
     return dict(TS=ts, UT=ut, S=slots, KS=ks, NS=-(-blocks // each))

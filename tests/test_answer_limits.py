@@ -103,3 +103,15 @@ def test_a_launch_has_fewer_than_2_to_the_32_threads(monkeypatch):
     # a wavefront for 16 tokens and a head of the keys or values, and for 32 heads of a token's queries
     refused_from(monkeypatch, lambda tokens: ops._cache_append_launch(Operand((tokens, 32, 64), bf16), Operand((tokens, 8, 64), bf16), Operand((tokens, 8, 64), bf16), cache, cache,
                                                                       scale, scale, Operand((tokens,), i64), Operand((tokens,), i32), Operand((100, 64), f32), False), (1 << 25) - 3)
+
+
+def test_adapters_parts_of_k_by_columns_and_k():
+    """From rank 64 on four parts of k turn into two where the second launch reads them too often, and are no more than k or the part has room for."""
+    def parts(tokens, adapters, n, k, rank):
+        return ops._add_adapters_form(tokens, adapters, n, k, rank, 128)["KS"]
+    for rank in (64, 128):
+        assert [parts(64, 64, 4096, k, rank) for k in (2048, 4096, 4104, 11008)] == [2, 2, 4, 4]
+        assert [parts(64, 64, n, 4096, rank) for n in (1024, 4088, 4096, 11008)] == [4, 4, 2, 2]
+        assert parts(128, 64, 4096, 11008, rank) == 2 and parts(5000, 3, 4096, 11008, rank) <= 4
+    assert parts(64, 64, 11008, 4096, 56) == 4
+    assert [parts(1, 1, 4096, k, 16) for k in (8, 1024, 1536, 2048, 11008)] == [1, 2, 2, 4, 4]
