@@ -210,7 +210,8 @@ __device__ __forceinline__ void ad_put(ad_y* z, int n, ad_yv v) {
 }
 
 // a as the sum of AD_PIECES 16-bit numbers of its sign, none of them 0 unless a is (or, in half precision, below 2^-23): an infinity of B times all of them
-// is one, as times a.  Each is cut off, so that what is left has a's sign; where nothing is left, or nothing finite, halves do.
+// is one, as times a.  Each is cut off, so that what is left has a's sign; where nothing is left, or nothing finite, halves of the first do (not of the last: a
+// matrix instruction drops digits below those of fp32).
 __device__ __forceinline__ void ad_split(float a, float (&p)[3]) {
 #if AD_F16
   p[0] = (float)__builtin_amdgcn_cvt_pkrtz(a, a)[0];
@@ -218,13 +219,11 @@ __device__ __forceinline__ void ad_split(float a, float (&p)[3]) {
   p[1] = a - a == 0.0f ? a - p[0] : a;
 #else
   auto cut = [](float v) { return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, v) & 0xffff0000u); };
-  p[0] = cut(a);
-  const float left = a - p[0], half = a * 0.5f, mine = __builtin_fabsf(left) > 0.0f ? left : half;
-  p[0] = __builtin_fabsf(left) > 0.0f ? p[0] : half;
-  p[1] = cut(mine);
-  const float rest = mine - p[1], quarter = mine * 0.5f;
-  p[1] = __builtin_fabsf(rest) > 0.0f ? p[1] : quarter;
-  p[2] = __builtin_fabsf(rest) > 0.0f ? rest : quarter;
+  const float high = cut(a), half = a * 0.5f, left = __builtin_fabsf(a - high) > 0.0f ? a - high : half, rest = left - cut(left);
+  p[0] = __builtin_fabsf(a - high) > 0.0f ? high : half;
+  p[1] = cut(left);
+  p[2] = __builtin_fabsf(rest) > 0.0f ? rest : p[0] * 0.5f;
+  p[0] = __builtin_fabsf(rest) > 0.0f ? p[0] : p[0] * 0.5f;
 #endif
 }
 
@@ -302,14 +301,14 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
 #pragma unroll
     for (int s = 0; s < AD_OWN; ++s) {
       const int q = s * 4 + g;
-      ad_v p[AD_PIECES];
+      ad_v p[AD_STEPS / AD_OWN];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float of[3];
         ad_split(AD_F16 ? h[s][e] * up : h[s][e], of);
         if (AD_CHUNKS % 4) of[0] = q < AD_CHUNKS ? of[0] : q < 2 * AD_CHUNKS ? of[1] : q < AD_PIECES * AD_CHUNKS ? of[AD_PIECES - 1] : 0.0f;
 #pragma unroll
-        for (int n = 0; n < AD_PIECES; ++n) p[n][e] = (ad_x)of[n];
+        for (int n = 0; n < AD_STEPS / AD_OWN; ++n) p[n][e] = (ad_x)of[n];
       }
 #pragma unroll
       for (int n = 0; n < AD_STEPS / AD_OWN; ++n) f[n * AD_OWN + s] = __builtin_bit_cast(kcg_u32x4, p[n]);

@@ -21,6 +21,8 @@ def test_adapters_h_enters_the_second_product_whole(dtype, out, tokens, n, rank)
     g = generator(tokens + rank)
     digits, unit = ((65536.0, 256.0, 1.0), 1.0) if dtype == "bf16" else ((2048.0, 1.0), 2.0 ** -7)
     values = [torch.randint(1, 256 if dtype == "bf16" else 2048, (tokens, rank), generator=g, device="cuda").double() * d * unit for d in digits]
+    for n, digit in enumerate(values):
+        digit[n::3, n::2] = 0.0           # (nothing left of one behind the others)
     x = torch.stack(values + [torch.zeros_like(values[0])] * (4 - len(digits)), -1).view(tokens, 4 * rank).to(DTYPE[dtype])
     a = torch.eye(rank, device="cuda").repeat_interleave(4, 1)[None].to(DTYPE[dtype])
     j = torch.arange(n, device="cuda") % rank
