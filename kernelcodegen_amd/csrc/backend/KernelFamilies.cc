@@ -1832,7 +1832,7 @@ bool emitAdapters(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::
 // token_logprobs, and logprobs_join, which finishes rows that several workgroups share: the same parameters.
 bool emitLogprobs(KernelSpec& s, std::string& src, KernelLaunchInfo& info, std::string& err) {
   const bool join = s.family == "logprobs_join";
-  // (an index of a number or a segment has 32 bits; the segments of a row are in LDS)
+  // (the keys by which alternatives are ordered have 19 bits for an index, beside the value's 32; the segments of a row are in LDS)
   if (!whole(s, "V", 1, 1 << 19, err) || !whole(s, "F16", 0, 2, err) || !whole(s, "TOP", 0, 32, err)) return false;
   const int64_t v = s.p["V"], esize = s.p["F16"] ? 2 : 4;
   if (s.p["TOP"] > v) { err = s.family + ": TOP must not be above V"; return false; }

@@ -5,21 +5,23 @@
 // Two launches, since every column needs all of h: adapters_down leaves h in fp32, in AD_KS parts of k; adapters_up adds the parts in order.
 // Tokens come in any order, and a step's requests may have an adapter each or share one.  A tile is 16 AD_TS tokens as they stand (of either launch its
 // own AD_TS); each adapter that occurs in it (found by comparing lanes) is multiplied with the whole tile, and of the result only its own tokens
-// are kept: rows of a matrix product do not touch one another.  A prompt's tiles have one adapter; a decoding step's have up to 16, which
-// workgroups share; those that find none are the last of the launch.
+// are kept: rows of a matrix product do not touch one another.  Up to 1024 tokens, which may all have different ones, tiles have 16 tokens in the first launch and 16,
+// 32 or 64 (ranks up to 16, up to 128, more) in the second, and workgroups share a tile's adapters; those that find none are the last of the launch.
+// More tokens are prompts', whose tiles have one adapter or a few: 16 tokens, or 32 for ranks of 65 to 128, and 64.
 // h is not rounded to 16 bits: it enters the second product as the sum of AD_PIECES 16-bit numbers, which the matrix instruction takes as AD_PIECES AD_RANK
-// values of k with B's columns as often.  Two of half precision have 22 bits, three of bfloat16 all of fp32's 24.  (Two of bfloat16 have 16: of 262144 results in
-// bfloat16, 64 tokens with 40 adapters, 295 were not the nearest to the formula, of the formula in fp32 53, of this 24; 9.3 and 9.5 us.)  In half precision h is brought below 2^15 by
-// a power of two of its row.
+// values of k with B's columns as often.  Two of half precision have 22 bits, three of bfloat16 all of fp32's 24.  (Two of bfloat16 have 16: of 262144
+// results in bfloat16, 64 tokens with 40 adapters, 295 were not the nearest to the formula, of the formula in fp32 53, of this 24; 9.3 and 9.5 us.)  In half
+// precision h is brought below 2^15 by a power of two of its row.
 // Both products have the tokens as their columns, so that a lane has four neighbouring numbers of one token in each result.
-// Reading and writing bound prompts: 5000 tokens, rank 64, K = N = 4096 in bfloat16 13 us (X, 3.1 TB/s, LDS under way 40 % of the time) and 21 (Y and Z, 3.9
-// TB/s); 2600 tokens, rank 32, N = 11008 in fp32 11.4 and 51 (4.5 TB/s).  Of few tokens each launch is a chain: which adapter, its numbers, a sum over
-// wavefronts, the store: one token 2.9 and 4.0 us, 64 tokens with 40 adapters between them 4.8 and 5.5.  Both in one launch, in which a workgroup has all
-// of h for its columns, take as long for a tile alone (6.8) and lose from there on (64 tokens: 11.1).
+// Reading and writing bound prompts: 5000 tokens, rank 64, K = N = 4096 in bfloat16 13.7 us (X, 3.0 TB/s, LDS under way 41 % of the time) and 22 (Y and Z, 3.7
+// TB/s); 2600 tokens, rank 32, N = 11008 in fp32 11.5 and 50 (4.6 TB/s).  Of few tokens each launch is a chain: which adapter, its numbers, a sum over
+// wavefronts, the store: one token 2.9 and 4.2 us, 64 tokens with 40 adapters between them 4.8 and 5.8.  Both in one launch, in which a workgroup has all
+// of h for its columns, take as long for a tile alone (6.8) and lose from there on (64 tokens: 11.1).  Hundreds of tokens in any order with tens of adapters read a
+// matrix once for each tile that has its adapter: 1000 tokens with 64 adapters of rank 16 54 us, where each matrix once would be 8.
 // Parameters: AD_NAME, AD_UP (this is adapters_up), AD_F16, AD_PIECES, AD_RANK, AD_K, AD_N, AD_XT, AD_YT, AD_ZT (strides of rows, elements), AD_YTYPE,
-// AD_YSIZE, AD_ALIGN (rows of Y and Z start on multiples of 16 bytes), AD_SCALE (0: no scales), AD_INPLACE, AD_TS, AD_KS, AD_MANY (a tile's adapters are
-// shared out; between how many workgroups, and how many there are along N, are arguments), AD_ONCE (there are as many along N as have columns:
-// each has one pass).
+// AD_YSIZE, AD_ALIGN (rows of Y and Z start on multiples of 16 bytes), AD_SCALE (0: no scales), AD_INPLACE, AD_TS, AD_KS, AD_DEPTH (steps of k under way), AD_MANY (a
+// tile's adapters are shared out; between how many workgroups, and how many there are along N, are arguments), AD_ONCE (there are as many along N
+// as have columns: each has one pass).  adapters_down has AD_F16, AD_RANK, AD_K, AD_XT, AD_TS, AD_KS, AD_DEPTH and AD_MANY of them.
 typedef _Float16 ad_f16x8 __attribute__((ext_vector_type(8)));
 #if AD_F16
 typedef _Float16 ad_x;

@@ -18,10 +18,11 @@
 // with c and s of row `position` of the table.  What becomes of a key jumps where 8 bits do, so it has to be the formula's: the two products
 // are exact in fp64 and their sum is rounded there once; on the way to fp32 what is cut off leaves its trace in the last bit (rounding to odd), so the
 // rounding to 8 bits is that of the 53-bit number, and so is the comparison with 448 that gives the scale.  Queries in fp32
-// are summed in fp64 as well and rounded once (7206 tokens of 32 query heads, 8 others, 64 us, summed in fp32 68); those of 16 bits in fp32, whose two roundings
-// are 2^-12 and less of their last (in half precision 43 us, all of it in fp64 79).  Wavefronts behind those of the cache take a token's queries, CW_QN
-// passes of CW_RPP heads for one reading of c and s.
-// Half precision moves 163 MB in these 43 us, 3.7 TB/s: the turns in fp64 of the keys and their 128 registers bound it, not memory (fp32: 310 MB, 4.8 TB/s).
+// are summed in fp64 as well and rounded once (7206 tokens of 32 query heads, 8 others, 64 us, summed in fp32 68); those of 16 bits in fp32, off
+// by 2^-24 of the product and of the sum before their own rounding (half precision 43 us; with sines in two parts, whose products are exact, 46; in fp64 79).
+// Wavefronts behind those of the cache take a token's queries, CW_QN passes of CW_RPP heads for one reading of c and s.
+// Half precision moves 163 MB in these 43 us, 3.7 TB/s, of which keys and values alone take about 23: the keys' turns in fp64 and their registers (two wavefronts a
+// SIMD) bound it, not memory.  fp32 moves 310 MB at 4.8 TB/s.
 // Measured, 8 heads of 128: 64 tokens of a page each 2.9 us (an empty launch 1.7); 9000 tokens of whole pages, half precision, 12.5 us, 4.4 TB/s.
 // Parameters: CW_NAME, CW_H, CW_D, CW_PAGE, CW_T (input type), CW_ESIZE, CW_WIN, strides as in cache_attention: CW_KP .. CW_VH (bytes), CW_XKT
 // CW_XKH CW_XVT CW_XVH (of k and v, elements); CW_ROT, and with it CW_R, CW_PAIRS, CW_HQ (heads of q), CW_QN, CW_XQT CW_XQH.

@@ -15,11 +15,11 @@
 // those of a wavefront the k-th is a bound, what reaches the highest bound is counted out against one another.
 // Vectors are the aligned ones of memory, the first and the last of a row maybe with elements outside of it, which are left out.
 // A row is a workgroup, or several parts (LP_SPLIT; how many is an argument), whose sums and segments logprobs_join (LP_JOIN) finishes.
-// Reading bounds large calls: 2000 rows of 32000 in bfloat16 26 us, 4.9 TB/s; with 20 alternatives 35, of which the two picks take 8 (some 500
-// instructions of each wavefront, a chain of LDS accesses and three barriers each, while others read).  64 rows of 128000 in fp32 in 16 parts
-// 8.3 us, 3.9 TB/s, and the join 2, or 5.7 with 20 alternatives.  One row of 32000 with 5 of them 7.1, a chain as well: four trips over the row, two
-// picks, a trip between.  Of many equal numbers (a masked row's -inf) each wavefront finds its LP_TOP largest one after the other: 64 rows of 128000 with
-// 8 left 22 us, not 12.
+// Reading bounds large calls, and their instructions nearly as much: 2000 rows of 32000 in bfloat16 26 us, 4.9 TB/s, vector instructions 88 % of the time; with
+// 20 alternatives 35, of which the two picks take 8 (some 500 instructions of each wavefront, a chain of LDS accesses and three barriers each, while others
+// read).  64 rows of 128000 in fp32 in 16 parts 8.4 us, 3.9 TB/s, and the join 2, or 5.9 with 20 alternatives.  One row of 32000 with 5 of them 7.0, a chain
+// as well: four trips over the row, two picks, a trip between.  Of many equal numbers (a masked row's -inf) each wavefront finds its LP_TOP largest one after
+// the other: 64 rows of 128000 with 8 left 24 us, not 13, 2000 of 32000 67, not 35.
 // Parameters: LP_NAME, LP_V, LP_T, LP_ES (element bytes), LP_STRIDE (of rows, elements), LP_SHIFT (rows may start off a multiple of 16 bytes), LP_TOP,
 // LP_SPLIT, LP_THREADS, LP_U, LP_JOIN.
 typedef LP_T lp_t;
