@@ -11,7 +11,7 @@
 // h is not rounded to 16 bits: it enters the second product as the sum of AD_PIECES 16-bit numbers, which the matrix instruction takes as AD_PIECES AD_RANK
 // values of k with B's columns as often.  Two of half precision have 22 bits, three of bfloat16 all of fp32's 24.  (Two of bfloat16 have 16: of 262144
 // results in bfloat16, 64 tokens with 40 adapters, 295 were not the nearest to the formula, of the formula in fp32 53, of this 24; 9.3 and 9.5 us.)  In half
-// precision h is brought below 2^15 by a power of two of its row.
+// precision h is brought below 2^15 by a power of two of its row's finite numbers.
 // Both products have the tokens as their columns, so that a lane has four neighbouring numbers of one token in each result.
 // Reading and writing bound prompts: 5000 tokens, rank 64, K = N = 4096 in bfloat16 13.7 us (X, 3.0 TB/s, LDS under way 41 % of the time) and 22 (Y and Z, 3.7
 // TB/s); 2600 tokens, rank 32, N = 11008 in fp32 11.5 and 50 (4.6 TB/s).  Of few tokens each launch is a chain: which adapter, its numbers, a sum over
@@ -289,7 +289,7 @@ void AD_NAME(const float* __restrict__ part, const ad_y* Y, const ad_x* __restri
 #pragma unroll
         for (int e = 0; e < 8; ++e) h[s][e] += parts[p][e / 4][e % 4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) most = fmaxf(most, __builtin_fabsf(h[s][e]));
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, __builtin_fabsf(h[s][e]) < __builtin_inff() ? __builtin_fabsf(h[s][e]) : 0.0f);        // (beside an infinity, the others)
     }
     float up = 1.0f;
     if (AD_F16) {

@@ -46,7 +46,7 @@ def test_adapters_of_infinite_numbers(dtype, out, n, rank):
     scale[1] = -1.5
     good = ops.add_adapters(y, x, a, b, which, scale)
     b[0, 3, 5], b[0, 17, 1], b[0, n - 1, rank - 1], b[0, 9, 0], b[0, 9, 7], b[1, 3, 2], b[1, 5, 4], b[2, 6, 1] = math.inf, -math.inf, math.inf, math.inf, math.inf, -math.inf, math.nan, -math.inf
-    a[2, 1, 7] = math.inf
+    a[2, 1, 7] = b[2, 8, 3] = math.inf          # (an infinity of x a beside one of b that meets another number)
     got = ops.add_adapters(y, x, a, b, which, scale)
     want = y.double()
     for r in range(3):
